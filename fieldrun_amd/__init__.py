@@ -19,6 +19,10 @@ The classes mirror the reference's interface for this path
                           unembed over an f32 / f16 / rowi8 (vocab, d) table,
                           and rowdot_f32_subset (995-1015)
 
+  KvCache                 a paged key / value cache in the caller's device
+                          memory: rows written (quantised) and read back,
+                          attention over it (decode and prompt rows)
+
 Errors the reference raises by panicking come back as FrqError carrying the
 library's status code and message.
 """
@@ -98,6 +102,11 @@ SIGNATURES = {
     "frq_gemma_set_graphs": (_I, [_P, _I]),
     "frq_gemma_generate": (_I, [_P, _P, _P, _S, _S, _P, _P]),
     "frq_gemma_generate_batch": (_I, [_P, _P, _P, _S, _S, _S, _P, _P]),
+    "frq_norm_quant_i8_dev": (_I, [_P, _P, _P, _P, C.c_double, _S, _S, _P, _P, _P, _P, _P]),
+    "frq_kv_write_dev": (_I, [_P, _P, _P, _P, _S, _P, _S]),
+    "frq_kv_read_dev": (_I, [_P, _P, _P, _S, _P, _P, _S]),
+    "frq_kv_attn_ws": (_S, [_P, _S, _S, _S, _S]),
+    "frq_kv_attn_dev": (_I, [_P, _P, _P, _S, _S, _S, _P, _S, _P, _P, _S, C.c_double, C.c_double, _S, _P, _S, _P, _S]),
     "frq_gemma_predict": (_I, [_P, _P, _P, _S, _P, _P]),
 }
 
@@ -167,6 +176,11 @@ class Context:
     def set_stream(self, stream_handle: int | None):
         _check(lib.frq_set_stream(self.h, stream_handle))
 
+    @property
+    def stream(self) -> int:
+        """The HIP stream calls are enqueued on (frq_get_stream)."""
+        return lib.frq_get_stream(self.h)
+
     def sync(self):
         _check(lib.frq_sync(self.h))
 
@@ -174,6 +188,13 @@ class Context:
                   oval_ptr: int):
         """Activation quant of the I8 arm on device pointers (a8 pitch quant_pitch(k))."""
         _check(lib.frq_quant_i8_dev(self.h, a_ptr, m, k, a8_ptr, sa_ptr, oidx_ptr, oval_ptr))
+
+    def norm_quant_dev(self, x_ptr: int, y_ptr: int | None, w_ptr: int, eps: float, m: int, k: int,
+                       sum_ptr: int | None, a8_ptr: int, sa_ptr: int, oidx_ptr: int, oval_ptr: int):
+        """Residual x + y (into sum_ptr), RMS norm with gain w, and the int8
+        rows quant_dev gives for it, on device pointers, for Weight.mm_q_dev."""
+        _check(lib.frq_norm_quant_i8_dev(self.h, x_ptr, y_ptr, w_ptr, eps, m, k, sum_ptr, a8_ptr, sa_ptr, oidx_ptr,
+                                         oval_ptr))
 
     # ---- uploads ----
     def upload_i8(self, wt_nk: np.ndarray, scale: np.ndarray) -> "Weight":
@@ -304,6 +325,63 @@ class Context:
         _check(lib.frq_moe_route(self.h, _ptr(logits), T, E, topk, int(norm_topk), _ptr(pes),
                                  _ptr(sel), _ptr(w)))
         return sel, w
+
+
+class _Kv(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("n_pages", C.c_size_t), ("page", C.c_size_t), ("n_kv", C.c_size_t),
+                ("hd", C.c_size_t), ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p),
+                ("v_scale", C.c_void_p), ("page_stride", C.c_size_t), ("scale_stride", C.c_size_t)]
+
+
+class KvCache:
+    """A paged key / value cache in the caller's device memory (frq_kv):
+    k (n_pages, n_kv, page, hd), v (n_pages, n_kv, hd, page) of kind 'f32',
+    'f16' or 'rowi8' (with f32 steps k_scale, v_scale (n_pages, n_kv, page)).
+    page_stride / scale_stride: values between pages where they are not
+    dense.  A token's slot is page id * page + place in the page.  The memory
+    stays the caller's and outlives the object's calls."""
+
+    KINDS = {"f32": FRQ_DT_F32, "f16": FRQ_DT_F16, "rowi8": FRQ_DT_ROWI8}
+
+    def __init__(self, ctx: Context, kind: str, n_pages: int, page: int, n_kv: int, hd: int, k_ptr: int, v_ptr: int,
+                 k_scale_ptr: int | None = None, v_scale_ptr: int | None = None, page_stride: int = 0,
+                 scale_stride: int = 0):
+        if kind not in self.KINDS:
+            raise FrqError(FRQ_ERR_DTYPE, f"unknown cache kind {kind!r}")
+        self.ctx = ctx
+        self.desc = _Kv(self.KINDS[kind], n_pages, page, n_kv, hd, k_ptr, v_ptr, k_scale_ptr, v_scale_ptr,
+                        page_stride, scale_stride)
+        self._ref = C.byref(self.desc)
+        self.row = n_kv * hd
+
+    def write_dev(self, k_ptr: int, v_ptr: int, slot_ptr: int, n: int, pitch: int | None = None):
+        """n rows of keys and values (pitch floats apart, default dense) into
+        the slots of slot_ptr (int64), on the context stream."""
+        _check(lib.frq_kv_write_dev(self.ctx.h, self._ref, k_ptr, v_ptr, self.row if pitch is None else pitch,
+                                    slot_ptr, n))
+
+    def read_dev(self, slot_ptr: int, n: int, k_ptr: int, v_ptr: int, pitch: int | None = None):
+        """The slots' keys and values back in f32."""
+        _check(lib.frq_kv_read_dev(self.ctx.h, self._ref, slot_ptr, n, k_ptr, v_ptr,
+                                   self.row if pitch is None else pitch))
+
+    def attn_ws_bytes(self, n_row: int, n_head: int, n_seq: int, pages_pitch: int) -> int:
+        """Bytes of the workspace attn_dev takes for such a call."""
+        return lib.frq_kv_attn_ws(self._ref, n_row, n_head, n_seq, pages_pitch)
+
+    def attn_dev(self, q_ptr: int, n_row: int, n_head: int, pages_ptr: int, pages_pitch: int, len_ptr: int,
+                 n_seq: int, out_ptr: int, first_ptr: int | None = None, scale: float | None = None,
+                 cap: float = 0.0, window: int = 0, q_pitch: int | None = None, out_pitch: int | None = None,
+                 ws_ptr: int | None = None, ws_bytes: int = 0):
+        """Attention of n_row query rows of n_seq sequences over the cache
+        (frq_kv_attn_dev); scale defaults to 1 / sqrt(hd), pitches to dense
+        rows, first_ptr None to one row a sequence."""
+        hd = self.desc.hd
+        wide = n_head * hd
+        _check(lib.frq_kv_attn_dev(self.ctx.h, self._ref, q_ptr, wide if q_pitch is None else q_pitch, n_row, n_head,
+                                   pages_ptr, pages_pitch, len_ptr, first_ptr, n_seq,
+                                   hd ** -0.5 if scale is None else scale, cap, window, out_ptr,
+                                   wide if out_pitch is None else out_pitch, ws_ptr, ws_bytes))
 
 
 class Weight:

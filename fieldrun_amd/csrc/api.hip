@@ -34,7 +34,7 @@ struct frq_ctx {
     hipStream_t stream = nullptr;
     void* ws = nullptr;
     size_t ws_bytes = 0;
-    int* err = nullptr;  // device word: kernels atomically OR 1 on NaN input
+    int* err = nullptr;  // device word: kernels atomically OR 1 on NaN input, 2 on a bad index (kv_attn.h)
 };
 
 // Scratch of frq_mm_dev_noalloc: one static array per GPU (each device that
@@ -216,6 +216,7 @@ int check_err_word(frq_ctx* c) {
     if (h) {
         const int zero = 0;
         HIPCHK(hipMemcpy(c->err, &zero, sizeof(int), hipMemcpyHostToDevice), "hipMemcpy(err)");
+        if (!(h & 1)) return fail(FRQ_ERR_ARG, "a page, slot, length or row offset of the cache was out of range");
         return fail(FRQ_ERR_NAN, "NaN in activations (the reference panics in partial_cmp().unwrap())");
     }
     return FRQ_OK;

@@ -1,0 +1,8 @@
+// kv_attn_f16.hip — paged attention over an f16 cache (kv_attn.h), gfx950.
+#include "kv_attn.h"
+
+namespace frq {
+namespace kv {
+hipError_t launch_decode_f16(const Args& a, const Launch& l) { return launch_decode<FRQ_DT_F16>(a, l); }
+}  // namespace kv
+}  // namespace frq

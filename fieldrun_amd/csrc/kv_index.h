@@ -1,0 +1,113 @@
+// kv_index.h — where the rows, keys and pages of a paged attention call lie
+// (plain functions, the same on the host and on the device).
+//
+// A call's work is cut into items: a tile of `tp` (query row, head) pairs of
+// one sequence and kv head times a run of `chunk` of its keys.  Lengths and row
+// offsets are device data, so every workgroup finds its own item from them:
+// the chunk length follows from the whole call's keys (kv_chunk), the items
+// are numbered sequence after sequence, and the grid is the host's bound of
+// their number (kv_max_items).  A sequence cut into several chunks leaves
+// partial results in slots, at most kv_max_slots.
+#pragma once
+
+#include <stdint.h>
+
+#ifdef __HIPCC__
+#define KV_HD __host__ __device__ inline
+#else
+#define KV_HD inline
+#endif
+
+namespace frq {
+namespace kv {
+
+constexpr int ALIGN = 32;  // a sequence's first key of a window is rounded down to this
+
+struct Call {
+    const int32_t* len;    // [n_seq] cached tokens
+    const int32_t* first;  // [n_seq + 1] row offsets, or null: row s is sequence s's
+    int n_seq, n_row;      // sequences; rows of q
+    int width, shift;      // page ids of a table row; log2 of the page
+    int rep;               // query heads a kv head
+    int window;            // keys seen at most (0: all)
+    int n_kv;
+    int tp;                // pairs a tile
+    int min_pairs, max_pairs;  // the sequences served: pairs in [min, max]
+    int64_t target;        // items wanted over all kv heads
+    int min_chunk;         // keys a chunk at least, a multiple of ALIGN
+};
+
+struct Seq {
+    int row0, rows;  // its rows of q
+    int len;         // its keys
+    int lo, ext;     // the first key any row sees (rounded down), keys from there
+    int tiles;       // 0: not served
+    bool bad;        // its length or offsets are out of range
+};
+
+KV_HD Seq seq_of(const Call& c, int len, int r0, int r1) {
+    Seq q{r0, r1 - r0, len, 0, 0, 0, false};
+    if (r0 < 0 || r1 < r0 || r1 > c.n_row) {
+        q.row0 = q.rows = q.len = 0;
+        q.bad = true;
+        return q;
+    }
+    if (len < 0 || (int64_t)len > ((int64_t)c.width << c.shift)) {
+        q.len = 0;
+        q.bad = true;
+    }
+    const int64_t pairs = (int64_t)q.rows * c.rep;
+    if (pairs < c.min_pairs || pairs > c.max_pairs) return q;
+    q.tiles = (int)((pairs + c.tp - 1) / c.tp);
+    if (c.window) {
+        const int64_t lo = (int64_t)q.len - q.rows - c.window + 1;
+        q.lo = lo > 0 ? (int)(lo / ALIGN * ALIGN) : 0;
+    }
+    q.ext = q.len - q.lo;
+    return q;
+}
+KV_HD Seq seq_at(const Call& c, int s) {
+    return c.first ? seq_of(c, c.len[s], c.first[s], c.first[s + 1]) : seq_of(c, c.len[s], s, s + 1);
+}
+KV_HD int64_t keys_of(const Seq& q) { return (int64_t)q.tiles * q.ext; }
+
+// Keys a chunk when the call's tiles read `total` keys a kv head.
+KV_HD int chunk_of(const Call& c, int64_t total) {
+    const int64_t per = (total * c.n_kv + c.target - 1) / c.target;
+    const int64_t up = (per + c.min_chunk - 1) / c.min_chunk * c.min_chunk, most = 0x7FFFFFFF / ALIGN * ALIGN;
+    return (int)(up < c.min_chunk ? c.min_chunk : up > most ? most : up);
+}
+KV_HD int chunks_of(const Seq& q, int chunk) {
+    const int n = (int)(((int64_t)q.ext + chunk - 1) / chunk);
+    return n < 1 ? 1 : n;
+}
+
+// Host bounds.  Tiles: sum of ceil(rows rep / tp) <= n_row rep / tp + n_seq;
+// items: sum of tiles ceil(ext / chunk) <= tiles + total / chunk and
+// total / chunk <= target / n_kv; slots, over the sequences of several
+// chunks only: ceil(x) < 2 x for x > 1.
+KV_HD int64_t max_tiles(int64_t n_row, int64_t n_seq, int rep, int tp) {
+    const int64_t by_row = n_row * ((rep + tp - 1) / tp);  // no tile for less than a row
+    const int64_t all = n_row * rep / tp + n_seq;
+    return all < by_row ? all : by_row;
+}
+KV_HD int64_t max_items(const Call& c) {
+    return max_tiles(c.n_row, c.n_seq, c.rep, c.tp) + c.target / c.n_kv + 1;
+}
+KV_HD int64_t max_slots(int64_t target, int n_kv) { return 2 * (target / n_kv + 1); }
+
+// The first key that the row at position pos sees (the last one is pos).
+KV_HD int key_lo(const Call& c, int pos) { return c.window && pos - c.window + 1 > 0 ? pos - c.window + 1 : 0; }
+
+// A key's page id where the table holds one, else -1.
+KV_HD int page_ok(int id, int64_t n_pages) { return id >= 0 && (int64_t)id < n_pages ? id : -1; }
+
+// A slot of the cache: page and place; false for one that is not in it.
+KV_HD bool slot_of(int64_t slot, int shift, int64_t n_pages, int64_t* page, int* off) {
+    *page = slot >> shift;
+    *off = (int)(slot & (((int64_t)1 << shift) - 1));
+    return slot >= 0 && *page < n_pages;
+}
+
+}  // namespace kv
+}  // namespace frq

@@ -64,6 +64,25 @@ typedef struct frq_bundle frq_bundle;
 typedef struct frq_gpt2 frq_gpt2;
 typedef struct frq_gemma frq_gemma;
 
+/* A paged key / value cache: pages in the caller's device memory, described
+ * here (plain data, read during a call; nothing keeps the pointer).  A page
+ * holds `page` tokens of every kv head.  dtype FRQ_DT_F32, FRQ_DT_F16 or
+ * FRQ_DT_ROWI8 (int8 with an f32 step per token and head). */
+typedef struct frq_kv {
+    int dtype;
+    size_t n_pages;       /* pages in the pool                                */
+    size_t page;          /* tokens a page: 16, 32, .. 1024                   */
+    size_t n_kv;          /* kv heads                                         */
+    size_t hd;            /* head width: a multiple of 16 up to 256           */
+    void* k;              /* (n_pages, n_kv, page, hd), 16-byte aligned       */
+    void* v;              /* (n_pages, n_kv, hd, page): a channel's tokens
+                             adjacent                                         */
+    float* k_scale;       /* FRQ_DT_ROWI8: (n_pages, n_kv, page), else unused */
+    float* v_scale;
+    size_t page_stride;   /* values between pages in k and in v, 0: dense     */
+    size_t scale_stride;  /* steps between pages, 0: dense                    */
+} frq_kv;
+
 /* Last error message of the calling thread ("" when none). */
 const char* frq_last_error(void);
 /* Library version string. */
@@ -80,7 +99,8 @@ void frq_free(frq_ctx* ctx);
 int frq_set_stream(frq_ctx* ctx, void* hip_stream);
 void* frq_get_stream(frq_ctx* ctx);
 /* Wait for the ctx stream; returns FRQ_ERR_NAN if a _dev call since the last
- * sync saw a NaN activation, else FRQ_OK / FRQ_ERR_HIP. */
+ * sync saw a NaN activation, FRQ_ERR_ARG if one saw an index of the paged
+ * cache out of range, else FRQ_OK / FRQ_ERR_HIP. */
 int frq_sync(frq_ctx* ctx);
 
 /* ---- weight upload (one-time, into persistent HBM) ---------------------- */
@@ -191,6 +211,66 @@ int frq_mm_i8_q_dev(frq_ctx* ctx, const frq_w* w, const int8_t* d_a8,
  * M <= 16 the skinny / GEMV dot. */
 int frq_mm_i8_acc_dev(frq_ctx* ctx, const frq_w* w, const int8_t* d_a8, size_t m,
                       int32_t* d_acc);
+
+/* The row between two int8 linears in one launch: s = x + y (y NULL: x),
+ * written to d_sum (nullable, may be d_x or d_y), then n = s / sqrt(mean(s^2)
+ * + eps) * w as Gemma::norm has it (src/gemma.rs:66-77, its sum taken in 64
+ * bits and n rounded to f32 once, where the engines fold in f32), then
+ * frq_quant_i8_dev's outputs for the rows n, which frq_mm_i8_q_dev takes.
+ * x, y (m,k) row-major f32, w [k]; k up to 28672.  A NaN in n is
+ * FRQ_ERR_NAN at the next frq_sync. */
+int frq_norm_quant_i8_dev(frq_ctx* ctx, const float* d_x, const float* d_y,
+                          const float* d_w, double eps, size_t m, size_t k,
+                          float* d_sum, int8_t* d_a8, float* d_sa,
+                          uint32_t* d_oidx, float* d_oval);
+
+/* ---- the paged cache and its attention -----------------------------------
+ * The cache of a program that runs its sequences' steps on the device-pointer
+ * linears (the engines below keep caches of their own: forward_block and
+ * forward_block_q, src/gemma.rs:242-363).  A token's slot is page id * page +
+ * place in the page.  Indices are device data; those out of range are skipped
+ * and reported by the next frq_sync as FRQ_ERR_ARG.
+ *
+ * frq_kv_write_dev: n tokens' keys and values (row i at d_k + i * pitch, its
+ * n_kv heads of hd adjacent; parts of a fused q|k|v row will do) into their
+ * slots, converted to the cache's dtype: f16 by rounding to nearest (beyond
+ * its range: infinity), int8 by forward_block_q's rule (src/gemma.rs:314-324:
+ * step = max(max|x| / 127, 1e-8), round(x / step) half away from zero, NaN 0).
+ * A negative slot is a row without a place: skipped.  Slots are distinct
+ * (two rows at one slot leave a mixture of both).
+ * frq_kv_read_dev: the way back, in f32 (int8 value times step); rows whose
+ * slot is skipped stay as they were. */
+int frq_kv_write_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_k,
+                     const float* d_v, size_t pitch, const int64_t* d_slot,
+                     size_t n);
+int frq_kv_read_dev(frq_ctx* ctx, const frq_kv* kv, const int64_t* d_slot,
+                    size_t n, float* d_k, float* d_v, size_t pitch);
+/* Attention of n_row query rows of n_seq sequences over their pages: sequence
+ * s holds d_len[s] cached tokens, token j in page d_pages[s * pages_pitch +
+ * j / page], and asks with the rows d_first[s] .. d_first[s + 1] - 1 of d_q
+ * (d_first [n_seq + 1] ascending; NULL: row s is sequence s's, a decode
+ * step).  The rows are the sequence's last tokens, written to the cache
+ * before: row i of r stands at position p = len - r + i and sees the tokens j
+ * <= p, with window > 0 those of p - j < window.  Query head h (n_head of hd
+ * a row, rows q_pitch apart) reads kv head h / (n_head / n_kv):
+ *   z_j = scale q . k_j, cap > 0: cap tanh(z_j / cap);  out = softmax(z) v
+ * (forward_block, src/gemma.rs:252-277) with f32 sums over each run of keys,
+ * the runs joined in a fixed order; a row that sees no token gets zeros.  Rows
+ * outside d_first[0] .. d_first[n_seq] - 1 stay as they were.  What a row
+ * does not see does not touch it, whatever it holds; a row that sees an
+ * infinity or a NaN gets infinities or NaN.
+ * d_ws: frq_kv_attn_ws bytes of device memory, 16-byte aligned, for this call
+ * alone until it is done (calls that may overlap, such as two graphs' replays,
+ * have one each); NULL takes the context's, which a call under graph capture
+ * may not. */
+size_t frq_kv_attn_ws(const frq_kv* kv, size_t n_row, size_t n_head,
+                      size_t n_seq, size_t pages_pitch);
+int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q,
+                    size_t q_pitch, size_t n_row, size_t n_head,
+                    const int32_t* d_pages, size_t pages_pitch,
+                    const int32_t* d_len, const int32_t* d_first, size_t n_seq,
+                    double scale, double cap, size_t window, float* d_out,
+                    size_t out_pitch, void* d_ws, size_t ws_bytes);
 
 /* ---- the unembed: Bundle::rowdot_f32 (src/bundle.rs:958-987) -----------
  * out[r] = dot(W[r], x) for every row of a frq_upload_rows table (out has
