@@ -165,6 +165,14 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const Move m) {
     }
 }
 
+// The decode launch's tiles, then the prompt launch's (grid_b 0: none).
+__global__ __launch_bounds__(256) void kv_join_kernel(const Args a, const Args b, unsigned grid_a) {
+    __shared__ f4 so[256];
+    __shared__ float sm[256], sl[256];
+    if (blockIdx.x < grid_a) join_item<16>(a, blockIdx.x, so, sm, sl);
+    else join_item<128>(b, blockIdx.x - grid_a, so, sm, sl);
+}
+
 struct Guard {
     int prev = -1;
     explicit Guard(int d) {
@@ -244,11 +252,15 @@ hipError_t launch_move(const Move& m, int dtype, hipStream_t s) {
     return hipGetLastError();
 }
 
-constexpr int64_t DEC_TARGET = 1024;  // decode items wanted: four workgroups a CU
+constexpr int64_t DEC_TARGET = 1024;    // decode items wanted: four workgroups a CU
+constexpr int64_t PROMPT_TARGET = 1024;
+constexpr int DEC_PAIRS = 64;           // a sequence of up to so many (row, head) pairs is the decode kernel's
 
-// Slots and floats of the parts of an attention call.
-size_t part_floats(size_t n_kv, size_t hd) {
-    return (size_t)max_slots(DEC_TARGET, (int)n_kv) * n_kv * 16 * (hd + 2);
+// Floats of the parts of an attention call: the decode tiles' and, where a
+// sequence may ask with several rows, the prompt tiles'.
+size_t dec_floats(size_t n_kv, size_t hd) { return (size_t)max_slots(DEC_TARGET, (int)n_kv) * n_kv * 16 * (hd + 2); }
+size_t prompt_floats(size_t n_kv, size_t hd) {
+    return (size_t)max_slots(PROMPT_TARGET, (int)n_kv) * n_kv * 128 * (hd + 2);
 }
 
 }  // namespace
@@ -289,12 +301,10 @@ int frq_kv_read_dev(frq_ctx* ctx, const frq_kv* kv, const int64_t* d_slot, size_
 }
 
 size_t frq_kv_attn_ws(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq, size_t max_pages) {
-    (void)n_row;
     (void)n_head;
-    (void)n_seq;
     (void)max_pages;
     if (!kv || !kv->n_kv || kv->n_kv > 65535 || kv->hd > MAX_HD) return 0;
-    return part_floats(kv->n_kv, kv->hd) * sizeof(float);
+    return (dec_floats(kv->n_kv, kv->hd) + (n_row > n_seq ? prompt_floats(kv->n_kv, kv->hd) : 0)) * sizeof(float);
 }
 
 int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, size_t n_row, size_t n_head,
@@ -340,30 +350,46 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_p
     a.c.rep = (int)(n_head / kv->n_kv);
     a.c.window = (int)window;
     a.c.n_kv = (int)kv->n_kv;
-    a.c.tp = 16;
-    a.c.min_pairs = 1;
-    a.c.max_pairs = 0x7FFFFFFF;
-    a.c.target = DEC_TARGET;
-    a.c.min_chunk = 256;
     a.q = d_q;
     a.q_pitch = (int64_t)q_pitch;
     a.out_pitch = (int64_t)out_pitch;
     a.pages_pitch = (int64_t)pages_pitch;
     a.pages = d_pages;
     a.out = d_out;
+    a.err = ctx_err(ctx);
+    a.scale = scale == 0.0 ? 1.0f : (float)(scale < 0.0 ? -scale : scale);
+    a.sign = scale == 0.0 ? 0.0f : scale < 0.0 ? -1.0f : 1.0f;
+    a.cap = (float)cap;
+    const int64_t TUNE_P = getenv("TUNE_P") ? atoi(getenv("TUNE_P")) : PROMPT_TARGET;
+    // Each sequence is served by the kernel of its number of pairs; one that
+    // no sequence can be for is not launched.
+    const bool prompts = d_first && kv->dtype != FRQ_DT_F32 && n_row * (size_t)a.c.rep > (size_t)DEC_PAIRS;
+    a.c.min_pairs = 1;
+    a.c.max_pairs = prompts ? DEC_PAIRS : 0x7FFFFFFF;
+    a.c.tp = 16;
+    a.c.target = DEC_TARGET;
+    a.c.min_chunk = 256;
     a.part = (float*)d_ws;
     a.slots = max_slots(DEC_TARGET, a.c.n_kv);
-    a.err = ctx_err(ctx);
-    a.scale = (float)scale;
-    a.cap = (float)cap;
-    const int64_t grid = max_items(a.c) * a.c.n_kv;
-    if (grid > 0x7FFFFFFF) return bad("too many rows or sequences");
-    const Launch l{(unsigned)grid, s};
-    hipError_t e = kv->dtype == FRQ_DT_F32   ? launch_decode_f32(a, l)
-                   : kv->dtype == FRQ_DT_F16 ? launch_decode_f16(a, l)
-                                             : launch_decode_i8(a, l);
+    Args b = a;
+    b.c.min_pairs = DEC_PAIRS + 1;
+    b.c.max_pairs = 0x7FFFFFFF;
+    b.c.tp = 128;
+    b.c.target = n_row > n_seq ? TUNE_P : 1;  // no room for parts: every tile's keys in one run
+    b.part = a.part + dec_floats(kv->n_kv, kv->hd);
+    b.slots = n_row > n_seq ? max_slots(PROMPT_TARGET, a.c.n_kv) : 0;
+    const int64_t ga = max_items(a.c) * a.c.n_kv, gb = prompts ? max_items(b.c) * b.c.n_kv : 0;
+    if (ga + gb > 0x7FFFFFFF) return bad("too many rows or sequences");
+    const Launch la{(unsigned)ga, s}, lb{(unsigned)gb, s};
+    hipError_t e = kv->dtype == FRQ_DT_F32   ? launch_decode_f32(a, la)
+                   : kv->dtype == FRQ_DT_F16 ? launch_decode_f16(a, la)
+                                             : launch_decode_i8(a, la);
     if (e != hipSuccess) return hip_bad(e, "launch kv_decode");
-    kv_join_kernel<16><<<dim3(l.grid), dim3(256), 0, s>>>(a);
+    if (prompts) {
+        e = kv->dtype == FRQ_DT_F16 ? launch_prompt_f16(b, lb) : launch_prompt_i8(b, lb);
+        if (e != hipSuccess) return hip_bad(e, "launch kv_prompt");
+    }
+    kv_join_kernel<<<dim3((unsigned)(ga + gb)), dim3(256), 0, s>>>(a, b, (unsigned)ga);
     e = hipGetLastError();
     return e == hipSuccess ? FRQ_OK : hip_bad(e, "launch kv_join");
 }

@@ -20,8 +20,8 @@
 //
 // 32-bit exactness on the f16 matrix cores: the cache's f16 and int8 entries
 // are exact f16; an f32 q row, scaled by a power of two to below 2, is the sum
-// of two f16 (22 bits and more), likewise the probabilities (scaled by 2^14,
-// so that what f16 cannot hold of them is below 2^-38 of the largest); the
+// of two f16 (22 bits and more), likewise the probabilities (scaled by 2^11,
+// so that what f16 cannot hold of them is below 2^-36 of the largest); the
 // products of both halves add up in the f32 accumulators.  An f32 cache uses
 // the f32 matrix cores.
 #pragma once
@@ -62,7 +62,7 @@ struct Args {
     float* part;  // slots of tp (hd + 2) floats a kv head: (m, sum) pairs, then out
     int64_t slots;
     int* err;
-    float scale, cap;
+    float scale, sign, cap;  // |scale| and the sign that q takes (0: scale 1)
 };
 
 // An item's place: its sequence, tile and chunk; every lane has the same.
@@ -93,8 +93,8 @@ __device__ __forceinline__ Item find_item(const Call& c, int64_t id, int* err) {
     if (c.n_seq == 1) {
         it.q = seq_at(c, 0);
         if (it.q.bad && threadIdx.x == 0 && id == 0) atomicOr(err, ERR_INDEX);
-        it.klen = chunk_of(c, keys_of(it.q));
-        it.chunks = chunks_of(it.q, it.klen);
+        it.chunks = chunks_of(it.q, chunk_of(c, keys_of(it.q)));
+        it.klen = even_chunk(it.q, it.chunks);
         it.found = id < (int64_t)it.q.tiles * it.chunks;
         it.tile = (int)(id / it.chunks);
         it.chunk = (int)(id % it.chunks);
@@ -111,12 +111,12 @@ __device__ __forceinline__ Item find_item(const Call& c, int64_t id, int* err) {
     }
 #pragma unroll
     for (int d = 32; d; d >>= 1) total += __shfl_xor((long long)total, d, 64);
-    it.klen = chunk_of(c, total);
+    const int klen = chunk_of(c, total);
     int64_t items = 0, slots = 0;  // of the sequences before
     for (int s0 = 0; s0 < c.n_seq; s0 += 64) {
         Seq q{};
         if (s0 + lane < c.n_seq) q = seq_at(c, s0 + lane);
-        const int n = q.tiles ? chunks_of(q, it.klen) : 1;
+        const int n = q.tiles ? chunks_of(q, klen) : 1;
         const int64_t mine = (int64_t)q.tiles * n;
         int64_t a = mine, b = n > 1 ? mine : 0;  // inclusive sums
 #pragma unroll
@@ -133,6 +133,7 @@ __device__ __forceinline__ Item find_item(const Call& c, int64_t id, int* err) {
             it.seq = s0 + l;
             it.q = seq_at(c, it.seq);
             it.chunks = lane_bcast(n, l);
+            it.klen = even_chunk(it.q, it.chunks);
             const int64_t at = id - items - (lane_bcast(a, l) - lane_bcast(mine, l));
             it.tile = (int)(at / it.chunks);
             it.chunk = (int)(at % it.chunks);
@@ -144,6 +145,23 @@ __device__ __forceinline__ Item find_item(const Call& c, int64_t id, int* err) {
         items += lane_bcast(a, 63);
         slots += lane_bcast(b, 63);
     }
+    return it;
+}
+
+// Every lane has the same item; said so, its fields live in scalar registers.
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ Item uniform_item(const Call& c, int64_t id, int* err) {
+    Item it = find_item(c, id, err);
+    it.q.row0 = uni(it.q.row0);
+    it.q.rows = uni(it.q.rows);
+    it.q.len = uni(it.q.len);
+    it.q.lo = uni(it.q.lo);
+    it.seq = uni(it.seq);
+    it.tile = uni(it.tile);
+    it.chunk = uni(it.chunk);
+    it.chunks = uni(it.chunks);
+    it.klen = uni(it.klen);
+    it.slot = lane_bcast(it.slot, 0);
     return it;
 }
 
@@ -185,17 +203,44 @@ __device__ __forceinline__ h8 i8_to_h8(u2 w) {
     return h8{r[0][0], r[0][1], r[1][0], r[1][1], r[2][0], r[2][1], r[3][0], r[3][1]};
 }
 
-// x = hi + lo, each rounded to nearest: 22 bits and the sign.
+// x = hi + lo, each rounded to nearest: 22 bits and the sign.  In pairs: a
+// packed conversion, x - hi as one mixed FMA (exact), a packed conversion.
+typedef float f2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void split8(const float (&x)[8], h8& hi, h8& lo) {
+    u4 a, b;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        hi[j] = (_Float16)x[j];
-        lo[j] = (_Float16)(x[j] - (float)hi[j]);
+    for (int j = 0; j < 8; j += 2) {
+        a[j / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{x[j], x[j + 1]}), h2));
+        f2 d;
+        float d0, d1;
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d0) : "v"(a[j / 2]), "v"(x[j]));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d1) : "v"(a[j / 2]), "v"(x[j + 1]));
+        d = f2{d0, d1};
+        b[j / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(d, h2));
     }
+    hi = __builtin_bit_cast(h8, a);
+    lo = __builtin_bit_cast(h8, b);
 }
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float P_BIAS = 14.0f;  // probabilities are held times 2^14
+// Probabilities are held times 2^P_BIAS against a maximum that moves only when
+// one would pass 2^(P_BIAS + P_SLACK) = 2^15 (f16 holds up to 2^16): after a
+// sequence's first keys out is hardly ever rescaled, and what f16 cannot hold
+// of a probability stays below 2^(-25 - P_BIAS) of the largest.
+constexpr float P_BIAS = 11.0f, P_SLACK = 4.0f;
+
+// int8: a key's value step goes into its probability, w = p step, and the
+// pair's weights are held over a power of two of their own, so that neither
+// steps of any size nor other rows' keys cost a pair its bits: ev is the
+// exponent field of the pair's largest weight so far, falling with the
+// maximum's rescaling (alpha), and weights and out are held times
+// 2^(W_EXP - ev), the largest weight thus below 2^15.
+constexpr int W_EXP = 127 + 14;
+__device__ __forceinline__ int weight_exp(int ev, float alpha, float wm) {
+    const int ea = (int)(__float_as_uint(alpha) >> 23) - 126;  // alpha < 2^ea; alpha == 1: one too many
+    const int was = alpha == 1.0f ? ev : max(0, ev + ea);
+    return max(was, (int)(__float_as_uint(wm) >> 23));
+}
 
 // What differs by the stored type: DT FRQ_DT_F32, F16 or ROWI8.
 template <int DT>
@@ -209,8 +254,19 @@ struct Type {
 };
 
 template <int DT>
+__device__ __forceinline__ float value_at(const char* p) {
+    if constexpr (DT == FRQ_DT_F32) return *reinterpret_cast<const float*>(p);
+    else return (float)*reinterpret_cast<const _Float16*>(p);
+}
+
+template <int DT>
 __device__ __forceinline__ typename Type<DT>::Raw load_raw(const char* p) {
     return __builtin_nontemporal_load(reinterpret_cast<const typename Type<DT>::Raw*>(p));
+}
+
+// Which of two f16 in a word are not finite, as a mask of their bits.
+__device__ __forceinline__ uint32_t odd_h2(uint32_t w) {
+    return ((w & 0x7C00u) == 0x7C00u ? 0x0000FFFFu : 0u) | ((w & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u);
 }
 
 // The 16 pairs of a lane's column: q times a power of two, as B operands.
@@ -224,7 +280,7 @@ struct QOp {
 
 // q points at the pair's hd values; lane group g takes PL of each step's KS.
 template <int DT, int NS, bool FULL>
-__device__ __forceinline__ void load_q(const float* q, int hd, int g, QOp<DT, NS>& o) {
+__device__ __forceinline__ void load_q(const float* q, float sign, int hd, int g, QOp<DT, NS>& o) {
     using T = Type<DT>;
     float x[NS][T::PL];
 #pragma unroll
@@ -235,7 +291,7 @@ __device__ __forceinline__ void load_q(const float* q, int hd, int g, QOp<DT, NS
         for (int j = 0; j < T::PL; j += 4) {
             const F4 f = *reinterpret_cast<const F4*>(q + (in ? c + j : 0));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[s][j + i] = in ? f.v[i] : 0.0f;
+            for (int i = 0; i < 4; ++i) x[s][j + i] = in ? f.v[i] * sign : 0.0f;
         }
     }
     if constexpr (T::F32) {
@@ -270,10 +326,9 @@ __global__ __launch_bounds__(64 * NW) void kv_decode_kernel(const Args a) {
     constexpr int ORow = 32 * N32 + 4;
     __shared__ float red[NW / 2][16][ORow];
     __shared__ float stat[NW][16][2];
-    __shared__ int stat_e[NW];
     const int n_kv = a.c.n_kv;
     const int kvh = blockIdx.x % n_kv;
-    const Item it = find_item(a.c, blockIdx.x / n_kv, a.err);
+    const Item it = uniform_item(a.c, blockIdx.x / n_kv, a.err);
     if (!it.found) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int col = lane & 15, g = lane >> 4;
@@ -284,16 +339,19 @@ __global__ __launch_bounds__(64 * NW) void kv_decode_kernel(const Args a) {
     const int pr = p0 + min(col, np - 1);
     const int row = pr / a.c.rep, head = kvh * a.c.rep + pr % a.c.rep;
     const int pos = it.q.len - it.q.rows + row;
-    const int pos_a = it.q.len - it.q.rows + p0 / a.c.rep;                 // the tile's first row
-    const int pos_b = it.q.len - it.q.rows + (p0 + np - 1) / a.c.rep;      // and last
+    // the tile's first and last row
+    const int pos_a = uni(it.q.len - it.q.rows + p0 / a.c.rep);
+    const int pos_b = uni(it.q.len - it.q.rows + (p0 + np - 1) / a.c.rep);
     const int see_lo = key_lo(a.c, pos), lo_a = key_lo(a.c, pos_a), lo_b = key_lo(a.c, pos_b);
-    const int beg = max(it.q.lo + it.chunk * it.klen, lo_a / ALIGN * ALIGN);
-    const int end = (int)min((int64_t)it.q.lo + (int64_t)(it.chunk + 1) * it.klen, (int64_t)pos_b + 1);
+    const int beg = uni(max(it.q.lo + it.chunk * it.klen, lo_a / ALIGN * ALIGN));
+    const int end = uni((int)min((int64_t)it.q.lo + (int64_t)(it.chunk + 1) * it.klen, (int64_t)pos_b + 1));
     const int tiles = end > beg ? (end - beg + KT - 1) / KT : 0;
     QOp<DT, NS> q;
-    load_q<DT, NS, FULL>(a.q + (int64_t)(it.q.row0 + row) * a.q_pitch + (int64_t)head * hd, hd, g, q);
-    const float scl = __builtin_ldexpf(a.scale, q.e) * (a.cap > 0.0f ? 1.0f : LOG2E);
-    const float rcap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
+    load_q<DT, NS, FULL>(a.q + (int64_t)(it.q.row0 + row) * a.q_pitch + (int64_t)head * hd, a.sign, hd, g, q);
+    // scores times mul are in the domain of exp2; with a cap they are made so
+    const bool capped = a.cap > 0.0f;
+    const float scl = fmaxf(__builtin_ldexpf(a.scale, q.e), 1.17549435e-38f);
+    const float mul = capped ? 1.0f : scl * LOG2E, rcap = capped ? scl / a.cap : 0.0f;
     const int32_t* table = a.pages + (int64_t)it.seq * a.pages_pitch;
     const int last_page = max(0, it.q.len - 1) >> shift;
     const char* kb = a.kv.k + (int64_t)kvh * page * hd * T::SZ;
@@ -305,17 +363,23 @@ __global__ __launch_bounds__(64 * NW) void kv_decode_kernel(const Args a) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t] = f4{0, 0, 0, 0};
     float m = -__builtin_inff(), l = 0.0f;
-    int ev = 0;  // int8: out is held times 2^(127 - ev)
+    int ev = 0;  // int8: out is held times 2^(W_EXP - ev)
+    uint32_t odd = 0;
+    const bool alike = lo_a == lo_b && pos_a == pos_b;  // every pair sees the same
 
-    // the page of key `base + d` (d < KT) as the lanes need it; a bad id is
-    // reported and reads page 0
-    int pid[2];
-    auto pages_of = [&](int base) {
+    // the page ids of a tile's two halves, loaded a tile ahead of the loads
+    // that use them; a bad one reads page 0 and is told at the end
+    int pid[2], nid[2];
+    bool bad = false;
+    auto ids = [&](int base) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) nid[h] = table[min((base + 16 * h) >> shift, last_page)];
+    };
+    auto pages = [&]() {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int at = min((base + 16 * h) >> shift, last_page);
-            const int id = page_ok(table[at], a.kv.n_pages);
-            if (id < 0 && lane == 0) atomicOr(a.err, ERR_INDEX);
+            const int id = page_ok(nid[h], a.kv.n_pages);
+            bad |= id < 0;
             pid[h] = __builtin_amdgcn_readfirstlane(max(id, 0));
         }
     };
@@ -353,7 +417,9 @@ __global__ __launch_bounds__(64 * NW) void kv_decode_kernel(const Args a) {
         }
     };
     if (wave < tiles) {
-        pages_of(beg + wave * KT);
+        ids(beg + wave * KT);
+        pages();
+        ids(beg + (wave + NW) * KT);
         load_k(beg + wave * KT);
         load_v(beg + wave * KT);
     }
@@ -388,7 +454,7 @@ __global__ __launch_bounds__(64 * NW) void kv_decode_kernel(const Args a) {
         float s[4 * NU];
 #pragma unroll
         for (int j = 0; j < 4 * NU; ++j) {
-            s[j] = sc[j / 4][j % 4] * scl;
+            s[j] = sc[j / 4][j % 4];
             if constexpr (T::I8) s[j] *= ksc[j];
         }
         float vcur[T::I8 ? 8 : 1];
@@ -397,10 +463,11 @@ __global__ __launch_bounds__(64 * NW) void kv_decode_kernel(const Args a) {
             for (int j = 0; j < 8; ++j) vcur[j] = vsc[j];
         }
         if (more) {
-            pages_of(next);
+            pages();
+            ids(next + NW * KT);
             load_k(next);
         }
-        if (a.cap > 0.0f) {
+        if (capped) {
 #pragma unroll
             for (int j = 0; j < 4 * NU; ++j) s[j] = (a.cap * LOG2E) * tanh_f(s[j] * rcap);
         }
@@ -411,154 +478,116 @@ __global__ __launch_bounds__(64 * NW) void kv_decode_kernel(const Args a) {
             for (int j = 0; j < 4 * NU; ++j) {
                 const int key = base + T::PL * g + j;
                 if (key < see_lo || key > pos) s[j] = -__builtin_inff();
-                if constexpr (T::I8)
-                    if (key < lo_a || key > pos_b) vcur[j] = 0.0f;
             }
         }
         // ---- running maximum and sum
         float mx = s[0];
 #pragma unroll
         for (int j = 1; j < 4 * NU; ++j) mx = fmaxf(mx, s[j]);
-        const float mn = fmaxf(m, fmax16(mx));
+        mx = fmax16(mx) * mul;
+        const float mn = mx > m + P_SLACK ? mx : m;
         const float mr = mn == -__builtin_inff() ? 0.0f : mn;
         float alpha = __builtin_amdgcn_exp2f(m - mr);
         bool moved = mn != m;
         m = mn;
+        const float mb = T::I8 ? -mr : P_BIAS - mr;
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < 4 * NU; ++j) {
-            s[j] = __builtin_amdgcn_exp2f(s[j] - mr + P_BIAS);
+            s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], mul, mb));
             sum += s[j];
         }
         l = l * alpha + sum;
         if constexpr (T::I8) {
-            // the values' steps go into the probabilities, over the largest
-            // step's power of two so far
-            float vm = 0.0f;
+            float wm = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) vm = fmaxf(vm, __builtin_fabsf(vcur[j]));
-            const int en = max(ev, (int)(__float_as_uint(fmax16(vm)) >> 23));
-            if (en != ev) {
-                alpha = __builtin_ldexpf(alpha, ev - en);
-                ev = en;
-                moved = true;
+            for (int j = 0; j < 8; ++j) {
+                s[j] = s[j] == 0.0f ? 0.0f : s[j] * vcur[j];
+                wm = fmaxf(wm, __builtin_fabsf(s[j]));
             }
+            const int en = weight_exp(ev, alpha, fmax16(wm));
+            moved |= en != ev;
+            alpha = __builtin_ldexpf(alpha, ev - en);
+            ev = en;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s[j] = s[j] == 0.0f ? 0.0f : s[j] * __builtin_ldexpf(vcur[j], 127 - ev);
+            for (int j = 0; j < 8; ++j) s[j] = __builtin_ldexpf(s[j], W_EXP - ev);
         }
         if (__builtin_amdgcn_ballot_w64(moved)) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) o[t] *= alpha;
         }
-        // ---- values
-        if constexpr (T::F32) {
+        // ---- values.  Keys that no pair sees may hold anything, and a zero
+        // probability would carry what is not finite to pairs that do not see
+        // it: both are zeroed in a tile that not every pair sees whole, the
+        // second noted and given to its pairs after the loop
+        if constexpr (!T::I8) {
             if (edge) {
+                constexpr int PW = T::F32 ? 1 : 2;  // values a word
+                u4 keep;
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int key = base + 4 * g + j;
-                        if (key < lo_a || key > pos_b) vr[t][j] = 0u;
-                    }
-            }
-            auto product = [&]() {
+                for (int j = 0; j < T::PL; ++j) {
+                    const int key = base + T::PL * g + j;
+                    const uint32_t w = key < lo_a || key > pos_b ? 0u : PW == 1 ? ~0u : j & 1 ? 0xFFFF0000u : 0x0000FFFFu;
+                    keep[j / PW] = j % PW ? keep[j / PW] | w : w;
+                }
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     if (!FULL && t * 16 >= hd) continue;
-                    const f4 x = __builtin_bit_cast(f4, vr[t]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], s[j], o[t], 0, 0, 0);
-                }
-            };
-            uint32_t odd = 0;
-            if (edge && lo_a + pos_a != lo_b + pos_b) {  // rows differ in what they see
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (FULL || t * 16 < hd) odd |= (vr[t][j] & 0x7F800000u) == 0x7F800000u;
-            }
-            if (!__builtin_amdgcn_ballot_w64(odd)) {
-                product();
-            } else {
-                // a value that is not finite, and a zero probability would
-                // carry it to rows that do not see it: key by key, each
-                // product kept by the pairs that see the key
-                for (int d = 0; d < KT; ++d) {
-                    const bool sees = base + d >= see_lo && base + d <= pos;
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        if (!FULL && t * 16 >= hd) continue;
-                        f4 y{0, 0, 0, 0};
+                    vr[t] &= keep;
+                    if (!alike) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const bool mine = 4 * g + j == d;
-                            y = __builtin_amdgcn_mfma_f32_16x16x4f32(mine ? __uint_as_float(vr[t][j]) : 0.0f,
-                                                                     mine ? s[j] : 0.0f, y, 0, 0, 0);
+                            const uint32_t x = vr[t][j];
+                            const uint32_t n = PW == 2 ? odd_h2(x) : (x & 0x7F800000u) == 0x7F800000u ? ~0u : 0u;
+                            odd |= n;
+                            vr[t][j] = x & ~n;
                         }
-                        if (sees) o[t] += y;
-                    }
-                }
-            }
-        } else {
-            h8 hi, lo;
-            split8(s, hi, lo);
-            uint32_t odd = 0;
-            if constexpr (!T::I8) {
-                if (edge) {
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const int key = base + 8 * g + j;
-                            if (key < lo_a || key > pos_b) vr[t][j / 2] &= j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-                        }
-                    if (lo_a + pos_a != lo_b + pos_b) {
-#pragma unroll
-                        for (int t = 0; t < NT; ++t)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                if (FULL || t * 16 < hd)
-                                    odd |= (vr[t][j] & 0x7C00u) == 0x7C00u || (vr[t][j] & 0x7C000000u) == 0x7C000000u;
-                    }
-                }
-            }
-            if (!__builtin_amdgcn_ballot_w64(odd)) {
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    if (!FULL && t * 16 >= hd) continue;
-                    h8 x;
-                    if constexpr (T::I8) x = i8_to_h8(vr[t]);
-                    else x = __builtin_bit_cast(h8, vr[t]);
-                    o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, hi, o[t], 0, 0, 0);
-                    o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, lo, o[t], 0, 0, 0);
-                }
-            } else if constexpr (!T::I8) {
-                for (int d = 0; d < KT; ++d) {  // as for f32 above
-                    const bool sees = base + d >= see_lo && base + d <= pos;
-                    h8 ph, pl;
-                    u4 keep;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const bool mine = 8 * g + j == d;
-                        ph[j] = mine ? hi[j] : (_Float16)0.0f;
-                        pl[j] = mine ? lo[j] : (_Float16)0.0f;
-                        if (j & 1) keep[j / 2] |= mine ? 0xFFFF0000u : 0u;
-                        else keep[j / 2] = mine ? 0x0000FFFFu : 0u;
-                    }
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        if (!FULL && t * 16 >= hd) continue;
-                        const h8 x = __builtin_bit_cast(h8, (u4)(vr[t] & keep));
-                        f4 y{0, 0, 0, 0};
-                        y = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ph, y, 0, 0, 0);
-                        y = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, pl, y, 0, 0, 0);
-                        if (sees) o[t] += y;
                     }
                 }
             }
         }
+        if constexpr (T::F32) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                if (!FULL && t * 16 >= hd) continue;
+                const f4 x = __builtin_bit_cast(f4, vr[t]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], s[j], o[t], 0, 0, 0);
+            }
+        } else {
+            h8 hi, lo;
+            split8(s, hi, lo);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                if (!FULL && t * 16 >= hd) continue;
+                h8 x;
+                if constexpr (T::I8) x = i8_to_h8(vr[t]);
+                else x = __builtin_bit_cast(h8, vr[t]);
+                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, hi, o[t], 0, 0, 0);
+                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, lo, o[t], 0, 0, 0);
+            }
+        }
         if (more) load_v(next);
+    }
+    if (bad && lane == 0) atomicOr(a.err, ERR_INDEX);
+    if constexpr (!T::I8) {
+        if (__builtin_amdgcn_ballot_w64(odd != 0)) {  // rare: the keys of those tiles again, one by one
+            for (int key = beg; key < end; ++key) {
+                const int t0 = (key - beg) / KT, base = beg + t0 * KT;
+                if (t0 % NW != wave || (base >= lo_b && base + KT - 1 <= pos_a)) continue;
+                const int64_t pg = max(page_ok(table[key >> shift], a.kv.n_pages), 0);
+                const char* p = vb + pg * a.kv.stride + (int64_t)(key & (page - 1)) * T::SZ;
+                const bool sees = key >= see_lo && key <= pos;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (!FULL && t * 16 >= hd) continue;
+                        const float x = value_at<DT>(p + (int64_t)(16 * t + 4 * g + i) * page * T::SZ);
+                        if (sees && !(x - x == 0.0f)) o[t][i] += x;
+                    }
+            }
+        }
     }
     // ---- the waves' parts: the largest maximum, then sums in a fixed order
     l = fsum16(l);
@@ -566,7 +595,6 @@ __global__ __launch_bounds__(64 * NW) void kv_decode_kernel(const Args a) {
         stat[wave][col][0] = m;
         stat[wave][col][1] = l;
     }
-    if (lane == 0) stat_e[wave] = ev;
     __syncthreads();
     float mm = -__builtin_inff();
 #pragma unroll
@@ -576,7 +604,7 @@ __global__ __launch_bounds__(64 * NW) void kv_decode_kernel(const Args a) {
 #pragma unroll
     for (int w = 0; w < NW; ++w) lsum += stat[w][col][1] * __builtin_amdgcn_exp2f(stat[w][col][0] - mr);
     float f = __builtin_amdgcn_exp2f(m - mr);
-    if constexpr (T::I8) f = __builtin_ldexpf(f, ev - 127);
+    if constexpr (T::I8) f = __builtin_ldexpf(f, ev - W_EXP);
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t] *= f;
 #pragma unroll
@@ -619,17 +647,451 @@ __global__ __launch_bounds__(64 * NW) void kv_decode_kernel(const Args a) {
     }
 }
 
+__device__ __forceinline__ int pick4(int j, int a, int b, int c, int d) {
+    const int lo = j & 1 ? b : a, hi = j & 1 ? d : c;
+    return j & 2 ? hi : lo;
+}
+
+// ---- prompt: 128 pairs a workgroup, keys and values through LDS -------------
+// Four waves of 32 pairs each on the 32 x 32 x 16 products; the workgroup's
+// key tiles (KT keys) are staged in LDS as f16, double-buffered, the next
+// tile's loads in flight under the current one's products.  A lane again owns
+// a pair (lane % 32): key row r of a score tile is the key whose bits 2 and 3
+// are r's swapped, so that the probabilities come out as the B operand of
+// O^T = V^T P^T.
+//
+// LDS rows are cut into 16-byte pieces, piece c of row r at c ^ (r mod a power
+// of two), so that the 32 rows a read takes the same piece of lie in
+// different banks.
+template <int DT, int N32>
+struct Prompt {
+    static constexpr int KT = N32 <= 4 ? 64 : 32;   // keys a tile
+    static constexpr int HP = 32 * N32;             // hd, padded
+    static constexpr int KC = HP / 8, VC = KT / 8;  // pieces of a key row, of a value row
+    static constexpr int KX = KC % 16 == 0 ? 15 : KC % 8 == 0 ? 7 : 3, VX = VC - 1;
+    static constexpr int IPW = KT * KC / 256;       // pieces a thread stages of each
+    static constexpr int BUF = KT * HP;             // f16 of one matrix's tile
+    static constexpr int LDS = 2 * 2 * BUF * 2 + (DT == FRQ_DT_ROWI8 ? 2 * 2 * KT * 4 : 0);
+};
+
+template <int DT, int N32, bool FULL>
+__global__ __launch_bounds__(256, N32 <= 4 ? 2 : 1) void kv_prompt_kernel(const Args a) {
+    using P = Prompt<DT, N32>;
+    constexpr bool I8 = DT == FRQ_DT_ROWI8;
+    constexpr int SZ = I8 ? 1 : 2;
+    constexpr int NS = 2 * N32, NH = N32, NK = P::KT / 32, KT = P::KT, IPW = P::IPW;
+    typedef float f16v __attribute__((ext_vector_type(16)));
+    extern __shared__ __align__(1024) char lds[];
+    __shared__ int flag;  // a value was taken out
+    _Float16* lk = reinterpret_cast<_Float16*>(lds);           // [2][KT][HP]
+    _Float16* lv = lk + 2 * P::BUF;                            // [2][HP][KT]
+    float* lks = reinterpret_cast<float*>(lv + 2 * P::BUF);    // [2][KT] int8 steps
+    float* lvs = lks + 2 * KT;
+    const int n_kv = a.c.n_kv;
+    const int kvh = blockIdx.x % n_kv;
+    const Item it = uniform_item(a.c, blockIdx.x / n_kv, a.err);
+    if (!it.found) return;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int col = lane & 31, h = lane >> 5;
+    const int hd = a.kv.hd, page = a.kv.page, shift = a.c.shift, rep = a.c.rep;
+    const int pairs = it.q.rows * rep, off = it.q.len - it.q.rows;
+    // the workgroup's pairs and keys
+    const int t0 = it.tile * 128, tn = min(128, pairs - t0);
+    const int wpos_a = uni(off + t0 / rep), wpos_b = uni(off + (t0 + tn - 1) / rep);  // its first and last row
+    const int beg = uni(max(it.q.lo + it.chunk * it.klen, key_lo(a.c, wpos_a) / ALIGN * ALIGN));
+    const int end = uni((int)min((int64_t)it.q.lo + (int64_t)(it.chunk + 1) * it.klen, (int64_t)wpos_b + 1));
+    const int tiles = end > beg ? (end - beg + KT - 1) / KT : 0;
+    // the wave's, the lane's; columns past the last pair repeat it
+    const int p0 = t0 + min(32 * wave, tn - 1), np = max(1, min(32, tn - 32 * wave));
+    const bool idle = 32 * wave >= tn;
+    const int pr = p0 + min(col, np - 1);
+    const int row = pr / rep, head = kvh * rep + pr % rep, pos = off + row;
+    const int pos_a = uni(off + p0 / rep), pos_b = uni(off + (p0 + np - 1) / rep);
+    const int see_lo = key_lo(a.c, pos), lo_a = key_lo(a.c, pos_a), lo_b = key_lo(a.c, pos_b);
+
+    // ---- q, times a power of two, as the B operands of the scores
+    h8 qh[NS], ql[NS];
+    int qe;
+    {
+        const float* q = a.q + (int64_t)(it.q.row0 + row) * a.q_pitch + (int64_t)head * hd;
+        float x[NS][8], mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const int c = 16 * s + 8 * h;
+            const bool in = FULL || c < hd;
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {
+                const F4 f = *reinterpret_cast<const F4*>(q + (in ? c + j : 0));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[s][j + i] = in ? f.v[i] * a.sign : 0.0f;
+                    mx = fmaxf(mx, __builtin_fabsf(x[s][j + i]));
+                }
+            }
+        }
+        mx = fmaxf(mx, __uint_as_float(xshfl<32>(__float_as_uint(mx))));
+        const int eb = (int)(__float_as_uint(mx) >> 23);
+        qe = eb == 0 || eb == 255 ? 0 : eb - 127;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[s][j] = __builtin_ldexpf(x[s][j], -qe);
+            split8(x[s], qh[s], ql[s]);
+        }
+    }
+    // scores times mul are in the domain of exp2; with a cap they are made so
+    const bool capped = a.cap > 0.0f;
+    const float scl = fmaxf(__builtin_ldexpf(a.scale, qe), 1.17549435e-38f);
+    const float mul = capped ? 1.0f : scl * LOG2E, rcap = capped ? scl / a.cap : 0.0f;
+
+    // ---- staging: this thread's pieces (the same place in every tile)
+    const int32_t* table = a.pages + (int64_t)it.seq * a.pages_pitch;
+    const int last_page = max(0, it.q.len - 1) >> shift;
+    const char* kb = a.kv.k + (int64_t)kvh * page * hd * SZ;
+    const char* vb = a.kv.v + (int64_t)kvh * page * hd * SZ;
+    // A thread stages pieces (wave IPW + i) 64 + lane of both tiles.  A wave's
+    // pieces of the keys are KT / 4 whole rows, one page's; its pieces of the
+    // values hold the same 8 tokens of different channels.  Page ids are
+    // scalar, loaded a tile ahead of the loads that use them and looked at
+    // only there; a bad one reads page 0 and is told at the end.
+    static_assert(64 / P::VC % P::VC == 0 && IPW * 64 * 4 == KT * P::KC && KT / 4 <= 16, "");
+    constexpr int VR = 64 / P::VC;                        // channels a wave's piece takes
+    const int vr0 = (wave * IPW * 64 + lane) / P::VC;     // channel of piece 0
+    const int vd = 8 * ((lane % P::VC) ^ (vr0 & P::VX));  // its first token
+    bool bad = false;
+    int g0 = 0, g1 = 0, g2 = 0, g3 = 0;  // the ids of the tile's 16-token groups
+    auto ids = [&](int base) {
+        g0 = table[min(base >> shift, last_page)];
+        g1 = table[min((base + 16) >> shift, last_page)];
+        if (KT == 64) {
+            g2 = table[min((base + 32) >> shift, last_page)];
+            g3 = table[min((base + 48) >> shift, last_page)];
+        }
+    };
+    auto page_of = [&](int id) -> int64_t {
+        const int ok = page_ok(id, a.kv.n_pages);
+        bad |= ok < 0;
+        return max(ok, 0);
+    };
+    u2 rk[I8 ? IPW : 1], rv[I8 ? IPW : 1];
+    float rs = 0.0f;
+    auto fetch = [&](int base, int buf) {
+        int ln = lane;
+        asm volatile("" : "+v"(ln));  // addresses are formed anew for every tile, not held over the products
+        const int r0 = wave * (IPW * VR) + ln / P::VC, tok = 8 * ((ln % P::VC) ^ (r0 & P::VX));
+        const char* rows = kb + page_of(pick4(wave * (KT / 4) / 16, g0, g1, g2, g3)) * a.kv.stride +
+                           (int64_t)((base + wave * (KT / 4)) & (page - 1)) * (hd * SZ);
+        const char* toks = vb + page_of(pick4(tok / 16, g0, g1, g2, g3)) * a.kv.stride + ((base + tok) & (page - 1)) * SZ;
+#pragma unroll
+        for (int i = 0; i < IPW; ++i) {
+            const int d = (i * 64 + ln) / P::KC, r = r0 + i * VR;
+            const int c = 8 * (((i * 64 + ln) % P::KC) ^ ((wave * (KT / 4) + d) & P::KX));
+            // past hd q is zero, any piece will do; channels past hd are not kept
+            const char* pk = rows + (d * hd + (FULL || c < hd ? c : 0)) * SZ;
+            const char* pv = toks + (FULL || r < hd ? r : 0) * page * SZ;
+            if constexpr (I8) {
+                rk[i] = *reinterpret_cast<const u2*>(pk);
+                rv[i] = *reinterpret_cast<const u2*>(pv);
+            } else {
+                dma16_lds(pk, lk + buf * P::BUF + (wave * IPW + i) * 512);
+                dma16_lds(pv, lv + buf * P::BUF + (wave * IPW + i) * 512);
+            }
+        }
+        if constexpr (I8) {
+            if (tid < 2 * KT) {  // the steps, a thread a key of each
+                const int d = tid % KT;
+                const int64_t at = page_of(pick4(d / 16, g0, g1, g2, g3)) * a.kv.sstride + kvh * page + ((base + d) & (page - 1));
+                rs = tid < KT ? a.kv.ks[at] : a.kv.vs[at];
+            }
+        }
+    };
+    auto land = [&](int buf) {
+        if constexpr (I8) {
+#pragma unroll
+            for (int i = 0; i < IPW; ++i) {
+                const int p = (wave * IPW + i) * 64 + lane;
+                *reinterpret_cast<h8*>(lk + buf * P::BUF + p * 8) = i8_to_h8(rk[i]);
+                *reinterpret_cast<h8*>(lv + buf * P::BUF + p * 8) = i8_to_h8(rv[i]);
+            }
+            if (tid < KT) lks[buf * KT + tid] = rs;
+            else if (tid < 2 * KT) lvs[buf * KT + tid - KT] = rs;
+        } else {
+            wait_vmcnt<0>();
+        }
+    };
+    // f16: in a tile that not every pair of the workgroup sees whole, values of
+    // keys that none sees (they may be anything) and values that are not
+    // finite (a zero probability would carry them to pairs that do not see
+    // them) are zeroed; the second are noted and given to their pairs after
+    // the loop
+    const int wlo_a = key_lo(a.c, wpos_a), wlo_b = key_lo(a.c, wpos_b);
+    auto clean = [&](int base, int buf) {
+        if (I8 || (base >= wlo_b && base + KT - 1 <= wpos_a)) return;
+        uint32_t odd = 0;
+#pragma unroll 1
+        for (int i = 0; i < IPW; ++i) {
+            u4* at = reinterpret_cast<u4*>(lv + buf * P::BUF + ((wave * IPW + i) * 64 + lane) * 8);
+            u4 v = *at;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int key = base + vd + j;
+                if (key < wlo_a || key > wpos_b) v[j / 2] &= j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t n = odd_h2(v[j]);
+                odd |= n;
+                v[j] &= ~n;
+            }
+            *at = v;
+        }
+        if (odd) flag = 1;
+    };
+
+    f16v o[NH];
+#pragma unroll
+    for (int t = 0; t < NH; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+    float m = -__builtin_inff(), l = 0.0f;
+    int ev = 0;
+    const int krow = (col & 19) | (col & 4) << 1 | (col & 8) >> 1;  // the key of this lane's score row
+    if (tid == 0) flag = 0;
+    __syncthreads();
+    if (tiles) {
+        ids(beg);
+        fetch(beg, 0);
+        land(0);
+        clean(beg, 0);
+        if (tiles > 1) ids(beg + KT);
+    }
+    __syncthreads();
+    for (int ti = 0; ti < tiles; ++ti) {
+        const int base = beg + ti * KT, buf = ti & 1;
+        if (ti + 1 < tiles) {
+            fetch(base + KT, buf ^ 1);
+            if (ti + 2 < tiles) ids(base + 2 * KT);
+        }
+        if (!idle) {
+#pragma unroll 1
+            for (int u = 0; u < NK; ++u) {
+                const int kb0 = base + 32 * u;
+                if (kb0 > pos_b || kb0 + 31 < lo_a) continue;
+                // operands are read a group ahead of their products, the
+                // first of the values ahead of the softmax
+                // piece (2 st + h) ^ (row mod) of the key row, 4 u + 2 k + h
+                // ^ (row mod) of the value row: the parts of the lane as they
+                // are, the step's by one xor-add
+                const char* tk = lds + buf * (2 * P::BUF);
+                const char* tv = lds + (2 + buf) * (2 * P::BUF);
+                const uint32_t ka = (32 * u + krow) * (P::KC * 16), kx = (h ^ (krow & P::KX)) * 16;
+                const uint32_t va = col * (P::VC * 16), vx = ((h ^ (col & P::VX)) ^ (4 * u)) * 16;
+                auto key_op = [&](int st) { return *reinterpret_cast<const h8*>(tk + ((kx ^ (32 * st)) + ka)); };
+                auto val_op = [&](int i) {  // channel rows 32 (i / 2) .., keys 16 (i % 2) + 8 h ..
+                    return *reinterpret_cast<const h8*>(tv + ((vx ^ (32 * (i % 2))) + va) + (i / 2) * (32 * P::VC * 16));
+                };
+                constexpr int G = 4;  // operands a group
+                h8 xa[G], xb[G];
+                f16v s;  // s[8 t + j] is key kb0 + 16 t + 8 h + j
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < G; ++i)
+                    if (FULL || 16 * i < hd) xa[i] = key_op(i);
+#pragma unroll
+                for (int g = 0; g < NS; g += 2 * G) {
+#pragma unroll
+                    for (int i = 0; i < G; ++i)
+                        if (g + G + i < NS && (FULL || 16 * (g + G + i) < hd)) xb[i] = key_op(g + G + i);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int i = 0; i < G; ++i) {
+                        if (!FULL && 16 * (g + i) >= hd) continue;
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[i], qh[g + i], s, 0, 0, 0);
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[i], ql[g + i], s, 0, 0, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int i = 0; i < G; ++i)
+                        if (g + 2 * G + i < NS && (FULL || 16 * (g + 2 * G + i) < hd)) xa[i] = key_op(g + 2 * G + i);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int i = 0; i < G; ++i) {
+                        if (g + G + i >= NS || (!FULL && 16 * (g + G + i) >= hd)) continue;
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(xb[i], qh[(g + G + i) % NS], s, 0, 0, 0);
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(xb[i], ql[(g + G + i) % NS], s, 0, 0, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int i = 0; i < G; ++i)
+                    if (i < 2 * NH && (FULL || 32 * (i / 2) < hd)) xa[i] = val_op(i);
+                const bool edge = kb0 < lo_b || kb0 + 31 > pos_a;
+                if constexpr (I8) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] *= lks[buf * KT + 32 * u + 16 * (i / 8) + 8 * h + i % 8];
+                }
+                if (capped) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] = (a.cap * LOG2E) * tanh_f(s[i] * rcap);
+                }
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int key = kb0 + 16 * (i / 8) + 8 * h + i % 8;
+                        if (key < see_lo || key > pos) s[i] = -__builtin_inff();
+                    }
+                }
+                float mx = s[0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+                mx = fmaxf(mx, __uint_as_float(xshfl<32>(__float_as_uint(mx)))) * mul;
+                const float mn = mx > m + P_SLACK ? mx : m;
+                const float mr = mn == -__builtin_inff() ? 0.0f : mn;
+                float alpha = __builtin_amdgcn_exp2f(m - mr);
+                bool moved = mn != m;
+                m = mn;
+                const float mb = I8 ? -mr : P_BIAS - mr;
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], mul, mb));
+                    sum += s[i];
+                }
+                l = l * alpha + sum;
+                if constexpr (I8) {
+                    float wm = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        s[i] = s[i] == 0.0f ? 0.0f : s[i] * lvs[buf * KT + 32 * u + 16 * (i / 8) + 8 * h + i % 8];
+                        wm = fmaxf(wm, __builtin_fabsf(s[i]));
+                    }
+                    wm = fmaxf(wm, __uint_as_float(xshfl<32>(__float_as_uint(wm))));
+                    const int en = weight_exp(ev, alpha, wm);
+                    moved |= en != ev;
+                    alpha = __builtin_ldexpf(alpha, ev - en);
+                    ev = en;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] = __builtin_ldexpf(s[i], W_EXP - ev);
+                }
+                if (__builtin_amdgcn_ballot_w64(moved)) {
+#pragma unroll
+                    for (int t = 0; t < NH; ++t) o[t] *= alpha;
+                }
+                h8 ph[2], pl[2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    float x[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = s[8 * t + j];
+                    split8(x, ph[t], pl[t]);
+                }
+#pragma unroll
+                for (int g = 0; g < 2 * NH; g += 2 * G) {
+#pragma unroll
+                    for (int i = 0; i < G; ++i)
+                        if (g + G + i < 2 * NH && (FULL || 32 * ((g + G + i) / 2) < hd)) xb[i] = val_op(g + G + i);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int i = 0; i < G; ++i) {
+                        const int t = (g + i) / 2;
+                        if (g + i >= 2 * NH || (!FULL && 32 * t >= hd)) continue;
+                        o[t % NH] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[i], ph[i % 2], o[t % NH], 0, 0, 0);
+                        o[t % NH] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[i], pl[i % 2], o[t % NH], 0, 0, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int i = 0; i < G; ++i)
+                        if (g + 2 * G + i < 2 * NH && (FULL || 32 * ((g + 2 * G + i) / 2) < hd)) xa[i] = val_op(g + 2 * G + i);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int i = 0; i < G; ++i) {
+                        const int t = (g + G + i) / 2;
+                        if (g + G + i >= 2 * NH || (!FULL && 32 * t >= hd)) continue;
+                        o[t % NH] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xb[i], ph[i % 2], o[t % NH], 0, 0, 0);
+                        o[t % NH] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xb[i], pl[i % 2], o[t % NH], 0, 0, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+        if (ti + 1 < tiles) {
+            land(buf ^ 1);
+            clean(base + KT, buf ^ 1);
+        }
+        __syncthreads();
+    }
+    if (bad) atomicOr(a.err, ERR_INDEX);
+    if constexpr (!I8) {
+        if (flag) {  // rare: the keys of those tiles again, one by one (the last barrier was after the last note)
+            for (int key = beg; key < end; ++key) {
+                const int base = beg + (key - beg) / KT * KT;
+                if (base >= wlo_b && base + KT - 1 <= wpos_a) continue;
+                const int64_t pg = max(page_ok(table[key >> shift], a.kv.n_pages), 0);
+                const char* p = vb + pg * a.kv.stride + (int64_t)(key & (page - 1)) * SZ;
+                const bool sees = key >= see_lo && key <= pos;
+#pragma unroll
+                for (int t = 0; t < NH; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int c = 32 * t + 8 * (i / 4) + 4 * h + i % 4;
+                        if (!FULL && c >= hd) continue;
+                        const float x = value_at<DT>(p + (int64_t)c * page * SZ);
+                        if (sees && !(x - x == 0.0f)) o[t][i] += x;
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+            }
+        }
+    }
+    if (idle || col >= np) return;
+    l += __uint_as_float(xshfl<32>(__float_as_uint(l)));
+    if (it.chunks == 1) {
+        const float r = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // no key seen: zeros
+        float* d = a.out + (int64_t)(it.q.row0 + row) * a.out_pitch + (int64_t)head * hd + 4 * h;
+#pragma unroll
+        for (int t = 0; t < NH; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int c = 32 * t + 2 * i;
+                if (!FULL && c >= hd) continue;
+                F4 y;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y.v[j] = (I8 ? __builtin_ldexpf(o[t][i + j], ev - W_EXP) : o[t][i + j]) * r;
+                *reinterpret_cast<F4*>(d + c) = y;
+            }
+    } else {
+        const int64_t slot = it.slot + it.chunk;
+        if (slot >= a.slots) return;  // the host's bound holds them all
+        float* d = a.part + (slot * n_kv + kvh) * (int64_t)(128 * (hd + 2));
+        const int pair = 32 * wave + col;
+        if (h == 0) {
+            d[2 * pair] = m;
+            d[2 * pair + 1] = l;
+        }
+        d += 256 + (int64_t)pair * hd + 4 * h;
+#pragma unroll
+        for (int t = 0; t < NH; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int c = 32 * t + 2 * i;
+                if (!FULL && c >= hd) continue;
+                f4 y;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = I8 ? __builtin_ldexpf(o[t][i + j], ev - W_EXP) : o[t][i + j];
+                *reinterpret_cast<f4*>(d + c) = y;
+            }
+    }
+}
+
 // ---- joining the chunks' parts ----------------------------------------------
 // The workgroup of a tile's chunk i joins the i-th share of the tile's
 // outputs, so that a long sequence's parts are read by many workgroups.
 // Threads are (float4 of the share, run of chunks); each folds its chunks,
 // then the runs are merged pairwise, always in the same order.
 template <int TP>
-__global__ __launch_bounds__(256) void kv_join_kernel(const Args a) {
-    __shared__ f4 so[256];
-    __shared__ float sm[256], sl[256];
-    const int n_kv = a.c.n_kv, kvh = blockIdx.x % n_kv;
-    const Item it = find_item(a.c, blockIdx.x / n_kv, a.err);
+__device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so, float* sm, float* sl) {
+    const int n_kv = a.c.n_kv, kvh = block % n_kv;
+    const Item it = find_item(a.c, block / n_kv, a.err);
     if (!it.found || it.chunks == 1 || it.slot + it.chunks > a.slots) return;
     const int hd = a.kv.hd, tid = threadIdx.x;
     const int p0 = it.tile * TP, np = min(TP, it.q.rows * a.c.rep - p0);
@@ -692,6 +1154,8 @@ struct Launch {
 hipError_t launch_decode_f32(const Args& a, const Launch& l);
 hipError_t launch_decode_f16(const Args& a, const Launch& l);
 hipError_t launch_decode_i8(const Args& a, const Launch& l);
+hipError_t launch_prompt_f16(const Args& a, const Launch& l);
+hipError_t launch_prompt_i8(const Args& a, const Launch& l);
 
 // The kernel of a head width: whole steps of 32 at the widths models have,
 // else the next of three with its last steps masked.
@@ -708,6 +1172,30 @@ hipError_t launch_decode(const Args& a, const Launch& l) {
     else if (hd <= 128) kv_decode_kernel<DT, 4, false, NW><<<g, b, 0, l.s>>>(a);
     else kv_decode_kernel<DT, 8, false, NW><<<g, b, 0, l.s>>>(a);
     return hipGetLastError();
+}
+
+template <int DT, int N32, bool FULL>
+hipError_t run_prompt(const Args& a, const Launch& l) {
+    constexpr int lds = Prompt<DT, N32>::LDS;
+    static_assert(lds <= 160 * 1024, "LDS of a CU");
+    if (lds > 48 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kv_prompt_kernel<DT, N32, FULL>),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+    }
+    kv_prompt_kernel<DT, N32, FULL><<<dim3(l.grid), dim3(256), lds, l.s>>>(a);
+    return hipGetLastError();
+}
+template <int DT>
+hipError_t launch_prompt(const Args& a, const Launch& l) {
+    const int hd = a.kv.hd;
+    if (hd == 64) return run_prompt<DT, 2, true>(a, l);
+    if (hd == 96) return run_prompt<DT, 3, true>(a, l);
+    if (hd == 128) return run_prompt<DT, 4, true>(a, l);
+    if (hd == 256) return run_prompt<DT, 8, true>(a, l);
+    if (hd <= 64) return run_prompt<DT, 2, false>(a, l);
+    if (hd <= 128) return run_prompt<DT, 4, false>(a, l);
+    return run_prompt<DT, 8, false>(a, l);
 }
 
 }  // namespace kv

@@ -81,19 +81,26 @@ KV_HD int chunks_of(const Seq& q, int chunk) {
     const int n = (int)(((int64_t)q.ext + chunk - 1) / chunk);
     return n < 1 ? 1 : n;
 }
+// A sequence's own chunk: its keys in n runs of equal length, whole STEPs.
+constexpr int STEP = 64;
+KV_HD int even_chunk(const Seq& q, int n) {
+    const int64_t per = ((int64_t)q.ext + n - 1) / n, up = (per + STEP - 1) / STEP * STEP;
+    return up > 0x7FFFFFFF ? 0x7FFFFFFF / STEP * STEP : up < STEP ? STEP : (int)up;
+}
 
-// Host bounds.  Tiles: sum of ceil(rows rep / tp) <= n_row rep / tp + n_seq;
+// Host bounds.  Tiles: sum of ceil(rows rep / tp) <= n_row rep / tp + n_seq,
+// and no more than a sequence of max_pairs has for each;
 // items: sum of tiles ceil(ext / chunk) <= tiles + total / chunk and
 // total / chunk <= target / n_kv; slots, over the sequences of several
 // chunks only: ceil(x) < 2 x for x > 1.
-KV_HD int64_t max_tiles(int64_t n_row, int64_t n_seq, int rep, int tp) {
-    const int64_t by_row = n_row * ((rep + tp - 1) / tp);  // no tile for less than a row
-    const int64_t all = n_row * rep / tp + n_seq;
-    return all < by_row ? all : by_row;
+KV_HD int64_t max_tiles(const Call& c) {
+    const int64_t by_row = (int64_t)c.n_row * ((c.rep + c.tp - 1) / c.tp);  // no tile for less than a row
+    const int64_t by_seq = (int64_t)c.n_seq * (((int64_t)c.max_pairs + c.tp - 1) / c.tp);
+    const int64_t all = (int64_t)c.n_row * c.rep / c.tp + c.n_seq;
+    const int64_t least = all < by_row ? all : by_row;
+    return least < by_seq ? least : by_seq;
 }
-KV_HD int64_t max_items(const Call& c) {
-    return max_tiles(c.n_row, c.n_seq, c.rep, c.tp) + c.target / c.n_kv + 1;
-}
+KV_HD int64_t max_items(const Call& c) { return max_tiles(c) + c.target / c.n_kv + 1; }
 KV_HD int64_t max_slots(int64_t target, int n_kv) { return 2 * (target / n_kv + 1); }
 
 // The first key that the row at position pos sees (the last one is pos).

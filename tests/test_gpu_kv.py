@@ -15,11 +15,11 @@ the probabilities and u = 2^-24 the rounding of an f32 step:
            and 16 for the products, the joining and the division; the
            probabilities as two f16: 2^-21.
   small    a weight far below the largest, w, is lost where its type ends: in
-           f32 (2^-126 w, flushed to zero), and as two f16 times 2^14, whose
-           steps end at 2^-24, so half a step is 2^-25 2^-14 = 2^-39 w a key
-           (int8: of the largest value step's power of two, at most the step,
-           times a value of up to 127 steps).  For n keys at most
-           2^-38 w n max|v|; f32 caches 2^-126 w n max|v|.
+           f32 (2^-126 w, flushed to zero), and as two f16 times 2^11, whose
+           steps end at 2^-24, so half a step is 2^-25 2^-11 = 2^-36 w a key
+           (int8: times 2^14, of the largest product of a weight and a value's
+           step, times a value of up to 127 steps).  For n keys at most
+           2^-35 w n max|v|; f32 caches 2^-126 w n max|v|.
 so |error| <= (e^2d - 1 + 2^-21 + u (keys / 16 + 16)) sum p |v| + the small.
 (A key that outweighs the others by 2^200 leaves an output that is the second
 key's alone, where the first one's value is 0: 64 bits hold 1e-63 there.)"""
@@ -253,7 +253,7 @@ class Batch:
                     out[r0 + i, h * rep:(h + 1) * rep] = w @ v
                     tol[r0 + i, h * rep:(h + 1) * rep] = (np.expm1(2 * d) + 2.0 ** -21 + u * ((hi - lo) / 16 + 16)
                                                           )[:, None] * (w @ np.abs(v))
-                    tol[r0 + i, h * rep:(h + 1) * rep] += (2.0 ** (-126 if self.p.kind == "f32" else -38) * w.max(1)
+                    tol[r0 + i, h * rep:(h + 1) * rep] += (2.0 ** (-126 if self.p.kind == "f32" else -35) * w.max(1)
                                                            * (hi - lo))[:, None] * np.abs(v).max()
         return out, tol
 

@@ -116,7 +116,7 @@ extern "C" int64_t plan(const int32_t* len, const int32_t* first, int n_seq, int
         const int m = chunks_of(q, klen);
         for (int t = 0; t < q.tiles; ++t)
             for (int k = 0; k < m; ++k) {
-                if (n < cap) out[n] = Row{s, t, k, m, q.row0, q.rows, q.len, q.lo, q.ext, klen, m > 1 ? slots : -1};
+                if (n < cap) out[n] = Row{s, t, k, m, q.row0, q.rows, q.len, q.lo, q.ext, even_chunk(q, m), m > 1 ? slots : -1};
                 ++n;
                 if (m > 1) ++slots;
             }
@@ -177,7 +177,7 @@ def test_items_cover_every_tile_and_key_once(host):
         rep, n_kv, tp = rng.choice([1, 3, 7, 8, 16, 20, 71]), rng.choice([1, 4, 8, 40]), rng.choice([16, 64, 128])
         window = rng.choice([0, 0, 1, 33, 4096])
         minp, maxp = rng.choice([(1, 0x7FFFFFFF), (1, 64), (65, 0x7FFFFFFF)])
-        target, least = rng.choice([256, 512, 1024]), rng.choice([32, 128, 256])
+        target, least = rng.choice([256, 512, 1024]), rng.choice([64, 128, 256])
         items, bounds, bad = plan(host, lens, first, rep, n_kv, tp, window, 8192, 4, minp, maxp, target, least)
         assert bad == 0
         assert len(items) <= bounds[0]                    # the grid holds them
@@ -195,7 +195,7 @@ def test_items_cover_every_tile_and_key_once(host):
         for (s, t), parts in seen.items():
             lo = min(p.lo for p in parts)
             assert lo % 32 == 0 and lo <= max(0, lens[s] - rows[s] - window + 1 if window else 0)
-            assert parts[0].klen % 32 == 0 and parts[0].klen >= least
+            assert parts[0].klen % 64 == 0 and (parts[0].klen >= least // 2 or len(parts) == 1)
             assert [p.chunk for p in parts] == list(range(parts[0].chunks))
             assert lo + parts[0].chunks * parts[0].klen >= lens[s]
             assert lo + (parts[0].chunks - 1) * parts[0].klen < max(1, lens[s])
