@@ -252,15 +252,45 @@ hipError_t launch_move(const Move& m, int dtype, hipStream_t s) {
     return hipGetLastError();
 }
 
-constexpr int64_t DEC_TARGET = 1024;    // decode items wanted: four workgroups a CU
-constexpr int64_t PROMPT_TARGET = 1024;
+constexpr int64_t DEC_TARGET = 1024;    // decode items wanted: two rounds of the chip's workgroups
+constexpr int64_t PROMPT_TARGET = 400;  // prompt items wanted: a round and not quite two a CU
 constexpr int DEC_PAIRS = 64;           // a sequence of up to so many (row, head) pairs is the decode kernel's
 
-// Floats of the parts of an attention call: the decode tiles' and, where a
-// sequence may ask with several rows, the prompt tiles'.
-size_t dec_floats(size_t n_kv, size_t hd) { return (size_t)max_slots(DEC_TARGET, (int)n_kv) * n_kv * 16 * (hd + 2); }
-size_t prompt_floats(size_t n_kv, size_t hd) {
-    return (size_t)max_slots(PROMPT_TARGET, (int)n_kv) * n_kv * 128 * (hd + 2);
+// The work of an attention call, and its workspace: the items' records, the
+// decode tiles' parts and, where a sequence may ask with several rows, the
+// prompt tiles'.
+struct Plan {
+    Call dec, prompt;
+    size_t rec_dec, rec_prompt, part_dec, part_prompt, bytes;  // offsets, the whole
+};
+Plan plan_of(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq) {
+    Plan p{};
+    Call& c = p.dec;
+    c.n_seq = (int)n_seq;
+    c.n_row = (int)n_row;
+    c.rep = (int)(n_head / kv->n_kv);
+    c.n_kv = (int)kv->n_kv;
+    c.min_chunk = 256;
+    c.min_pairs = 1;
+    c.max_pairs = 0x7FFFFFFF;
+    c.tp = 16;
+    c.target = DEC_TARGET;
+    p.prompt = c;
+    p.prompt.min_pairs = DEC_PAIRS + 1;
+    p.prompt.tp = 128;
+    p.prompt.target = n_row > n_seq ? PROMPT_TARGET : 1;  // no room for parts: every tile's keys in one run
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t r = at;
+        at += round_up(bytes, 256);
+        return r;
+    };
+    p.rec_dec = take((size_t)max_items(p.dec) * sizeof(Record));
+    p.rec_prompt = take((size_t)max_items(p.prompt) * sizeof(Record));
+    p.part_dec = take((size_t)max_slots(DEC_TARGET, c.n_kv) * c.n_kv * 16 * (kv->hd + 2) * 4);
+    p.part_prompt = take(n_row > n_seq ? (size_t)max_slots(PROMPT_TARGET, c.n_kv) * c.n_kv * 128 * (kv->hd + 2) * 4 : 0);
+    p.bytes = at;
+    return p;
 }
 
 }  // namespace
@@ -300,11 +330,12 @@ int frq_kv_read_dev(frq_ctx* ctx, const frq_kv* kv, const int64_t* d_slot, size_
     return e == hipSuccess ? FRQ_OK : hip_bad(e, "launch kv_read");
 }
 
-size_t frq_kv_attn_ws(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq, size_t max_pages) {
-    (void)n_head;
-    (void)max_pages;
-    if (!kv || !kv->n_kv || kv->n_kv > 65535 || kv->hd > MAX_HD) return 0;
-    return (dec_floats(kv->n_kv, kv->hd) + (n_row > n_seq ? prompt_floats(kv->n_kv, kv->hd) : 0)) * sizeof(float);
+size_t frq_kv_attn_ws(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq, size_t pages_pitch) {
+    (void)pages_pitch;
+    if (!kv || !kv->n_kv || kv->n_kv > 65535 || kv->hd > MAX_HD || !n_head || n_head % kv->n_kv ||
+        n_head / kv->n_kv > 65535 || n_row > 0x7FFFFFFF || n_seq > 0x7FFFFFFF)
+        return 0;
+    return plan_of(kv, n_row, n_head, n_seq).bytes;
 }
 
 int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, size_t n_row, size_t n_head,
@@ -328,7 +359,8 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_p
     if (d_ws && ((uintptr_t)d_ws & 15)) return bad("the workspace must be 16-byte aligned");
     if (!ctx) return bad("null context");
     if (!n_row || !n_seq) return FRQ_OK;
-    const size_t need = frq_kv_attn_ws(kv, n_row, n_head, n_seq, pages_pitch);
+    const Plan plan = plan_of(kv, n_row, n_head, n_seq);
+    const size_t need = plan.bytes;
     if (d_ws && ws_bytes < need) return bad("the workspace is below frq_kv_attn_ws");
     Guard g(ctx_device(ctx));
     hipStream_t s = (hipStream_t)frq_get_stream(ctx);
@@ -341,15 +373,12 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_p
         if (st != hipStreamCaptureStatusNone) return bad("under graph capture the caller gives the workspace");
         if (int rc = ctx_ws(ctx, need, &d_ws)) return rc;
     }
+    a.c = plan.dec;
     a.c.len = d_len;
     a.c.first = d_first;
-    a.c.n_seq = (int)n_seq;
-    a.c.n_row = (int)n_row;
     a.c.width = (int)pages_pitch;
     a.c.shift = shift;
-    a.c.rep = (int)(n_head / kv->n_kv);
     a.c.window = (int)window;
-    a.c.n_kv = (int)kv->n_kv;
     a.q = d_q;
     a.q_pitch = (int64_t)q_pitch;
     a.out_pitch = (int64_t)out_pitch;
@@ -360,23 +389,21 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_p
     a.scale = scale == 0.0 ? 1.0f : (float)(scale < 0.0 ? -scale : scale);
     a.sign = scale == 0.0 ? 0.0f : scale < 0.0 ? -1.0f : 1.0f;
     a.cap = (float)cap;
-    const int64_t TUNE_P = getenv("TUNE_P") ? atoi(getenv("TUNE_P")) : PROMPT_TARGET;
     // Each sequence is served by the kernel of its number of pairs; one that
     // no sequence can be for is not launched.
     const bool prompts = d_first && kv->dtype != FRQ_DT_F32 && n_row * (size_t)a.c.rep > (size_t)DEC_PAIRS;
-    a.c.min_pairs = 1;
     a.c.max_pairs = prompts ? DEC_PAIRS : 0x7FFFFFFF;
-    a.c.tp = 16;
-    a.c.target = DEC_TARGET;
-    a.c.min_chunk = 256;
-    a.part = (float*)d_ws;
+    char* ws = (char*)d_ws;
+    a.rec = (Record*)(ws + plan.rec_dec);
+    a.part = (float*)(ws + plan.part_dec);
     a.slots = max_slots(DEC_TARGET, a.c.n_kv);
     Args b = a;
-    b.c.min_pairs = DEC_PAIRS + 1;
-    b.c.max_pairs = 0x7FFFFFFF;
-    b.c.tp = 128;
-    b.c.target = n_row > n_seq ? TUNE_P : 1;  // no room for parts: every tile's keys in one run
-    b.part = a.part + dec_floats(kv->n_kv, kv->hd);
+    b.c.min_pairs = plan.prompt.min_pairs;
+    b.c.max_pairs = plan.prompt.max_pairs;
+    b.c.tp = plan.prompt.tp;
+    b.c.target = plan.prompt.target;
+    b.rec = (Record*)(ws + plan.rec_prompt);
+    b.part = (float*)(ws + plan.part_prompt);
     b.slots = n_row > n_seq ? max_slots(PROMPT_TARGET, a.c.n_kv) : 0;
     const int64_t ga = max_items(a.c) * a.c.n_kv, gb = prompts ? max_items(b.c) * b.c.n_kv : 0;
     if (ga + gb > 0x7FFFFFFF) return bad("too many rows or sequences");

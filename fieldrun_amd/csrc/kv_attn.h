@@ -52,6 +52,10 @@ struct Cache {  // frq_kv as the kernels take it
     int page, hd;
 };
 
+// An item as the joining launch reads it (chunks 1: nothing to join).
+struct Record {
+    int row0, rows, tile, chunk, chunks, slot, pad0, pad1;
+};
 struct Args {
     Call c;
     Cache kv;
@@ -59,6 +63,7 @@ struct Args {
     int64_t q_pitch, out_pitch, pages_pitch;
     const int32_t* pages;
     float* out;
+    Record* rec;  // an item each
     float* part;  // slots of tp (hd + 2) floats a kv head: (m, sum) pairs, then out
     int64_t slots;
     int* err;
@@ -69,10 +74,11 @@ struct Args {
 struct Item {
     Seq q;
     int seq, tile, chunk, chunks, klen;
-    int64_t slot;  // the chunk 0 slot of this tile (chunks > 1)
+    int slot;  // the chunk 0 slot of this tile (chunks > 1)
     bool found;
 };
 
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 template <typename T>
 __device__ __forceinline__ T lane_bcast(T v, int src) {
     if constexpr (sizeof(T) == 8) {
@@ -84,85 +90,95 @@ __device__ __forceinline__ T lane_bcast(T v, int src) {
     }
 }
 
+// Inclusive sums over the lanes (DPP: within rows of 16, then the rows' ends).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int x) {
+    return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int lane_sums(int x) {
+    x = dpp_add<0x111, 0xF>(x);
+    x = dpp_add<0x112, 0xF>(x);
+    x = dpp_add<0x114, 0xF>(x);
+    x = dpp_add<0x118, 0xF>(x);
+    x = dpp_add<0x142, 0xA>(x);
+    return dpp_add<0x143, 0xC>(x);
+}
+
 // Finds item `id`: each wave by itself, 64 sequences at a time, first the
-// call's keys (the chunk length), then the items before.  No memory but the
-// lengths and offsets, no barrier.
-__device__ __forceinline__ Item find_item(const Call& c, int64_t id, int* err) {
+// call's keys (the chunk length), then the items before.  Of each 64 those
+// with chunks longer than half the longest come first, so that the last
+// workgroups to start have the least to do; a sequence's last tiles come
+// first, which see the most.  No memory but the lengths and offsets, no
+// barrier.
+__device__ __forceinline__ Item find_item(const Call& c, int id, int* err) {
     const int lane = threadIdx.x & 63;
     Item it{};
-    if (c.n_seq == 1) {
-        it.q = seq_at(c, 0);
-        if (it.q.bad && threadIdx.x == 0 && id == 0) atomicOr(err, ERR_INDEX);
-        it.chunks = chunks_of(it.q, chunk_of(c, keys_of(it.q)));
-        it.klen = even_chunk(it.q, it.chunks);
-        it.found = id < (int64_t)it.q.tiles * it.chunks;
-        it.tile = (int)(id / it.chunks);
-        it.chunk = (int)(id % it.chunks);
-        it.slot = (int64_t)it.tile * it.chunks;
-        return it;
-    }
     int64_t total = 0;
+    Seq q{};
     for (int s0 = 0; s0 < c.n_seq; s0 += 64) {
+        q = Seq{};
         if (s0 + lane < c.n_seq) {
-            const Seq q = seq_at(c, s0 + lane);
+            q = seq_at(c, s0 + lane);
             total += keys_of(q);
             if (q.bad && id == 0 && threadIdx.x < 64) atomicOr(err, ERR_INDEX);
         }
     }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) total += __shfl_xor((long long)total, d, 64);
+    if (c.n_seq > 1) {
+        total += (int64_t)xshfl64<1>(total);
+        total += (int64_t)xshfl64<2>(total);
+        total += (int64_t)xshfl64<4>(total);
+        total += (int64_t)xshfl64<8>(total);
+        total += (int64_t)xshfl64<16>(total);
+        total += (int64_t)xshfl64<32>(total);
+    }
+    total = lane_bcast(total, 0);
     const int klen = chunk_of(c, total);
-    int64_t items = 0, slots = 0;  // of the sequences before
+    int items = 0, slots = 0;  // of the 64s before
     for (int s0 = 0; s0 < c.n_seq; s0 += 64) {
-        Seq q{};
-        if (s0 + lane < c.n_seq) q = seq_at(c, s0 + lane);
-        const int n = q.tiles ? chunks_of(q, klen) : 1;
-        const int64_t mine = (int64_t)q.tiles * n;
-        int64_t a = mine, b = n > 1 ? mine : 0;  // inclusive sums
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t x = __shfl_up((long long)a, d, 64), y = __shfl_up((long long)b, d, 64);
-            if (lane >= d) {
-                a += x;
-                b += y;
-            }
+        if (c.n_seq > 64) {
+            q = Seq{};
+            if (s0 + lane < c.n_seq) q = seq_at(c, s0 + lane);
         }
-        const uint64_t hit = __builtin_amdgcn_ballot_w64(items + a > id);
+        const int n = q.tiles ? chunks_of(q, klen) : 1, own = even_chunk(q, n), mine = q.tiles * n;
+        int most = own;
+        most = max(most, (int)xshfl<1>(most));
+        most = max(most, (int)xshfl<2>(most));
+        most = max(most, (int)xshfl<4>(most));
+        most = max(most, (int)xshfl<8>(most));
+        most = max(most, (int)xshfl<16>(most));
+        most = max(most, (int)xshfl<32>(most));
+        const bool first = own > most / 2;
+        const int parts = n > 1 ? mine : 0;
+        const int a = lane_sums(first ? mine : 0), b = lane_sums(first ? 0 : mine);
+        const int head = lane_bcast(a, 63);
+        const int at = id - items - (first ? a : head + b) + mine;
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(at >= 0 && at < mine);
+        const int sums = lane_sums(parts);
         if (hit) {
             const int l = __builtin_ctzll(hit);
             it.seq = s0 + l;
-            it.q = seq_at(c, it.seq);
+            it.q.row0 = lane_bcast(q.row0, l);
+            it.q.rows = lane_bcast(q.rows, l);
+            it.q.len = lane_bcast(q.len, l);
+            it.q.lo = lane_bcast(q.lo, l);
             it.chunks = lane_bcast(n, l);
-            it.klen = even_chunk(it.q, it.chunks);
-            const int64_t at = id - items - (lane_bcast(a, l) - lane_bcast(mine, l));
-            it.tile = (int)(at / it.chunks);
-            it.chunk = (int)(at % it.chunks);
-            it.slot = slots + lane_bcast(b, l) - (it.chunks > 1 ? lane_bcast(mine, l) : 0) +
-                      (int64_t)it.tile * it.chunks;
+            it.klen = lane_bcast(own, l);
+            const int i = lane_bcast(at, l), t = uni(i / it.chunks);
+            it.tile = lane_bcast(q.tiles, l) - 1 - t;
+            it.chunk = i - t * it.chunks;
+            it.slot = slots + lane_bcast(sums, l) - lane_bcast(parts, l) + it.tile * it.chunks;
             it.found = true;
             return it;
         }
-        items += lane_bcast(a, 63);
-        slots += lane_bcast(b, 63);
+        items += head + lane_bcast(b, 63);
+        slots += lane_bcast(sums, 63);
     }
     return it;
 }
 
-// Every lane has the same item; said so, its fields live in scalar registers.
-__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ Item uniform_item(const Call& c, int64_t id, int* err) {
-    Item it = find_item(c, id, err);
-    it.q.row0 = uni(it.q.row0);
-    it.q.rows = uni(it.q.rows);
-    it.q.len = uni(it.q.len);
-    it.q.lo = uni(it.q.lo);
-    it.seq = uni(it.seq);
-    it.tile = uni(it.tile);
-    it.chunk = uni(it.chunk);
-    it.chunks = uni(it.chunks);
-    it.klen = uni(it.klen);
-    it.slot = lane_bcast(it.slot, 0);
-    return it;
+__device__ __forceinline__ void note_item(Record* r, int id, const Item& it) {
+    if (threadIdx.x == 0)
+        r[id] = Record{it.q.row0, it.q.rows, it.tile, it.chunk, it.found ? it.chunks : 1, it.slot, 0, 0};
 }
 
 __device__ __forceinline__ float fmax16(float v) {  // over the four lane groups of a pair
@@ -328,7 +344,8 @@ __global__ __launch_bounds__(64 * NW) void kv_decode_kernel(const Args a) {
     __shared__ float stat[NW][16][2];
     const int n_kv = a.c.n_kv;
     const int kvh = blockIdx.x % n_kv;
-    const Item it = uniform_item(a.c, blockIdx.x / n_kv, a.err);
+    const Item it = find_item(a.c, blockIdx.x / n_kv, a.err);
+    if (kvh == 0) note_item(a.rec, blockIdx.x / n_kv, it);
     if (!it.found) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int col = lane & 15, g = lane >> 4;
@@ -502,7 +519,9 @@ __global__ __launch_bounds__(64 * NW) void kv_decode_kernel(const Args a) {
             float wm = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                s[j] = s[j] == 0.0f ? 0.0f : s[j] * vcur[j];
+                const float p = s[j];
+                s[j] = p * vcur[j];
+                if (edge) s[j] = p == 0.0f ? 0.0f : s[j];  // the step of a key that is not seen may be anything
                 wm = fmaxf(wm, __builtin_fabsf(s[j]));
             }
             const int en = weight_exp(ev, alpha, fmax16(wm));
@@ -634,7 +653,7 @@ __global__ __launch_bounds__(64 * NW) void kv_decode_kernel(const Args a) {
         }
     } else {
         const int64_t slot = it.slot + it.chunk;
-        if (slot >= a.slots) return;  // the host's bound holds them all
+        if (slot < 0 || slot >= a.slots) return;  // the host's bound holds them all
         float* d = a.part + (slot * n_kv + kvh) * (int64_t)(16 * (hd + 2));
         if (g == 0) {
             d[2 * col] = mm;
@@ -689,7 +708,8 @@ __global__ __launch_bounds__(256, N32 <= 4 ? 2 : 1) void kv_prompt_kernel(const 
     float* lvs = lks + 2 * KT;
     const int n_kv = a.c.n_kv;
     const int kvh = blockIdx.x % n_kv;
-    const Item it = uniform_item(a.c, blockIdx.x / n_kv, a.err);
+    const Item it = find_item(a.c, blockIdx.x / n_kv, a.err);
+    if (kvh == 0) note_item(a.rec, blockIdx.x / n_kv, it);
     if (!it.found) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int col = lane & 31, h = lane >> 5;
@@ -857,6 +877,9 @@ __global__ __launch_bounds__(256, N32 <= 4 ? 2 : 1) void kv_prompt_kernel(const 
     int ev = 0;
     const int krow = (col & 19) | (col & 4) << 1 | (col & 8) >> 1;  // the key of this lane's score row
     if (tid == 0) flag = 0;
+    // two workgroups share a CU, the second 256 behind the first: one ahead of
+    // the other keeps the one's products over the other's softmax
+    if ((blockIdx.x >> 8) & 1) __builtin_amdgcn_s_setprio(2);
     __syncthreads();
     if (tiles) {
         ids(beg);
@@ -963,7 +986,9 @@ __global__ __launch_bounds__(256, N32 <= 4 ? 2 : 1) void kv_prompt_kernel(const 
                     float wm = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        s[i] = s[i] == 0.0f ? 0.0f : s[i] * lvs[buf * KT + 32 * u + 16 * (i / 8) + 8 * h + i % 8];
+                        const float p = s[i];
+                        s[i] = p * lvs[buf * KT + 32 * u + 16 * (i / 8) + 8 * h + i % 8];
+                        if (edge) s[i] = p == 0.0f ? 0.0f : s[i];  // the step of a key that is not seen may be anything
                         wm = fmaxf(wm, __builtin_fabsf(s[i]));
                     }
                     wm = fmaxf(wm, __uint_as_float(xshfl<32>(__float_as_uint(wm))));
@@ -1061,7 +1086,7 @@ __global__ __launch_bounds__(256, N32 <= 4 ? 2 : 1) void kv_prompt_kernel(const 
             }
     } else {
         const int64_t slot = it.slot + it.chunk;
-        if (slot >= a.slots) return;  // the host's bound holds them all
+        if (slot < 0 || slot >= a.slots) return;  // the host's bound holds them all
         float* d = a.part + (slot * n_kv + kvh) * (int64_t)(128 * (hd + 2));
         const int pair = 32 * wave + col;
         if (h == 0) {
@@ -1091,10 +1116,10 @@ __global__ __launch_bounds__(256, N32 <= 4 ? 2 : 1) void kv_prompt_kernel(const 
 template <int TP>
 __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so, float* sm, float* sl) {
     const int n_kv = a.c.n_kv, kvh = block % n_kv;
-    const Item it = find_item(a.c, block / n_kv, a.err);
-    if (!it.found || it.chunks == 1 || it.slot + it.chunks > a.slots) return;
+    const Record it = a.rec[block / n_kv];
+    if (it.chunks <= 1 || it.slot < 0 || it.slot + it.chunks > a.slots) return;
     const int hd = a.kv.hd, tid = threadIdx.x;
-    const int p0 = it.tile * TP, np = min(TP, it.q.rows * a.c.rep - p0);
+    const int p0 = it.tile * TP, np = min(TP, it.rows * a.c.rep - p0);
     const int n4 = np * (hd / 4), per = (n4 + it.chunks - 1) / it.chunks;
     const int beg = it.chunk * per, end = min(n4, beg + per);
     int pe = 1;
@@ -1141,7 +1166,7 @@ __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so,
             F4 y;
 #pragma unroll
             for (int i = 0; i < 4; ++i) y.v[i] = o[i] * r;
-            *reinterpret_cast<F4*>(a.out + (int64_t)(it.q.row0 + row) * a.out_pitch + (int64_t)head * hd + 4 * c4) = y;
+            *reinterpret_cast<F4*>(a.out + (int64_t)(it.row0 + row) * a.out_pitch + (int64_t)head * hd + 4 * c4) = y;
         }
     }
 }
