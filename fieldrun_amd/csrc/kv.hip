@@ -29,139 +29,238 @@ struct Move {
 
 template <int DT>
 using Elem = std::conditional_t<DT == FRQ_DT_F32, float, std::conditional_t<DT == FRQ_DT_F16, _Float16, int8_t>>;
+template <typename E>
+struct __attribute__((packed, aligned(1))) Quad {  // four elements anywhere (global memory takes any alignment)
+    E v[4];
+};
 
-__device__ __forceinline__ int8_t q8(float x, float step) {
-    const float r = roundf(x / step);
-    return r != r ? (int8_t)0 : (int8_t)fminf(fmaxf(r, -127.0f), 127.0f);
+// round(x / step) of a row's values, |x| <= 127 step: the quotient as a
+// product with RN(1 / step) and one residual correction (Markstein; the
+// IEEE quotient, while 1 / step is a normal number), or the IEEE divide.
+__device__ __forceinline__ int8_t q8(float x, float step, float inv) {
+    float q = x * inv;
+    q = step < 1e37f ? __builtin_fmaf(__builtin_fmaf(-q, step, x), inv, q) : x / step;
+    const float t = __builtin_truncf(q);
+    const float r = __builtin_fabsf(q - t) >= 0.5f ? t + __builtin_copysignf(1.0f, q) : t;
+    return q != q ? (int8_t)0 : (int8_t)(int)__builtin_amdgcn_fmed3f(r, -127.0f, 127.0f);
 }
 
-// The places of the workgroup's rows: page (or -1: no place) and offset.
-__device__ __forceinline__ void places(const Move& m, int64_t r0, int64_t* pg, int* off) {
-    if (threadIdx.x < WR) {
-        int64_t p = -1;
-        int o = 0;
-        if (r0 + threadIdx.x < m.n) {
-            const int64_t s = m.slot[r0 + threadIdx.x];
-            if (!slot_of(s, m.shift, m.kv.n_pages, &p, &o)) {
-                p = -1;
-                if (s >= 0) atomicOr(m.err, ERR_INDEX);  // below zero: a row without a place
-            }
+// The places of the workgroup's rows: page (or -1: no place) and offset; then
+// which fours of rows lie side by side in a page.
+struct Places {
+    int64_t pg[WR];
+    int off[WR];
+    int four[WR / 4];
+};
+__device__ __forceinline__ void find_places(const Move& m, int64_t r0, int64_t slot, Places& p) {
+    const int r = threadIdx.x;
+    if (r < WR) {
+        int64_t pg = -1;
+        int off = 0;
+        if (r0 + r < m.n && !slot_of(slot, m.shift, m.kv.n_pages, &pg, &off)) {
+            pg = -1;
+            if (slot >= 0) atomicOr(m.err, ERR_INDEX);  // below zero: a row without a place
         }
-        pg[threadIdx.x] = p;
-        off[threadIdx.x] = o;
+        p.pg[r] = pg;
+        p.off[r] = off;
+    }
+    __syncthreads();
+    if (r < WR / 4) {
+        bool side = p.pg[4 * r] >= 0;
+        for (int j = 1; j < 4; ++j) side &= p.pg[4 * r + j] == p.pg[4 * r] && p.off[4 * r + j] == p.off[4 * r] + j;
+        p.four[r] = side;
     }
     __syncthreads();
 }
 
-// Workgroup (WR rows, kv head).  A wave takes a row at a time: its keys go
-// straight to the page, its values to LDS and from there token by token
-// along each channel, so that neighbouring slots make whole segments.
-template <int DT>
+// The largest of G lanes' values (G a power of two, the lanes aligned).
+template <int G>
+__device__ __forceinline__ float row_max(float v) {
+    auto step = [&](uint32_t o) { v = fmaxf(v, __uint_as_float(o)); };
+    step(xshfl<1>(__float_as_uint(v)));
+    step(xshfl<2>(__float_as_uint(v)));
+    step(xshfl<4>(__float_as_uint(v)));
+    if constexpr (G > 8) step(xshfl<8>(__float_as_uint(v)));
+    if constexpr (G > 16) step(xshfl<16>(__float_as_uint(v)));
+    if constexpr (G > 32) step(xshfl<32>(__float_as_uint(v)));
+    return v;
+}
+
+// Elements of a channel's LDS row: fours word-aligned, and channels 4 apart (a
+// wave's neighbouring lanes) 4 banks on (33 words, 17, 9).
+template <typename E>
+constexpr int lds_row() { return sizeof(E) == 4 ? 33 : sizeof(E) == 2 ? 34 : 36; }
+template <typename E>
+__device__ __forceinline__ Quad<E> from_lds(const E* p) {
+    uint32_t w[sizeof(E)];
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(E); ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    Quad<E> q;
+    __builtin_memcpy(&q, w, sizeof(q));
+    return q;
+}
+template <typename E>
+__device__ __forceinline__ void to_lds(E* p, const Quad<E>& q) {
+    uint32_t w[sizeof(E)];
+    __builtin_memcpy(w, &q, sizeof(q));
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(E); ++i) reinterpret_cast<uint32_t*>(p)[i] = w[i];
+}
+
+// Workgroup (WR rows, kv head); G lanes a row (a power of two >= hd / 4), four
+// channels a lane, every load issued up front.  Keys go straight to their
+// page; values through LDS, and from there four tokens of a channel at a time
+// where the rows lie side by side (a prompt's do).
+template <int DT, int G>
 __global__ __launch_bounds__(256) void kv_write_kernel(const Move m) {
     using E = Elem<DT>;
-    extern __shared__ char lds_raw[];
-    E* lv = reinterpret_cast<E*>(lds_raw);  // [hd][WR + pad]
-    constexpr int LP = WR + 4 / sizeof(E);
-    __shared__ int64_t pg[WR];
-    __shared__ int off[WR];
+    constexpr bool I8 = DT == FRQ_DT_ROWI8;
+    constexpr int RP = 256 / G < WR ? 256 / G : WR, NP = WR / RP;  // rows a pass, passes
+    constexpr int LP = lds_row<E>();
+    __shared__ __align__(16) E lv[4 * G * LP];
+    __shared__ Places at;
     const int kvh = blockIdx.x % m.n_kv, hd = m.kv.hd, page = m.kv.page;
     const int64_t r0 = (int64_t)(blockIdx.x / m.n_kv) * WR;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    places(m, r0, pg, off);
-    for (int r = wave; r < WR; r += 4) {
-        if (pg[r] < 0) continue;
-        const float* sk = m.wk + (r0 + r) * m.pitch + (int64_t)kvh * hd;
-        const float* sv = m.wv + (r0 + r) * m.pitch + (int64_t)kvh * hd;
-        E* dk = reinterpret_cast<E*>(const_cast<char*>(m.kv.k) + pg[r] * m.kv.stride) + ((int64_t)kvh * page + off[r]) * hd;
-        float x[MAX_HD / 64], y[MAX_HD / 64];
+    const int tid = threadIdx.x, c = 4 * (tid % G), pr = tid / G;
+    const int64_t slot = tid < WR && r0 + tid < m.n ? m.slot[r0 + tid] : -1;
+    const bool act = c < hd && pr < RP;
+    F4 x[NP], y[NP];
 #pragma unroll
-        for (int i = 0; i < MAX_HD / 64; ++i) {
-            const int c = lane + 64 * i;
-            x[i] = c < hd ? sk[c] : 0.0f;
-            y[i] = c < hd ? sv[c] : 0.0f;
+    for (int i = 0; i < NP; ++i) {
+        const int64_t row = r0 + i * RP + pr;
+        if (act && row < m.n) {
+            x[i] = *reinterpret_cast<const F4*>(m.wk + row * m.pitch + (int64_t)kvh * hd + c);
+            y[i] = *reinterpret_cast<const F4*>(m.wv + row * m.pitch + (int64_t)kvh * hd + c);
+        } else {
+            x[i] = y[i] = F4{{0.0f, 0.0f, 0.0f, 0.0f}};
         }
+    }
+    find_places(m, r0, slot, at);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const int r = i * RP + pr;
         float ks = 0.0f, vs = 0.0f;
-        if constexpr (DT == FRQ_DT_ROWI8) {
-            float mk = 0.0f, mv = 0.0f;
+        if constexpr (I8) {
 #pragma unroll
-            for (int i = 0; i < MAX_HD / 64; ++i) {
-                mk = fmaxf(mk, fabsf(x[i]));
-                mv = fmaxf(mv, fabsf(y[i]));
+            for (int j = 0; j < 4; ++j) {
+                ks = fmaxf(ks, fabsf(x[i].v[j]));
+                vs = fmaxf(vs, fabsf(y[i].v[j]));
             }
+            ks = row_max<G>(ks);
+            vs = row_max<G>(vs);
+            ks = fmaxf(ks / 127.0f, 1e-8f);
+            vs = fmaxf(vs / 127.0f, 1e-8f);
+        }
+        if (!act || at.pg[r] < 0) continue;
+        const float ki = 1.0f / ks, vi = 1.0f / vs;  // int8
+        Quad<E> k4;
 #pragma unroll
-            for (int d = 32; d; d >>= 1) {
-                mk = fmaxf(mk, __shfl_xor(mk, d, 64));
-                mv = fmaxf(mv, __shfl_xor(mv, d, 64));
-            }
-            ks = fmaxf(mk / 127.0f, 1e-8f);
-            vs = fmaxf(mv / 127.0f, 1e-8f);
-            if (lane == 0) {
-                const int64_t at = pg[r] * m.kv.sstride + kvh * page + off[r];
-                const_cast<float*>(m.kv.ks)[at] = ks;
-                const_cast<float*>(m.kv.vs)[at] = vs;
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (I8) {
+                k4.v[j] = q8(x[i].v[j], ks, ki);
+                lv[(c + j) * LP + r] = q8(y[i].v[j], vs, vi);
+            } else {
+                k4.v[j] = (E)x[i].v[j];
+                lv[(c + j) * LP + r] = (E)y[i].v[j];
             }
         }
-#pragma unroll
-        for (int i = 0; i < MAX_HD / 64; ++i) {
-            const int c = lane + 64 * i;
-            if (c >= hd) continue;
-            if constexpr (DT == FRQ_DT_ROWI8) {
-                dk[c] = q8(x[i], ks);
-                lv[c * LP + r] = q8(y[i], vs);
-            } else {
-                dk[c] = (E)x[i];
-                lv[c * LP + r] = (E)y[i];
-            }
+        const int64_t pg = at.pg[r];
+        E* dk = reinterpret_cast<E*>(const_cast<char*>(m.kv.k) + pg * m.kv.stride) + ((int64_t)kvh * page + at.off[r]) * hd;
+        *reinterpret_cast<Quad<E>*>(dk + c) = k4;
+        if (I8 && c == 0) {
+            const int64_t s = pg * m.kv.sstride + kvh * page + at.off[r];
+            const_cast<float*>(m.kv.ks)[s] = ks;
+            const_cast<float*>(m.kv.vs)[s] = vs;
         }
     }
     __syncthreads();
-    const int r = threadIdx.x % WR;
-    if (pg[r] < 0) return;
-    E* dv = reinterpret_cast<E*>(const_cast<char*>(m.kv.v) + pg[r] * m.kv.stride) + (int64_t)kvh * hd * page + off[r];
-    for (int c = threadIdx.x / WR; c < hd; c += 256 / WR) dv[(int64_t)c * page] = lv[c * LP + r];
+    const int f = tid % (WR / 4);
+    if (at.four[f]) {
+        E* dv = reinterpret_cast<E*>(const_cast<char*>(m.kv.v) + at.pg[4 * f] * m.kv.stride) + (int64_t)kvh * hd * page +
+                at.off[4 * f];
+        for (int ch = tid / (WR / 4); ch < hd; ch += 256 / (WR / 4))
+            *reinterpret_cast<Quad<E>*>(dv + (int64_t)ch * page) = from_lds(lv + ch * LP + 4 * f);
+    } else {
+        E* dv[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            dv[j] = at.pg[4 * f + j] < 0 ? nullptr
+                                         : reinterpret_cast<E*>(const_cast<char*>(m.kv.v) + at.pg[4 * f + j] * m.kv.stride) +
+                                               (int64_t)kvh * hd * page + at.off[4 * f + j];
+        for (int ch = tid / (WR / 4); ch < hd; ch += 256 / (WR / 4))
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (dv[j]) dv[j][(int64_t)ch * page] = lv[ch * LP + 4 * f + j];
+    }
 }
 
-// The way back: keys by rows, values through LDS.
-template <int DT>
+// The way back: keys by rows, values by fours of tokens into LDS and from
+// there by rows.
+template <int DT, int G>
 __global__ __launch_bounds__(256) void kv_read_kernel(const Move m) {
     using E = Elem<DT>;
-    extern __shared__ char lds_raw[];
-    E* lv = reinterpret_cast<E*>(lds_raw);
-    constexpr int LP = WR + 4 / sizeof(E);
-    __shared__ int64_t pg[WR];
-    __shared__ int off[WR];
+    constexpr bool I8 = DT == FRQ_DT_ROWI8;
+    constexpr int RP = 256 / G < WR ? 256 / G : WR, NP = WR / RP;
+    constexpr int LP = lds_row<E>();
+    __shared__ __align__(16) E lv[4 * G * LP];
+    __shared__ Places at;
     const int kvh = blockIdx.x % m.n_kv, hd = m.kv.hd, page = m.kv.page;
     const int64_t r0 = (int64_t)(blockIdx.x / m.n_kv) * WR;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    places(m, r0, pg, off);
-    {
-        const int r = threadIdx.x % WR;
-        if (pg[r] >= 0) {
-            const E* sv = reinterpret_cast<const E*>(m.kv.v + pg[r] * m.kv.stride) + (int64_t)kvh * hd * page + off[r];
-            for (int c = threadIdx.x / WR; c < hd; c += 256 / WR) lv[c * LP + r] = sv[(int64_t)c * page];
+    const int tid = threadIdx.x, c = 4 * (tid % G), pr = tid / G;
+    find_places(m, r0, tid < WR && r0 + tid < m.n ? m.slot[r0 + tid] : -1, at);
+    const bool act = c < hd && pr < RP;
+    Quad<E> k4[NP];
+    float ks[NP], vs[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const int r = i * RP + pr;
+        ks[i] = vs[i] = 1.0f;
+        if (!act || at.pg[r] < 0) continue;
+        const int64_t pg = at.pg[r];
+        k4[i] = *reinterpret_cast<const Quad<E>*>(reinterpret_cast<const E*>(m.kv.k + pg * m.kv.stride) +
+                                                  ((int64_t)kvh * page + at.off[r]) * hd + c);
+        if constexpr (I8) {
+            const int64_t s = pg * m.kv.sstride + kvh * page + at.off[r];
+            ks[i] = m.kv.ks[s];
+            vs[i] = m.kv.vs[s];
+        }
+    }
+    const int f = tid % (WR / 4);
+    if (at.four[f]) {
+        const E* sv = reinterpret_cast<const E*>(m.kv.v + at.pg[4 * f] * m.kv.stride) + (int64_t)kvh * hd * page + at.off[4 * f];
+#pragma unroll 4
+        for (int ch = tid / (WR / 4); ch < hd; ch += 256 / (WR / 4))
+            to_lds(lv + ch * LP + 4 * f, *reinterpret_cast<const Quad<E>*>(sv + (int64_t)ch * page));
+    } else {
+        // (rows without a place read the first page and are not kept)
+        const E* sv[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            sv[j] = reinterpret_cast<const E*>(m.kv.v + max(at.pg[4 * f + j], (int64_t)0) * m.kv.stride) +
+                    (int64_t)kvh * hd * page + at.off[4 * f + j];
+#pragma unroll 2
+        for (int ch = tid / (WR / 4); ch < hd; ch += 256 / (WR / 4)) {
+            E t[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[j] = sv[j][(int64_t)ch * page];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) lv[ch * LP + 4 * f + j] = t[j];
         }
     }
     __syncthreads();
-    for (int r = wave; r < WR; r += 4) {
-        if (pg[r] < 0) continue;
-        float* dk = m.k + (r0 + r) * m.pitch + (int64_t)kvh * hd;
-        float* dv = m.v + (r0 + r) * m.pitch + (int64_t)kvh * hd;
-        const E* sk = reinterpret_cast<const E*>(m.kv.k + pg[r] * m.kv.stride) + ((int64_t)kvh * page + off[r]) * hd;
-        float ks = 1.0f, vs = 1.0f;
-        if constexpr (DT == FRQ_DT_ROWI8) {
-            const int64_t at = pg[r] * m.kv.sstride + kvh * page + off[r];
-            ks = m.kv.ks[at];
-            vs = m.kv.vs[at];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const int r = i * RP + pr;
+        if (!act || at.pg[r] < 0) continue;
+        F4 x, y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x.v[j] = (float)k4[i].v[j] * ks[i];
+            y.v[j] = (float)lv[(c + j) * LP + r] * vs[i];
         }
-        for (int c = lane; c < hd; c += 64) {
-            float x = (float)sk[c], y = (float)lv[c * LP + r];
-            if constexpr (DT == FRQ_DT_ROWI8) {
-                x *= ks;
-                y *= vs;
-            }
-            dk[c] = x;
-            dv[c] = y;
-        }
+        const int64_t d = (r0 + r) * m.pitch + (int64_t)kvh * hd + c;
+        *reinterpret_cast<F4*>(m.k + d) = x;
+        *reinterpret_cast<F4*>(m.v + d) = y;
     }
 }
 
@@ -238,21 +337,29 @@ int check_rows(const frq_kv* h, const void* k, const void* v, size_t pitch, cons
     return FRQ_OK;
 }
 
+template <bool WRITE, int DT>
+void launch_move_g(const Move& m, const dim3& g, hipStream_t s) {
+    const dim3 b(256);
+    auto go = [&](auto lanes) {
+        constexpr int G = decltype(lanes)::value;
+        if constexpr (WRITE) kv_write_kernel<DT, G><<<g, b, 0, s>>>(m);
+        else kv_read_kernel<DT, G><<<g, b, 0, s>>>(m);
+    };
+    if (m.kv.hd <= 32) go(std::integral_constant<int, 8>{});
+    else if (m.kv.hd <= 64) go(std::integral_constant<int, 16>{});
+    else if (m.kv.hd <= 128) go(std::integral_constant<int, 32>{});
+    else go(std::integral_constant<int, 64>{});
+}
 template <bool WRITE>
 hipError_t launch_move(const Move& m, int dtype, hipStream_t s) {
-    const dim3 g((unsigned)((m.n + WR - 1) / WR * m.n_kv)), b(256);
-    const size_t sz = elem_size(dtype), lds = (size_t)m.kv.hd * (WR * sz + 4);
-#define KV_MOVE(DT)                                              \
-    if (WRITE) kv_write_kernel<DT><<<g, b, lds, s>>>(m);         \
-    else kv_read_kernel<DT><<<g, b, lds, s>>>(m)
-    if (dtype == FRQ_DT_F32) { KV_MOVE(FRQ_DT_F32); }
-    else if (dtype == FRQ_DT_F16) { KV_MOVE(FRQ_DT_F16); }
-    else { KV_MOVE(FRQ_DT_ROWI8); }
-#undef KV_MOVE
+    const dim3 g((unsigned)((m.n + WR - 1) / WR * m.n_kv));
+    if (dtype == FRQ_DT_F32) launch_move_g<WRITE, FRQ_DT_F32>(m, g, s);
+    else if (dtype == FRQ_DT_F16) launch_move_g<WRITE, FRQ_DT_F16>(m, g, s);
+    else launch_move_g<WRITE, FRQ_DT_ROWI8>(m, g, s);
     return hipGetLastError();
 }
 
-constexpr int64_t DEC_TARGET = 1024;    // decode items wanted: two rounds of the chip's workgroups
+constexpr int64_t DEC_TARGET = 512;    // decode items wanted: the chip's workgroups at two a CU
 constexpr int64_t PROMPT_TARGET = 400;  // prompt items wanted: a round and not quite two a CU
 constexpr int DEC_PAIRS = 64;           // a sequence of up to so many (row, head) pairs is the decode kernel's
 

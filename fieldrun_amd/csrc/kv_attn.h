@@ -277,7 +277,7 @@ __device__ __forceinline__ float value_at(const char* p) {
 
 template <int DT>
 __device__ __forceinline__ typename Type<DT>::Raw load_raw(const char* p) {
-    return __builtin_nontemporal_load(reinterpret_cast<const typename Type<DT>::Raw*>(p));
+    return *reinterpret_cast<const typename Type<DT>::Raw*>(p);
 }
 
 // Which of two f16 in a word are not finite, as a mask of their bits.
@@ -335,7 +335,7 @@ __device__ __forceinline__ void load_q(const float* q, float sign, int hd, int g
 // NS steps of hd (hd <= 32 NS; FULL: equal).  NW waves share a chunk's tiles
 // and join in LDS.
 template <int DT, int N32, bool FULL, int NW>
-__global__ __launch_bounds__(64 * NW) void kv_decode_kernel(const Args a) {
+__global__ __launch_bounds__(64 * NW, FULL && N32 <= 4 ? 2 : 1) void kv_decode_kernel(const Args a) {
     using T = Type<DT>;
     constexpr int NS = 32 * N32 / T::KS, NT = 2 * N32;  // steps of hd in the scores, 16-wide tiles of hd in the values
     constexpr int KT = T::KT, NU = KT / 16;
@@ -494,7 +494,10 @@ __global__ __launch_bounds__(64 * NW) void kv_decode_kernel(const Args a) {
 #pragma unroll
             for (int j = 0; j < 4 * NU; ++j) {
                 const int key = base + T::PL * g + j;
-                if (key < see_lo || key > pos) s[j] = -__builtin_inff();
+                if (key < see_lo || key > pos) {
+                    s[j] = -__builtin_inff();
+                    if constexpr (T::I8) vcur[j] = 0.0f;  // its step may be anything
+                }
             }
         }
         // ---- running maximum and sum
@@ -519,9 +522,7 @@ __global__ __launch_bounds__(64 * NW) void kv_decode_kernel(const Args a) {
             float wm = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float p = s[j];
-                s[j] = p * vcur[j];
-                if (edge) s[j] = p == 0.0f ? 0.0f : s[j];  // the step of a key that is not seen may be anything
+                s[j] *= vcur[j];
                 wm = fmaxf(wm, __builtin_fabsf(s[j]));
             }
             const int en = weight_exp(ev, alpha, fmax16(wm));
@@ -986,9 +987,10 @@ __global__ __launch_bounds__(256, N32 <= 4 ? 2 : 1) void kv_prompt_kernel(const 
                     float wm = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float p = s[i];
-                        s[i] = p * lvs[buf * KT + 32 * u + 16 * (i / 8) + 8 * h + i % 8];
-                        if (edge) s[i] = p == 0.0f ? 0.0f : s[i];  // the step of a key that is not seen may be anything
+                        const int d = 16 * (i / 8) + 8 * h + i % 8;
+                        const float step = lvs[buf * KT + 32 * u + d];
+                        // the step of a key that is not seen may be anything
+                        s[i] *= edge && (kb0 + d < see_lo || kb0 + d > pos) ? 0.0f : step;
                         wm = fmaxf(wm, __builtin_fabsf(s[i]));
                     }
                     wm = fmaxf(wm, __uint_as_float(xshfl<32>(__float_as_uint(wm))));
