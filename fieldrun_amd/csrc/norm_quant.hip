@@ -5,14 +5,14 @@
 // The mean and the norm are formed in 64 bits and rounded to f32 once, so the
 // int8 rows do not depend on an order of summation; the quantisation is
 // quant_core.h's (frq_quant_i8_dev's bytes for the rows n).  A row is read
-// once and stays in registers (a copy in LDS serves the selection of rows
-// with many equal magnitudes).
+// once and stays in registers; only the selection of rows with many equal
+// magnitudes puts it into LDS, over the candidates it has done with.
 #include "quant_core.h"
 
 namespace frq {
 namespace {
 
-constexpr int MAX_K = 28672;  // the LDS copy of a row, 112 KB, beside the selection's 30 KB
+constexpr int MAX_K = 28672;  // a row in LDS, 112 KB, beside the selection's 15 KB
 
 struct NormArgs {
     const float *x, *y, *w;
@@ -30,6 +30,8 @@ struct __attribute__((packed, aligned(4))) F4u {
     float x, y, z, w;
 };
 
+__host__ __device__ constexpr int bitmap_quads(int kp) { return ((kp + 31) / 32 + 3) / 4; }
+
 // Four values of a row at 4 i (rows of any alignment; zero past k).
 __device__ __forceinline__ float4 row4(const float* p, int i, int k) {
     if (4 * i + 3 < k) {
@@ -43,12 +45,12 @@ __device__ __forceinline__ float4 row4(const float* p, int i, int k) {
 template <int NV4, int NT>
 __global__ __launch_bounds__(NT) void norm_quant_kernel(const NormArgs a) {
     __shared__ qc::RowLdsT<NT> L;
-    __shared__ unsigned long long cand[qc::FCAP];
     __shared__ double wsum[NT / 64];
-    extern __shared__ float4 lds4[];  // the row n, then the bitmap
+    extern __shared__ float4 lds4[];  // the bitmap, then the candidates or the row n
     const int tid = threadIdx.x, k = a.k, k4 = (k + 3) >> 2;
     const size_t row = blockIdx.x;
-    uint32_t* bitmap = reinterpret_cast<uint32_t*>(lds4 + k4);
+    uint32_t* bitmap = reinterpret_cast<uint32_t*>(lds4);
+    float4* lrow = lds4 + bitmap_quads(a.kp);
     const float* x = a.x + row * k;
     float4 v[NV4], w[NV4];
 #pragma unroll
@@ -109,15 +111,21 @@ __global__ __launch_bounds__(NT) void norm_quant_kernel(const NormArgs a) {
         if (left < 3) v[i].z = 0.0f;
         if (left < 2) v[i].y = 0.0f;
         if (left < 1) v[i].x = 0.0f;
-        if (tid + NT * i < k4) lds4[tid + NT * i] = v[i];
     }
-    __syncthreads();
     int8_t* a8 = a.a8 + row * a.kp;
     uint32_t* a8w = reinterpret_cast<uint32_t*>(a8);
     uint32_t* oi = a.oidx + row * FRQ_T;
     float* ov = a.oval + row * FRQ_T;
-    const float* n = reinterpret_cast<const float*>(lds4);
+    auto put = [&]() {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NV4; ++i)
+            if (tid + NT * i < k4) lrow[tid + NT * i] = v[i];
+        __syncthreads();
+    };
+    const float* n = reinterpret_cast<const float*>(lrow);
     if (k <= FRQ_T) {  // every channel is an outlier
+        put();
         for (int i = tid; i < a.kp / 4; i += NT) a8w[i] = 0u;
         if (tid < FRQ_T) {
             oi[tid] = tid < k ? (uint32_t)tid : 0u;
@@ -127,7 +135,8 @@ __global__ __launch_bounds__(NT) void norm_quant_kernel(const NormArgs a) {
         return;
     }
     // zeros past k are the last to be taken, and k > 32 channels come first
-    const qc::RowSel s = qc::row_select<NV4, NT>(n, 4 * k4, v, L, cand, bitmap, (a.kp + 31) / 32);
+    const qc::RowSel s = qc::row_select<NV4, NT>(n, 4 * k4, v, L, reinterpret_cast<unsigned long long*>(lrow), bitmap,
+                                                   (a.kp + 31) / 32, put);
     if (s.nan) {  // frq_quant_i8_dev's placeholders, reported by frq_sync
         if (tid == 0) atomicOr(a.err, 1);
         for (int i = tid; i < k4; i += NT) a8w[i] = 0u;
@@ -144,7 +153,8 @@ __global__ __launch_bounds__(NT) void norm_quant_kernel(const NormArgs a) {
 
 template <int NV4, int NT>
 hipError_t launch(const NormArgs& a, size_t m, hipStream_t s) {
-    const size_t lds = (size_t)((a.k + 3) / 4) * 16 + (size_t)(a.kp + 31) / 32 * 4;
+    const size_t row = (size_t)((a.k + 3) / 4) * 16, cand = qc::FCAP * sizeof(unsigned long long);
+    const size_t lds = (size_t)bitmap_quads(a.kp) * 16 + (row > cand ? row : cand);
     if (lds > 32 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(norm_quant_kernel<NV4, NT>),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -177,7 +187,10 @@ extern "C" int frq_norm_quant_i8_dev(frq_ctx* ctx, const float* d_x, const float
     hipStream_t s = (hipStream_t)frq_get_stream(ctx);
     const size_t k4 = (k + 3) / 4;
     hipError_t e;
-    if (k4 <= 256) e = launch<1, 256>(a, m, s);
+    // 256 threads a row; few rows of 2049 .. 4096 channels 512 (K = 3584: one row
+    // 7.0 us against 7.7; 4096 rows of 4096 69.6 against 63.5)
+    if (m <= 256 && k4 > 512 && k4 <= 1024) e = launch<2, 512>(a, m, s);
+    else if (k4 <= 256) e = launch<1, 256>(a, m, s);
     else if (k4 <= 512) e = launch<2, 256>(a, m, s);
     else if (k4 <= 1024) e = launch<4, 256>(a, m, s);
     else if (k4 <= 2048) e = launch<8, 256>(a, m, s);

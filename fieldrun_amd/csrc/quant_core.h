@@ -241,9 +241,15 @@ struct RowSel {
 // here.  Ends with a barrier; then sel_i / sel_v hold the 32 outliers in
 // channel order and bitmap marks them, and cand is free.  A NaN row returns
 // nan (uniformly) with sel_i[q] = q, sel_v[q] = 0 and an empty bitmap.
-template <int NV4, int NT = BLOCK>
-__device__ RowSel row_select(const float* __restrict__ a, int K, const float4 (&v)[NV4], RowLdsT<NT>& L,
-                             unsigned long long* cand, uint32_t* bitmap, int nbw) {
+// row(): called by every thread before a is read, and only then (the
+// selection beyond FCAP candidates): a row that is nowhere but in v is put at a
+// there, which may be cand's memory.
+struct RowInPlace {
+    __device__ __forceinline__ void operator()() const {}
+};
+template <int NV4, int NT = BLOCK, typename Row = RowInPlace>
+__device__ RowSel row_select(const float* a, int K, const float4 (&v)[NV4], RowLdsT<NT>& L,
+                             unsigned long long* cand, uint32_t* bitmap, int nbw, Row row = {}) {
     constexpr int NW = NT / 64, BLOCK = NT;
     static_assert(NW == 4 || NW == 8 || NW == 16, "4, 8 or 16 waves");
     constexpr int TOPW = 3;  // lane maxima a wave contributes (16 waves)
@@ -402,7 +408,8 @@ __device__ RowSel row_select(const float* __restrict__ a, int K, const float4 (&
         }
     } else {
         // many near-equal magnitudes (e.g. constant rows): exact select over
-        // the row in global memory, outliers by ordered chunks
+        // the row in memory, outliers by ordered chunks
+        row();
         bulk = radix_select_desc<BLOCK>([&](int i) { return absbits(a[i]); }, K, (uint32_t)FRQ_T,
                                         L.hist, L.bc);
         const int C = (K + BLOCK - 1) / BLOCK;
