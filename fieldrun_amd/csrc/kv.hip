@@ -361,7 +361,7 @@ hipError_t launch_move(const Move& m, int dtype, hipStream_t s) {
 
 constexpr int64_t DEC_TARGET = 512;    // decode items wanted: the chip's workgroups at two a CU
 constexpr int64_t PROMPT_TARGET = 400;  // prompt items wanted: a round and not quite two a CU
-constexpr int DEC_PAIRS = 64;           // a sequence of up to so many (row, head) pairs is the decode kernel's
+constexpr int DEC_PAIRS = 128;          // a sequence of up to so many (row, head) pairs is the decode kernel's
 
 // The work of an attention call, and its workspace: the items' records, the
 // decode tiles' parts and, where a sequence may ask with several rows, the
@@ -498,7 +498,10 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_p
     a.cap = (float)cap;
     // Each sequence is served by the kernel of its number of pairs; one that
     // no sequence can be for is not launched.
-    const bool prompts = d_first && kv->dtype != FRQ_DT_F32 && n_row * (size_t)a.c.rep > (size_t)DEC_PAIRS;
+    // (f32 keys of over 128 channels stay with the decode kernel: three parts of
+    // q do not fit the registers; 8 heads of 256, 2048 rows: 1.6 ms against 1.9.)
+    const bool prompts = d_first && n_row * (size_t)a.c.rep > (size_t)DEC_PAIRS &&
+                         !(kv->dtype == FRQ_DT_F32 && kv->hd > 128);
     a.c.max_pairs = prompts ? DEC_PAIRS : 0x7FFFFFFF;
     char* ws = (char*)d_ws;
     a.rec = (Record*)(ws + plan.rec_dec);
@@ -520,7 +523,9 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_p
                                              : launch_decode_i8(a, la);
     if (e != hipSuccess) return hip_bad(e, "launch kv_decode");
     if (prompts) {
-        e = kv->dtype == FRQ_DT_F16 ? launch_prompt_f16(b, lb) : launch_prompt_i8(b, lb);
+        e = kv->dtype == FRQ_DT_F32   ? launch_prompt_f32(b, lb)
+            : kv->dtype == FRQ_DT_F16 ? launch_prompt_f16(b, lb)
+                                      : launch_prompt_i8(b, lb);
         if (e != hipSuccess) return hip_bad(e, "launch kv_prompt");
     }
     kv_join_kernel<<<dim3((unsigned)(ga + gb)), dim3(256), 0, s>>>(a, b, (unsigned)ga);

@@ -683,29 +683,69 @@ __device__ __forceinline__ int pick4(int j, int a, int b, int c, int d) {
 // LDS rows are cut into 16-byte pieces, piece c of row r at c ^ (r mod a power
 // of two), so that the 32 rows a read takes the same piece of lie in
 // different banks.
+// An f32 cache is staged as three bf16 (exact: 8 bits each), q and the
+// probabilities likewise, and a product is the six of theirs that reach 2^-24
+// of it: six matrix instructions, where the f32 ones would take the time of
+// sixteen.  Its tiles are loaded into registers and have one buffer.
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ void split8(const float (&x)[8], b8 (&y)[3]) {
+    u4 w[3];
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        float r[2] = {x[j], x[j + 1]};
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            w[k][j / 2] = __builtin_amdgcn_perm(__float_as_uint(r[1]), __float_as_uint(r[0]), 0x07060302u);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) r[i] -= __uint_as_float(__float_as_uint(r[i]) & 0xFFFF0000u);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) y[k] = __builtin_bit_cast(b8, w[k]);
+}
+__device__ __forceinline__ void split8(const float (&x)[8], h8 (&y)[2]) { split8(x, y[0], y[1]); }
+typedef float f16v __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ f16v product(const h8 (&x)[1], const h8 (&y)[2], f16v c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[0], y[0], c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(x[0], y[1], c, 0, 0, 0);
+}
+__device__ __forceinline__ f16v product(const b8 (&x)[3], const b8 (&y)[3], f16v c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], y[2], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[2], y[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], y[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], y[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], y[0], c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], y[0], c, 0, 0, 0);
+}
+
 template <int DT, int N32>
 struct Prompt {
-    static constexpr int KT = N32 <= 4 ? 64 : 32;   // keys a tile
+    static constexpr bool F32 = DT == FRQ_DT_F32;
+    using Op = std::conditional_t<F32, b8, h8>;
+    static constexpr int NA = F32 ? 3 : 1, NB = F32 ? 3 : 2;  // parts of a cache operand, of q and p
+    static constexpr int NBUF = F32 ? 1 : 2;                  // buffers
+    static constexpr int WAVES = !F32 && N32 <= 4 ? 2 : 1;    // a SIMD
+    static constexpr int KT = N32 == 3 || (!F32 && N32 <= 4) ? 64 : 32;  // keys a tile
     static constexpr int HP = 32 * N32;             // hd, padded
     static constexpr int KC = HP / 8, VC = KT / 8;  // pieces of a key row, of a value row
     static constexpr int KX = KC % 16 == 0 ? 15 : KC % 8 == 0 ? 7 : 3, VX = VC - 1;
     static constexpr int IPW = KT * KC / 256;       // pieces a thread stages of each
-    static constexpr int BUF = KT * HP;             // f16 of one matrix's tile
-    static constexpr int LDS = 2 * 2 * BUF * 2 + (DT == FRQ_DT_ROWI8 ? 2 * 2 * KT * 4 : 0);
+    static constexpr int BUF = KT * HP;             // elements of one matrix's tile (of one part)
+    static constexpr int LDS = 2 * NBUF * NA * BUF * 2 + (DT == FRQ_DT_ROWI8 ? 2 * 2 * KT * 4 : 0);
 };
 
 template <int DT, int N32, bool FULL>
-__global__ __launch_bounds__(256, N32 <= 4 ? 2 : 1) void kv_prompt_kernel(const Args a) {
+__global__ __launch_bounds__(256, (Prompt<DT, N32>::WAVES)) void kv_prompt_kernel(const Args a) {
     using P = Prompt<DT, N32>;
-    constexpr bool I8 = DT == FRQ_DT_ROWI8;
-    constexpr int SZ = I8 ? 1 : 2;
+    using Op = typename P::Op;
+    constexpr bool I8 = DT == FRQ_DT_ROWI8, F32 = P::F32, F16 = !I8 && !F32;
+    constexpr int SZ = I8 ? 1 : F32 ? 4 : 2, NA = P::NA, NB = P::NB, NBUF = P::NBUF;
     constexpr int NS = 2 * N32, NH = N32, NK = P::KT / 32, KT = P::KT, IPW = P::IPW;
-    typedef float f16v __attribute__((ext_vector_type(16)));
     extern __shared__ __align__(1024) char lds[];
     __shared__ int flag;  // a value was taken out
-    _Float16* lk = reinterpret_cast<_Float16*>(lds);           // [2][KT][HP]
-    _Float16* lv = lk + 2 * P::BUF;                            // [2][HP][KT]
-    float* lks = reinterpret_cast<float*>(lv + 2 * P::BUF);    // [2][KT] int8 steps
+    uint16_t* lk = reinterpret_cast<uint16_t*>(lds);                   // [NBUF][NA][KT][HP]
+    uint16_t* lv = lk + NBUF * NA * P::BUF;                            // [NBUF][NA][HP][KT]
+    float* lks = reinterpret_cast<float*>(lv + NBUF * NA * P::BUF);    // [2][KT] int8 steps
     float* lvs = lks + 2 * KT;
     const int n_kv = a.c.n_kv;
     const int kvh = blockIdx.x % n_kv;
@@ -730,8 +770,8 @@ __global__ __launch_bounds__(256, N32 <= 4 ? 2 : 1) void kv_prompt_kernel(const 
     const int pos_a = uni(off + p0 / rep), pos_b = uni(off + (p0 + np - 1) / rep);
     const int see_lo = key_lo(a.c, pos), lo_a = key_lo(a.c, pos_a), lo_b = key_lo(a.c, pos_b);
 
-    // ---- q, times a power of two, as the B operands of the scores
-    h8 qh[NS], ql[NS];
+    // ---- q, times a power of two (f16), as the B operands of the scores
+    Op qv[NS][NB];
     int qe;
     {
         const float* q = a.q + (int64_t)(it.q.row0 + row) * a.q_pitch + (int64_t)head * hd;
@@ -752,12 +792,12 @@ __global__ __launch_bounds__(256, N32 <= 4 ? 2 : 1) void kv_prompt_kernel(const 
         }
         mx = fmaxf(mx, __uint_as_float(xshfl<32>(__float_as_uint(mx))));
         const int eb = (int)(__float_as_uint(mx) >> 23);
-        qe = eb == 0 || eb == 255 ? 0 : eb - 127;
+        qe = F32 || eb == 0 || eb == 255 ? 0 : eb - 127;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[s][j] = __builtin_ldexpf(x[s][j], -qe);
-            split8(x[s], qh[s], ql[s]);
+            split8(x[s], qv[s]);
         }
     }
     // scores times mul are in the domain of exp2; with a cap they are made so
@@ -794,7 +834,9 @@ __global__ __launch_bounds__(256, N32 <= 4 ? 2 : 1) void kv_prompt_kernel(const 
         bad |= ok < 0;
         return max(ok, 0);
     };
-    u2 rk[I8 ? IPW : 1], rv[I8 ? IPW : 1];
+    using Raw = std::conditional_t<I8, u2, u4>;
+    constexpr int NR = F32 ? 2 : 1;  // loads a piece
+    Raw rk[F16 ? 1 : IPW][NR], rv[F16 ? 1 : IPW][NR];
     float rs = 0.0f;
     auto fetch = [&](int base, int buf) {
         int ln = lane;
@@ -810,9 +852,12 @@ __global__ __launch_bounds__(256, N32 <= 4 ? 2 : 1) void kv_prompt_kernel(const 
             // past hd q is zero, any piece will do; channels past hd are not kept
             const char* pk = rows + (d * hd + (FULL || c < hd ? c : 0)) * SZ;
             const char* pv = toks + (FULL || r < hd ? r : 0) * page * SZ;
-            if constexpr (I8) {
-                rk[i] = *reinterpret_cast<const u2*>(pk);
-                rv[i] = *reinterpret_cast<const u2*>(pv);
+            if constexpr (!F16) {
+#pragma unroll
+                for (int x = 0; x < NR; ++x) {
+                    rk[i][x] = reinterpret_cast<const Raw*>(pk)[x];
+                    rv[i][x] = reinterpret_cast<const Raw*>(pv)[x];
+                }
             } else {
                 dma16_lds(pk, lk + buf * P::BUF + (wave * IPW + i) * 512);
                 dma16_lds(pv, lv + buf * P::BUF + (wave * IPW + i) * 512);
@@ -826,47 +871,73 @@ __global__ __launch_bounds__(256, N32 <= 4 ? 2 : 1) void kv_prompt_kernel(const 
             }
         }
     };
-    auto land = [&](int buf) {
+    // In a tile that not every pair of the workgroup sees whole, values of keys
+    // that none sees (they may be anything) and values that are not finite (a
+    // zero probability would carry them to pairs that do not see them) are
+    // zeroed; the second are noted and given to their pairs after the loop.
+    // (int8 values are finite, and a key that is not seen has weight zero.)
+    const int wlo_a = key_lo(a.c, wpos_a), wlo_b = key_lo(a.c, wpos_b);
+    auto land = [&](int base, int buf) {
+        const bool edge = base < wlo_b || base + KT - 1 > wpos_a;
         if constexpr (I8) {
 #pragma unroll
             for (int i = 0; i < IPW; ++i) {
                 const int p = (wave * IPW + i) * 64 + lane;
-                *reinterpret_cast<h8*>(lk + buf * P::BUF + p * 8) = i8_to_h8(rk[i]);
-                *reinterpret_cast<h8*>(lv + buf * P::BUF + p * 8) = i8_to_h8(rv[i]);
+                *reinterpret_cast<h8*>(lk + buf * P::BUF + p * 8) = i8_to_h8(rk[i][0]);
+                *reinterpret_cast<h8*>(lv + buf * P::BUF + p * 8) = i8_to_h8(rv[i][0]);
             }
             if (tid < KT) lks[buf * KT + tid] = rs;
             else if (tid < 2 * KT) lvs[buf * KT + tid - KT] = rs;
+        } else if constexpr (F32) {
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < IPW; ++i) {
+                const int p = (wave * IPW + i) * 64 + lane;
+                float x[8], y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    x[j] = __uint_as_float(rk[i][j / 4][j % 4]);
+                    y[j] = __uint_as_float(rv[i][j / 4][j % 4]);
+                    if (edge) {
+                        const int key = base + vd + j;
+                        const bool seen = key >= wlo_a && key <= wpos_b, fin = y[j] - y[j] == 0.0f;
+                        odd |= seen && !fin;
+                        y[j] = seen && fin ? y[j] : 0.0f;
+                    }
+                }
+                b8 xs[3], ys[3];
+                split8(x, xs);
+                split8(y, ys);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) {
+                    *reinterpret_cast<b8*>(lk + (buf * NA + k) * P::BUF + p * 8) = xs[k];
+                    *reinterpret_cast<b8*>(lv + (buf * NA + k) * P::BUF + p * 8) = ys[k];
+                }
+            }
+            if (odd) flag = 1;
         } else {
             wait_vmcnt<0>();
-        }
-    };
-    // f16: in a tile that not every pair of the workgroup sees whole, values of
-    // keys that none sees (they may be anything) and values that are not
-    // finite (a zero probability would carry them to pairs that do not see
-    // them) are zeroed; the second are noted and given to their pairs after
-    // the loop
-    const int wlo_a = key_lo(a.c, wpos_a), wlo_b = key_lo(a.c, wpos_b);
-    auto clean = [&](int base, int buf) {
-        if (I8 || (base >= wlo_b && base + KT - 1 <= wpos_a)) return;
-        uint32_t odd = 0;
+            if (!edge) return;
+            uint32_t odd = 0;
 #pragma unroll 1
-        for (int i = 0; i < IPW; ++i) {
-            u4* at = reinterpret_cast<u4*>(lv + buf * P::BUF + ((wave * IPW + i) * 64 + lane) * 8);
-            u4 v = *at;
+            for (int i = 0; i < IPW; ++i) {
+                u4* at = reinterpret_cast<u4*>(lv + buf * P::BUF + ((wave * IPW + i) * 64 + lane) * 8);
+                u4 v = *at;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int key = base + vd + j;
-                if (key < wlo_a || key > wpos_b) v[j / 2] &= j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-            }
+                for (int j = 0; j < 8; ++j) {
+                    const int key = base + vd + j;
+                    if (key < wlo_a || key > wpos_b) v[j / 2] &= j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t n = odd_h2(v[j]);
-                odd |= n;
-                v[j] &= ~n;
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t n = odd_h2(v[j]);
+                    odd |= n;
+                    v[j] &= ~n;
+                }
+                *at = v;
             }
-            *at = v;
+            if (odd) flag = 1;
         }
-        if (odd) flag = 1;
     };
 
     f16v o[NH];
@@ -885,15 +956,14 @@ __global__ __launch_bounds__(256, N32 <= 4 ? 2 : 1) void kv_prompt_kernel(const 
     if (tiles) {
         ids(beg);
         fetch(beg, 0);
-        land(0);
-        clean(beg, 0);
+        land(beg, 0);
         if (tiles > 1) ids(beg + KT);
     }
     __syncthreads();
     for (int ti = 0; ti < tiles; ++ti) {
-        const int base = beg + ti * KT, buf = ti & 1;
+        const int base = beg + ti * KT, buf = NBUF == 1 ? 0 : ti & 1, other = NBUF - 1 - buf;
         if (ti + 1 < tiles) {
-            fetch(base + KT, buf ^ 1);
+            fetch(base + KT, other);
             if (ti + 2 < tiles) ids(base + 2 * KT);
         }
         if (!idle) {
@@ -906,50 +976,55 @@ __global__ __launch_bounds__(256, N32 <= 4 ? 2 : 1) void kv_prompt_kernel(const 
                 // piece (2 st + h) ^ (row mod) of the key row, 4 u + 2 k + h
                 // ^ (row mod) of the value row: the parts of the lane as they
                 // are, the step's by one xor-add
-                const char* tk = lds + buf * (2 * P::BUF);
-                const char* tv = lds + (2 + buf) * (2 * P::BUF);
+                const char* tk = lds + buf * NA * (2 * P::BUF);
+                const char* tv = lds + (NBUF + buf) * NA * (2 * P::BUF);
                 const uint32_t ka = (32 * u + krow) * (P::KC * 16), kx = (h ^ (krow & P::KX)) * 16;
                 const uint32_t va = col * (P::VC * 16), vx = ((h ^ (col & P::VX)) ^ (4 * u)) * 16;
-                auto key_op = [&](int st) { return *reinterpret_cast<const h8*>(tk + ((kx ^ (32 * st)) + ka)); };
-                auto val_op = [&](int i) {  // channel rows 32 (i / 2) .., keys 16 (i % 2) + 8 h ..
-                    return *reinterpret_cast<const h8*>(tv + ((vx ^ (32 * (i % 2))) + va) + (i / 2) * (32 * P::VC * 16));
+                auto key_op = [&](int st, Op(&x)[NA]) {
+#pragma unroll
+                    for (int k = 0; k < NA; ++k)
+                        x[k] = *reinterpret_cast<const Op*>(tk + ((kx ^ (32 * st)) + ka) + k * (2 * P::BUF));
                 };
-                constexpr int G = 4;  // operands a group
-                h8 xa[G], xb[G];
+                auto val_op = [&](int i, Op(&x)[NA]) {  // channel rows 32 (i / 2) .., keys 16 (i % 2) + 8 h ..
+#pragma unroll
+                    for (int k = 0; k < NA; ++k)
+                        x[k] = *reinterpret_cast<const Op*>(tv + ((vx ^ (32 * (i % 2))) + va) + (i / 2) * (32 * P::VC * 16) +
+                                                            k * (2 * P::BUF));
+                };
+                constexpr int G = F32 ? 2 : 4;  // operands a group
+                Op xa[G][NA], xb[G][NA];
                 f16v s;  // s[8 t + j] is key kb0 + 16 t + 8 h + j
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < G; ++i)
-                    if (FULL || 16 * i < hd) xa[i] = key_op(i);
+                    if (FULL || 16 * i < hd) key_op(i, xa[i]);
 #pragma unroll
                 for (int g = 0; g < NS; g += 2 * G) {
 #pragma unroll
                     for (int i = 0; i < G; ++i)
-                        if (g + G + i < NS && (FULL || 16 * (g + G + i) < hd)) xb[i] = key_op(g + G + i);
+                        if (g + G + i < NS && (FULL || 16 * (g + G + i) < hd)) key_op(g + G + i, xb[i]);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int i = 0; i < G; ++i) {
                         if (!FULL && 16 * (g + i) >= hd) continue;
-                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[i], qh[g + i], s, 0, 0, 0);
-                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[i], ql[g + i], s, 0, 0, 0);
+                        s = product(xa[i], qv[g + i], s);
                     }
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int i = 0; i < G; ++i)
-                        if (g + 2 * G + i < NS && (FULL || 16 * (g + 2 * G + i) < hd)) xa[i] = key_op(g + 2 * G + i);
+                        if (g + 2 * G + i < NS && (FULL || 16 * (g + 2 * G + i) < hd)) key_op(g + 2 * G + i, xa[i]);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int i = 0; i < G; ++i) {
                         if (g + G + i >= NS || (!FULL && 16 * (g + G + i) >= hd)) continue;
-                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(xb[i], qh[(g + G + i) % NS], s, 0, 0, 0);
-                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(xb[i], ql[(g + G + i) % NS], s, 0, 0, 0);
+                        s = product(xb[i], qv[(g + G + i) % NS], s);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
 #pragma unroll
                 for (int i = 0; i < G; ++i)
-                    if (i < 2 * NH && (FULL || 32 * (i / 2) < hd)) xa[i] = val_op(i);
+                    if (i < 2 * NH && (FULL || 32 * (i / 2) < hd)) val_op(i, xa[i]);
                 const bool edge = kb0 < lo_b || kb0 + 31 > pos_a;
                 if constexpr (I8) {
 #pragma unroll
@@ -984,13 +1059,17 @@ __global__ __launch_bounds__(256, N32 <= 4 ? 2 : 1) void kv_prompt_kernel(const 
                 }
                 l = l * alpha + sum;
                 if constexpr (I8) {
-                    float wm = 0.0f;
+                    float wm = 0.0f, step[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) step[i] = lvs[buf * KT + 32 * u + 16 * (i / 8) + 8 * h + i % 8];
+                    if (edge) {  // the step of a key that is not seen may be anything
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) step[i] = s[i] == 0.0f ? 0.0f : step[i];
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int d = 16 * (i / 8) + 8 * h + i % 8;
-                        const float step = lvs[buf * KT + 32 * u + d];
-                        // the step of a key that is not seen may be anything
-                        s[i] *= edge && (kb0 + d < see_lo || kb0 + d > pos) ? 0.0f : step;
+                        s[i] *= step[i];
                         wm = fmaxf(wm, __builtin_fabsf(s[i]));
                     }
                     wm = fmaxf(wm, __uint_as_float(xshfl<32>(__float_as_uint(wm))));
@@ -1005,47 +1084,43 @@ __global__ __launch_bounds__(256, N32 <= 4 ? 2 : 1) void kv_prompt_kernel(const 
 #pragma unroll
                     for (int t = 0; t < NH; ++t) o[t] *= alpha;
                 }
-                h8 ph[2], pl[2];
+                Op pv[2][NB];
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     float x[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) x[j] = s[8 * t + j];
-                    split8(x, ph[t], pl[t]);
+                    split8(x, pv[t]);
                 }
 #pragma unroll
                 for (int g = 0; g < 2 * NH; g += 2 * G) {
 #pragma unroll
                     for (int i = 0; i < G; ++i)
-                        if (g + G + i < 2 * NH && (FULL || 32 * ((g + G + i) / 2) < hd)) xb[i] = val_op(g + G + i);
+                        if (g + G + i < 2 * NH && (FULL || 32 * ((g + G + i) / 2) < hd)) val_op(g + G + i, xb[i]);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int i = 0; i < G; ++i) {
                         const int t = (g + i) / 2;
                         if (g + i >= 2 * NH || (!FULL && 32 * t >= hd)) continue;
-                        o[t % NH] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[i], ph[i % 2], o[t % NH], 0, 0, 0);
-                        o[t % NH] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[i], pl[i % 2], o[t % NH], 0, 0, 0);
+                        o[t % NH] = product(xa[i], pv[i % 2], o[t % NH]);
                     }
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int i = 0; i < G; ++i)
-                        if (g + 2 * G + i < 2 * NH && (FULL || 32 * ((g + 2 * G + i) / 2) < hd)) xa[i] = val_op(g + 2 * G + i);
+                        if (g + 2 * G + i < 2 * NH && (FULL || 32 * ((g + 2 * G + i) / 2) < hd)) val_op(g + 2 * G + i, xa[i]);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int i = 0; i < G; ++i) {
                         const int t = (g + G + i) / 2;
                         if (g + G + i >= 2 * NH || (!FULL && 32 * t >= hd)) continue;
-                        o[t % NH] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xb[i], ph[i % 2], o[t % NH], 0, 0, 0);
-                        o[t % NH] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xb[i], pl[i % 2], o[t % NH], 0, 0, 0);
+                        o[t % NH] = product(xb[i], pv[i % 2], o[t % NH]);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
-        if (ti + 1 < tiles) {
-            land(buf ^ 1);
-            clean(base + KT, buf ^ 1);
-        }
+        if (NBUF == 1) __syncthreads();
+        if (ti + 1 < tiles) land(base + KT, other);
         __syncthreads();
     }
     if (bad) atomicOr(a.err, ERR_INDEX);
@@ -1181,6 +1256,7 @@ struct Launch {
 hipError_t launch_decode_f32(const Args& a, const Launch& l);
 hipError_t launch_decode_f16(const Args& a, const Launch& l);
 hipError_t launch_decode_i8(const Args& a, const Launch& l);
+hipError_t launch_prompt_f32(const Args& a, const Launch& l);
 hipError_t launch_prompt_f16(const Args& a, const Launch& l);
 hipError_t launch_prompt_i8(const Args& a, const Launch& l);
 
@@ -1219,10 +1295,13 @@ hipError_t launch_prompt(const Args& a, const Launch& l) {
     if (hd == 64) return run_prompt<DT, 2, true>(a, l);
     if (hd == 96) return run_prompt<DT, 3, true>(a, l);
     if (hd == 128) return run_prompt<DT, 4, true>(a, l);
-    if (hd == 256) return run_prompt<DT, 8, true>(a, l);
     if (hd <= 64) return run_prompt<DT, 2, false>(a, l);
     if (hd <= 128) return run_prompt<DT, 4, false>(a, l);
-    return run_prompt<DT, 8, false>(a, l);
+    if constexpr (DT != FRQ_DT_F32) {
+        if (hd == 256) return run_prompt<DT, 8, true>(a, l);
+        return run_prompt<DT, 8, false>(a, l);
+    }
+    return hipErrorNotSupported;
 }
 
 }  // namespace kv

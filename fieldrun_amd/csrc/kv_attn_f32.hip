@@ -4,5 +4,6 @@
 namespace frq {
 namespace kv {
 hipError_t launch_decode_f32(const Args& a, const Launch& l) { return launch_decode<FRQ_DT_F32>(a, l); }
+hipError_t launch_prompt_f32(const Args& a, const Launch& l) { return launch_prompt<FRQ_DT_F32>(a, l); }
 }  // namespace kv
 }  // namespace frq
