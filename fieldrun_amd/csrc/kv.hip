@@ -459,9 +459,12 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_p
     const size_t width = n_head * kv->hd;
     if (q_pitch < width || out_pitch < width || q_pitch > ((size_t)1 << 40) || out_pitch > ((size_t)1 << 40))
         return bad("pitch is below the heads' width");
-    if (pages_pitch > 0x7FFFFFFF || (pages_pitch << shift) > 0x7FFFFFFF) return bad("a table holds up to 2^31 - 1 tokens");
+    // (keys past a sequence's last are counted to the end of a tile: room below 2^31)
+    if (pages_pitch > 0x7FFFFFFF || (pages_pitch << shift) > 0x7FFFFFFF - 1024)
+        return bad("a table holds up to 2^31 - 1024 tokens");
     if (window > 0x7FFFFFFF) window = 0;  // wider than any sequence
-    if (!(scale - scale == 0.0) || !(cap >= 0.0) || cap > 1e30) return bad("scale must be finite, cap 0 or positive");
+    if (!(scale >= -1e30 && scale <= 1e30) || !(cap >= 0.0 && cap <= 1e30))
+        return bad("scale must be within 1e30, cap 0 or positive");
     if (n_row && n_seq && (!d_q || !d_out || !d_len || (!d_pages && pages_pitch))) return bad("null pointer");
     if (d_ws && ((uintptr_t)d_ws & 15)) return bad("the workspace must be 16-byte aligned");
     if (!ctx) return bad("null context");

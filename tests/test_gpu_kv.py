@@ -309,6 +309,23 @@ def test_long_and_many(ctx, kind):
     Batch(ctx, kind, 16, 1, 2, 32, lens, rows, seed=3).check()
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "rowi8"])
+def test_rows_no_more_than_sequences(ctx, kind):
+    """One sequence asks with many rows, the others with none: no room for
+    parts is held then, and the long tiles run whole."""
+    n = 300
+    rows, lens = [0] * n, [0] * n
+    rows[131], lens[131] = 150, 900
+    rows[7], lens[7] = 3, 40
+    lens[250] = 77  # cached, not asking
+    Batch(ctx, kind, 16, 1, 2, 64, lens, rows, seed=4).check()
+
+
+def test_thousand_sequences(ctx):
+    rng = np.random.default_rng(6)
+    Batch(ctx, "f16", 16, 1, 1, 32, [int(x) for x in rng.integers(0, 40, 1000)], seed=5).check()
+
+
 def test_large_and_small_scores(ctx):
     """Rows of q over the whole range of f32 (scores that saturate one key, or
     none), equal scores, and a zero row."""

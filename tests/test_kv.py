@@ -60,7 +60,7 @@ def attn(d=None, q=A, qp=256, n_row=3, n_head=4, pages=A, width=5, lens=A, first
     (dict(n_head=3), "n_head"), (dict(n_head=0), "n_head"), (dict(n_row=4), "one row"), (dict(qp=255), "pitch"),
     (dict(op=100), "pitch"), (dict(n_row=1 << 31, n_seq=1 << 31), "too many"), (dict(width=1 << 28), "2^31"),
     (dict(n_row=1 << 30, n_seq=1 << 30, n_head=8, qp=512, op=512), "too many"),
-    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(cap=-1.0), "cap"),
+    (dict(width=(1 << 27) - 63), "2^31"), (dict(scale=1e300), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(cap=-1.0), "cap"),
     (dict(cap=float("nan")), "cap"), (dict(q=None), "null"), (dict(out=None), "null"), (dict(lens=None), "null"),
     (dict(pages=None), "null"), (dict(ws=A + 4), "16-byte"), ({}, "null context"),
 ])
