@@ -272,6 +272,61 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const Args a, const Args b
     else join_item<128>(b, blockIdx.x - grid_a, so, sm, sl);
 }
 
+// The plans of many sequences (workgroup 0: the decode launch's, 1: the
+// prompt's): the call's keys, then the items and slots before each 64
+// sequences.  16 waves, 64 sequences each at a time, bound by the latency of
+// two passes over the lengths.
+__global__ __launch_bounds__(1024) void kv_plan_kernel(const Call ca, const Call cb, int32_t* plan_a, int32_t* plan_b,
+                                                       int* err) {
+    __shared__ int64_t keys[16];
+    const bool dec = blockIdx.x == 0;
+    const Call c = dec ? ca : cb;
+    int32_t* plan = dec ? plan_a : plan_b;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, blocks = (c.n_seq + 63) / 64;
+    int64_t total = 0;
+    for (int64_t s = threadIdx.x; s < c.n_seq; s += 1024) {
+        const Seq q = seq_at(c, (int)s);
+        total += keys_of(q);
+        if (q.bad && dec) atomicOr(err, ERR_INDEX);
+    }
+    total = wave_total(total);
+    if (lane == 0) keys[w] = total;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) total += keys[i];
+    const int klen = chunk_of(c, total);
+    for (int b = w; b < blocks; b += 16) {
+        Seq q{};
+        if (b * 64 + lane < c.n_seq) q = seq_at(c, b * 64 + lane);
+        const int n = q.tiles ? chunks_of(q, klen) : 1, mine = q.tiles * n;
+        const int items = lane_sums(mine), slots = lane_sums(n > 1 ? mine : 0);
+        if (lane == 63) {
+            plan[2 + 2 * (int64_t)b] = items;
+            plan[3 + 2 * (int64_t)b] = slots;
+        }
+    }
+    __syncthreads();
+    if (w) return;
+    if (lane == 0) {
+        plan[0] = klen;
+        plan[1] = 0;
+    }
+    int items = 0, slots = 0;
+    for (int b0 = 0; b0 < blocks; b0 += 64) {
+        const bool in = b0 + lane < blocks;
+        int32_t* at = plan + 2 + 2 * (int64_t)(b0 + lane);
+        const int x = in ? at[0] : 0, y = in ? at[1] : 0;
+        const int xs = lane_sums(x), ys = lane_sums(y);
+        if (in) {
+            at[0] = items + xs - x;
+            at[1] = slots + ys - y;
+        }
+        items += lane_bcast(xs, 63);
+        slots += lane_bcast(ys, 63);
+    }
+}
+
 struct Guard {
     int prev = -1;
     explicit Guard(int d) {
@@ -364,11 +419,11 @@ constexpr int64_t PROMPT_TARGET = 400;  // prompt items wanted: a round and not 
 constexpr int DEC_PAIRS = 128;          // a sequence of up to so many (row, head) pairs is the decode kernel's
 
 // The work of an attention call, and its workspace: the items' records, the
-// decode tiles' parts and, where a sequence may ask with several rows, the
-// prompt tiles'.
+// decode tiles' parts, where a sequence may ask with several rows the prompt
+// tiles', and for many sequences both launches' plans.
 struct Plan {
     Call dec, prompt;
-    size_t rec_dec, rec_prompt, part_dec, part_prompt, bytes;  // offsets, the whole
+    size_t rec_dec, rec_prompt, part_dec, part_prompt, plan_dec, plan_prompt, bytes;  // offsets, the whole
 };
 Plan plan_of(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq) {
     Plan p{};
@@ -396,6 +451,8 @@ Plan plan_of(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq) {
     p.rec_prompt = take((size_t)max_items(p.prompt) * sizeof(Record));
     p.part_dec = take((size_t)max_slots(DEC_TARGET, c.n_kv) * c.n_kv * 16 * (kv->hd + 2) * 4);
     p.part_prompt = take(n_row > n_seq ? (size_t)max_slots(PROMPT_TARGET, c.n_kv) * c.n_kv * 128 * (kv->hd + 2) * 4 : 0);
+    p.plan_dec = take((size_t)plan_words(c.n_seq) * 4);
+    p.plan_prompt = take((size_t)plan_words(c.n_seq) * 4);
     p.bytes = at;
     return p;
 }
@@ -521,7 +578,16 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_p
     const int64_t ga = max_items(a.c) * a.c.n_kv, gb = prompts ? max_items(b.c) * b.c.n_kv : 0;
     if (ga + gb > 0x7FFFFFFF) return bad("too many rows or sequences");
     const Launch la{(unsigned)ga, s}, lb{(unsigned)gb, s};
-    hipError_t e = kv->dtype == FRQ_DT_F32   ? launch_decode_f32(a, la)
+    hipError_t e = hipSuccess;
+    if (n_seq > (size_t)PLAN_SEQS) {
+        int32_t *pa = (int32_t*)(ws + plan.plan_dec), *pb = (int32_t*)(ws + plan.plan_prompt);
+        kv_plan_kernel<<<dim3(prompts ? 2 : 1), dim3(1024), 0, s>>>(a.c, b.c, pa, pb, a.err);
+        e = hipGetLastError();
+        if (e != hipSuccess) return hip_bad(e, "launch kv_plan");
+        a.c.plan = pa;
+        b.c.plan = pb;
+    }
+    e = kv->dtype == FRQ_DT_F32   ? launch_decode_f32(a, la)
                    : kv->dtype == FRQ_DT_F16 ? launch_decode_f16(a, la)
                                              : launch_decode_i8(a, la);
     if (e != hipSuccess) return hip_bad(e, "launch kv_decode");

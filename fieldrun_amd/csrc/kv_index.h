@@ -35,6 +35,7 @@ struct Call {
     int min_pairs, max_pairs;  // the sequences served: pairs in [min, max]
     int64_t target;        // items wanted over all kv heads
     int min_chunk;         // keys a chunk at least, a multiple of ALIGN
+    const int32_t* plan;   // of many sequences: the chunk length and 0, then before each 64 sequences (items, slots)
 };
 
 struct Seq {
@@ -101,6 +102,9 @@ KV_HD int64_t max_tiles(const Call& c) {
     return least < by_seq ? least : by_seq;
 }
 KV_HD int64_t max_items(const Call& c) { return max_tiles(c) + c.target / c.n_kv + 1; }
+// More sequences than this are summed once for the call, into a plan.
+constexpr int PLAN_SEQS = 64;
+KV_HD int64_t plan_words(int64_t n_seq) { return n_seq > PLAN_SEQS ? 2 + (n_seq + 63) / 64 * 2 : 0; }
 KV_HD int64_t max_slots(int64_t target, int n_kv) { return 2 * (target / n_kv + 1); }
 
 // The first key that the row at position pos sees (the last one is pos).

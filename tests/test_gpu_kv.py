@@ -326,6 +326,41 @@ def test_thousand_sequences(ctx):
     Batch(ctx, "f16", 16, 1, 1, 32, [int(x) for x in rng.integers(0, 40, 1000)], seed=5).check()
 
 
+@pytest.mark.parametrize("n", [64, 65, 128, 200])
+def test_more_than_64_sequences(ctx, n):
+    """Rows for both kernels, several chunks, idle and empty sequences, on both
+    sides of the number from which the sequences are summed beforehand."""
+    rng = np.random.default_rng(n)
+    lens = [int(x) for x in rng.integers(0, 60, n)]
+    rows = [int(x) for x in rng.integers(0, 3, n)]
+    for s, l, r in ((0, 1500, 1), (n // 2, 1300, 60), (n - 1, 900, 70), (n - 2, 2100, 2)):
+        lens[s], rows[s] = l, r
+    b = Batch(ctx, "f16", 16, 2, 3, 64, lens, rows, seed=n)
+    b.check()
+    b.check(window=33)
+
+
+def test_over_4096_sequences(ctx):
+    rng = np.random.default_rng(8)
+    lens = [int(x) for x in rng.integers(0, 9, 4300)]
+    lens[4200], lens[7], lens[4096] = 3000, 2000, 1000
+    Batch(ctx, "f16", 16, 1, 1, 16, lens, seed=9).check()
+
+
+@pytest.mark.parametrize("at", [0, 100, 299])
+def test_a_bad_length_among_many(ctx, at):
+    b = Batch(ctx, "f16", 16, 1, 2, 32, [20] * 300)
+    want = b.run()
+    lens = np.full(300, 20, np.int32)
+    lens[at] = 1 << 20
+    b.dev[1] = hip.DeviceArray.from_numpy(lens)
+    with pytest.raises(fa.FrqError) as e:
+        b.run()
+    assert e.value.code == fa.FRQ_ERR_ARG
+    b.dev[1] = hip.DeviceArray.from_numpy(np.full(300, 20, np.int32))
+    np.testing.assert_array_equal(b.run(), want)
+
+
 def test_large_and_small_scores(ctx):
     """Rows of q over the whole range of f32 (scores that saturate one key, or
     none), equal scores, and a zero row."""
