@@ -14,7 +14,10 @@ namespace frq {
 namespace kv {
 namespace {
 
-constexpr int WR = 32;   // rows a workgroup of the write and read kernels
+// Rows a workgroup of the write and read kernels (64, whole lines of int8
+// values, were slower for their fewer waves: 8192 rows of 4 heads of 128
+// written in 19.4 us against 16.8, read in 11.2 against 9.7).
+constexpr int WR = 32;
 constexpr int MAX_HD = 256;
 
 struct Move {
@@ -110,7 +113,11 @@ __device__ __forceinline__ void to_lds(E* p, const Quad<E>& q) {
 // Workgroup (WR rows, kv head); G lanes a row (a power of two >= hd / 4), four
 // channels a lane, every load issued up front.  Keys go straight to their
 // page; values through LDS, and from there four tokens of a channel at a time
-// where the rows lie side by side (a prompt's do).
+// where the rows lie side by side (a prompt's do).  Bound by memory for long
+// prompts: 8192 rows of 4 heads of 128 channels into int8, 42 MB, in 16.8 us
+// (2.5 TB/s: the values' pieces are half lines), back in 9.7 (4.3 TB/s); one token,
+// 2.6 us, by latency.  (A token at a time both ways 29.5 us against 25.1, calls
+// included.)
 template <int DT, int G>
 __global__ __launch_bounds__(256) void kv_write_kernel(const Move m) {
     using E = Elem<DT>;
@@ -414,9 +421,20 @@ hipError_t launch_move(const Move& m, int dtype, hipStream_t s) {
     return hipGetLastError();
 }
 
-constexpr int64_t DEC_TARGET = 512;    // decode items wanted: the chip's workgroups at two a CU
-constexpr int64_t PROMPT_TARGET = 400;  // prompt items wanted: a round and not quite two a CU
-constexpr int DEC_PAIRS = 128;          // a sequence of up to so many (row, head) pairs is the decode kernel's
+// Decode items wanted: the chip's workgroups at two a CU (256, 512, 768, 1024:
+// 48 int8 sequences of up to 6001 tokens 65, 47, 55, 56 us; one of 131071 f16
+// 103, 109, 115, 109; 16 f32 windows of 4096 164, 124, 123, 133).
+constexpr int64_t DEC_TARGET = 512;
+// Prompt items wanted: a round and not quite two a CU; more cost the joining
+// more than the balance gives (400, 640, 1024, 1536: kernel and join of 7 ragged
+// int8 prompts 123 + 8, 127 + 18, 110 + 24, 108 + 24 us; of 2048 rows over 8192
+// keys 503 + 5 at 400, 486 + 25 at 1024).
+constexpr int64_t PROMPT_TARGET = 400;
+// A sequence of up to so many (row, head) pairs is the decode kernel's (decode
+// against prompt kernel: 126 pairs over 1000 tokens 14.4, 31.3 us, over 8192
+// 27.9, 35.7, 8 times over 2000 45.5, 39.2; 252 pairs over 1000 15.2, 31.7, but
+// 8 times over 2000 71, 49.5).
+constexpr int DEC_PAIRS = 128;
 
 // The work of an attention call, and its workspace: the items' records, the
 // decode tiles' parts, where a sequence may ask with several rows the prompt

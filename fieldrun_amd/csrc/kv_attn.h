@@ -18,12 +18,13 @@
 // transposed (hd, page), so both operands are 16-byte loads straight from the
 // pages and nothing goes through LDS.
 //
-// 32-bit exactness on the f16 matrix cores: the cache's f16 and int8 entries
+// 32-bit exactness on the 16-bit matrix cores: the cache's f16 and int8 entries
 // are exact f16; an f32 q row, scaled by a power of two to below 2, is the sum
 // of two f16 (22 bits and more), likewise the probabilities (scaled by 2^11,
 // so that what f16 cannot hold of them is below 2^-36 of the largest); the
 // products of both halves add up in the f32 accumulators.  An f32 cache uses
-// the f32 matrix cores.
+// the f32 matrix cores for decoding, where memory bounds the call, and three
+// bf16 parts of both operands for prompts.
 #pragma once
 
 #include "frq_internal.h"
@@ -54,7 +55,7 @@ struct Cache {  // frq_kv as the kernels take it
 
 // An item as the joining launch reads it (chunks 1: nothing to join).
 struct Record {
-    int row0, rows, tile, chunk, chunks, slot, pad0, pad1;
+    int row0, rows, tile, chunk, chunks, slot, len, pad;
 };
 struct Args {
     Call c;
@@ -182,7 +183,7 @@ __device__ __forceinline__ Item find_item(const Call& c, int id, int* err) {
 
 __device__ __forceinline__ void note_item(Record* r, int id, const Item& it) {
     if (threadIdx.x == 0)
-        r[id] = Record{it.q.row0, it.q.rows, it.tile, it.chunk, it.found ? it.chunks : 1, it.slot, 0, 0};
+        r[id] = Record{it.q.row0, it.q.rows, it.tile, it.chunk, it.found ? it.chunks : 1, it.slot, it.q.len, 0};
 }
 
 __device__ __forceinline__ float fmax16(float v) {  // over the four lane groups of a pair
@@ -192,6 +193,12 @@ __device__ __forceinline__ float fmax16(float v) {  // over the four lane groups
 __device__ __forceinline__ float fsum16(float v) {
     v += __uint_as_float(xshfl<16>(__float_as_uint(v)));
     return v + __uint_as_float(xshfl<32>(__float_as_uint(v)));
+}
+
+// What out is multiplied by: a row that sees no key (its position below 0) is
+// zeros, one whose scores are all -inf is NaN, as the formula has it.
+__device__ __forceinline__ float over(float l, int pos) {
+    return l > 0.0f || l != l ? 1.0f / l : pos < 0 ? 0.0f : __builtin_nanf("");
 }
 
 // tanh to about 2e-7 of its value: a polynomial near zero, where
@@ -338,6 +345,20 @@ __device__ __forceinline__ void load_q(const float* q, float sign, int hd, int g
 // ---- decode: a wave takes whole key tiles for 16 pairs ----------------------
 // NS steps of hd (hd <= 32 NS; FULL: equal).  NW waves share a chunk's tiles
 // and join in LDS.
+//
+// Bound by the reading of keys and values, each once for 16 heads and rows: a
+// wave's loads of the next tile's keys are in flight under the softmax, of its
+// values under the next scores, straight into registers (LDS would add a pass
+// and a barrier a tile), page ids a tile ahead.  With two workgroups of four
+// waves a CU (the kernel alone; a large copy reaches 4.8 TB/s): f16, one
+// sequence of 131071 tokens, 8 kv heads of 128 channels, 95 us, 5.6 TB/s; f32, a
+// window of 4096, 16 sequences, 4 kv heads of 256, 111 us, 4.6 TB/s; int8, 48
+// sequences of up to 6001, 4 kv heads of 128 with 7 heads each, 42 us, 3.5 TB/s:
+// there the unpacking, the steps and the softmax of half the bytes keep the
+// vector units busy 40% of the time, and waves wait the other half.  Slower
+// (batch, long, window): loads past the caches 47, 110, 122 us; eight waves a
+// workgroup 55 and 168 (batch, window); a wave's tiles side by side 107 and 131
+// (long, window).
 template <int DT, int N32, bool FULL, int NW>
 __global__ __launch_bounds__(64 * NW, FULL && N32 <= 4 ? 2 : 1) void kv_decode_kernel(const Args a) {
     using T = Type<DT>;
@@ -646,7 +667,7 @@ __global__ __launch_bounds__(64 * NW, FULL && N32 <= 4 ? 2 : 1) void kv_decode_k
     }
     if (wave != 0 || col >= np) return;
     if (it.chunks == 1) {
-        const float r = lsum > 0.0f || lsum != lsum ? 1.0f / lsum : 0.0f;  // no key seen: zeros
+        const float r = over(lsum, pos);
         float* d = a.out + (int64_t)(it.q.row0 + row) * a.out_pitch + (int64_t)head * hd + 4 * g;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -690,7 +711,8 @@ __device__ __forceinline__ int pick4(int j, int a, int b, int c, int d) {
 // An f32 cache is staged as three bf16 (exact: 8 bits each), q and the
 // probabilities likewise, and a product is the six of theirs that reach 2^-24
 // of it: six matrix instructions, where the f32 ones would take the time of
-// sixteen.  Its tiles are loaded into registers and have one buffer.
+// sixteen (the f16 case over an f32 cache 1671 us against 2768).  Its tiles are
+// loaded into registers and have one buffer.
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ void split8(const float (&x)[8], b8 (&y)[3]) {
     u4 w[3];
@@ -1152,7 +1174,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, N32>::WAVES)) void kv_prompt_kerne
     if (idle || col >= np) return;
     l += __uint_as_float(xshfl<32>(__float_as_uint(l)));
     if (it.chunks == 1) {
-        const float r = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // no key seen: zeros
+        const float r = over(l, pos);
         float* d = a.out + (int64_t)(it.q.row0 + row) * a.out_pitch + (int64_t)head * hd + 4 * h;
 #pragma unroll
         for (int t = 0; t < NH; ++t)
@@ -1193,7 +1215,8 @@ __global__ __launch_bounds__(256, (Prompt<DT, N32>::WAVES)) void kv_prompt_kerne
 // The workgroup of a tile's chunk i joins the i-th share of the tile's
 // outputs, so that a long sequence's parts are read by many workgroups.
 // Threads are (float4 of the share, run of chunks); each folds its chunks,
-// then the runs are merged pairwise, always in the same order.
+// then the runs are merged pairwise, always in the same order.  Bound by
+// latency: 4.5 to 5.3 us at 60 to 280 chunks of 16 pairs of 128 channels.
 template <int TP>
 __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so, float* sm, float* sl) {
     const int n_kv = a.c.n_kv, kvh = block % n_kv;
@@ -1243,7 +1266,7 @@ __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so,
         }
         if (run == 0 && in) {
             const int pr = p0 + pair, row = pr / a.c.rep, head = kvh * a.c.rep + pr % a.c.rep;
-            const float r = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            const float r = over(l, it.len - it.rows + row);
             F4 y;
 #pragma unroll
             for (int i = 0; i < 4; ++i) y.v[i] = o[i] * r;

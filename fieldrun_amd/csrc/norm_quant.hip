@@ -7,6 +7,12 @@
 // quant_core.h's (frq_quant_i8_dev's bytes for the rows n).  A row is read
 // once and stays in registers; only the selection of rows with many equal
 // magnitudes puts it into LDS, over the candidates it has done with.
+//
+// Bound by the selection's passes over the registers, with the loads of other
+// workgroups behind them: 4096 rows of 4096 channels, 219 MB, in 63 us (3.5
+// TB/s; a large copy reaches 4.8), waves waiting for memory and at barriers
+// 57% of their time; one row of 3584 in 7.1 us, by latency.  With the row n
+// always in LDS the large case took 66 us.
 #include "quant_core.h"
 
 namespace frq {

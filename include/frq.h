@@ -258,7 +258,8 @@ int frq_kv_read_dev(frq_ctx* ctx, const frq_kv* kv, const int64_t* d_slot,
  * the runs joined in a fixed order; a row that sees no token gets zeros.  Rows
  * outside d_first[0] .. d_first[n_seq] - 1 stay as they were.  What a row
  * does not see does not touch it, whatever it holds; a row that sees an
- * infinity or a NaN gets infinities or NaN.
+ * infinity or a NaN gets infinities or NaN, or, where an infinite key leaves
+ * a score of -inf, possibly the formula's value.
  * d_ws: frq_kv_attn_ws bytes of device memory, 16-byte aligned, for this call
  * alone until it is done (calls that may overlap, such as two graphs' replays,
  * have one each); NULL takes the context's, which a call under graph capture

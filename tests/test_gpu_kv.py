@@ -376,6 +376,29 @@ def test_large_and_small_scores(ctx):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_scores_that_are_all_minus_infinity(ctx, kind):
+    """Such a row is NaN, as its softmax is; a row that sees no key is zeros.
+    One chunk and several, rows for both kernels.  Where one score is not -inf
+    the f32 decode row is that key's value; over f16 keys it is NaN: q's entry
+    1.0 is the halves 1 and 0, and -inf * 1 + -inf * 0 is NaN."""
+    def poison(ks, vs):
+        for s in (0, 1, 2, 4):
+            ks[s][:, 0, 3] = -np.inf
+        ks[4][-1, 0, 3] = 0.25
+
+    b = Batch(ctx, kind, 16, 1, 3, 64, [40, 1400, 300, 5, 70], [1, 2, 60, 9, 1], poison=poison)
+    b.q[:, :, 3] = 1.0
+    got = b.run()
+    at = b.first
+    assert np.isnan(got[at[0]:at[3]]).all()
+    assert (got[at[3]:at[3] + 4] == 0).all() and np.isfinite(got[at[3]:at[4]]).all()
+    if kind == "f32":
+        assert np.abs(got[at[4]] - b.v[4][-1]).max() <= 2.0 ** -20 * np.abs(b.v[4][-1]).max()
+    else:
+        assert np.isnan(got[at[4]]).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
 @pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
 def test_what_is_not_finite_stays_with_rows_that_see_it(ctx, kind, bad):
     def poison(ks, vs):
