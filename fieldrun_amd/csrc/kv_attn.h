@@ -306,14 +306,14 @@ struct QOp {
 };
 
 // q points at the pair's hd values; lane group g takes PL of each step's KS.
-template <int DT, int NS, bool FULL>
-__device__ __forceinline__ void load_q(const float* q, float sign, int hd, int g, QOp<DT, NS>& o) {
+template <int DT, int HD, int NS>
+__device__ __forceinline__ void load_q(const float* q, float sign, int g, QOp<DT, NS>& o) {
     using T = Type<DT>;
     float x[NS][T::PL];
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
         const int c = s * T::KS + g * T::PL;
-        const bool in = FULL || c < hd;
+        const bool in = HD % T::KS == 0 || c < HD;
 #pragma unroll
         for (int j = 0; j < T::PL; j += 4) {
             const F4 f = *reinterpret_cast<const F4*>(q + (in ? c + j : 0));
@@ -343,8 +343,8 @@ __device__ __forceinline__ void load_q(const float* q, float sign, int hd, int g
 }
 
 // ---- decode: a wave takes whole key tiles for 16 pairs ----------------------
-// NS steps of hd (hd <= 32 NS; FULL: equal).  NW waves share a chunk's tiles
-// and join in LDS.
+// HD channels: NS steps of the scores (the last half empty where HD is 16 mod
+// 32), NT tiles of the values.  NW waves share a chunk's tiles and join in LDS.
 //
 // Bound by the reading of keys and values, each once for 16 heads and rows: a
 // wave's loads of the next tile's keys are in flight under the softmax, of its
@@ -359,12 +359,13 @@ __device__ __forceinline__ void load_q(const float* q, float sign, int hd, int g
 // (batch, long, window): loads past the caches 47, 110, 122 us; eight waves a
 // workgroup 55 and 168 (batch, window); a wave's tiles side by side 107 and 131
 // (long, window).
-template <int DT, int N32, bool FULL, int NW>
-__global__ __launch_bounds__(64 * NW, FULL && N32 <= 4 ? 2 : 1) void kv_decode_kernel(const Args a) {
+template <int DT, int HD, int NW>
+__global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(const Args a) {
     using T = Type<DT>;
-    constexpr int NS = 32 * N32 / T::KS, NT = 2 * N32;  // steps of hd in the scores, 16-wide tiles of hd in the values
+    constexpr int NS = (HD + T::KS - 1) / T::KS, NT = HD / 16;
+    constexpr bool WHOLE = HD % T::KS == 0;
     constexpr int KT = T::KT, NU = KT / 16;
-    constexpr int ORow = 32 * N32 + 4;
+    constexpr int ORow = HD + 4;
     __shared__ float red[NW / 2][16][ORow];
     __shared__ float stat[NW][16][2];
     const int n_kv = a.c.n_kv;
@@ -374,7 +375,8 @@ __global__ __launch_bounds__(64 * NW, FULL && N32 <= 4 ? 2 : 1) void kv_decode_k
     if (!it.found) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int col = lane & 15, g = lane >> 4;
-    const int hd = a.kv.hd, page = a.kv.page, shift = a.c.shift;
+    constexpr int hd = HD;
+    const int page = a.kv.page, shift = a.c.shift;
     // the pair of this lane's column; columns past the last pair repeat it
     const int pairs = it.q.rows * a.c.rep;
     const int p0 = it.tile * 16, np = min(16, pairs - p0);
@@ -389,7 +391,7 @@ __global__ __launch_bounds__(64 * NW, FULL && N32 <= 4 ? 2 : 1) void kv_decode_k
     const int end = uni((int)min((int64_t)it.q.lo + (int64_t)(it.chunk + 1) * it.klen, (int64_t)pos_b + 1));
     const int tiles = end > beg ? (end - beg + KT - 1) / KT : 0;
     QOp<DT, NS> q;
-    load_q<DT, NS, FULL>(a.q + (int64_t)(it.q.row0 + row) * a.q_pitch + (int64_t)head * hd, a.sign, hd, g, q);
+    load_q<DT, HD, NS>(a.q + (int64_t)(it.q.row0 + row) * a.q_pitch + (int64_t)head * hd, a.sign, g, q);
     // scores times mul are in the domain of exp2; with a cap they are made so
     const bool capped = a.cap > 0.0f;
     const float scl = fmaxf(__builtin_ldexpf(a.scale, q.e), 1.17549435e-38f);
@@ -433,9 +435,8 @@ __global__ __launch_bounds__(64 * NW, FULL && N32 <= 4 ? 2 : 1) void kv_decode_k
             const char* p = kb + pg * a.kv.stride + (int64_t)((base + d) & (page - 1)) * hd * T::SZ;
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
-                if (!FULL && s * T::KS >= hd) continue;
                 const int c = s * T::KS + g * T::PL;
-                kr[u][s] = load_raw<DT>(p + (FULL || c < hd ? c : 0) * T::SZ);
+                kr[u][s] = load_raw<DT>(p + (WHOLE || c < hd ? c : 0) * T::SZ);
             }
         }
         if constexpr (T::I8) {
@@ -451,7 +452,7 @@ __global__ __launch_bounds__(64 * NW, FULL && N32 <= 4 ? 2 : 1) void kv_decode_k
         const char* p = vb + pg * a.kv.stride + ((int64_t)col * page + at) * T::SZ;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
-            if (FULL || t * 16 < hd) vr[t] = load_raw<DT>(p + (int64_t)t * 16 * page * T::SZ);
+            vr[t] = load_raw<DT>(p + (int64_t)t * 16 * page * T::SZ);
         if constexpr (T::I8) {
             const float* s = a.kv.vs + pg * a.kv.sstride + kvh * page + at;
 #pragma unroll
@@ -476,10 +477,9 @@ __global__ __launch_bounds__(64 * NW, FULL && N32 <= 4 ? 2 : 1) void kv_decode_k
             sc[u] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
-                if (!FULL && s * T::KS >= hd) continue;
                 if constexpr (T::F32) {
                     f4 x = __builtin_bit_cast(f4, kr[u][s]);
-                    if (!FULL && s * T::KS + g * T::PL >= hd) x = f4{0, 0, 0, 0};
+                    if (!WHOLE && s * T::KS + g * T::PL >= hd) x = f4{0, 0, 0, 0};
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         sc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], q.x[s][j], sc[u], 0, 0, 0);
@@ -487,7 +487,7 @@ __global__ __launch_bounds__(64 * NW, FULL && N32 <= 4 ? 2 : 1) void kv_decode_k
                     h8 x;
                     if constexpr (T::I8) x = i8_to_h8(kr[u][s]);
                     else x = __builtin_bit_cast(h8, kr[u][s]);
-                    if (!FULL && s * T::KS + g * T::PL >= hd) x = h8{0, 0, 0, 0, 0, 0, 0, 0};
+                    if (!WHOLE && s * T::KS + g * T::PL >= hd) x = h8{0, 0, 0, 0, 0, 0, 0, 0};
                     sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.hi[s], sc[u], 0, 0, 0);
                     sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q.lo[s], sc[u], 0, 0, 0);
                 }
@@ -577,7 +577,6 @@ __global__ __launch_bounds__(64 * NW, FULL && N32 <= 4 ? 2 : 1) void kv_decode_k
                 }
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    if (!FULL && t * 16 >= hd) continue;
                     vr[t] &= keep;
                     if (!alike) {
 #pragma unroll
@@ -594,7 +593,6 @@ __global__ __launch_bounds__(64 * NW, FULL && N32 <= 4 ? 2 : 1) void kv_decode_k
         if constexpr (T::F32) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                if (!FULL && t * 16 >= hd) continue;
                 const f4 x = __builtin_bit_cast(f4, vr[t]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], s[j], o[t], 0, 0, 0);
@@ -604,7 +602,6 @@ __global__ __launch_bounds__(64 * NW, FULL && N32 <= 4 ? 2 : 1) void kv_decode_k
             split8(s, hi, lo);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                if (!FULL && t * 16 >= hd) continue;
                 h8 x;
                 if constexpr (T::I8) x = i8_to_h8(vr[t]);
                 else x = __builtin_bit_cast(h8, vr[t]);
@@ -627,7 +624,6 @@ __global__ __launch_bounds__(64 * NW, FULL && N32 <= 4 ? 2 : 1) void kv_decode_k
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        if (!FULL && t * 16 >= hd) continue;
                         const float x = value_at<DT>(p + (int64_t)(16 * t + 4 * g + i) * page * T::SZ);
                         if (sees && !(x - x == 0.0f)) o[t][i] += x;
                     }
@@ -671,7 +667,6 @@ __global__ __launch_bounds__(64 * NW, FULL && N32 <= 4 ? 2 : 1) void kv_decode_k
         float* d = a.out + (int64_t)(it.q.row0 + row) * a.out_pitch + (int64_t)head * hd + 4 * g;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            if (!FULL && t * 16 >= hd) continue;
             F4 y;
 #pragma unroll
             for (int i = 0; i < 4; ++i) y.v[i] = o[t][i] * r;
@@ -688,7 +683,7 @@ __global__ __launch_bounds__(64 * NW, FULL && N32 <= 4 ? 2 : 1) void kv_decode_k
         d += 32 + (int64_t)col * hd + 4 * g;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
-            if (FULL || t * 16 < hd) *reinterpret_cast<f4*>(d + 16 * t) = o[t];
+            *reinterpret_cast<f4*>(d + 16 * t) = o[t];
     }
 }
 
@@ -744,15 +739,16 @@ __device__ __forceinline__ f16v product(const b8 (&x)[3], const b8 (&y)[3], f16v
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], y[0], c, 0, 0, 0);
 }
 
-template <int DT, int N32>
+template <int DT, int HD>
 struct Prompt {
     static constexpr bool F32 = DT == FRQ_DT_F32;
+    static constexpr int N32 = (HD + 31) / 32;
     using Op = std::conditional_t<F32, b8, h8>;
     static constexpr int NA = F32 ? 3 : 1, NB = F32 ? 3 : 2;  // parts of a cache operand, of q and p
     static constexpr int NBUF = F32 ? 1 : 2;                  // buffers
     static constexpr int WAVES = !F32 && N32 <= 4 ? 2 : 1;    // a SIMD
-    static constexpr int KT = N32 == 3 || (!F32 && N32 <= 4) ? 64 : 32;  // keys a tile
-    static constexpr int HP = 32 * N32;             // hd, padded
+    static constexpr int KT = N32 % 2 || (!F32 && N32 <= 4) ? 64 : 32;  // keys a tile
+    static constexpr int HP = 32 * N32;             // HD, padded
     static constexpr int KC = HP / 8, VC = KT / 8;  // pieces of a key row, of a value row
     static constexpr int KX = KC % 16 == 0 ? 15 : KC % 8 == 0 ? 7 : 3, VX = VC - 1;
     static constexpr int IPW = KT * KC / 256;       // pieces a thread stages of each
@@ -760,13 +756,13 @@ struct Prompt {
     static constexpr int LDS = 2 * NBUF * NA * BUF * 2 + (DT == FRQ_DT_ROWI8 ? 2 * 2 * KT * 4 : 0);
 };
 
-template <int DT, int N32, bool FULL>
-__global__ __launch_bounds__(256, (Prompt<DT, N32>::WAVES)) void kv_prompt_kernel(const Args a) {
-    using P = Prompt<DT, N32>;
+template <int DT, int HD>
+__global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel(const Args a) {
+    using P = Prompt<DT, HD>;
     using Op = typename P::Op;
     constexpr bool I8 = DT == FRQ_DT_ROWI8, F32 = P::F32, F16 = !I8 && !F32;
     constexpr int SZ = I8 ? 1 : F32 ? 4 : 2, NA = P::NA, NB = P::NB, NBUF = P::NBUF;
-    constexpr int NS = 2 * N32, NH = N32, NK = P::KT / 32, KT = P::KT, IPW = P::IPW;
+    constexpr int NS = HD / 16, NH = P::N32, NK = P::KT / 32, KT = P::KT, IPW = P::IPW;
     extern __shared__ __align__(1024) char lds[];
     __shared__ int flag;  // a value was taken out
     uint16_t* lk = reinterpret_cast<uint16_t*>(lds);                   // [NBUF][NA][KT][HP]
@@ -780,7 +776,8 @@ __global__ __launch_bounds__(256, (Prompt<DT, N32>::WAVES)) void kv_prompt_kerne
     if (!it.found) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int col = lane & 31, h = lane >> 5;
-    const int hd = a.kv.hd, page = a.kv.page, shift = a.c.shift, rep = a.c.rep;
+    constexpr int hd = HD;
+    const int page = a.kv.page, shift = a.c.shift, rep = a.c.rep;
     const int pairs = it.q.rows * rep, off = it.q.len - it.q.rows;
     // the workgroup's pairs and keys
     const int t0 = it.tile * 128, tn = min(128, pairs - t0);
@@ -805,13 +802,12 @@ __global__ __launch_bounds__(256, (Prompt<DT, N32>::WAVES)) void kv_prompt_kerne
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             const int c = 16 * s + 8 * h;
-            const bool in = FULL || c < hd;
 #pragma unroll
             for (int j = 0; j < 8; j += 4) {
-                const F4 f = *reinterpret_cast<const F4*>(q + (in ? c + j : 0));
+                const F4 f = *reinterpret_cast<const F4*>(q + c + j);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[s][j + i] = in ? f.v[i] * a.sign : 0.0f;
+                    x[s][j + i] = f.v[i] * a.sign;
                     mx = fmaxf(mx, __builtin_fabsf(x[s][j + i]));
                 }
             }
@@ -876,8 +872,8 @@ __global__ __launch_bounds__(256, (Prompt<DT, N32>::WAVES)) void kv_prompt_kerne
             const int d = (i * 64 + ln) / P::KC, r = r0 + i * VR;
             const int c = 8 * (((i * 64 + ln) % P::KC) ^ ((wave * (KT / 4) + d) & P::KX));
             // past hd q is zero, any piece will do; channels past hd are not kept
-            const char* pk = rows + (d * hd + (FULL || c < hd ? c : 0)) * SZ;
-            const char* pv = toks + (FULL || r < hd ? r : 0) * page * SZ;
+            const char* pk = rows + (d * hd + (P::HP == hd || c < hd ? c : 0)) * SZ;
+            const char* pv = toks + (P::HP == hd || r < hd ? r : 0) * page * SZ;
             if constexpr (!F16) {
 #pragma unroll
                 for (int x = 0; x < NR; ++x) {
@@ -1024,33 +1020,33 @@ __global__ __launch_bounds__(256, (Prompt<DT, N32>::WAVES)) void kv_prompt_kerne
                 for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < G; ++i)
-                    if (FULL || 16 * i < hd) key_op(i, xa[i]);
+                    if (i < NS) key_op(i, xa[i]);
 #pragma unroll
                 for (int g = 0; g < NS; g += 2 * G) {
 #pragma unroll
                     for (int i = 0; i < G; ++i)
-                        if (g + G + i < NS && (FULL || 16 * (g + G + i) < hd)) key_op(g + G + i, xb[i]);
+                        if (g + G + i < NS) key_op(g + G + i, xb[i]);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int i = 0; i < G; ++i) {
-                        if (!FULL && 16 * (g + i) >= hd) continue;
-                        s = product(xa[i], qv[g + i], s);
+                        if (g + i >= NS) continue;
+                        s = product(xa[i], qv[(g + i) % NS], s);
                     }
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int i = 0; i < G; ++i)
-                        if (g + 2 * G + i < NS && (FULL || 16 * (g + 2 * G + i) < hd)) key_op(g + 2 * G + i, xa[i]);
+                        if (g + 2 * G + i < NS) key_op(g + 2 * G + i, xa[i]);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int i = 0; i < G; ++i) {
-                        if (g + G + i >= NS || (!FULL && 16 * (g + G + i) >= hd)) continue;
+                        if (g + G + i >= NS) continue;
                         s = product(xb[i], qv[(g + G + i) % NS], s);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
 #pragma unroll
                 for (int i = 0; i < G; ++i)
-                    if (i < 2 * NH && (FULL || 32 * (i / 2) < hd)) val_op(i, xa[i]);
+                    if (i < 2 * NH) val_op(i, xa[i]);
                 const bool edge = kb0 < lo_b || kb0 + 31 > pos_a;
                 if constexpr (I8) {
 #pragma unroll
@@ -1122,23 +1118,23 @@ __global__ __launch_bounds__(256, (Prompt<DT, N32>::WAVES)) void kv_prompt_kerne
                 for (int g = 0; g < 2 * NH; g += 2 * G) {
 #pragma unroll
                     for (int i = 0; i < G; ++i)
-                        if (g + G + i < 2 * NH && (FULL || 32 * ((g + G + i) / 2) < hd)) val_op(g + G + i, xb[i]);
+                        if (g + G + i < 2 * NH) val_op(g + G + i, xb[i]);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int i = 0; i < G; ++i) {
                         const int t = (g + i) / 2;
-                        if (g + i >= 2 * NH || (!FULL && 32 * t >= hd)) continue;
+                        if (g + i >= 2 * NH) continue;
                         o[t % NH] = product(xa[i], pv[i % 2], o[t % NH]);
                     }
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int i = 0; i < G; ++i)
-                        if (g + 2 * G + i < 2 * NH && (FULL || 32 * ((g + 2 * G + i) / 2) < hd)) val_op(g + 2 * G + i, xa[i]);
+                        if (g + 2 * G + i < 2 * NH) val_op(g + 2 * G + i, xa[i]);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int i = 0; i < G; ++i) {
                         const int t = (g + G + i) / 2;
-                        if (g + G + i >= 2 * NH || (!FULL && 32 * t >= hd)) continue;
+                        if (g + G + i >= 2 * NH) continue;
                         o[t % NH] = product(xb[i], pv[i % 2], o[t % NH]);
                     }
                     __builtin_amdgcn_sched_barrier(0);
@@ -1163,7 +1159,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, N32>::WAVES)) void kv_prompt_kerne
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int c = 32 * t + 8 * (i / 4) + 4 * h + i % 4;
-                        if (!FULL && c >= hd) continue;
+                        if (c >= hd) continue;
                         const float x = value_at<DT>(p + (int64_t)c * page * SZ);
                         if (sees && !(x - x == 0.0f)) o[t][i] += x;
                         __builtin_amdgcn_sched_barrier(0);
@@ -1181,7 +1177,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, N32>::WAVES)) void kv_prompt_kerne
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const int c = 32 * t + 2 * i;
-                if (!FULL && c >= hd) continue;
+                if (c >= hd) continue;
                 F4 y;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) y.v[j] = (I8 ? __builtin_ldexpf(o[t][i + j], ev - W_EXP) : o[t][i + j]) * r;
@@ -1202,7 +1198,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, N32>::WAVES)) void kv_prompt_kerne
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const int c = 32 * t + 2 * i;
-                if (!FULL && c >= hd) continue;
+                if (c >= hd) continue;
                 f4 y;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) y[j] = I8 ? __builtin_ldexpf(o[t][i + j], ev - W_EXP) : o[t][i + j];
@@ -1287,48 +1283,62 @@ hipError_t launch_prompt_f32(const Args& a, const Launch& l);
 hipError_t launch_prompt_f16(const Args& a, const Launch& l);
 hipError_t launch_prompt_i8(const Args& a, const Launch& l);
 
-// The kernel of a head width: whole steps of 32 at the widths models have,
-// else the next of three with its last steps masked.
-template <int DT>
-hipError_t launch_decode(const Args& a, const Launch& l) {
-    constexpr int NW = 4;
-    const int hd = a.kv.hd;
-    const dim3 g(l.grid), b(64 * NW);
-    if (hd == 64) kv_decode_kernel<DT, 2, true, NW><<<g, b, 0, l.s>>>(a);
-    else if (hd == 96) kv_decode_kernel<DT, 3, true, NW><<<g, b, 0, l.s>>>(a);
-    else if (hd == 128) kv_decode_kernel<DT, 4, true, NW><<<g, b, 0, l.s>>>(a);
-    else if (hd == 256) kv_decode_kernel<DT, 8, true, NW><<<g, b, 0, l.s>>>(a);
-    else if (hd <= 64) kv_decode_kernel<DT, 2, false, NW><<<g, b, 0, l.s>>>(a);
-    else if (hd <= 128) kv_decode_kernel<DT, 4, false, NW><<<g, b, 0, l.s>>>(a);
-    else kv_decode_kernel<DT, 8, false, NW><<<g, b, 0, l.s>>>(a);
-    return hipGetLastError();
+// Every width has a kernel of its own: with the steps of a width known only at
+// run time (the next of 64, 128 and 256, masked) 192 channels took 21 us where
+// 256 took 10, 16 channels the time of 64.
+template <int HD>
+using Width = std::integral_constant<int, HD>;
+template <int MOST, typename F>
+hipError_t by_width(int hd, F&& f) {
+    switch (hd) {
+        case 16: return f(Width<16>{});
+        case 32: return f(Width<32>{});
+        case 48: return f(Width<48>{});
+        case 64: return f(Width<64>{});
+        case 80: return f(Width<80>{});
+        case 96: return f(Width<96>{});
+        case 112: return f(Width<112>{});
+        case 128: return f(Width<128>{});
+    }
+    if constexpr (MOST > 128) {
+        switch (hd) {
+            case 144: return f(Width<144>{});
+            case 160: return f(Width<160>{});
+            case 176: return f(Width<176>{});
+            case 192: return f(Width<192>{});
+            case 208: return f(Width<208>{});
+            case 224: return f(Width<224>{});
+            case 240: return f(Width<240>{});
+            case 256: return f(Width<256>{});
+        }
+    }
+    return hipErrorNotSupported;  // not a width that the checks let through
 }
 
-template <int DT, int N32, bool FULL>
+template <int DT>
+hipError_t launch_decode(const Args& a, const Launch& l) {
+    return by_width<256>(a.kv.hd, [&](auto w) {
+        kv_decode_kernel<DT, decltype(w)::value, 4><<<dim3(l.grid), dim3(256), 0, l.s>>>(a);
+        return hipGetLastError();
+    });
+}
+
+template <int DT, int HD>
 hipError_t run_prompt(const Args& a, const Launch& l) {
-    constexpr int lds = Prompt<DT, N32>::LDS;
+    constexpr int lds = Prompt<DT, HD>::LDS;
     static_assert(lds <= 160 * 1024, "LDS of a CU");
     if (lds > 48 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kv_prompt_kernel<DT, N32, FULL>),
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kv_prompt_kernel<DT, HD>),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
     }
-    kv_prompt_kernel<DT, N32, FULL><<<dim3(l.grid), dim3(256), lds, l.s>>>(a);
+    kv_prompt_kernel<DT, HD><<<dim3(l.grid), dim3(256), lds, l.s>>>(a);
     return hipGetLastError();
 }
 template <int DT>
 hipError_t launch_prompt(const Args& a, const Launch& l) {
-    const int hd = a.kv.hd;
-    if (hd == 64) return run_prompt<DT, 2, true>(a, l);
-    if (hd == 96) return run_prompt<DT, 3, true>(a, l);
-    if (hd == 128) return run_prompt<DT, 4, true>(a, l);
-    if (hd <= 64) return run_prompt<DT, 2, false>(a, l);
-    if (hd <= 128) return run_prompt<DT, 4, false>(a, l);
-    if constexpr (DT != FRQ_DT_F32) {
-        if (hd == 256) return run_prompt<DT, 8, true>(a, l);
-        return run_prompt<DT, 8, false>(a, l);
-    }
-    return hipErrorNotSupported;
+    return by_width<DT == FRQ_DT_F32 ? 128 : 256>(a.kv.hd,
+                                                  [&](auto w) { return run_prompt<DT, decltype(w)::value>(a, l); });
 }
 
 }  // namespace kv

@@ -326,6 +326,16 @@ def test_thousand_sequences(ctx):
     Batch(ctx, "f16", 16, 1, 1, 32, [int(x) for x in rng.integers(0, 40, 1000)], seed=5).check()
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "rowi8"])
+@pytest.mark.parametrize("hd", range(16, 257, 16))
+def test_every_width(ctx, kind, hd):
+    """Decode and prompt rows in one call, one chunk and several, a page's end
+    inside a tile."""
+    b = Batch(ctx, kind, 16, 2, 5, hd, [70, 333, 1400, 41], [1, 60, 2, 41], seed=hd)
+    b.check()
+    b.check(window=50, cap=20.0)
+
+
 @pytest.mark.parametrize("n", [64, 65, 128, 200])
 def test_more_than_64_sequences(ctx, n):
     """Rows for both kernels, several chunks, idle and empty sequences, on both
