@@ -590,6 +590,7 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_p
     b.c.max_pairs = plan.prompt.max_pairs;
     b.c.tp = plan.prompt.tp;
     b.c.target = plan.prompt.target;
+    b.c.min_chunk = plan.prompt.min_chunk;
     b.rec = (Record*)(ws + plan.rec_prompt);
     b.part = (float*)(ws + plan.part_prompt);
     b.slots = n_row > n_seq ? max_slots(PROMPT_TARGET, a.c.n_kv) : 0;

@@ -169,7 +169,6 @@ __device__ __forceinline__ Item find_item(const Call& c, int id, int* err) {
         it.q.row0 = lane_bcast(q.row0, l);
         it.q.rows = lane_bcast(q.rows, l);
         it.q.len = lane_bcast(q.len, l);
-        it.q.lo = lane_bcast(q.lo, l);
         it.chunks = lane_bcast(n, l);
         it.klen = lane_bcast(own, l);
         const int i = lane_bcast(at, l), t = uni(i / it.chunks);
@@ -387,8 +386,9 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
     const int pos_a = uni(it.q.len - it.q.rows + p0 / a.c.rep);
     const int pos_b = uni(it.q.len - it.q.rows + (p0 + np - 1) / a.c.rep);
     const int see_lo = key_lo(a.c, pos), lo_a = key_lo(a.c, pos_a), lo_b = key_lo(a.c, pos_b);
-    const int beg = uni(max(it.q.lo + it.chunk * it.klen, lo_a / ALIGN * ALIGN));
-    const int end = uni((int)min((int64_t)it.q.lo + (int64_t)(it.chunk + 1) * it.klen, (int64_t)pos_b + 1));
+    const int64_t beg64 = tile_lo(a.c, pos_a) + (int64_t)it.chunk * it.klen;
+    const int end = uni((int)min(beg64 + it.klen, (int64_t)pos_b + 1));
+    const int beg = uni((int)min(beg64, (int64_t)max(end, 0)));
     const int tiles = end > beg ? (end - beg + KT - 1) / KT : 0;
     QOp<DT, NS> q;
     load_q<DT, HD, NS>(a.q + (int64_t)(it.q.row0 + row) * a.q_pitch + (int64_t)head * hd, a.sign, g, q);
@@ -782,8 +782,9 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     // the workgroup's pairs and keys
     const int t0 = it.tile * 128, tn = min(128, pairs - t0);
     const int wpos_a = uni(off + t0 / rep), wpos_b = uni(off + (t0 + tn - 1) / rep);  // its first and last row
-    const int beg = uni(max(it.q.lo + it.chunk * it.klen, key_lo(a.c, wpos_a) / ALIGN * ALIGN));
-    const int end = uni((int)min((int64_t)it.q.lo + (int64_t)(it.chunk + 1) * it.klen, (int64_t)wpos_b + 1));
+    const int64_t beg64 = tile_lo(a.c, wpos_a) + (int64_t)it.chunk * it.klen;
+    const int end = uni((int)min(beg64 + it.klen, (int64_t)wpos_b + 1));
+    const int beg = uni((int)min(beg64, (int64_t)max(end, 0)));
     const int tiles = end > beg ? (end - beg + KT - 1) / KT : 0;
     // the wave's, the lane's; columns past the last pair repeat it
     const int p0 = t0 + min(32 * wave, tn - 1), np = max(1, min(32, tn - 32 * wave));
@@ -1227,6 +1228,54 @@ __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so,
     const int runs = 256 / pe, run = tid / pe;
     const int64_t pitch = (int64_t)TP * (hd + 2) * n_kv;
     const float* part = a.part + (it.slot * n_kv + kvh) * (int64_t)(TP * (hd + 2));
+    auto store = [&](int pair, int c4, f4 o, float l) {
+        const int pr = p0 + pair, row = pr / a.c.rep, head = kvh * a.c.rep + pr % a.c.rep;
+        const float r = over(l, it.len - it.rows + row);
+        F4 y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y.v[i] = o[i] * r;
+        *reinterpret_cast<F4*>(a.out + (int64_t)(it.row0 + row) * a.out_pitch + (int64_t)head * hd + 4 * c4) = y;
+    };
+    if (runs == 1) {  // large shares: U float4 a thread at once
+        constexpr int U = 4;
+        for (int b = beg + tid; b < end; b += 256 * U) {
+            int pair[U], c4[U];
+            float m[U], l[U];
+            f4 o[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int e = min(b + 256 * u, end - 1);
+                pair[u] = e / (hd / 4);
+                c4[u] = e % (hd / 4);
+                m[u] = -__builtin_inff();
+                l[u] = 0.0f;
+                o[u] = f4{0, 0, 0, 0};
+            }
+            for (int c = 0; c < it.chunks; ++c) {
+                const float* d = part + c * pitch;
+                float mc[U], lc[U];
+                f4 oc[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    mc[u] = d[2 * pair[u]];
+                    lc[u] = d[2 * pair[u] + 1];
+                    oc[u] = *reinterpret_cast<const f4*>(d + 2 * TP + (int64_t)pair[u] * hd + 4 * c4[u]);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const float mn = fmaxf(m[u], mc[u]), mr = mn == -__builtin_inff() ? 0.0f : mn;
+                    const float x = __builtin_amdgcn_exp2f(m[u] - mr), y = __builtin_amdgcn_exp2f(mc[u] - mr);
+                    m[u] = mn;
+                    l[u] = l[u] * x + lc[u] * y;
+                    o[u] = o[u] * x + oc[u] * y;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (b + 256 * u < end) store(pair[u], c4[u], o[u], l[u]);
+        }
+        return;
+    }
     for (int b = beg; b < end; b += pe) {
         const int e = b + tid % pe;
         const bool in = e < end;
@@ -1260,14 +1309,7 @@ __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so,
             }
             __syncthreads();
         }
-        if (run == 0 && in) {
-            const int pr = p0 + pair, row = pr / a.c.rep, head = kvh * a.c.rep + pr % a.c.rep;
-            const float r = over(l, it.len - it.rows + row);
-            F4 y;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y.v[i] = o[i] * r;
-            *reinterpret_cast<F4*>(a.out + (int64_t)(it.row0 + row) * a.out_pitch + (int64_t)head * hd + 4 * c4) = y;
-        }
+        if (run == 0 && in) store(pair, c4, o, l);
     }
 }
 

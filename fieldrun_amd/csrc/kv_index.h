@@ -21,7 +21,7 @@
 namespace frq {
 namespace kv {
 
-constexpr int ALIGN = 32;  // a sequence's first key of a window is rounded down to this
+constexpr int ALIGN = 32;  // a tile's first key of a window is rounded down to this
 
 struct Call {
     const int32_t* len;    // [n_seq] cached tokens
@@ -41,13 +41,13 @@ struct Call {
 struct Seq {
     int row0, rows;  // its rows of q
     int len;         // its keys
-    int lo, ext;     // the first key any row sees (rounded down), keys from there
+    int ext;         // keys that a tile of it spans, at most
     int tiles;       // 0: not served
     bool bad;        // its length or offsets are out of range
 };
 
 KV_HD Seq seq_of(const Call& c, int len, int r0, int r1) {
-    Seq q{r0, r1 - r0, len, 0, 0, 0, false};
+    Seq q{r0, r1 - r0, len, 0, 0, false};
     if (r0 < 0 || r1 < r0 || r1 > c.n_row) {
         q.row0 = q.rows = q.len = 0;
         q.bad = true;
@@ -60,11 +60,10 @@ KV_HD Seq seq_of(const Call& c, int len, int r0, int r1) {
     const int64_t pairs = (int64_t)q.rows * c.rep;
     if (pairs < c.min_pairs || pairs > c.max_pairs) return q;
     q.tiles = (int)((pairs + c.tp - 1) / c.tp);
-    if (c.window) {
-        const int64_t lo = (int64_t)q.len - q.rows - c.window + 1;
-        q.lo = lo > 0 ? (int)(lo / ALIGN * ALIGN) : 0;
-    }
-    q.ext = q.len - q.lo;
+    // its window and its rows after the first, and the rounding of tile_lo
+    const int most = (c.tp - 1) / c.rep + 2, rows = q.rows < most ? q.rows : most;
+    const int64_t span = (int64_t)c.window + rows - 1 + ALIGN - 1;
+    q.ext = c.window && span < q.len ? (int)span : q.len;
     return q;
 }
 KV_HD Seq seq_at(const Call& c, int s) {
@@ -107,8 +106,11 @@ constexpr int PLAN_SEQS = 64;
 KV_HD int64_t plan_words(int64_t n_seq) { return n_seq > PLAN_SEQS ? 2 + (n_seq + 63) / 64 * 2 : 0; }
 KV_HD int64_t max_slots(int64_t target, int n_kv) { return 2 * (target / n_kv + 1); }
 
-// The first key that the row at position pos sees (the last one is pos).
+// The first key that the row at position pos sees (the last one is pos), and
+// where the chunks of a tile begin whose first row is at pos.
 KV_HD int key_lo(const Call& c, int pos) { return c.window && pos - c.window + 1 > 0 ? pos - c.window + 1 : 0; }
+
+KV_HD int tile_lo(const Call& c, int pos) { return key_lo(c, pos) / ALIGN * ALIGN; }
 
 // A key's page id where the table holds one, else -1.
 KV_HD int page_ok(int id, int64_t n_pages) { return id >= 0 && (int64_t)id < n_pages ? id : -1; }

@@ -116,7 +116,8 @@ extern "C" int64_t plan(const int32_t* len, const int32_t* first, int n_seq, int
         const int m = chunks_of(q, klen);
         for (int t = 0; t < q.tiles; ++t)
             for (int k = 0; k < m; ++k) {
-                if (n < cap) out[n] = Row{s, t, k, m, q.row0, q.rows, q.len, q.lo, q.ext, even_chunk(q, m), m > 1 ? slots : -1};
+                if (n < cap) out[n] = Row{s, t, k, m, q.row0, q.rows, q.len,
+                                       tile_lo(c, q.len - q.rows + (int)((int64_t)t * tp / rep)), q.ext, even_chunk(q, m), m > 1 ? slots : -1};
                 ++n;
                 if (m > 1) ++slots;
             }
@@ -193,12 +194,14 @@ def test_items_cover_every_tile_and_key_once(host):
             tiles = [t for q, t in seen if q == s]
             assert sorted(tiles) == list(range(-(-pairs // tp) if served else 0))
         for (s, t), parts in seen.items():
-            lo = min(p.lo for p in parts)
-            assert lo % 32 == 0 and lo <= max(0, lens[s] - rows[s] - window + 1 if window else 0)
+            lo = parts[0].lo
+            first_pos = lens[s] - rows[s] + t * tp // rep
+            last_pos = lens[s] - rows[s] + (min((t + 1) * tp, rows[s] * rep) - 1) // rep
+            assert lo % 32 == 0 and lo <= max(0, first_pos - window + 1 if window else 0)
             assert parts[0].klen % 64 == 0 and (parts[0].klen >= least // 2 or len(parts) == 1)
             assert [p.chunk for p in parts] == list(range(parts[0].chunks))
-            assert lo + parts[0].chunks * parts[0].klen >= lens[s]
-            assert lo + (parts[0].chunks - 1) * parts[0].klen < max(1, lens[s])
+            assert lo + parts[0].chunks * parts[0].klen >= last_pos + 1
+            assert (parts[0].chunks - 1) * parts[0].klen < max(1, parts[0].ext)
 
 
 def test_bad_lengths_and_offsets_are_told(host):
