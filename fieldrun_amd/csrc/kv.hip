@@ -428,8 +428,10 @@ constexpr int64_t DEC_TARGET = 512;
 // Prompt items wanted: a round and not quite two a CU; more cost the joining
 // more than the balance gives (400, 640, 1024, 1536: kernel and join of 7 ragged
 // int8 prompts 123 + 8, 127 + 18, 110 + 24, 108 + 24 us; of 2048 rows over 8192
-// keys 503 + 5 at 400, 486 + 25 at 1024).
-constexpr int64_t PROMPT_TARGET = 400;
+// keys 503 + 5 at 400, 486 + 25 at 1024).  Where one workgroup fills a CU (over
+// 128 channels) less than a round: 189 rows of 32 heads of 256 over 2611 int8
+// keys 135 us at 400, 92 at 240.
+constexpr int64_t PROMPT_TARGET = 400, PROMPT_TARGET_WIDE = 240;
 // A sequence of up to so many (row, head) pairs is the decode kernel's (decode
 // against prompt kernel: 126 pairs over 1000 tokens 14.4, 31.3 us, over 8192
 // 27.9, 35.7, 8 times over 2000 45.5, 39.2; 252 pairs over 1000 15.2, 31.7, but
@@ -450,7 +452,12 @@ Plan plan_of(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq) {
     c.n_row = (int)n_row;
     c.rep = (int)(n_head / kv->n_kv);
     c.n_kv = (int)kv->n_kv;
-    c.min_chunk = 256;
+    // Two tiles a wave at least; prompts two or four a workgroup (256 instead: one
+    // f32 sequence of 959 tokens, 15 heads of 256, 27 us against 21; 108 f32 rows
+    // of 16 heads of 64 over 400 tokens 33 against 25.  f16 at 128: 113 sequences of
+    // up to 579 tokens 31 us against 26; prompts at 64: 4 sequences of 166 rows
+    // with a window of 8 42 us against 23).
+    c.min_chunk = kv->dtype == FRQ_DT_F32 ? 128 : 256;
     c.min_pairs = 1;
     c.max_pairs = 0x7FFFFFFF;
     c.tp = 16;
@@ -458,7 +465,9 @@ Plan plan_of(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq) {
     p.prompt = c;
     p.prompt.min_pairs = DEC_PAIRS + 1;
     p.prompt.tp = 128;
-    p.prompt.target = n_row > n_seq ? PROMPT_TARGET : 1;  // no room for parts: every tile's keys in one run
+    // (n_row <= n_seq: no room for parts, every tile's keys in one run)
+    p.prompt.target = n_row <= n_seq ? 1 : kv->hd > 128 ? PROMPT_TARGET_WIDE : PROMPT_TARGET;
+    p.prompt.min_chunk = 128;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t r = at;
@@ -468,7 +477,7 @@ Plan plan_of(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq) {
     p.rec_dec = take((size_t)max_items(p.dec) * sizeof(Record));
     p.rec_prompt = take((size_t)max_items(p.prompt) * sizeof(Record));
     p.part_dec = take((size_t)max_slots(DEC_TARGET, c.n_kv) * c.n_kv * 16 * (kv->hd + 2) * 4);
-    p.part_prompt = take(n_row > n_seq ? (size_t)max_slots(PROMPT_TARGET, c.n_kv) * c.n_kv * 128 * (kv->hd + 2) * 4 : 0);
+    p.part_prompt = take(n_row > n_seq ? (size_t)max_slots(p.prompt.target, c.n_kv) * c.n_kv * 128 * (kv->hd + 2) * 4 : 0);
     p.plan_dec = take((size_t)plan_words(c.n_seq) * 4);
     p.plan_prompt = take((size_t)plan_words(c.n_seq) * 4);
     p.bytes = at;
@@ -593,7 +602,7 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_p
     b.c.min_chunk = plan.prompt.min_chunk;
     b.rec = (Record*)(ws + plan.rec_prompt);
     b.part = (float*)(ws + plan.part_prompt);
-    b.slots = n_row > n_seq ? max_slots(PROMPT_TARGET, a.c.n_kv) : 0;
+    b.slots = n_row > n_seq ? max_slots(b.c.target, a.c.n_kv) : 0;
     const int64_t ga = max_items(a.c) * a.c.n_kv, gb = prompts ? max_items(b.c) * b.c.n_kv : 0;
     if (ga + gb > 0x7FFFFFFF) return bad("too many rows or sequences");
     const Launch la{(unsigned)ga, s}, lb{(unsigned)gb, s};

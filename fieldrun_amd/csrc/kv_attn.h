@@ -114,6 +114,15 @@ __device__ __forceinline__ int64_t wave_total(int64_t v) {
     return lane_bcast(v + (int64_t)xshfl64<32>(v), 0);
 }
 
+__device__ __forceinline__ int wave_most(int v) {
+    v = max(v, (int)xshfl<1>(v));
+    v = max(v, (int)xshfl<2>(v));
+    v = max(v, (int)xshfl<4>(v));
+    v = max(v, (int)xshfl<8>(v));
+    v = max(v, (int)xshfl<16>(v));
+    return uni(max(v, (int)xshfl<32>(v)));
+}
+
 // Finds item `id`, each wave by itself: up to 64 sequences from their lengths
 // and offsets alone, first the call's keys (the chunk length), then the items
 // before; more from the call's plan, which holds the chunk length and the
@@ -146,16 +155,11 @@ __device__ __forceinline__ Item find_item(const Call& c, int id, int* err) {
     if (s0 + lane < c.n_seq) q = seq_at(c, s0 + lane);
     if (!c.plan) {
         if (q.bad && id == 0 && threadIdx.x < 64) atomicOr(err, ERR_INDEX);
-        klen = chunk_of(c, c.n_seq > 1 ? wave_total(keys_of(q)) : lane_bcast(keys_of(q), 0));
+        const int64_t total = c.n_seq > 1 ? wave_total(keys_of(q)) : lane_bcast(keys_of(q), 0);
+        klen = chunk_of(c, total);
     }
     const int n = q.tiles ? chunks_of(q, klen) : 1, own = even_chunk(q, n), mine = q.tiles * n;
-    int most = own;
-    most = max(most, (int)xshfl<1>(most));
-    most = max(most, (int)xshfl<2>(most));
-    most = max(most, (int)xshfl<4>(most));
-    most = max(most, (int)xshfl<8>(most));
-    most = max(most, (int)xshfl<16>(most));
-    most = max(most, (int)xshfl<32>(most));
+    const int most = wave_most(own);
     const bool first = own > most / 2;
     const int parts = n > 1 ? mine : 0;
     const int a = lane_sums(first ? mine : 0), b = lane_sums(first ? 0 : mine);

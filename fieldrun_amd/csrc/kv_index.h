@@ -34,7 +34,7 @@ struct Call {
     int tp;                // pairs a tile
     int min_pairs, max_pairs;  // the sequences served: pairs in [min, max]
     int64_t target;        // items wanted over all kv heads
-    int min_chunk;         // keys a chunk at least, a multiple of ALIGN
+    int min_chunk;         // keys a chunk at least, 64, 128 or 256
     const int32_t* plan;   // of many sequences: the chunk length and 0, then before each 64 sequences (items, slots)
 };
 
@@ -71,23 +71,30 @@ KV_HD Seq seq_at(const Call& c, int s) {
 }
 KV_HD int64_t keys_of(const Seq& q) { return (int64_t)q.tiles * q.ext; }
 
-// Keys a chunk when the call's tiles read `total` keys a kv head.
+// Keys a chunk when the call's tiles read `total` keys a kv head.  (32-bit
+// divisions wherever the numbers allow: a 64-bit one is a hundred instructions
+// and more, in every workgroup.)
+constexpr int MOST = 0x7FFFFFFF / 64 * 64;
+KV_HD int round_keys(uint32_t keys, int step) {  // up to a multiple of step, a power of two up to 256
+    const uint32_t up = (keys + (uint32_t)step - 1) & ~((uint32_t)step - 1);
+    return up > (uint32_t)MOST ? MOST : (int)up;
+}
 KV_HD int chunk_of(const Call& c, int64_t total) {
-    const int64_t per = (total * c.n_kv + c.target - 1) / c.target;
-    const int64_t up = (per + c.min_chunk - 1) / c.min_chunk * c.min_chunk, most = 0x7FFFFFFF / ALIGN * ALIGN;
-    return (int)(up < c.min_chunk ? c.min_chunk : up > most ? most : up);
+    const uint64_t x = (uint64_t)total * (uint64_t)c.n_kv + (uint64_t)c.target - 1;
+    const uint64_t per = x >> 32 ? x / (uint64_t)c.target : (uint64_t)((uint32_t)x / (uint32_t)c.target);
+    const int up = round_keys(per > (uint64_t)MOST ? (uint32_t)MOST : (uint32_t)per, c.min_chunk);
+    return up < c.min_chunk ? c.min_chunk : up;
 }
 KV_HD int chunks_of(const Seq& q, int chunk) {
-    const int n = (int)(((int64_t)q.ext + chunk - 1) / chunk);
+    const int n = (int)(((uint32_t)q.ext + (uint32_t)chunk - 1) / (uint32_t)chunk);
     return n < 1 ? 1 : n;
 }
 // A sequence's own chunk: its keys in n runs of equal length, whole STEPs.
 constexpr int STEP = 64;
 KV_HD int even_chunk(const Seq& q, int n) {
-    const int64_t per = ((int64_t)q.ext + n - 1) / n, up = (per + STEP - 1) / STEP * STEP;
-    return up > 0x7FFFFFFF ? 0x7FFFFFFF / STEP * STEP : up < STEP ? STEP : (int)up;
+    const int up = round_keys(((uint32_t)q.ext + (uint32_t)n - 1) / (uint32_t)n, STEP);
+    return up < STEP ? STEP : up;
 }
-
 // Host bounds.  Tiles: sum of ceil(rows rep / tp) <= n_row rep / tp + n_seq,
 // and no more than a sequence of max_pairs has for each;
 // items: sum of tiles ceil(ext / chunk) <= tiles + total / chunk and
