@@ -707,6 +707,15 @@ __device__ __forceinline__ int pick4(int j, int a, int b, int c, int d) {
 // LDS rows are cut into 16-byte pieces, piece c of row r at c ^ (r mod a power
 // of two), so that the 32 rows a read takes the same piece of lie in
 // different banks.
+//
+// Bound by the matrix cores, and by the clock under them (1.7 GHz, the cores
+// busy half the time): f16, 28 heads of 128 channels over 4, 2048 rows after
+// 6144 cached tokens, is 210 GFLOP of the formula, which the two halves of q
+// and p make 420, in 490 us; int8, 7 sequences of up to 1501 tokens, 24 GFLOP,
+// in 111.  One f16 for p would cost its bits below 2^-11.  128 pairs a workgroup
+// let two fit a CU (64 KB of LDS, 256 registers); equal priorities of both 503 us
+// against 481.
+//
 // An f32 cache is staged as three bf16 (exact: 8 bits each), q and the
 // probabilities likewise, and a product is the six of theirs that reach 2^-24
 // of it: six matrix instructions, where the f32 ones would take the time of
@@ -1217,7 +1226,9 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
 // outputs, so that a long sequence's parts are read by many workgroups.
 // Threads are (float4 of the share, run of chunks); each folds its chunks,
 // then the runs are merged pairwise, always in the same order.  Bound by
-// latency: 4.5 to 5.3 us at 60 to 280 chunks of 16 pairs of 128 channels.
+// latency: 4.5 to 5.5 us at 60 to 280 chunks of 16 pairs of 128 channels, 11 us for
+// 7 prompts' 128 pairs (a float4 a thread at a time: 585 rows of 8 heads of 256
+// 64 us in all against 57).
 template <int TP>
 __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so, float* sm, float* sl) {
     const int n_kv = a.c.n_kv, kvh = block % n_kv;
