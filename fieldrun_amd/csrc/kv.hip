@@ -14,10 +14,6 @@ namespace frq {
 namespace kv {
 namespace {
 
-// Rows a workgroup of the write and read kernels (64, whole lines of int8
-// values, were slower for their fewer waves: 8192 rows of 4 heads of 128
-// written in 19.4 us against 16.8, read in 11.2 against 9.7).
-constexpr int WR = 32;
 constexpr int MAX_HD = 256;
 
 struct Move {
@@ -50,12 +46,14 @@ __device__ __forceinline__ int8_t q8(float x, float step, float inv) {
 
 // The places of the workgroup's rows: page (or -1: no place) and offset; then
 // which fours of rows lie side by side in a page.
+template <int WR>
 struct Places {
     int64_t pg[WR];
     int off[WR];
     int four[WR / 4];
 };
-__device__ __forceinline__ void find_places(const Move& m, int64_t r0, int64_t slot, Places& p) {
+template <int WR>
+__device__ __forceinline__ void find_places(const Move& m, int64_t r0, int64_t slot, Places<WR>& p) {
     const int r = threadIdx.x;
     if (r < WR) {
         int64_t pg = -1;
@@ -118,14 +116,14 @@ __device__ __forceinline__ void to_lds(E* p, const Quad<E>& q) {
 // (2.5 TB/s: the values' pieces are half lines), back in 9.7 (4.3 TB/s); one token,
 // 2.6 us, by latency.  (A token at a time both ways 29.5 us against 25.1, calls
 // included.)
-template <int DT, int G>
+template <int DT, int G, int WR>
 __global__ __launch_bounds__(256) void kv_write_kernel(const Move m) {
     using E = Elem<DT>;
     constexpr bool I8 = DT == FRQ_DT_ROWI8;
     constexpr int RP = 256 / G < WR ? 256 / G : WR, NP = WR / RP;  // rows a pass, passes
     constexpr int LP = lds_row<E>();
     __shared__ __align__(16) E lv[4 * G * LP];
-    __shared__ Places at;
+    __shared__ Places<WR> at;
     const int kvh = blockIdx.x % m.n_kv, hd = m.kv.hd, page = m.kv.page;
     const int64_t r0 = (int64_t)(blockIdx.x / m.n_kv) * WR;
     const int tid = threadIdx.x, c = 4 * (tid % G), pr = tid / G;
@@ -203,14 +201,14 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const Move m) {
 
 // The way back: keys by rows, values by fours of tokens into LDS and from
 // there by rows.
-template <int DT, int G>
+template <int DT, int G, int WR>
 __global__ __launch_bounds__(256) void kv_read_kernel(const Move m) {
     using E = Elem<DT>;
     constexpr bool I8 = DT == FRQ_DT_ROWI8;
     constexpr int RP = 256 / G < WR ? 256 / G : WR, NP = WR / RP;
     constexpr int LP = lds_row<E>();
     __shared__ __align__(16) E lv[4 * G * LP];
-    __shared__ Places at;
+    __shared__ Places<WR> at;
     const int kvh = blockIdx.x % m.n_kv, hd = m.kv.hd, page = m.kv.page;
     const int64_t r0 = (int64_t)(blockIdx.x / m.n_kv) * WR;
     const int tid = threadIdx.x, c = 4 * (tid % G), pr = tid / G;
@@ -391,7 +389,7 @@ int check_rows(const frq_kv* h, const void* k, const void* v, size_t pitch, cons
     if (int rc = check(h, &m->kv, &m->shift)) return rc;
     if (n && (!k || !v || !slot)) return bad("null pointer");
     if (pitch < h->n_kv * h->hd || pitch > ((size_t)1 << 40)) return bad("pitch is below the kv heads' width");
-    if (n > ((size_t)1 << 31) || (n + WR - 1) / WR * h->n_kv > 0x7FFFFFFF) return bad("too many rows");
+    if (n > ((size_t)1 << 31) || (n + 31) / 32 * h->n_kv > 0x7FFFFFFF) return bad("too many rows");
     m->slot = slot;
     m->n = (int64_t)n;
     m->pitch = (int64_t)pitch;
@@ -399,25 +397,38 @@ int check_rows(const frq_kv* h, const void* k, const void* v, size_t pitch, cons
     return FRQ_OK;
 }
 
-template <bool WRITE, int DT>
-void launch_move_g(const Move& m, const dim3& g, hipStream_t s) {
-    const dim3 b(256);
+// Rows a workgroup: 32, or 8 where workgroups of 32 leave the chip unfilled and
+// the latency of one bounds the call (61 f32 rows of 5 heads of 80 written in
+// 3.9 us against 5.0 and read in 3.8 against 5.1; there and back with the calls:
+// 1500 int8 rows of 4 heads of 128, 188 workgroups of 32, 10.1 us against 14.1).
+// More calls for 32: 1500 f32 rows of 5 heads of 256, 235 workgroups, 20.5 us
+// against 23.0; 8192 int8 rows read in 9.6 against 13.8 (at 64, whole lines of
+// int8 values, 11.2, and written in 19.4 against 16.6).
+template <bool WRITE, int DT, int WR>
+void launch_move_g(const Move& m, int64_t groups, hipStream_t s) {
+    const dim3 g((unsigned)groups), b(256);
     auto go = [&](auto lanes) {
         constexpr int G = decltype(lanes)::value;
-        if constexpr (WRITE) kv_write_kernel<DT, G><<<g, b, 0, s>>>(m);
-        else kv_read_kernel<DT, G><<<g, b, 0, s>>>(m);
+        if constexpr (WRITE) kv_write_kernel<DT, G, WR><<<g, b, 0, s>>>(m);
+        else kv_read_kernel<DT, G, WR><<<g, b, 0, s>>>(m);
     };
     if (m.kv.hd <= 32) go(std::integral_constant<int, 8>{});
     else if (m.kv.hd <= 64) go(std::integral_constant<int, 16>{});
     else if (m.kv.hd <= 128) go(std::integral_constant<int, 32>{});
     else go(std::integral_constant<int, 64>{});
 }
+template <bool WRITE, int DT>
+void launch_move_r(const Move& m, hipStream_t s) {
+    const int64_t groups = (m.n + 31) / 32 * m.n_kv;
+    constexpr int64_t few = DT == FRQ_DT_F32 ? 128 : 256;
+    if (groups < few) launch_move_g<WRITE, DT, 8>(m, (m.n + 7) / 8 * m.n_kv, s);
+    else launch_move_g<WRITE, DT, 32>(m, groups, s);
+}
 template <bool WRITE>
 hipError_t launch_move(const Move& m, int dtype, hipStream_t s) {
-    const dim3 g((unsigned)((m.n + WR - 1) / WR * m.n_kv));
-    if (dtype == FRQ_DT_F32) launch_move_g<WRITE, FRQ_DT_F32>(m, g, s);
-    else if (dtype == FRQ_DT_F16) launch_move_g<WRITE, FRQ_DT_F16>(m, g, s);
-    else launch_move_g<WRITE, FRQ_DT_ROWI8>(m, g, s);
+    if (dtype == FRQ_DT_F32) launch_move_r<WRITE, FRQ_DT_F32>(m, s);
+    else if (dtype == FRQ_DT_F16) launch_move_r<WRITE, FRQ_DT_F16>(m, s);
+    else launch_move_r<WRITE, FRQ_DT_ROWI8>(m, s);
     return hipGetLastError();
 }
 
