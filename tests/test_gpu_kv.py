@@ -604,3 +604,34 @@ def test_captured_and_replayed(ctx):
         last = outs[0]
     for g in graphs:
         g.close()
+
+
+def test_many_sequences_captured(ctx):
+    """A call of decode and prompt rows of 150 sequences in a graph, replayed
+    over changing lengths and queries with eager calls between."""
+    rng = np.random.default_rng(12)
+    lens = [int(x) for x in rng.integers(1, 80, 150)]
+    rows = [1] * 150
+    lens[3], lens[70], lens[149], rows[70], rows[149] = 1500, 700, 400, 50, 90
+    b = Batch(ctx, "f16", 16, 2, 4, 32, lens, rows, seed=4)
+    b.check()
+    graph = Graph(ctx, b.call)
+    held, last = list(b.lens), None
+    for i in range(4):
+        b.lens = [max(1, n - 7 * i) if r == 1 else n - 20 * i for n, r in zip(held, rows)]
+        put(b.dev[1], np.array(b.lens, np.int32))
+        b.q = rng.standard_normal(b.q.shape).astype(np.float32)
+        put(b.dq, b.q.reshape(b.dq.shape))
+        outs = []
+        for how in (graph.replay, b.call, graph.replay):
+            put(b.do, np.full(b.do.shape, 7.0, np.float32))
+            how()
+            ctx.sync()
+            outs.append(b.do.numpy())
+        assert all(same(o, outs[0]) for o in outs[1:])
+        b.k, b.v = [k[:n] for k, n in zip(b.k, b.lens)], [v[:n] for v, n in zip(b.v, b.lens)]
+        want, tol = b.want()
+        assert (np.abs(outs[0][:b.n_row].reshape(want.shape) - want) <= tol).all()
+        assert last is None or not same(outs[0], last)
+        last = outs[0]
+    graph.close()
