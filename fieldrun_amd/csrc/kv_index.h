@@ -4,10 +4,10 @@
 // A call's work is cut into items: a tile of `tp` (query row, head) pairs of
 // one sequence and kv head times a run of `chunk` of its keys.  Lengths and row
 // offsets are device data, so every workgroup finds its own item from them:
-// the chunk length follows from the whole call's keys (kv_chunk), the items
+// the chunk length follows from the whole call's keys (chunk_of), the items
 // are numbered sequence after sequence, and the grid is the host's bound of
-// their number (kv_max_items).  A sequence cut into several chunks leaves
-// partial results in slots, at most kv_max_slots.
+// their number (max_items).  A tile cut into several chunks leaves partial
+// results in slots, at most max_slots.
 #pragma once
 
 #include <stdint.h>
