@@ -159,6 +159,17 @@ def _context():
     return _ctx
 
 
+def _take_stream():
+    """The program has one stream: the context's, which waits for no other,
+    becomes torch's current one.  So inputs are there when a call reads them,
+    what torch does with the outputs comes behind the call, and freed memory is
+    not given away under it."""
+    stream = _context()[1]
+    if torch.cuda.current_stream() != stream:
+        stream.wait_stream(torch.cuda.current_stream())
+        torch.cuda.set_stream(stream)
+
+
 def _handle(case, k, v, ks, vs):
     import fieldrun_amd as fa
     at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
@@ -167,6 +178,8 @@ def _handle(case, k, v, ks, vs):
 
 
 def prepare(case, seed):
+    if own:
+        _take_stream()
     g = torch.Generator(device="cuda")
     g.manual_seed(int(seed) & 0x7FFFFFFF)
     if case["kind"] == "norm":
@@ -307,14 +320,13 @@ def run(state):
         return state["out"]
     if not own:
         return _plain_norm(state)
-    ctx, stream = _context()
+    ctx = _context()[0]
     x, y, a8, sa = state["x"], state["y"], state["a8"], state["sa"]
     total = x if y is None else state["sum"]
     ctx.norm_quant_dev(x.data_ptr(), None if y is None else y.data_ptr(), state["w"].data_ptr(), EPS, x.shape[0],
                        x.shape[1], None if y is None else total.data_ptr(), a8.data_ptr(), sa.data_ptr(),
                        state["index"].data_ptr(), state["outlier"].data_ptr())
-    with torch.cuda.stream(stream):
-        values = a8[:, :x.shape[1]] * sa[:, None]  # what the bytes stand for
+    values = a8[:, :x.shape[1]] * sa[:, None]  # what the bytes stand for
     return {"sum": total, "values": values, "sa": sa, "index": state["index"], "outlier": state["outlier"]}
 
 
