@@ -415,27 +415,29 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
     uint32_t odd = 0;
     const bool alike = lo_a == lo_b && pos_a == pos_b;  // every pair sees the same
 
-    // the page ids of a tile's two halves, loaded a tile ahead of the loads
-    // that use them; a bad one reads page 0 and is told at the end
-    int pid[2], nid[2];
+    // the page ids of a tile's 16-token groups, loaded a tile ahead of the loads
+    // that use them.  A bad one reads page 0; it is told at the end where a row
+    // sees a key of the group (pages are of 16 tokens and more, a tile begins at
+    // a multiple of 32: a page wholly before the window may be gone)
+    int pid[NU], nid[NU];
     bool bad = false;
     auto ids = [&](int base) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) nid[h] = table[min((base + 16 * h) >> shift, last_page)];
+        for (int h = 0; h < NU; ++h) nid[h] = table[min((base + 16 * h) >> shift, last_page)];
     };
-    auto pages = [&]() {
+    auto pages = [&](int base) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int id = page_ok(nid[h], a.kv.n_pages);
-            bad |= id < 0;
-            pid[h] = __builtin_amdgcn_readfirstlane(max(id, 0));
+        for (int h = 0; h < NU; ++h) {
+            const int id = uni(page_ok(nid[h], a.kv.n_pages));
+            bad |= id < 0 && base + 16 * h + 15 >= lo_a && base + 16 * h <= pos_b;
+            pid[h] = max(id, 0);
         }
     };
     auto load_k = [&](int base) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
             const int d = T::F32 ? col : 8 * (col >> 2) + 4 * u + (col & 3);
-            const int64_t pg = d >= 16 ? pid[1] : pid[0];
+            const int64_t pg = d >= 16 ? pid[NU - 1] : pid[0];
             const char* p = kb + pg * a.kv.stride + (int64_t)((base + d) & (page - 1)) * hd * T::SZ;
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
@@ -444,14 +446,14 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
             }
         }
         if constexpr (T::I8) {
-            const int64_t pg = g >= 2 ? pid[1] : pid[0];
+            const int64_t pg = g >= 2 ? pid[NU - 1] : pid[0];
             const float* p = a.kv.ks + pg * a.kv.sstride + kvh * page + ((base + 8 * g) & (page - 1));
 #pragma unroll
             for (int j = 0; j < 8; j += 4) *reinterpret_cast<f4*>(ksc + j) = *reinterpret_cast<const f4*>(p + j);
         }
     };
     auto load_v = [&](int base) {
-        const int64_t pg = T::PL * g >= 16 ? pid[1] : pid[0];
+        const int64_t pg = T::PL * g >= 16 ? pid[NU - 1] : pid[0];
         const int at = (base + T::PL * g) & (page - 1);
         const char* p = vb + pg * a.kv.stride + ((int64_t)col * page + at) * T::SZ;
 #pragma unroll
@@ -465,7 +467,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
     };
     if (wave < tiles) {
         ids(beg + wave * KT);
-        pages();
+        pages(beg + wave * KT);
         ids(beg + (wave + NW) * KT);
         load_k(beg + wave * KT);
         load_v(beg + wave * KT);
@@ -509,7 +511,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
             for (int j = 0; j < 8; ++j) vcur[j] = vsc[j];
         }
         if (more) {
-            pages();
+            pages(next);
             ids(next + NW * KT);
             load_k(next);
         }
@@ -841,6 +843,8 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     const float scl = fmaxf(__builtin_ldexpf(a.scale, qe), 1.17549435e-38f);
     const float mul = capped ? 1.0f : scl * LOG2E, rcap = capped ? scl / a.cap : 0.0f;
 
+    const int wlo_a = key_lo(a.c, wpos_a), wlo_b = key_lo(a.c, wpos_b);
+
     // ---- staging: this thread's pieces (the same place in every tile)
     const int32_t* table = a.pages + (int64_t)it.seq * a.pages_pitch;
     const int last_page = max(0, it.q.len - 1) >> shift;
@@ -850,7 +854,8 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     // pieces of the keys are KT / 4 whole rows, one page's; its pieces of the
     // values hold the same 8 tokens of different channels.  Page ids are
     // scalar, loaded a tile ahead of the loads that use them and looked at
-    // only there; a bad one reads page 0 and is told at the end.
+    // only there; a bad one reads page 0 and is told at the end where a row of
+    // the workgroup sees a key of its group.
     static_assert(64 / P::VC % P::VC == 0 && IPW * 64 * 4 == KT * P::KC && KT / 4 <= 16, "");
     constexpr int VR = 64 / P::VC;                        // channels a wave's piece takes
     const int vr0 = (wave * IPW * 64 + lane) / P::VC;     // channel of piece 0
@@ -865,16 +870,19 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
             g3 = table[min((base + 48) >> shift, last_page)];
         }
     };
-    auto page_of = [&](int id) -> int64_t {
-        const int ok = page_ok(id, a.kv.n_pages);
-        bad |= ok < 0;
-        return max(ok, 0);
+    auto page_of = [&](int id) -> int64_t { return max(page_ok(id, a.kv.n_pages), 0); };
+    auto look = [&](int base) {
+#pragma unroll
+        for (int h = 0; h < KT / 16; ++h)
+            bad |= page_ok(pick4(h, g0, g1, g2, g3), a.kv.n_pages) < 0 && base + 16 * h + 15 >= wlo_a &&
+                   base + 16 * h <= wpos_b;
     };
     using Raw = std::conditional_t<I8, u2, u4>;
     constexpr int NR = F32 ? 2 : 1;  // loads a piece
     Raw rk[F16 ? 1 : IPW][NR], rv[F16 ? 1 : IPW][NR];
     float rs = 0.0f;
     auto fetch = [&](int base, int buf) {
+        look(base);
         int ln = lane;
         asm volatile("" : "+v"(ln));  // addresses are formed anew for every tile, not held over the products
         const int r0 = wave * (IPW * VR) + ln / P::VC, tok = 8 * ((ln % P::VC) ^ (r0 & P::VX));
@@ -912,7 +920,6 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     // zero probability would carry them to pairs that do not see them) are
     // zeroed; the second are noted and given to their pairs after the loop.
     // (int8 values are finite, and a key that is not seen has weight zero.)
-    const int wlo_a = key_lo(a.c, wpos_a), wlo_b = key_lo(a.c, wpos_b);
     auto land = [&](int base, int buf) {
         const bool edge = base < wlo_b || base + KT - 1 > wpos_a;
         if constexpr (I8) {
@@ -1159,7 +1166,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
         if (ti + 1 < tiles) land(base + KT, other);
         __syncthreads();
     }
-    if (bad) atomicOr(a.err, ERR_INDEX);
+    if (bad && tid == 0) atomicOr(a.err, ERR_INDEX);
     if constexpr (!I8) {
         if (flag) {  // rare: the keys of those tiles again, one by one (the last barrier was after the last note)
             for (int key = beg; key < end; ++key) {

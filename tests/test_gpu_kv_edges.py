@@ -1,0 +1,79 @@
+"""The paged attention where a call is allowed and unusual: pages that are gone
+or out of range, scores, caps and values of any size, entries that are not
+finite.  Held to the definition in 64 bits as test_gpu_kv.py holds the rest;
+its tolerance is derived there."""
+import numpy as np
+import pytest
+
+import fieldrun_amd as fa
+from fieldrun_amd import hip
+from test_gpu_kv import Batch, put
+
+pytestmark = pytest.mark.gpu
+KINDS = ["f32", "f16", "rowi8"]
+
+
+def expect(b, gone=None, scale=None, cap=0.0, window=0):
+    """Outputs and tolerances of batch b, the keys of gone ({sequence: keys})
+    left out; a row that sees no key is zeros."""
+    kv, hd, rep, kind = b.p.kv, b.p.hd, b.rep, b.p.kind
+    scale = hd ** -0.5 if scale is None else scale
+    out = np.zeros((b.n_row, kv * rep, hd))
+    tol = np.zeros_like(out)
+    u = 2.0 ** -24
+    for s, n in enumerate(b.lens):
+        for i in range(b.rows[s]):
+            p = n - b.rows[s] + i
+            keys = np.arange(max(0, p - window + 1) if window else 0, p + 1)
+            keys = np.setdiff1d(keys, list((gone or {}).get(s, ())))
+            if not len(keys):
+                continue
+            r = int(b.first[s]) + i
+            for h in range(kv):
+                k, v = (x[s][keys, h].astype(np.float64) for x in (b.k, b.v))
+                q = b.q[r, h * rep:(h + 1) * rep].astype(np.float64)
+                z = scale * (q @ k.T)
+                d = u * (4 * hd ** 0.5 + 8) * abs(scale) * (np.abs(q) @ np.abs(k).T).max(1)
+                if kind != "f32":
+                    d += 2.0 ** -22 * abs(scale) * np.abs(q).max(1) * np.abs(k).sum(1).max()
+                if cap:
+                    z = cap * np.tanh(z / cap)
+                    d += 4e-7 * np.abs(z).max(1)
+                w = np.exp(z - z.max(1, keepdims=True))
+                w /= w.sum(1, keepdims=True)
+                at = slice(h * rep, (h + 1) * rep)
+                out[r, at] = w @ v
+                tol[r, at] = (np.expm1(2 * d) + 2.0 ** -21 + u * (len(keys) / 16 + 16))[:, None] * (w @ np.abs(v))
+                tol[r, at] += (2.0 ** (-126 if kind == "f32" else -35) * w.max(1) * len(keys))[:, None] * np.abs(
+                    v[np.isfinite(v)]).max()
+    return out, tol
+
+
+def hold(got, want, tol):
+    off = np.abs(got - want)
+    bad = ~(off <= tol)
+    assert not bad.any(), (np.argwhere(bad)[:4], got[bad][:4], want[bad][:4], tol[bad][:4])
+
+
+def set_table(b, table):
+    put(b.dev[0], np.ascontiguousarray(table, np.int32))
+
+
+# ---- pages ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("window", [1, 16, 33])
+@pytest.mark.parametrize("many", [False, True])
+def test_pages_before_the_window_may_be_gone(ctx, kind, window, many):
+    """A program frees the pages that no later row sees and marks them -1: no
+    error and the same outputs, whatever place in its page the window begins
+    at (every length mod 32), decode rows and prompt rows."""
+    lens = [300 + i for i in range(32)] * (3 if many else 1) + [5, 1001, 16]
+    for rows in (None, [(1, 2, 50)[i % 3] for i in range(len(lens) - 3)] + [1, 60, 16]):
+        b = Batch(ctx, kind, 16, 1, 3, 64, lens, rows, seed=window)
+        table = b.table.copy()
+        for s, n in enumerate(lens):
+            table[s, :max(0, n - b.rows[s] - window + 1) // 16] = -1
+        assert (table[:, 0] == -1).sum() >= len(lens) - 3
+        set_table(b, table)
+        hold(b.run(window=window), *expect(b, window=window))
