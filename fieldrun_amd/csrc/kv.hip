@@ -594,6 +594,7 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_p
     a.scale = scale == 0.0 ? 1.0f : (float)(scale < 0.0 ? -scale : scale);
     a.sign = scale == 0.0 ? 0.0f : scale < 0.0 ? -1.0f : 1.0f;
     a.cap = (float)cap;
+    a.dtype = kv->dtype;
     // Each sequence is served by the kernel of its number of pairs; one that
     // no sequence can be for is not launched.
     // (f32 keys of over 128 channels stay with the decode kernel: three parts of

@@ -53,9 +53,10 @@ struct Cache {  // frq_kv as the kernels take it
     int page, hd;
 };
 
-// An item as the joining launch reads it (chunks 1: nothing to join).
+// An item as the joining launch reads it (chunks 1: nothing to join; seq: its
+// complement where a row sees a key under a page id out of range).
 struct Record {
-    int row0, rows, tile, chunk, chunks, slot, len, pad;
+    int row0, rows, tile, chunk, chunks, slot, len, seq;
 };
 struct Args {
     Call c;
@@ -69,6 +70,7 @@ struct Args {
     int64_t slots;
     int* err;
     float scale, sign, cap;  // |scale| and the sign that q takes (0: scale 1)
+    int dtype;
 };
 
 // An item's place: its sequence, tile and chunk; every lane has the same.
@@ -112,6 +114,17 @@ __device__ __forceinline__ int64_t wave_total(int64_t v) {
     v += (int64_t)xshfl64<8>(v);
     v += (int64_t)xshfl64<16>(v);
     return lane_bcast(v + (int64_t)xshfl64<32>(v), 0);
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+    auto step = [&](uint32_t o) { v += __uint_as_float(o); };
+    step(xshfl<1>(__float_as_uint(v)));
+    step(xshfl<2>(__float_as_uint(v)));
+    step(xshfl<4>(__float_as_uint(v)));
+    step(xshfl<8>(__float_as_uint(v)));
+    step(xshfl<16>(__float_as_uint(v)));
+    step(xshfl<32>(__float_as_uint(v)));
+    return v;
 }
 
 __device__ __forceinline__ int wave_most(int v) {
@@ -186,7 +199,14 @@ __device__ __forceinline__ Item find_item(const Call& c, int id, int* err) {
 
 __device__ __forceinline__ void note_item(Record* r, int id, const Item& it) {
     if (threadIdx.x == 0)
-        r[id] = Record{it.q.row0, it.q.rows, it.tile, it.chunk, it.found ? it.chunks : 1, it.slot, it.q.len, 0};
+        r[id] = Record{it.q.row0, it.q.rows, it.tile, it.chunk, it.found ? it.chunks : 1, it.slot, it.q.len, it.seq};
+}
+
+__device__ __forceinline__ void note_hole(const Args& a, int id, int seq) {
+    if (threadIdx.x == 0) {
+        atomicOr(a.err, ERR_INDEX);
+        if (blockIdx.x % a.c.n_kv == 0) a.rec[id].seq = ~seq;  // as note_item; every kv head finds the same
+    }
 }
 
 __device__ __forceinline__ float fmax16(float v) {  // over the four lane groups of a pair
@@ -202,6 +222,19 @@ __device__ __forceinline__ float fsum16(float v) {
 // zeros, one whose scores are all -inf is NaN, as the formula has it.
 __device__ __forceinline__ float over(float l, int pos) {
     return l > 0.0f || l != l ? 1.0f / l : pos < 0 ? 0.0f : __builtin_nanf("");
+}
+
+// The loops read page 0 for a page id out of range.  Such an id is an error
+// where a row would see a key under it (pages are of 16 tokens and more, a tile
+// begins at a multiple of 32: a page wholly before the window may be gone).
+// Then the tile's results are formed anew behind the joining, without those
+// keys: a chunk says so by this in the place of its sums.
+constexpr float HOLE = -1.0f;
+__device__ __forceinline__ bool page_bad(const Args& a, int seq, int lo, int hi) {
+    const int32_t* table = a.pages + (int64_t)seq * a.pages_pitch;
+    for (int pg = lo >> a.c.shift; lo <= hi && pg <= hi >> a.c.shift; ++pg)
+        if (page_ok(table[pg], a.kv.n_pages) < 0) return true;
+    return false;
 }
 
 // tanh to about 2e-7 of its value: a polynomial near zero, where
@@ -371,6 +404,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
     constexpr int ORow = HD + 4;
     __shared__ float red[NW / 2][16][ORow];
     __shared__ float stat[NW][16][2];
+    __shared__ int holes[NW];
     const int n_kv = a.c.n_kv;
     const int kvh = blockIdx.x % n_kv;
     const Item it = find_item(a.c, blockIdx.x / n_kv, a.err);
@@ -415,29 +449,27 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
     uint32_t odd = 0;
     const bool alike = lo_a == lo_b && pos_a == pos_b;  // every pair sees the same
 
-    // the page ids of a tile's 16-token groups, loaded a tile ahead of the loads
-    // that use them.  A bad one reads page 0; it is told at the end where a row
-    // sees a key of the group (pages are of 16 tokens and more, a tile begins at
-    // a multiple of 32: a page wholly before the window may be gone)
-    int pid[NU], nid[NU];
+    // the page ids of a tile's two halves, loaded a tile ahead of the loads
+    // that use them; a bad one reads page 0 and is looked into at the end
+    int pid[2], nid[2];
     bool bad = false;
     auto ids = [&](int base) {
 #pragma unroll
-        for (int h = 0; h < NU; ++h) nid[h] = table[min((base + 16 * h) >> shift, last_page)];
+        for (int h = 0; h < 2; ++h) nid[h] = table[min((base + 16 * h) >> shift, last_page)];
     };
-    auto pages = [&](int base) {
+    auto pages = [&]() {
 #pragma unroll
-        for (int h = 0; h < NU; ++h) {
-            const int id = uni(page_ok(nid[h], a.kv.n_pages));
-            bad |= id < 0 && base + 16 * h + 15 >= lo_a && base + 16 * h <= pos_b;
-            pid[h] = max(id, 0);
+        for (int h = 0; h < 2; ++h) {
+            const int id = page_ok(nid[h], a.kv.n_pages);
+            bad |= id < 0;
+            pid[h] = __builtin_amdgcn_readfirstlane(max(id, 0));
         }
     };
     auto load_k = [&](int base) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
             const int d = T::F32 ? col : 8 * (col >> 2) + 4 * u + (col & 3);
-            const int64_t pg = d >= 16 ? pid[NU - 1] : pid[0];
+            const int64_t pg = d >= 16 ? pid[1] : pid[0];
             const char* p = kb + pg * a.kv.stride + (int64_t)((base + d) & (page - 1)) * hd * T::SZ;
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
@@ -446,14 +478,14 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
             }
         }
         if constexpr (T::I8) {
-            const int64_t pg = g >= 2 ? pid[NU - 1] : pid[0];
+            const int64_t pg = g >= 2 ? pid[1] : pid[0];
             const float* p = a.kv.ks + pg * a.kv.sstride + kvh * page + ((base + 8 * g) & (page - 1));
 #pragma unroll
             for (int j = 0; j < 8; j += 4) *reinterpret_cast<f4*>(ksc + j) = *reinterpret_cast<const f4*>(p + j);
         }
     };
     auto load_v = [&](int base) {
-        const int64_t pg = T::PL * g >= 16 ? pid[NU - 1] : pid[0];
+        const int64_t pg = T::PL * g >= 16 ? pid[1] : pid[0];
         const int at = (base + T::PL * g) & (page - 1);
         const char* p = vb + pg * a.kv.stride + ((int64_t)col * page + at) * T::SZ;
 #pragma unroll
@@ -467,7 +499,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
     };
     if (wave < tiles) {
         ids(beg + wave * KT);
-        pages(beg + wave * KT);
+        pages();
         ids(beg + (wave + NW) * KT);
         load_k(beg + wave * KT);
         load_v(beg + wave * KT);
@@ -511,7 +543,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
             for (int j = 0; j < 8; ++j) vcur[j] = vsc[j];
         }
         if (more) {
-            pages(next);
+            pages();
             ids(next + NW * KT);
             load_k(next);
         }
@@ -617,7 +649,6 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
         }
         if (more) load_v(next);
     }
-    if (bad && lane == 0) atomicOr(a.err, ERR_INDEX);
     if constexpr (!T::I8) {
         if (__builtin_amdgcn_ballot_w64(odd != 0)) {  // rare: the keys of those tiles again, one by one
             for (int key = beg; key < end; ++key) {
@@ -642,6 +673,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
         stat[wave][col][0] = m;
         stat[wave][col][1] = l;
     }
+    if (lane == 0) holes[wave] = bad;
     __syncthreads();
     float mm = -__builtin_inff();
 #pragma unroll
@@ -667,7 +699,15 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
         }
         __syncthreads();
     }
-    if (wave != 0 || col >= np) return;
+    if (wave != 0) return;
+    int hole = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) hole |= holes[w];
+    if (hole && page_bad(a, it.seq, max(lo_a, beg), min(pos_b, end - 1))) {
+        note_hole(a, blockIdx.x / n_kv, it.seq);
+        lsum = HOLE;
+    }
+    if (col >= np) return;
     if (it.chunks == 1) {
         const float r = over(lsum, pos);
         float* d = a.out + (int64_t)(it.q.row0 + row) * a.out_pitch + (int64_t)head * hd + 4 * g;
@@ -779,7 +819,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     constexpr int SZ = I8 ? 1 : F32 ? 4 : 2, NA = P::NA, NB = P::NB, NBUF = P::NBUF;
     constexpr int NS = HD / 16, NH = P::N32, NK = P::KT / 32, KT = P::KT, IPW = P::IPW;
     extern __shared__ __align__(1024) char lds[];
-    __shared__ int flag;  // a value was taken out
+    __shared__ int flag, hole;  // a value was taken out; a page id was bad
     uint16_t* lk = reinterpret_cast<uint16_t*>(lds);                   // [NBUF][NA][KT][HP]
     uint16_t* lv = lk + NBUF * NA * P::BUF;                            // [NBUF][NA][HP][KT]
     float* lks = reinterpret_cast<float*>(lv + NBUF * NA * P::BUF);    // [2][KT] int8 steps
@@ -843,8 +883,6 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     const float scl = fmaxf(__builtin_ldexpf(a.scale, qe), 1.17549435e-38f);
     const float mul = capped ? 1.0f : scl * LOG2E, rcap = capped ? scl / a.cap : 0.0f;
 
-    const int wlo_a = key_lo(a.c, wpos_a), wlo_b = key_lo(a.c, wpos_b);
-
     // ---- staging: this thread's pieces (the same place in every tile)
     const int32_t* table = a.pages + (int64_t)it.seq * a.pages_pitch;
     const int last_page = max(0, it.q.len - 1) >> shift;
@@ -854,8 +892,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     // pieces of the keys are KT / 4 whole rows, one page's; its pieces of the
     // values hold the same 8 tokens of different channels.  Page ids are
     // scalar, loaded a tile ahead of the loads that use them and looked at
-    // only there; a bad one reads page 0 and is told at the end where a row of
-    // the workgroup sees a key of its group.
+    // only there; a bad one reads page 0 and is looked into at the end.
     static_assert(64 / P::VC % P::VC == 0 && IPW * 64 * 4 == KT * P::KC && KT / 4 <= 16, "");
     constexpr int VR = 64 / P::VC;                        // channels a wave's piece takes
     const int vr0 = (wave * IPW * 64 + lane) / P::VC;     // channel of piece 0
@@ -870,19 +907,16 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
             g3 = table[min((base + 48) >> shift, last_page)];
         }
     };
-    auto page_of = [&](int id) -> int64_t { return max(page_ok(id, a.kv.n_pages), 0); };
-    auto look = [&](int base) {
-#pragma unroll
-        for (int h = 0; h < KT / 16; ++h)
-            bad |= page_ok(pick4(h, g0, g1, g2, g3), a.kv.n_pages) < 0 && base + 16 * h + 15 >= wlo_a &&
-                   base + 16 * h <= wpos_b;
+    auto page_of = [&](int id) -> int64_t {
+        const int ok = page_ok(id, a.kv.n_pages);
+        bad |= ok < 0;
+        return max(ok, 0);
     };
     using Raw = std::conditional_t<I8, u2, u4>;
     constexpr int NR = F32 ? 2 : 1;  // loads a piece
     Raw rk[F16 ? 1 : IPW][NR], rv[F16 ? 1 : IPW][NR];
     float rs = 0.0f;
     auto fetch = [&](int base, int buf) {
-        look(base);
         int ln = lane;
         asm volatile("" : "+v"(ln));  // addresses are formed anew for every tile, not held over the products
         const int r0 = wave * (IPW * VR) + ln / P::VC, tok = 8 * ((ln % P::VC) ^ (r0 & P::VX));
@@ -920,6 +954,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     // zero probability would carry them to pairs that do not see them) are
     // zeroed; the second are noted and given to their pairs after the loop.
     // (int8 values are finite, and a key that is not seen has weight zero.)
+    const int wlo_a = key_lo(a.c, wpos_a), wlo_b = key_lo(a.c, wpos_b);
     auto land = [&](int base, int buf) {
         const bool edge = base < wlo_b || base + KT - 1 > wpos_a;
         if constexpr (I8) {
@@ -991,7 +1026,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     float m = -__builtin_inff(), l = 0.0f;
     int ev = 0;
     const int krow = (col & 19) | (col & 4) << 1 | (col & 8) >> 1;  // the key of this lane's score row
-    if (tid == 0) flag = 0;
+    if (tid == 0) flag = hole = 0;
     // two workgroups share a CU, the second 256 behind the first: one ahead of
     // the other keeps the one's products over the other's softmax
     if ((blockIdx.x >> 8) & 1) __builtin_amdgcn_s_setprio(2);
@@ -1166,7 +1201,8 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
         if (ti + 1 < tiles) land(base + KT, other);
         __syncthreads();
     }
-    if (bad && tid == 0) atomicOr(a.err, ERR_INDEX);
+    if (bad) hole = 1;  // (each wave has looked at the ids of its own pieces)
+    __syncthreads();
     if constexpr (!I8) {
         if (flag) {  // rare: the keys of those tiles again, one by one (the last barrier was after the last note)
             for (int key = beg; key < end; ++key) {
@@ -1188,8 +1224,12 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
             }
         }
     }
-    if (idle || col >= np) return;
     l += __uint_as_float(xshfl<32>(__float_as_uint(l)));
+    if (hole && page_bad(a, it.seq, max(wlo_a, beg), min(wpos_b, end - 1))) {
+        note_hole(a, blockIdx.x / n_kv, it.seq);
+        l = HOLE;
+    }
+    if (idle || col >= np) return;
     if (it.chunks == 1) {
         const float r = over(l, pos);
         float* d = a.out + (int64_t)(it.q.row0 + row) * a.out_pitch + (int64_t)head * hd + 4 * h;
@@ -1228,6 +1268,74 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     }
 }
 
+template <int DT>
+__device__ __forceinline__ float entry(const char* p) {  // a stored key's or value's
+    if constexpr (DT == FRQ_DT_ROWI8) return (float)*reinterpret_cast<const int8_t*>(p);
+    else return value_at<DT>(p);
+}
+// The outputs beg .. end - 1 of the tile (float4 of pairs), key by key without
+// those under page ids out of range: a wave a pair, a lane every 64th channel.
+template <int DT, int TP>
+__device__ __forceinline__ void redo_share(const Args& a, const Record& it, int kvh, int beg, int end) {
+    constexpr bool I8 = DT == FRQ_DT_ROWI8;
+    constexpr int SZ = DT == FRQ_DT_F32 ? 4 : I8 ? 1 : 2;
+    const int lane = threadIdx.x & 63, hd = a.kv.hd, page = a.kv.page, rep = a.c.rep;
+    const int32_t* table = a.pages + (int64_t)(it.seq < 0 ? ~it.seq : it.seq) * a.pages_pitch;
+    const int p0 = it.tile * TP, h4 = hd / 4;
+    for (int pair = beg / h4 + uni(threadIdx.x >> 6); pair * h4 < end; pair += 4) {
+        const int row = (p0 + pair) / rep, head = kvh * rep + (p0 + pair) % rep, pos = it.len - it.rows + row;
+        const float* q = a.q + (int64_t)(it.row0 + row) * a.q_pitch + (int64_t)head * hd;
+        float x[4], o[4], m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = 64 * i + lane < hd ? q[64 * i + lane] * a.sign : 0.0f;
+            o[i] = 0.0f;
+        }
+        int seen = -1;  // (over's place of a row: below 0 if it sees nothing)
+#pragma unroll 1
+        for (int key = key_lo(a.c, pos); key <= pos; ++key) {
+            const int64_t pg = page_ok(table[key >> a.c.shift], a.kv.n_pages);
+            if (pg < 0) continue;
+            const int at = key & (page - 1);
+            const char* k = a.kv.k + pg * a.kv.stride + ((int64_t)kvh * page + at) * hd * SZ;
+            const char* v = a.kv.v + pg * a.kv.stride + ((int64_t)kvh * hd * page + at) * SZ;
+            const int64_t step = pg * a.kv.sstride + kvh * page + at;
+            float z = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (64 * i + lane < hd) z = __builtin_fmaf(x[i], entry<DT>(k + (64 * i + lane) * SZ), z);
+            z = wave_sum(z);
+            if constexpr (I8) z *= a.kv.ks[step];
+            z *= a.scale;
+            z = LOG2E * (a.cap > 0.0f ? a.cap * tanh_f(z / a.cap) : z);
+            const float mn = fmaxf(m, z), mr = mn == -__builtin_inff() ? 0.0f : mn;
+            const float alpha = __builtin_amdgcn_exp2f(m - mr);
+            float w = __builtin_amdgcn_exp2f(z - mr);
+            m = mn;
+            l = l * alpha + w;
+            if constexpr (I8) w *= a.kv.vs[step];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (64 * i + lane < hd)
+                    o[i] = o[i] * alpha + w * entry<DT>(v + (int64_t)(64 * i + lane) * page * SZ);
+            seen = 0;
+        }
+        const float r = over(l, seen);
+        float* d = a.out + (int64_t)(it.row0 + row) * a.out_pitch + (int64_t)head * hd;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = 64 * i + lane, e = pair * h4 + c / 4;
+            if (c < hd && e >= beg && e < end) d[c] = o[i] * r;
+        }
+    }
+}
+template <int TP>
+__device__ __forceinline__ void redo_share(const Args& a, const Record& it, int kvh, int beg, int end) {
+    if (a.dtype == FRQ_DT_F32) redo_share<FRQ_DT_F32, TP>(a, it, kvh, beg, end);
+    else if (a.dtype == FRQ_DT_F16) redo_share<FRQ_DT_F16, TP>(a, it, kvh, beg, end);
+    else redo_share<FRQ_DT_ROWI8, TP>(a, it, kvh, beg, end);
+}
+
 // ---- joining the chunks' parts ----------------------------------------------
 // The workgroup of a tile's chunk i joins the i-th share of the tile's
 // outputs, so that a long sequence's parts are read by many workgroups.
@@ -1240,7 +1348,11 @@ template <int TP>
 __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so, float* sm, float* sl) {
     const int n_kv = a.c.n_kv, kvh = block % n_kv;
     const Record it = a.rec[block / n_kv];
-    if (it.chunks <= 1 || it.slot < 0 || it.slot + it.chunks > a.slots) return;
+    if (it.chunks <= 1) {
+        if (it.seq < 0) redo_share<TP>(a, it, kvh, 0, min(TP, it.rows * a.c.rep - it.tile * TP) * (a.kv.hd / 4));
+        return;
+    }
+    if (it.slot < 0 || it.slot + it.chunks > a.slots) return;
     const int hd = a.kv.hd, tid = threadIdx.x;
     const int p0 = it.tile * TP, np = min(TP, it.rows * a.c.rep - p0);
     const int n4 = np * (hd / 4), per = (n4 + it.chunks - 1) / it.chunks;
@@ -1258,6 +1370,7 @@ __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so,
         for (int i = 0; i < 4; ++i) y.v[i] = o[i] * r;
         *reinterpret_cast<F4*>(a.out + (int64_t)(it.row0 + row) * a.out_pitch + (int64_t)head * hd + 4 * c4) = y;
     };
+    bool hole = false;
     if (runs == 1) {  // large shares: U float4 a thread at once
         constexpr int U = 4;
         for (int b = beg + tid; b < end; b += 256 * U) {
@@ -1281,6 +1394,7 @@ __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so,
                 for (int u = 0; u < U; ++u) {
                     mc[u] = d[2 * pair[u]];
                     lc[u] = d[2 * pair[u] + 1];
+                    hole |= lc[u] == HOLE;
                     oc[u] = *reinterpret_cast<const f4*>(d + 2 * TP + (int64_t)pair[u] * hd + 4 * c4[u]);
                 }
 #pragma unroll
@@ -1296,9 +1410,8 @@ __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so,
             for (int u = 0; u < U; ++u)
                 if (b + 256 * u < end) store(pair[u], c4[u], o[u], l[u]);
         }
-        return;
     }
-    for (int b = beg; b < end; b += pe) {
+    for (int b = beg; runs > 1 && b < end; b += pe) {
         const int e = b + tid % pe;
         const bool in = e < end;
         const int pair = in ? e / (hd / 4) : 0, c4 = in ? e % (hd / 4) : 0;
@@ -1307,6 +1420,7 @@ __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so,
         for (int c = run; c < it.chunks; c += runs) {
             const float* d = part + c * pitch;
             const float mc = d[2 * pair], lc = d[2 * pair + 1];
+            hole |= lc == HOLE;
             const f4 oc = *reinterpret_cast<const f4*>(d + 2 * TP + (int64_t)pair * hd + 4 * c4);
             const float mn = fmaxf(m, mc), mr = mn == -__builtin_inff() ? 0.0f : mn;
             const float x = __builtin_amdgcn_exp2f(m - mr), y = __builtin_amdgcn_exp2f(mc - mr);
@@ -1333,6 +1447,7 @@ __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so,
         }
         if (run == 0 && in) store(pair, c4, o, l);
     }
+    if (__syncthreads_or(hole)) redo_share<TP>(a, it, kvh, beg, end);
 }
 
 // The launchers of one stored type (each in a file of its own).

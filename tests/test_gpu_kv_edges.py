@@ -77,3 +77,74 @@ def test_pages_before_the_window_may_be_gone(ctx, kind, window, many):
         assert (table[:, 0] == -1).sum() >= len(lens) - 3
         set_table(b, table)
         hold(b.run(window=window), *expect(b, window=window))
+
+
+def seed_with(lens, page, owner):
+    """A seed whose Batch of lens gives page 0 to sequence `owner` (None: to none)."""
+    held = [-(-n // page) for n in lens]
+    for seed in range(1000):
+        at = int(np.argwhere(np.random.default_rng(seed).permutation(sum(held) + 2) == 0)[0, 0])
+        who = next((s for s in range(len(lens)) if sum(held[:s]) <= at < sum(held[:s + 1])), None)
+        if who == owner:
+            return seed
+    raise AssertionError
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("owner", [None, 0])
+@pytest.mark.parametrize("rows", [None, [3, 4, 2], [40, 90, 60]])
+@pytest.mark.parametrize("window,cap", [(0, 0.0), (20, 30.0)])
+def test_pages_out_of_range_take_no_part(ctx, kind, owner, rows, window, cap):
+    """Keys under a page id out of range are left out and reported, whatever
+    page 0 holds (unwritten: NaN and infinities; another sequence's rows, here
+    large ones); a row that is left without a key gets zeros."""
+    lens = [200, 300, 70]
+
+    def poison(ks, vs):
+        ks[0] *= 3
+        vs[0] += 1000
+
+    b = Batch(ctx, kind, 16, 2, 3, 64, lens, rows, seed=seed_with(lens, 16, owner), poison=poison)
+    assert (b.table[0] == 0).any() == (owner == 0)
+    clean = b.run(window=window, cap=cap)
+    hold(clean, *expect(b, window=window, cap=cap))
+    table = b.table.copy()
+    holes = {1: (3, 10, 17, 18), 2: (0, 1, 2, 3, 4)}
+    ids = [-1, b.p.n_pages, 2 ** 31 - 1, -2 ** 31]
+    for s, pages in holes.items():
+        for i, p in enumerate(pages):
+            table[s, p] = ids[i % 4]
+    gone = {s: {j for p in pages for j in range(16 * p, 16 * p + 16)} for s, pages in holes.items()}
+    set_table(b, table)
+    with pytest.raises(fa.FrqError) as e:
+        b.run(window=window, cap=cap)
+    assert e.value.code == fa.FRQ_ERR_ARG
+    ctx.sync()
+    got = b.do.numpy()[:b.n_row].reshape(clean.shape)
+    want, tol = expect(b, gone, window=window, cap=cap)
+    hold(got, want, tol)
+    assert (got[b.first[2]:] == 0).all()  # every page of it is gone
+    assert np.array_equal(got[:b.first[1]], clean[:b.first[1]])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_gone_pages_beside_values_that_are_not_finite(ctx, kind):
+    """A seen value that is not finite reaches the rows that see it and no
+    other, in a tile with a page out of range too."""
+    def poison(ks, vs):
+        vs[0][70, 0, 5] = np.inf
+        vs[0][58, 0, 9] = np.nan  # in the page that goes
+
+    b = Batch(ctx, kind, 16, 1, 3, 64, [100], [64], poison=poison)
+    table = b.table.copy()
+    table[0, 3] = -1  # keys 48 .. 63
+    set_table(b, table)
+    with pytest.raises(fa.FrqError):
+        b.run()
+    got = b.do.numpy()[:64].reshape(64, 3, 64)
+    with np.errstate(invalid="ignore"):
+        want, tol = expect(b, {0: set(range(48, 64))})
+    hold(got[:34], want[:34], tol[:34])  # rows at 36 .. 69
+    rest = np.delete(np.arange(64), 5)
+    hold(got[34:][:, :, rest], want[34:][:, :, rest], tol[34:][:, :, rest])
+    assert (got[34:, :, 5] == np.inf).all()
