@@ -214,8 +214,8 @@ int check_err_word(frq_ctx* c) {
     int h = 0;
     HIPCHK(hipMemcpy(&h, c->err, sizeof(int), hipMemcpyDeviceToHost), "hipMemcpy(err)");
     if (h) {
-        const int zero = 0;
-        HIPCHK(hipMemcpy(c->err, &zero, sizeof(int), hipMemcpyHostToDevice), "hipMemcpy(err)");
+        const int left = h & 1 ? h & ~1 : 0;  // one error a call; the index is told by the next
+        HIPCHK(hipMemcpy(c->err, &left, sizeof(int), hipMemcpyHostToDevice), "hipMemcpy(err)");
         if (!(h & 1)) return fail(FRQ_ERR_ARG, "a page, slot, length or row offset of the cache was out of range");
         return fail(FRQ_ERR_NAN, "NaN in activations (the reference panics in partial_cmp().unwrap())");
     }

@@ -100,7 +100,8 @@ int frq_set_stream(frq_ctx* ctx, void* hip_stream);
 void* frq_get_stream(frq_ctx* ctx);
 /* Wait for the ctx stream; returns FRQ_ERR_NAN if a _dev call since the last
  * sync saw a NaN activation, FRQ_ERR_ARG if one saw an index of the paged
- * cache out of range, else FRQ_OK / FRQ_ERR_HIP. */
+ * cache out of range (of both the NaN first, the index by the next frq_sync),
+ * else FRQ_OK / FRQ_ERR_HIP. */
 int frq_sync(frq_ctx* ctx);
 
 /* ---- weight upload (one-time, into persistent HBM) ---------------------- */

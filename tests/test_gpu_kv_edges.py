@@ -148,3 +148,27 @@ def test_gone_pages_beside_values_that_are_not_finite(ctx, kind):
     rest = np.delete(np.arange(64), 5)
     hold(got[34:][:, :, rest], want[34:][:, :, rest], tol[34:][:, :, rest])
     assert (got[34:, :, 5] == np.inf).all()
+
+
+def test_a_bad_index_and_a_nan_are_both_reported(ctx):
+    b = Batch(ctx, "f16", 16, 1, 2, 32, [20])
+    b.run()
+    table = b.table.copy()
+    table[0, 1] = -1
+    x = hip.DeviceArray.from_numpy(np.full((1, 64), np.nan, np.float32))
+    a8, sa = hip.DeviceArray((1, fa.quant_pitch(64)), np.int8), hip.DeviceArray((1,), np.float32)
+    oi, ov = hip.DeviceArray((1, 32), np.uint32), hip.DeviceArray((1, 32), np.float32)
+    for first in (0, 1):
+        set_table(b, table)
+        for i in (first, 1 - first):
+            if i:
+                b.call()
+            else:
+                ctx.quant_dev(x.ptr, 1, 64, a8.ptr, sa.ptr, oi.ptr, ov.ptr)
+        codes = []
+        for _ in range(2):
+            with pytest.raises(fa.FrqError) as e:
+                ctx.sync()
+            codes.append(e.value.code)
+        assert sorted(codes) == sorted([fa.FRQ_ERR_NAN, fa.FRQ_ERR_ARG])
+        ctx.sync()  # each told once
