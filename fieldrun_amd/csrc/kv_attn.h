@@ -292,6 +292,39 @@ constexpr float LOG2E = 1.4426950408889634f;
 // of a probability stays below 2^(-25 - P_BIAS) of the largest.
 constexpr float P_BIAS = 11.0f, P_SLACK = 4.0f;
 
+// A pair's running maximum m, one of the scores as the products leave them,
+// their factor mul not in it, and what the weights of scores s are formed with,
+// exp2(s mul + mb): one FMA each, right while m mul rounds by less than 2^-4, to
+// all weights alike.  Beyond FAR (to the end of f32, where a rounding is more than
+// the slack) the scores of the tile have m taken off first, which mb then has not.
+constexpr float FAR = 1048576.0f;  // 2^20
+struct Top {
+    float m, mb;
+    bool far;  // of any pair of the wave
+    __device__ __forceinline__ explicit Top(float bias) : m(-__builtin_inff()), mb(bias), far(false) {}
+    __device__ __forceinline__ float base() const { return m == -__builtin_inff() ? 0.0f : m; }
+    // Whether a tile's largest score has to become some pair's maximum.
+    __device__ __forceinline__ bool moves(float mx, float mul) const {
+        return __builtin_amdgcn_ballot_w64((mx - m) * mul > P_SLACK) != 0;
+    }
+    // Then: what the pair's sums so far count.
+    __device__ __forceinline__ float move(float mx, float mul, float bias) {
+        const float was = m;
+        m = (mx - m) * mul > P_SLACK ? mx : m;
+        const float z = base() * mul;
+        far = __builtin_amdgcn_ballot_w64(__builtin_fabsf(z) > FAR) != 0;
+        mb = far ? bias : bias - z;
+        return __builtin_amdgcn_exp2f((was - base()) * mul);
+    }
+};
+// The scale of scores of q times 2^-e: not zero, and no larger than what f32
+// can multiply such scores by (over f16 and int8 keys they are 0 or more than
+// 2^-52, and differ by 2^-76 or not at all, so that 2^100 parts them as any
+// larger factor would).
+__device__ __forceinline__ float score_scale(float scale, int e) {
+    return fminf(fmaxf(__builtin_ldexpf(scale, e), 1.17549435e-38f), 1.2676506002282294e30f);
+}
+
 // int8: a key's value step goes into its probability, w = p step, and the
 // pair's weights are held over a power of two of their own, so that neither
 // steps of any size nor other rows' keys cost a pair its bits: ev is the
@@ -432,7 +465,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
     load_q<DT, HD, NS>(a.q + (int64_t)(it.q.row0 + row) * a.q_pitch + (int64_t)head * hd, a.sign, g, q);
     // scores times mul are in the domain of exp2; with a cap they are made so
     const bool capped = a.cap > 0.0f;
-    const float scl = fmaxf(__builtin_ldexpf(a.scale, q.e), 1.17549435e-38f);
+    const float scl = score_scale(a.scale, q.e);
     const float mul = capped ? 1.0f : scl * LOG2E, rcap = capped ? scl / a.cap : 0.0f;
     const int32_t* table = a.pages + (int64_t)it.seq * a.pages_pitch;
     const int last_page = max(0, it.q.len - 1) >> shift;
@@ -444,7 +477,9 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
     f4 o[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t] = f4{0, 0, 0, 0};
-    float m = -__builtin_inff(), l = 0.0f;
+    constexpr float BIAS = T::I8 ? 0.0f : P_BIAS;
+    Top top(BIAS);
+    float l = 0.0f;
     int ev = 0;  // int8: out is held times 2^(W_EXP - ev)
     uint32_t odd = 0;
     const bool alike = lo_a == lo_b && pos_a == pos_b;  // every pair sees the same
@@ -567,20 +602,27 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
         float mx = s[0];
 #pragma unroll
         for (int j = 1; j < 4 * NU; ++j) mx = fmaxf(mx, s[j]);
-        mx = fmax16(mx) * mul;
-        const float mn = mx > m + P_SLACK ? mx : m;
-        const float mr = mn == -__builtin_inff() ? 0.0f : mn;
-        float alpha = __builtin_amdgcn_exp2f(m - mr);
-        bool moved = mn != m;
-        m = mn;
-        const float mb = T::I8 ? -mr : P_BIAS - mr;
+        mx = fmax16(mx);
+        float alpha = 1.0f;
+        if (T::I8 || top.moves(mx, mul)) {  // (int8 has a branch of its own behind the weights)
+            alpha = top.move(mx, mul, BIAS);
+            l *= alpha;
+            if constexpr (!T::I8) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) o[t] *= alpha;
+            }
+        }
+        if (top.far) {
+#pragma unroll
+            for (int j = 0; j < 4 * NU; ++j) s[j] -= top.base();
+        }
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < 4 * NU; ++j) {
-            s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], mul, mb));
+            s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], mul, top.mb));
             sum += s[j];
         }
-        l = l * alpha + sum;
+        l += sum;
         if constexpr (T::I8) {
             float wm = 0.0f;
 #pragma unroll
@@ -589,15 +631,15 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
                 wm = fmaxf(wm, __builtin_fabsf(s[j]));
             }
             const int en = weight_exp(ev, alpha, fmax16(wm));
-            moved |= en != ev;
+            const bool moved = alpha != 1.0f || en != ev;
             alpha = __builtin_ldexpf(alpha, ev - en);
             ev = en;
 #pragma unroll
             for (int j = 0; j < 8; ++j) s[j] = __builtin_ldexpf(s[j], W_EXP - ev);
-        }
-        if (__builtin_amdgcn_ballot_w64(moved)) {
+            if (__builtin_amdgcn_ballot_w64(moved)) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) o[t] *= alpha;
+                for (int t = 0; t < NT; ++t) o[t] *= alpha;
+            }
         }
         // ---- values.  Keys that no pair sees may hold anything, and a zero
         // probability would carry what is not finite to pairs that do not see
@@ -669,6 +711,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
     }
     // ---- the waves' parts: the largest maximum, then sums in a fixed order
     l = fsum16(l);
+    const float m = top.m * mul;
     if (g == 0) {
         stat[wave][col][0] = m;
         stat[wave][col][1] = l;
@@ -880,7 +923,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     }
     // scores times mul are in the domain of exp2; with a cap they are made so
     const bool capped = a.cap > 0.0f;
-    const float scl = fmaxf(__builtin_ldexpf(a.scale, qe), 1.17549435e-38f);
+    const float scl = score_scale(a.scale, qe);
     const float mul = capped ? 1.0f : scl * LOG2E, rcap = capped ? scl / a.cap : 0.0f;
 
     // ---- staging: this thread's pieces (the same place in every tile)
@@ -1023,7 +1066,9 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     for (int t = 0; t < NH; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
-    float m = -__builtin_inff(), l = 0.0f;
+    constexpr float BIAS = I8 ? 0.0f : P_BIAS;
+    Top top(BIAS);
+    float l = 0.0f;
     int ev = 0;
     const int krow = (col & 19) | (col & 4) << 1 | (col & 8) >> 1;  // the key of this lane's score row
     if (tid == 0) flag = hole = 0;
@@ -1122,20 +1167,27 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
                 float mx = s[0];
 #pragma unroll
                 for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-                mx = fmaxf(mx, __uint_as_float(xshfl<32>(__float_as_uint(mx)))) * mul;
-                const float mn = mx > m + P_SLACK ? mx : m;
-                const float mr = mn == -__builtin_inff() ? 0.0f : mn;
-                float alpha = __builtin_amdgcn_exp2f(m - mr);
-                bool moved = mn != m;
-                m = mn;
-                const float mb = I8 ? -mr : P_BIAS - mr;
+                mx = fmaxf(mx, __uint_as_float(xshfl<32>(__float_as_uint(mx))));
+                float alpha = 1.0f;
+                if (top.moves(mx, mul)) {
+                    alpha = top.move(mx, mul, BIAS);
+                    l *= alpha;
+                    if constexpr (!I8) {
+#pragma unroll
+                        for (int t = 0; t < NH; ++t) o[t] *= alpha;
+                    }
+                }
+                if (top.far) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] -= top.base();
+                }
                 float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], mul, mb));
+                    s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], mul, top.mb));
                     sum += s[i];
                 }
-                l = l * alpha + sum;
+                l += sum;
                 if constexpr (I8) {
                     float wm = 0.0f, step[16];
 #pragma unroll
@@ -1152,15 +1204,15 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
                     }
                     wm = fmaxf(wm, __uint_as_float(xshfl<32>(__float_as_uint(wm))));
                     const int en = weight_exp(ev, alpha, wm);
-                    moved |= en != ev;
+                    const bool moved = alpha != 1.0f || en != ev;
                     alpha = __builtin_ldexpf(alpha, ev - en);
                     ev = en;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[i] = __builtin_ldexpf(s[i], W_EXP - ev);
-                }
-                if (__builtin_amdgcn_ballot_w64(moved)) {
+                    if (__builtin_amdgcn_ballot_w64(moved)) {
 #pragma unroll
-                    for (int t = 0; t < NH; ++t) o[t] *= alpha;
+                        for (int t = 0; t < NH; ++t) o[t] *= alpha;
+                    }
                 }
                 Op pv[2][NB];
 #pragma unroll
@@ -1230,6 +1282,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
         l = HOLE;
     }
     if (idle || col >= np) return;
+    const float m = top.m * mul;
     if (it.chunks == 1) {
         const float r = over(l, pos);
         float* d = a.out + (int64_t)(it.q.row0 + row) * a.out_pitch + (int64_t)head * hd + 4 * h;
@@ -1286,11 +1339,18 @@ __device__ __forceinline__ void redo_share(const Args& a, const Record& it, int 
         const int row = (p0 + pair) / rep, head = kvh * rep + (p0 + pair) % rep, pos = it.len - it.rows + row;
         const float* q = a.q + (int64_t)(it.row0 + row) * a.q_pitch + (int64_t)head * hd;
         float x[4], o[4], m = -__builtin_inff(), l = 0.0f;
+        int e = 0;  // q is held times 2^-e, as by the loops
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             x[i] = 64 * i + lane < hd ? q[64 * i + lane] * a.sign : 0.0f;
             o[i] = 0.0f;
+            e = max(e, (int)(__float_as_uint(__builtin_fabsf(x[i])) >> 23));
         }
+        e = wave_most(e);
+        e = DT == FRQ_DT_F32 || e == 0 || e == 255 ? 0 : e - 127;
+        const float scl = score_scale(a.scale, e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __builtin_ldexpf(x[i], -e);
         int seen = -1;  // (over's place of a row: below 0 if it sees nothing)
 #pragma unroll 1
         for (int key = key_lo(a.c, pos); key <= pos; ++key) {
@@ -1306,8 +1366,7 @@ __device__ __forceinline__ void redo_share(const Args& a, const Record& it, int 
                 if (64 * i + lane < hd) z = __builtin_fmaf(x[i], entry<DT>(k + (64 * i + lane) * SZ), z);
             z = wave_sum(z);
             if constexpr (I8) z *= a.kv.ks[step];
-            z *= a.scale;
-            z = LOG2E * (a.cap > 0.0f ? a.cap * tanh_f(z / a.cap) : z);
+            z = a.cap > 0.0f ? (a.cap * LOG2E) * tanh_f(z * (scl / a.cap)) : z * (scl * LOG2E);
             const float mn = fmaxf(m, z), mr = mn == -__builtin_inff() ? 0.0f : mn;
             const float alpha = __builtin_amdgcn_exp2f(m - mr);
             float w = __builtin_amdgcn_exp2f(z - mr);

@@ -255,8 +255,9 @@ int frq_kv_read_dev(frq_ctx* ctx, const frq_kv* kv, const int64_t* d_slot,
  * <= p, with window > 0 those of p - j < window.  Query head h (n_head of hd
  * a row, rows q_pitch apart) reads kv head h / (n_head / n_kv):
  *   z_j = scale q . k_j, cap > 0: cap tanh(z_j / cap);  out = softmax(z) v
- * (forward_block, src/gemma.rs:252-277) with f32 sums over each run of keys,
- * the runs joined in a fixed order; a row that sees no token gets zeros.  Rows
+ * (forward_block, src/gemma.rs:252-277) with f32 scores and sums over each run
+ * of keys, the runs joined in a fixed order (a score beyond f32 makes its row
+ * NaN); a row that sees no token gets zeros.  Rows
  * outside d_first[0] .. d_first[n_seq] - 1 stay as they were; d_out and d_q
  * lie apart.  What a row does not see does not touch it, whatever it holds
  * (pages behind the windows of all of a sequence's rows may be gone: their

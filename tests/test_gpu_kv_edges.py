@@ -172,3 +172,69 @@ def test_a_bad_index_and_a_nan_are_both_reported(ctx):
             codes.append(e.value.code)
         assert sorted(codes) == sorted([fa.FRQ_ERR_NAN, fa.FRQ_ERR_ARG])
         ctx.sync()  # each told once
+
+
+# ---- sizes ----------------------------------------------------------------------
+
+def patterned(b, rows_of, value):
+    """Keys of few kinds: key j of every sequence has value(j) in channel 0 and
+    zeros beside it, so that scores are exact and tie exactly."""
+    for s, n in enumerate(b.lens):
+        if not n:
+            continue
+        k = np.zeros((n, b.p.kv, b.p.hd), np.float32)
+        k[:, :, 0] = np.array([value(j) for j in range(n)], np.float32)[:, None]
+        j = np.arange(n)
+        b.p.write(k, b.v[s].astype(np.float32), b.table[s, j // b.p.page].astype(np.int64) * b.p.page + j % b.p.page)
+        b.k[s] = b.p.stored(k)
+        b.v[s] = b.p.stored(b.v[s].astype(np.float32))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows", [None, [60, 90]])
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 24 * 1.5, 2.0 ** 27, 2.0 ** 31, 2.0 ** 40 * 1.25, 2.0 ** 70, 2.0 ** 110])
+def test_scores_of_any_size(ctx, kind, rows, size):
+    """Scores far beyond the steps of f32 at 1: the keys that share the largest
+    share the output, evenly and exactly as many as there are, over one chunk
+    and several; a second head asks the other way, a third with zeros."""
+    b = Batch(ctx, kind, 16, 1, 3, 64, [90, 5000], rows, seed=4)
+    patterned(b, rows, lambda j: (j * 5) % 7 - 3)
+    b.q[:] = 0.0
+    b.q[:, 0, 0] = size
+    b.q[:, 1, 0] = -size
+    got = b.run()
+    u = 2.0 ** -24
+    for s, n in enumerate(b.lens):
+        for i in range(b.rows[s]):
+            p = n - b.rows[s] + i
+            k0, v = b.k[s][:p + 1, 0, 0], b.v[s][:p + 1, 0].astype(np.float64)
+            for h, top in ((0, k0.max()), (1, k0.min()), (2, None)):
+                keys = np.flatnonzero(k0 == top) if h < 2 else np.arange(p + 1)
+                want = v[keys].mean(0)
+                # no score is rounded: the weights' split, sums, joining and division, as in test_gpu_kv.py
+                tol = (2.0 ** -21 + u * ((p + 1) / 16 + 16)) * np.abs(v[keys]).mean(0)
+                tol += 2.0 ** -35 * (p + 1) / len(keys) * np.abs(v).max() * (kind != "f32")
+                assert (np.abs(got[b.first[s] + i, h] - want) <= tol).all(), (s, i, h)
+
+
+@pytest.mark.parametrize("kind", ["f16", "rowi8"])
+@pytest.mark.parametrize("cap", [0.0, 50.0])
+def test_large_scale_and_rows_of_q(ctx, kind, cap):
+    """scale times the size of q beyond f32, over keys of zeros among others."""
+    b = Batch(ctx, kind, 16, 1, 2, 64, [300, 70], [70, 1], seed=2)
+    patterned(b, None, lambda j: j % 3)
+    b.q[:] = 0.0
+    b.q[:, 0, 0] = 3e38
+    b.q[:, 1, 0] = -3e38
+    got = b.run(scale=1e25, cap=cap)
+    for s, n in enumerate(b.lens):
+        for i in range(b.rows[s]):
+            p = n - b.rows[s] + i
+            v, k0 = b.v[s][:p + 1, 0].astype(np.float64), b.k[s][:p + 1, 0, 0]
+            for h, sign in ((0, 1), (1, -1)):
+                z = sign * cap * np.sign(k0.astype(np.float64)) if cap else None
+                w = np.exp(z - z.max()) if cap else 1.0 * (k0 == (k0.max() if h == 0 else k0.min()))
+                w /= w.sum()
+                d = 4e-7 * cap
+                tol = (np.expm1(2 * d) + 2.0 ** -21 + 2.0 ** -24 * ((p + 1) / 16 + 16)) * (w @ np.abs(v))
+                assert (np.abs(got[b.first[s] + i, h] - w @ v) <= tol + 2.0 ** -35 * w.max() * (p + 1) * np.abs(v).max()).all()
