@@ -593,7 +593,9 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_p
     a.err = ctx_err(ctx);
     a.scale = scale == 0.0 ? 1.0f : (float)(scale < 0.0 ? -scale : scale);
     a.sign = scale == 0.0 ? 0.0f : scale < 0.0 ? -1.0f : 1.0f;
-    a.cap = (float)cap;
+    // (below 2^-27 every cap gives weights within a rounding of equal ones; there
+    // score_scale's 2^100 over the cap would leave f32, or the cap be zero in it)
+    a.cap = cap > 0.0 && cap < 7.450580596923828e-9 ? 7.450580596923828e-9f : (float)cap;
     a.dtype = kv->dtype;
     // Each sequence is served by the kernel of its number of pairs; one that
     // no sequence can be for is not launched.

@@ -238,3 +238,13 @@ def test_large_scale_and_rows_of_q(ctx, kind, cap):
                 d = 4e-7 * cap
                 tol = (np.expm1(2 * d) + 2.0 ** -21 + 2.0 ** -24 * ((p + 1) / 16 + 16)) * (w @ np.abs(v))
                 assert (np.abs(got[b.first[s] + i, h] - w @ v) <= tol + 2.0 ** -35 * w.max() * (p + 1) * np.abs(v).max()).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("cap", [1e-300, 1e-42, 1e-38, 1e-20, 1e-9, 1e-6])
+def test_tiny_caps(ctx, kind, cap):
+    """A cap leaves no score larger than itself: a tiny one is the mean."""
+    b = Batch(ctx, kind, 16, 1, 3, 64, [40, 700], [1, 60], seed=3)
+    b.q[0, 0] = 0.0
+    hold(b.run(cap=cap), *expect(b, cap=cap))
+    hold(b.run(cap=cap, window=9), *expect(b, cap=cap, window=9))
