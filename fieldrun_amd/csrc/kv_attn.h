@@ -291,6 +291,11 @@ constexpr float LOG2E = 1.4426950408889634f;
 // sequence's first keys out is hardly ever rescaled, and what f16 cannot hold
 // of a probability stays below 2^(-25 - P_BIAS) of the largest.
 constexpr float P_BIAS = 11.0f, P_SLACK = 4.0f;
+// f32 and int8 values may be as large as f32 goes: there the weights (int8: the
+// finished sums) are held times 2^-down, with the slack and the keys' number in
+// it, so that no sum is larger than the largest value.  (Values below about
+// 2^(down - 126) lose bits in turn, 1e-33 at 4096 keys.)
+__device__ __forceinline__ int down_of(int keys) { return 5 + 32 - __builtin_clz(keys | 1); }
 
 // A pair's running maximum m, one of the scores as the products leave them,
 // their factor mul not in it, and what the weights of scores s are formed with,
@@ -477,7 +482,8 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
     f4 o[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t] = f4{0, 0, 0, 0};
-    constexpr float BIAS = T::I8 ? 0.0f : P_BIAS;
+    constexpr float BIAS = T::I8 || T::F32 ? 0.0f : P_BIAS;
+    const int down = down_of(it.q.len);
     Top top(BIAS);
     float l = 0.0f;
     int ev = 0;  // int8: out is held times 2^(W_EXP - ev)
@@ -620,6 +626,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
 #pragma unroll
         for (int j = 0; j < 4 * NU; ++j) {
             s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], mul, top.mb));
+            if constexpr (T::F32) s[j] = __builtin_ldexpf(s[j], -down);
             sum += s[j];
         }
         l += sum;
@@ -710,7 +717,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
         }
     }
     // ---- the waves' parts: the largest maximum, then sums in a fixed order
-    l = fsum16(l);
+    l = fsum16(T::I8 ? __builtin_ldexpf(l, -down) : l);
     const float m = top.m * mul;
     if (g == 0) {
         stat[wave][col][0] = m;
@@ -726,7 +733,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
 #pragma unroll
     for (int w = 0; w < NW; ++w) lsum += stat[w][col][1] * __builtin_amdgcn_exp2f(stat[w][col][0] - mr);
     float f = __builtin_amdgcn_exp2f(m - mr);
-    if constexpr (T::I8) f = __builtin_ldexpf(f, ev - W_EXP);
+    if constexpr (T::I8) f = __builtin_ldexpf(f, ev - W_EXP - down);
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t] *= f;
 #pragma unroll
@@ -1066,7 +1073,8 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     for (int t = 0; t < NH; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
-    constexpr float BIAS = I8 ? 0.0f : P_BIAS;
+    constexpr float BIAS = I8 || F32 ? 0.0f : P_BIAS;
+    const int down = down_of(it.q.len);
     Top top(BIAS);
     float l = 0.0f;
     int ev = 0;
@@ -1185,6 +1193,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], mul, top.mb));
+                    if constexpr (F32) s[i] = __builtin_ldexpf(s[i], -down);
                     sum += s[i];
                 }
                 l += sum;
@@ -1276,6 +1285,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
             }
         }
     }
+    if constexpr (I8) l = __builtin_ldexpf(l, -down);
     l += __uint_as_float(xshfl<32>(__float_as_uint(l)));
     if (hole && page_bad(a, it.seq, max(wlo_a, beg), min(wpos_b, end - 1))) {
         note_hole(a, blockIdx.x / n_kv, it.seq);
@@ -1294,7 +1304,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
                 if (c >= hd) continue;
                 F4 y;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) y.v[j] = (I8 ? __builtin_ldexpf(o[t][i + j], ev - W_EXP) : o[t][i + j]) * r;
+                for (int j = 0; j < 4; ++j) y.v[j] = (I8 ? __builtin_ldexpf(o[t][i + j], ev - W_EXP - down) : o[t][i + j]) * r;
                 *reinterpret_cast<F4*>(d + c) = y;
             }
     } else {
@@ -1315,7 +1325,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
                 if (c >= hd) continue;
                 f4 y;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) y[j] = I8 ? __builtin_ldexpf(o[t][i + j], ev - W_EXP) : o[t][i + j];
+                for (int j = 0; j < 4; ++j) y[j] = I8 ? __builtin_ldexpf(o[t][i + j], ev - W_EXP - down) : o[t][i + j];
                 *reinterpret_cast<f4*>(d + c) = y;
             }
     }
@@ -1349,6 +1359,7 @@ __device__ __forceinline__ void redo_share(const Args& a, const Record& it, int 
         e = wave_most(e);
         e = DT == FRQ_DT_F32 || e == 0 || e == 255 ? 0 : e - 127;
         const float scl = score_scale(a.scale, e);
+        const int down = down_of(it.len);
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = __builtin_ldexpf(x[i], -e);
         int seen = -1;  // (over's place of a row: below 0 if it sees nothing)
@@ -1369,7 +1380,7 @@ __device__ __forceinline__ void redo_share(const Args& a, const Record& it, int 
             z = a.cap > 0.0f ? (a.cap * LOG2E) * tanh_f(z * (scl / a.cap)) : z * (scl * LOG2E);
             const float mn = fmaxf(m, z), mr = mn == -__builtin_inff() ? 0.0f : mn;
             const float alpha = __builtin_amdgcn_exp2f(m - mr);
-            float w = __builtin_amdgcn_exp2f(z - mr);
+            float w = __builtin_ldexpf(__builtin_amdgcn_exp2f(z - mr), -down);
             m = mn;
             l = l * alpha + w;
             if constexpr (I8) w *= a.kv.vs[step];

@@ -248,3 +248,29 @@ def test_tiny_caps(ctx, kind, cap):
     b.q[0, 0] = 0.0
     hold(b.run(cap=cap), *expect(b, cap=cap))
     hold(b.run(cap=cap, window=9), *expect(b, cap=cap, window=9))
+
+
+@pytest.mark.parametrize("kind", ["f32", "rowi8"])
+@pytest.mark.parametrize("lens,rows", [([1, 77, 3000], None), ([90, 1500], [60, 90])])
+def test_values_up_to_the_largest(ctx, kind, lens, rows):
+    """An average of finite values is finite: values up to 3e38, of one sign
+    and of both, over one chunk and several."""
+    def poison(ks, vs):
+        rng = np.random.default_rng(1)
+        for v in vs:
+            v[:] = rng.uniform(1e38, 3e38, v.shape)
+            v[:, :, ::2] *= rng.choice([-1, 1], v[:, :, ::2].shape)
+
+    b = Batch(ctx, kind, 16, 1, 3, 64, lens, rows, seed=3, poison=poison)
+    hold(b.run(), *expect(b))
+
+
+@pytest.mark.parametrize("rows", [None, [60, 90]])
+def test_small_values_keep_their_bits(ctx, rows):
+    """f32 values down to 1e-25 (products with probabilities stay normal numbers)."""
+    def poison(ks, vs):
+        for v in vs:
+            v *= np.float32(1e-25)
+
+    b = Batch(ctx, "f32", 16, 1, 3, 64, [77, 1500], rows, seed=3, poison=poison)
+    hold(b.run(), *expect(b))
