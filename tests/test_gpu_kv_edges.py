@@ -274,3 +274,55 @@ def test_small_values_keep_their_bits(ctx, rows):
 
     b = Batch(ctx, "f32", 16, 1, 3, 64, [77, 1500], rows, seed=3, poison=poison)
     hold(b.run(), *expect(b))
+
+
+# ---- entries that are not finite ---------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("inf", [np.inf, -np.inf])
+@pytest.mark.parametrize("lens,rows", [([100, 1400], [64, 3]), ([76, 1400], None)])
+@pytest.mark.parametrize("window", [0, 9])
+def test_rows_that_see_an_infinite_key(ctx, kind, inf, lens, rows, window):
+    """A score of +inf makes its row NaN, as the softmax is; one of -inf leaves
+    the other keys' value or makes the row NaN; other rows are right."""
+    def poison(ks, vs):
+        ks[0][75, 0, 3] = inf
+        ks[1][1398, 0, 3] = inf
+
+    b = Batch(ctx, kind, 16, 1, 3, 64, lens, rows, seed=6, poison=poison)
+    at = {0: 75, 1: 1398}
+    got = b.run(window=window)
+    with np.errstate(invalid="ignore"):
+        want, tol = expect(b, {s: {j} for s, j in at.items()}, window=window)
+    for s, n in enumerate(lens):
+        for i in range(b.rows[s]):
+            p, r = n - b.rows[s] + i, int(b.first[s]) + i
+            for h in range(3):
+                sees = at[s] <= p and not (window and p - at[s] >= window)
+                if sees and b.q[r, h, 3] * inf > 0:
+                    assert np.isnan(got[r, h]).all(), (s, i, h)
+                elif sees and np.isnan(got[r, h]).all():
+                    continue
+                else:
+                    assert (np.abs(got[r, h] - want[r, h]) <= tol[r, h]).all(), (s, i, h)
+
+
+@pytest.mark.parametrize("lens,rows", [([100], [64]), ([75], None), ([71], None)])
+@pytest.mark.parametrize("window", [0, 4])
+def test_rows_that_see_an_infinite_step(ctx, lens, rows, window):
+    """An infinite value gives its int8 row an infinite step over zeros: NaN in
+    every channel of the rows that see it; the others are right."""
+    def poison(ks, vs):
+        vs[0][70, 0, 5] = np.inf
+
+    b = Batch(ctx, "rowi8", 16, 1, 3, 64, lens, rows, seed=7, poison=poison)
+    assert np.isnan(b.v[0][70, 0]).all()
+    got = b.run(window=window)
+    with np.errstate(invalid="ignore"):
+        want, tol = expect(b, {0: {70}}, window=window)
+    for i in range(b.rows[0]):
+        p = lens[0] - b.rows[0] + i
+        if 70 <= p and not (window and p - 70 >= window):
+            assert np.isnan(got[i]).all(), i
+        else:
+            assert (np.abs(got[i] - want[i]) <= tol[i]).all(), i
