@@ -548,7 +548,8 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_p
     int shift = 0;
     if (int rc = check(kv, &a.kv, &shift)) return rc;
     if (!n_head || n_head % kv->n_kv || n_head / kv->n_kv > 65535) return bad("n_head must be a multiple of n_kv");
-    if (n_row > 0x7FFFFFFF || n_seq > 0x7FFFFFFF || n_row * (n_head / kv->n_kv) > 0x7FFFFFFF)
+    // (sequences are counted in 64s: room for 63 more)
+    if (n_row > 0x7FFFFFFF || n_seq > 0x7FFFFFFF - 63 || n_row * (n_head / kv->n_kv) > 0x7FFFFFFF)
         return bad("too many rows or sequences");
     if (!d_first && n_row != n_seq) return bad("without row offsets every sequence has one row");
     const size_t width = n_head * kv->hd;

@@ -224,3 +224,10 @@ def test_slots_and_pages(host):
     # a slot past 2^31 in a large pool
     assert host.slot(2 ** 33 + 5, 4, 2 ** 30, C.byref(page), C.byref(off)) and page.value == 2 ** 29 and off.value == 5
     assert [host.page(i, 7) for i in (0, 6, 7, -1, 2 ** 31 - 1, -2 ** 31)] == [0, 6, -1, -1, -1, -1]
+
+
+@pytest.mark.parametrize("n_seq", [2 ** 31 - 1, 2 ** 31 - 63])
+def test_sequences_beyond_their_count_in_64s_are_refused(n_seq):
+    """Sequences are counted in 64s in 32 bits: up to 2^31 - 64 of them."""
+    assert attn(n_seq=n_seq, first=A) == fa.FRQ_ERR_ARG and "too many" in message(), message()
+    assert attn(n_seq=2 ** 31 - 64, first=A) == fa.FRQ_ERR_ARG and "null context" in message(), message()
