@@ -219,7 +219,8 @@ int frq_mm_i8_acc_dev(frq_ctx* ctx, const frq_w* w, const int8_t* d_a8, size_t m
  * bits and n rounded to f32 once, where the engines fold in f32), then
  * frq_quant_i8_dev's outputs for the rows n, which frq_mm_i8_q_dev takes.
  * x, y (m,k) row-major f32, w [k]; k up to 28672.  A NaN in n is
- * FRQ_ERR_NAN at the next frq_sync. */
+ * FRQ_ERR_NAN at the next frq_sync; rows of up to 32 channels, all of them
+ * outliers, carry it in oval, as frq_quant_i8_dev's do. */
 int frq_norm_quant_i8_dev(frq_ctx* ctx, const float* d_x, const float* d_y,
                           const float* d_w, double eps, size_t m, size_t k,
                           float* d_sum, int8_t* d_a8, float* d_sa,

@@ -136,3 +136,17 @@ def test_feeds_the_int8_linear(ctx, m):
     want = weight.mm(norm(x + y, w, 1e-6))
     got = out.numpy()
     assert np.array_equal(got, want) if m <= 16 else np.abs(got - want).max() <= 1e-5 * np.abs(want).max()
+
+
+@pytest.mark.parametrize("k", [1, 7, 32])
+def test_nan_in_rows_of_outliers_alone(ctx, k):
+    """Up to 32 channels nothing is selected: a NaN goes through as an outlier,
+    unreported, as frq_quant_i8_dev hands it on."""
+    x, y, w = data(3, k, 5)
+    x[1, k // 2] = np.nan
+    c = Call(ctx, x, None, w)
+    with np.errstate(invalid="ignore"):
+        want = quantise(ctx, norm(x, w, 1e-6))
+    for got, exp in zip(c.parts, want):
+        assert np.array_equal(got, exp, equal_nan=got.dtype.kind == "f")
+    assert np.isnan(c.parts[3][1, :k]).all()
