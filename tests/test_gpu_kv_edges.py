@@ -2,6 +2,8 @@
 or out of range, scores, caps and values of any size, entries that are not
 finite.  Held to the definition in 64 bits as test_gpu_kv.py holds the rest;
 its tolerance is derived there."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -326,3 +328,72 @@ def test_rows_that_see_an_infinite_step(ctx, lens, rows, window):
             assert np.isnan(got[i]).all(), i
         else:
             assert (np.abs(got[i] - want[i]) <= tol[i]).all(), i
+
+
+# ---- layouts ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("page", [32, 64, 128, 256, 512, 1024])
+def test_prompts_over_every_page_size(ctx, kind, page):
+    """Decode rows and prompts in one call, lengths around the ends of pages."""
+    b = Batch(ctx, kind, page, 2, 3, 64, [page - 1, page, page + 1, 2 * page + 17], [60, 1, 45, 70], seed=page)
+    hold(b.run(), *expect(b))
+    hold(b.run(window=40, cap=25.0), *expect(b, window=40, cap=25.0))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rep,rows", [(150, None), (150, [1, 3]), (129, [2, 1]), (300, [5, 1])])
+def test_many_heads_a_kv_head(ctx, kind, rep, rows):
+    """More heads than a tile has pairs: a row spans several tiles."""
+    b = Batch(ctx, kind, 16, 1, rep, 32, [77, 1300], rows, seed=rep)
+    hold(b.run(), *expect(b))
+    hold(b.run(window=20), *expect(b, window=20))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows", [[1, 2], [60, 90]])
+def test_pages_beyond_32_bits(ctx, kind, rows):
+    """Pages, and int8 steps, more than 2^32 bytes apart, written, read back and
+    attended to."""
+    rng = np.random.default_rng(5)
+    page, kv, hd, n_pages, rep = 256, 1, 64, 2, 3
+    size = {"f32": 4, "f16": 2, "rowi8": 1}[kind]
+    stride, sstride = (1 << 32) // size + 1024, (1 << 30) + 64
+    last = kv * page * hd
+    k, v = (hip.DeviceArray(((stride * (n_pages - 1) + last) * size,), np.int8) for _ in "kv")
+    ks = vs = None
+    if kind == "rowi8":
+        ks, vs = (hip.DeviceArray((sstride * (n_pages - 1) + kv * page,), np.float32) for _ in "kv")
+    c = fa.KvCache(ctx, kind, n_pages, page, kv, hd, k.ptr, v.ptr, ks and ks.ptr, vs and vs.ptr, stride, sstride)
+    b = Batch(ctx, kind, page, kv, rep, hd, [200, 250], rows, seed=3)  # the same data, beside it
+    table = np.array([[1], [0]], np.int32)
+    for s, n in enumerate(b.lens):
+        dk, dv = (hip.DeviceArray.from_numpy(x[s].astype(np.float32)) for x in (b.k, b.v))
+        slot = hip.DeviceArray.from_numpy(table[s, 0] * page + np.arange(n, dtype=np.int64))
+        c.write_dev(dk.ptr, dv.ptr, slot.ptr, n)
+        ok, ov = (hip.DeviceArray((n, kv, hd), np.float32) for _ in "kv")
+        c.read_dev(slot.ptr, n, ok.ptr, ov.ptr)
+        ctx.sync()
+        b.k[s], b.v[s] = b.p.stored(b.k[s].astype(np.float32)), b.p.stored(b.v[s].astype(np.float32))
+        assert np.array_equal(ok.numpy(), b.k[s]) and np.array_equal(ov.numpy(), b.v[s])
+    q, first, lens = (hip.DeviceArray.from_numpy(x) for x in (b.q, b.first, np.asarray(b.lens, np.int32)))
+    t, out = hip.DeviceArray.from_numpy(table), hip.DeviceArray(b.q.shape, np.float32)
+    c.attn_dev(q.ptr, b.n_row, kv * rep, t.ptr, 1, lens.ptr, 2, out.ptr, first_ptr=first.ptr)
+    ctx.sync()
+    hold(out.numpy(), *expect(b))
+
+
+def test_calls_on_another_stream(ctx):
+    """On a stream of the caller's, and back on the context's own."""
+    b = Batch(ctx, "f16", 16, 2, 3, 64, [300, 70], [70, 1])
+    want = b.check()
+    other = C.c_void_p()
+    hip._chk(hip._hip.hipStreamCreate(C.byref(other)), "hipStreamCreate")
+    try:
+        ctx.set_stream(other.value)
+        assert np.array_equal(b.run(), want)
+    finally:
+        ctx.sync()
+        ctx.set_stream(None)
+        hip._chk(hip._hip.hipStreamDestroy(other), "hipStreamDestroy")
+    assert np.array_equal(b.run(), want)
