@@ -112,9 +112,9 @@ __device__ __forceinline__ void to_lds(E* p, const Quad<E>& q) {
 // channels a lane, every load issued up front.  Keys go straight to their
 // page; values through LDS, and from there four tokens of a channel at a time
 // where the rows lie side by side (a prompt's do).  Bound by memory for long
-// prompts: 8192 rows of 4 heads of 128 channels into int8, 42 MB, in 16.8 us
-// (2.5 TB/s: the values' pieces are half lines), back in 9.7 (4.3 TB/s); one token,
-// 2.6 us, by latency.  (A token at a time both ways 29.5 us against 25.1, calls
+// prompts: 8192 rows of 4 heads of 128 channels into int8, 42 MB, in 15.9 us
+// (2.7 TB/s: the values' pieces are 32 bytes), back in 9.2 (4.6 TB/s), into f16 13.2
+// and back 11.8 (50 MB), f32 15.0 and 13.8 (67 MB); one token, 2.9 us, by latency.  (A token at a time both ways 29.5 us against 25.1, calls
 // included.)
 template <int DT, int G, int WR>
 __global__ __launch_bounds__(256) void kv_write_kernel(const Move m) {
@@ -601,7 +601,10 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_p
     // Each sequence is served by the kernel of its number of pairs; one that
     // no sequence can be for is not launched.
     // (f32 keys of over 128 channels stay with the decode kernel: three parts of
-    // q do not fit the registers; 8 heads of 256, 2048 rows: 1.6 ms against 1.9.)
+    // q leave the prompt kernel one wave a SIMD.  2048 rows of 8 heads over 4, the
+    // decode kernel against the prompt kernel: 256 channels 288, 340 us over
+    // themselves, 72, 78 at 600 rows, 1612, 1508 over 8192 tokens; 192 channels 225,
+    // 202 and 1280, 676.  Widths of an odd number of 32s do not fit the LDS.)
     const bool prompts = d_first && n_row * (size_t)a.c.rep > (size_t)DEC_PAIRS &&
                          !(kv->dtype == FRQ_DT_F32 && kv->hd > 128);
     a.c.max_pairs = prompts ? DEC_PAIRS : 0x7FFFFFFF;

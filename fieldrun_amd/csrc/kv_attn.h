@@ -18,13 +18,14 @@
 // transposed (hd, page), so both operands are 16-byte loads straight from the
 // pages and nothing goes through LDS.
 //
-// 32-bit exactness on the 16-bit matrix cores: the cache's f16 and int8 entries
-// are exact f16; an f32 q row, scaled by a power of two to below 2, is the sum
-// of two f16 (22 bits and more), likewise the probabilities (scaled by 2^11,
-// so that what f16 cannot hold of them is below 2^-36 of the largest); the
-// products of both halves add up in the f32 accumulators.  An f32 cache uses
-// the f32 matrix cores for decoding, where memory bounds the call, and three
-// bf16 parts of both operands for prompts.
+// On the 16-bit matrix cores: the cache's f16 and int8 entries are exact f16;
+// an f32 q row, scaled by a power of two to below 2, is the sum of two f16, 22
+// bits of its larger entries and down to 2^-25 of the largest for all (f32 would
+// hold more of a small entry that meets a large key's), likewise the
+// probabilities (scaled by 2^11, so that what f16 cannot hold of them is below
+// 2^-36 of the largest); the products of both halves add up in the f32
+// accumulators.  An f32 cache uses the f32 matrix cores for decoding, where
+// memory bounds the call, and three bf16 parts of both operands for prompts.
 #pragma once
 
 #include "frq_internal.h"
@@ -426,8 +427,8 @@ __device__ __forceinline__ void load_q(const float* q, float sign, int g, QOp<DT
 // and a barrier a tile), page ids a tile ahead.  With two workgroups of four
 // waves a CU (the kernel alone; a large copy reaches 4.8 TB/s): f16, one
 // sequence of 131071 tokens, 8 kv heads of 128 channels, 95 us, 5.6 TB/s; f32, a
-// window of 4096, 16 sequences, 4 kv heads of 256, 111 us, 4.6 TB/s; int8, 48
-// sequences of up to 6001, 4 kv heads of 128 with 7 heads each, 42 us, 3.5 TB/s:
+// window of 4096, 16 sequences, 4 kv heads of 256, 108 us, 4.8 TB/s; int8, 48
+// sequences of up to 6001, 4 kv heads of 128 with 7 heads each, 41 us, 3.7 TB/s:
 // there the unpacking, the steps and the softmax of half the bytes keep the
 // vector units busy 40% of the time, and waves wait the other half.  Slower
 // (batch, long, window): loads past the caches 47, 110, 122 us; eight waves a
@@ -795,15 +796,15 @@ __device__ __forceinline__ int pick4(int j, int a, int b, int c, int d) {
 // Bound by the matrix cores, and by the clock under them (1.7 GHz, the cores
 // busy half the time): f16, 28 heads of 128 channels over 4, 2048 rows after
 // 6144 cached tokens, is 210 GFLOP of the formula, which the two halves of q
-// and p make 420, in 490 us; int8, 7 sequences of up to 1501 tokens, 24 GFLOP,
-// in 111.  One f16 for p would cost its bits below 2^-11.  128 pairs a workgroup
+// and p make 420, in 464 us; int8, 7 sequences of up to 1501 tokens, 24 GFLOP,
+// in 101.  One f16 for p would cost its bits below 2^-11.  128 pairs a workgroup
 // let two fit a CU (64 KB of LDS, 256 registers); equal priorities of both 503 us
 // against 481.
 //
 // An f32 cache is staged as three bf16 (exact: 8 bits each), q and the
 // probabilities likewise, and a product is the six of theirs that reach 2^-24
 // of it: six matrix instructions, where the f32 ones would take the time of
-// sixteen (the f16 case over an f32 cache 1671 us against 2768).  Its tiles are
+// sixteen (the f16 case over an f32 cache 1637 us against 2768).  Its tiles are
 // loaded into registers and have one buffer.
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ void split8(const float (&x)[8], b8 (&y)[3]) {
@@ -1422,7 +1423,7 @@ __device__ __forceinline__ void redo_share(const Args& a, const Record& it, int 
 // outputs, so that a long sequence's parts are read by many workgroups.
 // Threads are (float4 of the share, run of chunks); each folds its chunks,
 // then the runs are merged pairwise, always in the same order.  Bound by
-// latency: 4.5 to 5.5 us at 60 to 280 chunks of 16 pairs of 128 channels, 11 us for
+// latency: 4.5 to 5.5 us at 60 to 280 chunks of 16 pairs of 128 channels, 10 us for
 // 7 prompts' 128 pairs (a float4 a thread at a time: 585 rows of 8 heads of 256
 // 64 us in all against 57).
 template <int TP>

@@ -9,9 +9,9 @@
 // magnitudes puts it into LDS, over the candidates it has done with.
 //
 // Bound by the selection's passes over the registers, with the loads of other
-// workgroups behind them: 4096 rows of 4096 channels, 219 MB, in 63 us (3.5
+// workgroups behind them: 4096 rows of 4096 channels, 219 MB, in 61 us (3.6
 // TB/s; a large copy reaches 4.8), waves waiting for memory and at barriers
-// 57% of their time; one row of 3584 in 7.1 us, by latency.  With the row n
+// 57% of their time; one row of 3584 in 7.7 us, by latency.  With the row n
 // always in LDS the large case took 66 us.
 #include "quant_core.h"
 
@@ -193,8 +193,10 @@ extern "C" int frq_norm_quant_i8_dev(frq_ctx* ctx, const float* d_x, const float
     hipStream_t s = (hipStream_t)frq_get_stream(ctx);
     const size_t k4 = (k + 3) / 4;
     hipError_t e;
-    // 256 threads a row; few rows of 2049 .. 4096 channels 512 (K = 3584: one row
-    // 7.0 us against 7.7; 4096 rows of 4096 69.6 against 63.5)
+    // 256 threads a row; up to 256 rows, a row a CU, of 2049 .. 4096 channels 512
+    // (512 against 256, calls one after the other: K = 2304 one row 7.0, 7.5 us, 256
+    // rows 8.1, 8.3, 512 rows 11.2, 9.6; K = 4096 7.3, 8.0, then 8.8, 9.2, then 12.8,
+    // 11.2; 4096 rows 58.1, 51.5)
     if (m <= 256 && k4 > 512 && k4 <= 1024) e = launch<2, 512>(a, m, s);
     else if (k4 <= 256) e = launch<1, 256>(a, m, s);
     else if (k4 <= 512) e = launch<2, 256>(a, m, s);
