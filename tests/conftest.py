@@ -1,3 +1,4 @@
+import gc
 import os
 import sys
 
@@ -20,3 +21,11 @@ def ctx():
     c = fa.Context(0)
     yield c
     c.close()
+
+
+@pytest.fixture(autouse=True, scope="module")
+def memory_given_back():
+    """What a file's tests leave in reference cycles, device memory with it, is
+    freed at its end and not inside a later test."""
+    yield
+    gc.collect()

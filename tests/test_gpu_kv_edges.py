@@ -3,6 +3,7 @@ or out of range, scores, caps and values of any size, entries that are not
 finite.  Held to the definition in 64 bits as test_gpu_kv.py holds the rest;
 its tolerance is derived there."""
 import ctypes as C
+import gc
 
 import numpy as np
 import pytest
@@ -13,6 +14,13 @@ from test_gpu_kv import Batch, put
 
 pytestmark = pytest.mark.gpu
 KINDS = ["f32", "f16", "rowi8"]
+
+
+@pytest.fixture(autouse=True)
+def freed():
+    """A batch refers to itself: its device memory is given back here."""
+    yield
+    gc.collect()
 
 
 def expect(b, gone=None, scale=None, cap=0.0, window=0):
