@@ -113,9 +113,9 @@ __device__ __forceinline__ void to_lds(E* p, const Quad<E>& q) {
 // page; values through LDS, and from there four tokens of a channel at a time
 // where the rows lie side by side (a prompt's do).  Bound by memory for long
 // prompts: 8192 rows of 4 heads of 128 channels into int8, 42 MB, in 15.9 us
-// (2.7 TB/s: the values' pieces are 32 bytes), back in 9.2 (4.6 TB/s), into f16 13.2
-// and back 11.8 (50 MB), f32 15.0 and 13.8 (67 MB); one token, 2.9 us, by latency.  (A token at a time both ways 29.5 us against 25.1, calls
-// included.)
+// (2.7 TB/s: the values' pieces are 32 bytes), back in 9.2 (4.6 TB/s), into f16
+// 13.2 and back 11.8 (50 MB), f32 15.0 and 13.8 (67 MB); one token, 2.9 us, by
+// latency.  (A token at a time both ways 29.5 us against 25.1, calls included.)
 template <int DT, int G, int WR>
 __global__ __launch_bounds__(256) void kv_write_kernel(const Move m) {
     using E = Elem<DT>;

@@ -692,7 +692,8 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
         if (more) load_v(next);
     }
     if constexpr (!T::I8) {
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0) != 0, 0)) {  // rare: the keys of those tiles again, one by one
+        // rare: the keys of those tiles again, one by one
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0) != 0, 0)) {
             for (int key = beg; key < end; ++key) {
                 const int t0 = (key - beg) / KT, base = beg + t0 * KT;
                 if (t0 % NW != wave || (base >= lo_b && base + KT - 1 <= pos_a)) continue;
@@ -1298,7 +1299,8 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
                 if (c >= hd) continue;
                 F4 y;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) y.v[j] = (I8 ? __builtin_ldexpf(o[t][i + j], ev - W_EXP - down) : o[t][i + j]) * r;
+                for (int j = 0; j < 4; ++j)
+                    y.v[j] = (I8 ? __builtin_ldexpf(o[t][i + j], ev - W_EXP - down) : o[t][i + j]) * r;
                 *reinterpret_cast<F4*>(d + c) = y;
             }
     } else {
@@ -1375,7 +1377,8 @@ __device__ __forceinline__ void redo_share(const Args& a, const Record& it, int 
                 z[u] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (64 * i + lane < hd) z[u] = __builtin_fmaf(x[i], entry<DT>(k + (u * hd + 64 * i + lane) * SZ), z[u]);
+                    if (64 * i + lane < hd)
+                        z[u] = __builtin_fmaf(x[i], entry<DT>(k + (u * hd + 64 * i + lane) * SZ), z[u]);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -1431,7 +1434,8 @@ __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so,
     const int n_kv = a.c.n_kv, kvh = block % n_kv;
     const Record it = a.rec[block / n_kv];
     if (it.chunks <= 1) {
-        if (__builtin_expect(it.seq < 0, 0)) redo_share<TP>(a, it, kvh, 0, min(TP, it.rows * a.c.rep - it.tile * TP) * (a.kv.hd / 4));
+        if (__builtin_expect(it.seq < 0, 0))
+            redo_share<TP>(a, it, kvh, 0, min(TP, it.rows * a.c.rep - it.tile * TP) * (a.kv.hd / 4));
         return;
     }
     if (it.slot < 0 || it.slot + it.chunks > a.slots) return;

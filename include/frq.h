@@ -257,15 +257,15 @@ int frq_kv_read_dev(frq_ctx* ctx, const frq_kv* kv, const int64_t* d_slot,
  * a row, rows q_pitch apart) reads kv head h / (n_head / n_kv):
  *   z_j = scale q . k_j, cap > 0: cap tanh(z_j / cap);  out = softmax(z) v
  * (forward_block, src/gemma.rs:252-277) with f32 scores and sums over each run
- * of keys, the runs joined in a fixed order (a score beyond f32 makes its row
- * NaN); a row that sees no token gets zeros.  Rows
- * outside d_first[0] .. d_first[n_seq] - 1 stay as they were; d_out and d_q
- * lie apart.  What a row does not see does not touch it, whatever it holds
- * (pages behind the windows of all of a sequence's rows may be gone: their
- * entries in d_pages are anything); a row that sees an infinity or a NaN gets
- * infinities or NaN, or, where an infinite key leaves a score of -inf, possibly
- * the formula's value.  Tokens under a page id out of range are not seen; a
- * length out of range counts as 0, and rows whose offsets are stay as they were.
+ * of keys, the runs joined in a fixed order (a score beyond f32 can make its
+ * row NaN); a row that sees no token gets zeros.  Rows outside d_first[0] ..
+ * d_first[n_seq] - 1 stay as they were; d_out and d_q lie apart.  What a row
+ * does not see does not touch it, whatever it holds (pages behind the windows
+ * of all of a sequence's rows may be gone: their entries in d_pages are
+ * anything); a row that sees an infinity or a NaN gets infinities or NaN, or,
+ * where an infinite key leaves a score of -inf, possibly the formula's value.
+ * Tokens under a page id out of range are not seen; a length out of range
+ * counts as 0, and rows whose offsets are out of range stay as they were.
  * d_ws: frq_kv_attn_ws bytes of device memory, 16-byte aligned, for this call
  * alone until it is done (calls that may overlap, such as two graphs' replays,
  * have one each); NULL takes the context's, which a call under graph capture

@@ -160,6 +160,41 @@ def test_gone_pages_beside_values_that_are_not_finite(ctx, kind):
     assert (got[34:, :, 5] == np.inf).all()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows", [[3, 4, 2], [60, 70, 80]])
+@pytest.mark.parametrize("many", [False, True])
+def test_bad_lengths_and_offsets_stay_with_their_sequences(ctx, kind, rows, many):
+    """A length out of range counts as 0, its rows are zeros; rows between
+    offsets out of range stay as they were; the others are right."""
+    lens = [300, 90, 200] + [5] * (100 if many else 0)
+    rows = rows + [1] * (len(lens) - 3)
+    b = Batch(ctx, kind, 16, 1, 3, 64, lens, rows, seed=11)
+    clean = b.run()
+    hold(clean, *expect(b))
+    at = b.first
+    want, tol = expect(b)
+    for change, value in (("length", b.width * 16 + 1), ("length", -1), ("offset", b.n_row + 1), ("offset", -1)):
+        n, f = np.asarray(lens, np.int32), b.first.copy()
+        if change == "length":
+            n[1] = value
+        else:
+            f[2] = value  # the end of sequence 1 and the beginning of 2
+        put(b.dev[1], n)
+        put(b.dev[2], f)
+        with pytest.raises(fa.FrqError) as e:
+            b.run()
+        assert e.value.code == fa.FRQ_ERR_ARG
+        ctx.sync()
+        got = b.do.numpy()[:b.n_row].reshape(clean.shape)
+        lost = slice(at[1], at[2] if change == "length" else at[3])
+        assert (got[lost] == (0.0 if change == "length" else 7.0)).all()
+        # (the others' keys are cut into other runs than before: not the same bits)
+        hold(*(np.delete(x, np.r_[lost], 0) for x in (got, want, tol)))
+        put(b.dev[1], np.asarray(lens, np.int32))
+        put(b.dev[2], b.first)
+    assert np.array_equal(b.run(), clean)
+
+
 def test_a_bad_index_and_a_nan_are_both_reported(ctx):
     b = Batch(ctx, "f16", 16, 1, 2, 32, [20])
     b.run()
