@@ -137,6 +137,31 @@ def test_pages_out_of_range_take_no_part(ctx, kind, owner, rows, window, cap):
     assert np.array_equal(got[:b.first[1]], clean[:b.first[1]])
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd,kv,rep,many", [(16, 2, 5, False), (80, 3, 20, False), (256, 1, 3, False), (48, 2, 3, True)])
+def test_gone_pages_at_any_width(ctx, kind, hd, kv, rep, many):
+    """Strided pages, heads of every kind of width, decode and prompt rows in one
+    call, on both sides of 64 sequences; the same bits again."""
+    lens = [400, 150, 90] + [7] * (80 if many else 0)
+    rows = [1, 60, 2] + [1] * (len(lens) - 3)
+    b = Batch(ctx, kind, 16, kv, rep, hd, lens, rows, seed=hd, pad=1)
+    table = b.table.copy()
+    for s, pages in ((0, (2, 24)), (1, (0, 8)), (2, (5,))):
+        table[s, list(pages)] = b.p.n_pages + s
+    gone = {s: {j for p in np.flatnonzero(table[s, :-(-lens[s] // 16)] >= b.p.n_pages) for j in range(16 * p, 16 * p + 16)}
+            for s in range(3)}
+    set_table(b, table)
+    runs = []
+    for _ in range(2):
+        with pytest.raises(fa.FrqError) as e:
+            b.run(cap=20.0)
+        assert e.value.code == fa.FRQ_ERR_ARG
+        ctx.sync()
+        runs.append(b.do.numpy()[:b.n_row].reshape(b.n_row, kv * rep, hd))
+    hold(runs[0], *expect(b, gone, cap=20.0))
+    assert np.array_equal(runs[0], runs[1])
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16"])
 def test_gone_pages_beside_values_that_are_not_finite(ctx, kind):
     """A seen value that is not finite reaches the rows that see it and no
