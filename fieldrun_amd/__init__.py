@@ -105,6 +105,7 @@ SIGNATURES = {
     "frq_norm_quant_i8_dev": (_I, [_P, _P, _P, _P, C.c_double, _S, _S, _P, _P, _P, _P, _P]),
     "frq_kv_write_dev": (_I, [_P, _P, _P, _P, _S, _P, _S]),
     "frq_kv_read_dev": (_I, [_P, _P, _P, _S, _P, _P, _S]),
+    "frq_kv_append_dev": (_I, [_P, _P, _P, _P, _S, _S, _P, _P, _S, _P, _S]),
     "frq_kv_attn_ws": (_S, [_P, _S, _S, _S, _S]),
     "frq_kv_attn_dev": (_I, [_P, _P, _P, _S, _S, _S, _P, _S, _P, _P, _S, C.c_double, C.c_double, _S, _P, _S, _P, _S]),
     "frq_gemma_predict": (_I, [_P, _P, _P, _S, _P, _P]),
@@ -333,6 +334,24 @@ class _Kv(C.Structure):
                 ("v_scale", C.c_void_p), ("page_stride", C.c_size_t), ("scale_stride", C.c_size_t)]
 
 
+class _Rotary(C.Structure):
+    _fields_ = [("bias", C.c_void_p), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("eps", C.c_double),
+                ("freq", C.c_void_p), ("rot", C.c_size_t), ("pairs", C.c_int)]
+
+
+class Rotary:
+    """What happens to fused q | k | v rows before attention (frq_rotary), on
+    device pointers: biases, the norm of every query and key head (gains of hd
+    channels), and the rotation of each head's first rot channels by position
+    times freq (rot / 2 radians, float64), planes of halves or (pairs) of
+    neighbours.  The memory stays the caller's and outlives the object's calls."""
+
+    def __init__(self, rot: int, freq_ptr: int | None, pairs: bool = False, bias_ptr: int | None = None,
+                 q_norm_ptr: int | None = None, k_norm_ptr: int | None = None, eps: float = 1e-6):
+        self.desc = _Rotary(bias_ptr, q_norm_ptr, k_norm_ptr, eps, freq_ptr, rot, int(pairs))
+        self._ref = C.byref(self.desc)
+
+
 class KvCache:
     """A paged key / value cache in the caller's device memory (frq_kv):
     k (n_pages, n_kv, page, hd), v (n_pages, n_kv, hd, page) of kind 'f32',
@@ -364,6 +383,17 @@ class KvCache:
         """The slots' keys and values back in f32."""
         _check(lib.frq_kv_read_dev(self.ctx.h, self._ref, slot_ptr, n, k_ptr, v_ptr,
                                    self.row if pitch is None else pitch))
+
+    def append_dev(self, qkv_ptr: int, n_head: int, pos_ptr: int | None, slot_ptr: int, n: int, q_ptr: int,
+                   how: Rotary, pitch: int | None = None, q_pitch: int | None = None):
+        """n fused q | k | v rows: biases, norms and rotation as `how` says,
+        by the positions of pos_ptr (int32); q to q_ptr in f32 (qkv_ptr itself
+        with its pitch will do), keys and values into the slots of slot_ptr
+        (int64), on the context stream.  Pitches default to dense rows."""
+        hd = self.desc.hd
+        _check(lib.frq_kv_append_dev(self.ctx.h, self._ref, how._ref, qkv_ptr,
+                                     n_head * hd + 2 * self.row if pitch is None else pitch, n_head, pos_ptr, slot_ptr,
+                                     n, q_ptr, n_head * hd if q_pitch is None else q_pitch))
 
     def attn_ws_bytes(self, n_row: int, n_head: int, n_seq: int, pages_pitch: int) -> int:
         """Bytes of the workspace attn_dev takes for such a call."""

@@ -83,6 +83,21 @@ typedef struct frq_kv {
     size_t scale_stride;  /* steps between pages, 0: dense                    */
 } frq_kv;
 
+/* What happens to fused q | k | v rows before attention (plain data, read
+ * during a call; the arrays are device memory): biases, the norm of every head
+ * and the rotation by position. */
+typedef struct frq_rotary {
+    const float* bias;    /* [(n_head + 2 n_kv) hd], or NULL                  */
+    const float* q_norm;  /* [hd] gains of the query heads' norm, or NULL     */
+    const float* k_norm;  /* [hd] of the key heads', or NULL                  */
+    double eps;           /* the norms'                                       */
+    const double* freq;   /* [rot / 2] radians a position                     */
+    size_t rot;           /* channels turned, the first of each head: a
+                             multiple of 8 up to hd; 0: none                  */
+    int pairs;            /* plane j: 0 channels (j, j + rot / 2), 1 the
+                             neighbours (2 j, 2 j + 1)                        */
+} frq_rotary;
+
 /* Last error message of the calling thread ("" when none). */
 const char* frq_last_error(void);
 /* Library version string. */
@@ -247,6 +262,20 @@ int frq_kv_write_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_k,
                      size_t n);
 int frq_kv_read_dev(frq_ctx* ctx, const frq_kv* kv, const int64_t* d_slot,
                     size_t n, float* d_k, float* d_v, size_t pitch);
+/* Fused q | k | v rows (row i at d_qkv + i * pitch: n_head query heads, n_kv key
+ * heads, n_kv value heads, of hd each) made ready and appended in one launch:
+ *   y = x + bias;  q, k with gains: y = y / sqrt(mean(y^2) + eps) * gain;
+ *   q, k: plane (a, b) = (a cos t - b sin t, b cos t + a sin t), t = d_pos[i] freq[j]
+ * (Rope::proj, head_norm and rope, src/rope.rs:72-117; src/gemma.rs:79-94), in 64
+ * bits and rounded to f32 once (angles up to 2^30 radians).  q goes to d_q (row
+ * i at d_q + i * q_pitch; d_q may be d_qkv with its pitch, else it lies apart),
+ * keys and values into their slots as frq_kv_write_dev puts them there; a row
+ * without a place leaves its q alone.  d_pos (may be below 0) and freq may be
+ * NULL where rot is 0. */
+int frq_kv_append_dev(frq_ctx* ctx, const frq_kv* kv, const frq_rotary* how,
+                      const float* d_qkv, size_t pitch, size_t n_head,
+                      const int32_t* d_pos, const int64_t* d_slot, size_t n,
+                      float* d_q, size_t q_pitch);
 /* Attention of n_row query rows of n_seq sequences over their pages: sequence
  * s holds d_len[s] cached tokens, token j in page d_pages[s * pages_pitch +
  * j / page], and asks with the rows d_first[s] .. d_first[s + 1] - 1 of d_q
