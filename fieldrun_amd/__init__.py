@@ -108,6 +108,10 @@ SIGNATURES = {
     "frq_kv_append_dev": (_I, [_P, _P, _P, _P, _S, _S, _P, _P, _S, _P, _S]),
     "frq_kv_attn_ws": (_S, [_P, _S, _S, _S, _S]),
     "frq_kv_attn_dev": (_I, [_P, _P, _P, _S, _S, _S, _P, _S, _P, _P, _S, C.c_double, C.c_double, _S, _P, _S, _P, _S]),
+    "frq_kv_attn_sink_dev": (_I, [_P, _P, _P, _S, _S, _S, _P, _S, _P, _P, _S, C.c_double, C.c_double, _S, _S, _P, _S, _P,
+                                  _S]),
+    "frq_kv_attn_tree_dev": (_I, [_P, _P, _P, _S, _S, _S, _P, _S, _P, _P, _S, C.c_double, C.c_double, _S, _S, _P, _S, _P,
+                                  _S, _P, _S]),
     "frq_gemma_predict": (_I, [_P, _P, _P, _S, _P, _P]),
 }
 
@@ -402,16 +406,25 @@ class KvCache:
     def attn_dev(self, q_ptr: int, n_row: int, n_head: int, pages_ptr: int, pages_pitch: int, len_ptr: int,
                  n_seq: int, out_ptr: int, first_ptr: int | None = None, scale: float | None = None,
                  cap: float = 0.0, window: int = 0, q_pitch: int | None = None, out_pitch: int | None = None,
-                 ws_ptr: int | None = None, ws_bytes: int = 0):
+                 ws_ptr: int | None = None, ws_bytes: int = 0, sinks: int = 0, tree_ptr: int | None = None,
+                 tree_pitch: int = 1):
         """Attention of n_row query rows of n_seq sequences over the cache
         (frq_kv_attn_dev); scale defaults to 1 / sqrt(hd), pitches to dense
-        rows, first_ptr None to one row a sequence."""
+        rows, first_ptr None to one row a sequence.  sinks: first tokens that
+        stay seen beside a window (frq_kv_attn_sink_dev); tree_ptr: the rows
+        are drafted tokens, each seeing those of its bit mask of tree_pitch
+        64-bit words (frq_kv_attn_tree_dev)."""
         hd = self.desc.hd
         wide = n_head * hd
-        _check(lib.frq_kv_attn_dev(self.ctx.h, self._ref, q_ptr, wide if q_pitch is None else q_pitch, n_row, n_head,
-                                   pages_ptr, pages_pitch, len_ptr, first_ptr, n_seq,
-                                   hd ** -0.5 if scale is None else scale, cap, window, out_ptr,
-                                   wide if out_pitch is None else out_pitch, ws_ptr, ws_bytes))
+        args = (self.ctx.h, self._ref, q_ptr, wide if q_pitch is None else q_pitch, n_row, n_head, pages_ptr,
+                pages_pitch, len_ptr, first_ptr, n_seq, hd ** -0.5 if scale is None else scale, cap, window)
+        to = (out_ptr, wide if out_pitch is None else out_pitch, ws_ptr, ws_bytes)
+        if tree_ptr is not None:
+            _check(lib.frq_kv_attn_tree_dev(*args, sinks, tree_ptr, tree_pitch, *to))
+        elif sinks:
+            _check(lib.frq_kv_attn_sink_dev(*args, sinks, *to))
+        else:
+            _check(lib.frq_kv_attn_dev(*args, *to))
 
 
 class Weight:

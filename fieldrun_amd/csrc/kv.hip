@@ -159,11 +159,12 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const Move m) {
 }
 
 // The decode launch's tiles, then the prompt launch's (grid_b 0: none).
+template <bool EX>
 __global__ __launch_bounds__(256) void kv_join_kernel(const Args a, const Args b, unsigned grid_a) {
     __shared__ f4 so[256];
     __shared__ float sm[256], sl[256];
-    if (blockIdx.x < grid_a) join_item<16>(a, blockIdx.x, so, sm, sl);
-    else join_item<128>(b, blockIdx.x - grid_a, so, sm, sl);
+    if (blockIdx.x < grid_a) join_item<16, EX>(a, blockIdx.x, so, sm, sl);
+    else join_item<128, EX>(b, blockIdx.x - grid_a, so, sm, sl);
 }
 
 // The plans of many sequences (workgroup 0: the decode launch's, 1: the
@@ -319,6 +320,130 @@ Plan plan_of(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq) {
     return p;
 }
 
+struct More {  // than every attention call has
+    size_t sinks;
+    const uint64_t* tree;
+    size_t tree_pitch;
+    bool trees;
+};
+int attend(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, size_t n_row, size_t n_head,
+           const int32_t* d_pages, size_t pages_pitch, const int32_t* d_len, const int32_t* d_first, size_t n_seq,
+           double scale, double cap, size_t window, const More& more, float* d_out, size_t out_pitch, void* d_ws,
+           size_t ws_bytes) {
+    Args a{};
+    int shift = 0;
+    if (int rc = check(kv, &a.kv, &shift)) return rc;
+    if (!n_head || n_head % kv->n_kv || n_head / kv->n_kv > 65535) return bad("n_head must be a multiple of n_kv");
+    // (sequences are counted in 64s: room for 63 more)
+    if (n_row > 0x7FFFFFFF || n_seq > 0x7FFFFFFF - 63 || n_row * (n_head / kv->n_kv) > 0x7FFFFFFF)
+        return bad("too many rows or sequences");
+    if (!d_first && n_row != n_seq) return bad("without row offsets every sequence has one row");
+    const size_t width = n_head * kv->hd;
+    if (q_pitch < width || out_pitch < width || q_pitch > ((size_t)1 << 40) || out_pitch > ((size_t)1 << 40))
+        return bad("pitch is below the heads' width");
+    // (keys past a sequence's last are counted to the end of a tile: room below 2^31)
+    if (pages_pitch > 0x7FFFFFFF || (pages_pitch << shift) > 0x7FFFFFFF - 1024)
+        return bad("a table holds up to 2^31 - 1024 tokens");
+    if (window > 0x7FFFFFFF) window = 0;  // wider than any sequence
+    // (sinks beyond every table: all is seen)
+    size_t sinks = window ? more.sinks : 0;
+    if (sinks > (pages_pitch << shift)) window = sinks = 0;
+    if (more.trees && (!more.tree_pitch || more.tree_pitch > ((size_t)1 << 40))) return bad("a tree has masks of a word or more");
+    if (!(scale >= -1e30 && scale <= 1e30) || !(cap >= 0.0 && cap <= 1e30))
+        return bad("scale must be within 1e30, cap 0 or positive");
+    if (n_row && n_seq && (!d_q || !d_out || !d_len || (!d_pages && pages_pitch))) return bad("null pointer");
+    if (more.trees && n_row && n_seq && !more.tree) return bad("null pointer");
+    if (d_ws && ((uintptr_t)d_ws & 15)) return bad("the workspace must be 16-byte aligned");
+    if (!ctx) return bad("null context");
+    if (!n_row || !n_seq) return FRQ_OK;
+    const Plan plan = plan_of(kv, n_row, n_head, n_seq);
+    const size_t need = plan.bytes;
+    if (d_ws && ws_bytes < need) return bad("the workspace is below frq_kv_attn_ws");
+    Guard g(ctx_device(ctx));
+    hipStream_t s = (hipStream_t)frq_get_stream(ctx);
+    if (!d_ws) {
+        // the context's workspace may move with a later call: a graph would
+        // keep its old address
+        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+        const hipError_t e = hipStreamIsCapturing(s, &st);
+        if (e != hipSuccess) return hip_bad(e, "hipStreamIsCapturing");
+        if (st != hipStreamCaptureStatusNone) return bad("under graph capture the caller gives the workspace");
+        if (int rc = ctx_ws(ctx, need, &d_ws)) return rc;
+    }
+    a.c = plan.dec;
+    a.c.len = d_len;
+    a.c.first = d_first;
+    a.c.width = (int)pages_pitch;
+    a.c.shift = shift;
+    a.c.window = (int)window;
+    a.c.sinks = (int)sinks;
+    a.c.sink_span = sink_keys((int64_t)sinks, 32);
+    a.c.tree = more.tree;
+    a.c.tree_pitch = (int64_t)more.tree_pitch;
+    a.q = d_q;
+    a.q_pitch = (int64_t)q_pitch;
+    a.out_pitch = (int64_t)out_pitch;
+    a.pages_pitch = (int64_t)pages_pitch;
+    a.pages = d_pages;
+    a.out = d_out;
+    a.err = ctx_err(ctx);
+    a.scale = scale == 0.0 ? 1.0f : (float)(scale < 0.0 ? -scale : scale);
+    a.sign = scale == 0.0 ? 0.0f : scale < 0.0 ? -1.0f : 1.0f;
+    // (below 2^-27 every cap gives weights within a rounding of equal ones; there
+    // score_scale's 2^100 over the cap would leave f32, or the cap be zero in it)
+    a.cap = cap > 0.0 && cap < 7.450580596923828e-9 ? 7.450580596923828e-9f : (float)cap;
+    a.dtype = kv->dtype;
+    // Each sequence is served by the kernel of its number of pairs; one that
+    // no sequence can be for is not launched.
+    // (f32 keys of over 128 channels stay with the decode kernel: three parts of
+    // q leave the prompt kernel one wave a SIMD.  2048 rows of 8 heads over 4, the
+    // decode kernel against the prompt kernel: 256 channels 288, 340 us over
+    // themselves, 72, 78 at 600 rows, 1612, 1508 over 8192 tokens; 192 channels 225,
+    // 202 and 1280, 676.  Widths of an odd number of 32s do not fit the LDS.)
+    const bool prompts = d_first && n_row * (size_t)a.c.rep > (size_t)DEC_PAIRS &&
+                         !(kv->dtype == FRQ_DT_F32 && kv->hd > 128);
+    a.c.max_pairs = prompts ? DEC_PAIRS : 0x7FFFFFFF;
+    char* ws = (char*)d_ws;
+    a.rec = (Record*)(ws + plan.rec_dec);
+    a.part = (float*)(ws + plan.part_dec);
+    a.slots = max_slots(DEC_TARGET, a.c.n_kv);
+    Args b = a;
+    b.c.min_pairs = plan.prompt.min_pairs;
+    b.c.max_pairs = plan.prompt.max_pairs;
+    b.c.tp = plan.prompt.tp;
+    b.c.target = plan.prompt.target;
+    b.c.min_chunk = plan.prompt.min_chunk;
+    b.c.sink_span = sink_keys((int64_t)sinks, 64);
+    b.rec = (Record*)(ws + plan.rec_prompt);
+    b.part = (float*)(ws + plan.part_prompt);
+    b.slots = n_row > n_seq ? max_slots(b.c.target, a.c.n_kv) : 0;
+    const int64_t ga = max_items(a.c) * a.c.n_kv, gb = prompts ? max_items(b.c) * b.c.n_kv : 0;
+    if (ga + gb > 0x7FFFFFFF) return bad("too many rows or sequences");
+    const Launch la{(unsigned)ga, s}, lb{(unsigned)gb, s};
+    hipError_t e = hipSuccess;
+    if (n_seq > (size_t)PLAN_SEQS) {
+        int32_t *pa = (int32_t*)(ws + plan.plan_dec), *pb = (int32_t*)(ws + plan.plan_prompt);
+        kv_plan_kernel<<<dim3(prompts ? 2 : 1), dim3(1024), 0, s>>>(a.c, b.c, pa, pb, a.err);
+        e = hipGetLastError();
+        if (e != hipSuccess) return hip_bad(e, "launch kv_plan");
+        a.c.plan = pa;
+        b.c.plan = pb;
+    }
+    const bool ex = sinks || more.trees, f32 = kv->dtype == FRQ_DT_F32, f16 = kv->dtype == FRQ_DT_F16;
+    if (ex) e = f32 ? launch_decode_ex_f32(a, la) : f16 ? launch_decode_ex_f16(a, la) : launch_decode_ex_i8(a, la);
+    else e = f32 ? launch_decode_f32(a, la) : f16 ? launch_decode_f16(a, la) : launch_decode_i8(a, la);
+    if (e != hipSuccess) return hip_bad(e, "launch kv_decode");
+    if (prompts) {
+        if (ex) e = f32 ? launch_prompt_ex_f32(b, lb) : f16 ? launch_prompt_ex_f16(b, lb) : launch_prompt_ex_i8(b, lb);
+        else e = f32 ? launch_prompt_f32(b, lb) : f16 ? launch_prompt_f16(b, lb) : launch_prompt_i8(b, lb);
+        if (e != hipSuccess) return hip_bad(e, "launch kv_prompt");
+    }
+    if (ex) kv_join_kernel<true><<<dim3((unsigned)(ga + gb)), dim3(256), 0, s>>>(a, b, (unsigned)ga);
+    else kv_join_kernel<false><<<dim3((unsigned)(ga + gb)), dim3(256), 0, s>>>(a, b, (unsigned)ga);
+    e = hipGetLastError();
+    return e == hipSuccess ? FRQ_OK : hip_bad(e, "launch kv_join");
+}
+
 }  // namespace
 }  // namespace kv
 }  // namespace frq
@@ -368,108 +493,24 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_p
                     const int32_t* d_pages, size_t pages_pitch, const int32_t* d_len, const int32_t* d_first,
                     size_t n_seq, double scale, double cap, size_t window, float* d_out, size_t out_pitch, void* d_ws,
                     size_t ws_bytes) {
-    Args a{};
-    int shift = 0;
-    if (int rc = check(kv, &a.kv, &shift)) return rc;
-    if (!n_head || n_head % kv->n_kv || n_head / kv->n_kv > 65535) return bad("n_head must be a multiple of n_kv");
-    // (sequences are counted in 64s: room for 63 more)
-    if (n_row > 0x7FFFFFFF || n_seq > 0x7FFFFFFF - 63 || n_row * (n_head / kv->n_kv) > 0x7FFFFFFF)
-        return bad("too many rows or sequences");
-    if (!d_first && n_row != n_seq) return bad("without row offsets every sequence has one row");
-    const size_t width = n_head * kv->hd;
-    if (q_pitch < width || out_pitch < width || q_pitch > ((size_t)1 << 40) || out_pitch > ((size_t)1 << 40))
-        return bad("pitch is below the heads' width");
-    // (keys past a sequence's last are counted to the end of a tile: room below 2^31)
-    if (pages_pitch > 0x7FFFFFFF || (pages_pitch << shift) > 0x7FFFFFFF - 1024)
-        return bad("a table holds up to 2^31 - 1024 tokens");
-    if (window > 0x7FFFFFFF) window = 0;  // wider than any sequence
-    if (!(scale >= -1e30 && scale <= 1e30) || !(cap >= 0.0 && cap <= 1e30))
-        return bad("scale must be within 1e30, cap 0 or positive");
-    if (n_row && n_seq && (!d_q || !d_out || !d_len || (!d_pages && pages_pitch))) return bad("null pointer");
-    if (d_ws && ((uintptr_t)d_ws & 15)) return bad("the workspace must be 16-byte aligned");
-    if (!ctx) return bad("null context");
-    if (!n_row || !n_seq) return FRQ_OK;
-    const Plan plan = plan_of(kv, n_row, n_head, n_seq);
-    const size_t need = plan.bytes;
-    if (d_ws && ws_bytes < need) return bad("the workspace is below frq_kv_attn_ws");
-    Guard g(ctx_device(ctx));
-    hipStream_t s = (hipStream_t)frq_get_stream(ctx);
-    if (!d_ws) {
-        // the context's workspace may move with a later call: a graph would
-        // keep its old address
-        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-        const hipError_t e = hipStreamIsCapturing(s, &st);
-        if (e != hipSuccess) return hip_bad(e, "hipStreamIsCapturing");
-        if (st != hipStreamCaptureStatusNone) return bad("under graph capture the caller gives the workspace");
-        if (int rc = ctx_ws(ctx, need, &d_ws)) return rc;
-    }
-    a.c = plan.dec;
-    a.c.len = d_len;
-    a.c.first = d_first;
-    a.c.width = (int)pages_pitch;
-    a.c.shift = shift;
-    a.c.window = (int)window;
-    a.q = d_q;
-    a.q_pitch = (int64_t)q_pitch;
-    a.out_pitch = (int64_t)out_pitch;
-    a.pages_pitch = (int64_t)pages_pitch;
-    a.pages = d_pages;
-    a.out = d_out;
-    a.err = ctx_err(ctx);
-    a.scale = scale == 0.0 ? 1.0f : (float)(scale < 0.0 ? -scale : scale);
-    a.sign = scale == 0.0 ? 0.0f : scale < 0.0 ? -1.0f : 1.0f;
-    // (below 2^-27 every cap gives weights within a rounding of equal ones; there
-    // score_scale's 2^100 over the cap would leave f32, or the cap be zero in it)
-    a.cap = cap > 0.0 && cap < 7.450580596923828e-9 ? 7.450580596923828e-9f : (float)cap;
-    a.dtype = kv->dtype;
-    // Each sequence is served by the kernel of its number of pairs; one that
-    // no sequence can be for is not launched.
-    // (f32 keys of over 128 channels stay with the decode kernel: three parts of
-    // q leave the prompt kernel one wave a SIMD.  2048 rows of 8 heads over 4, the
-    // decode kernel against the prompt kernel: 256 channels 288, 340 us over
-    // themselves, 72, 78 at 600 rows, 1612, 1508 over 8192 tokens; 192 channels 225,
-    // 202 and 1280, 676.  Widths of an odd number of 32s do not fit the LDS.)
-    const bool prompts = d_first && n_row * (size_t)a.c.rep > (size_t)DEC_PAIRS &&
-                         !(kv->dtype == FRQ_DT_F32 && kv->hd > 128);
-    a.c.max_pairs = prompts ? DEC_PAIRS : 0x7FFFFFFF;
-    char* ws = (char*)d_ws;
-    a.rec = (Record*)(ws + plan.rec_dec);
-    a.part = (float*)(ws + plan.part_dec);
-    a.slots = max_slots(DEC_TARGET, a.c.n_kv);
-    Args b = a;
-    b.c.min_pairs = plan.prompt.min_pairs;
-    b.c.max_pairs = plan.prompt.max_pairs;
-    b.c.tp = plan.prompt.tp;
-    b.c.target = plan.prompt.target;
-    b.c.min_chunk = plan.prompt.min_chunk;
-    b.rec = (Record*)(ws + plan.rec_prompt);
-    b.part = (float*)(ws + plan.part_prompt);
-    b.slots = n_row > n_seq ? max_slots(b.c.target, a.c.n_kv) : 0;
-    const int64_t ga = max_items(a.c) * a.c.n_kv, gb = prompts ? max_items(b.c) * b.c.n_kv : 0;
-    if (ga + gb > 0x7FFFFFFF) return bad("too many rows or sequences");
-    const Launch la{(unsigned)ga, s}, lb{(unsigned)gb, s};
-    hipError_t e = hipSuccess;
-    if (n_seq > (size_t)PLAN_SEQS) {
-        int32_t *pa = (int32_t*)(ws + plan.plan_dec), *pb = (int32_t*)(ws + plan.plan_prompt);
-        kv_plan_kernel<<<dim3(prompts ? 2 : 1), dim3(1024), 0, s>>>(a.c, b.c, pa, pb, a.err);
-        e = hipGetLastError();
-        if (e != hipSuccess) return hip_bad(e, "launch kv_plan");
-        a.c.plan = pa;
-        b.c.plan = pb;
-    }
-    e = kv->dtype == FRQ_DT_F32   ? launch_decode_f32(a, la)
-                   : kv->dtype == FRQ_DT_F16 ? launch_decode_f16(a, la)
-                                             : launch_decode_i8(a, la);
-    if (e != hipSuccess) return hip_bad(e, "launch kv_decode");
-    if (prompts) {
-        e = kv->dtype == FRQ_DT_F32   ? launch_prompt_f32(b, lb)
-            : kv->dtype == FRQ_DT_F16 ? launch_prompt_f16(b, lb)
-                                      : launch_prompt_i8(b, lb);
-        if (e != hipSuccess) return hip_bad(e, "launch kv_prompt");
-    }
-    kv_join_kernel<<<dim3((unsigned)(ga + gb)), dim3(256), 0, s>>>(a, b, (unsigned)ga);
-    e = hipGetLastError();
-    return e == hipSuccess ? FRQ_OK : hip_bad(e, "launch kv_join");
+    return attend(ctx, kv, d_q, q_pitch, n_row, n_head, d_pages, pages_pitch, d_len, d_first, n_seq, scale, cap, window,
+                  More{0, nullptr, 0, false}, d_out, out_pitch, d_ws, ws_bytes);
+}
+
+int frq_kv_attn_sink_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, size_t n_row, size_t n_head,
+                         const int32_t* d_pages, size_t pages_pitch, const int32_t* d_len, const int32_t* d_first,
+                         size_t n_seq, double scale, double cap, size_t window, size_t sinks, float* d_out,
+                         size_t out_pitch, void* d_ws, size_t ws_bytes) {
+    return attend(ctx, kv, d_q, q_pitch, n_row, n_head, d_pages, pages_pitch, d_len, d_first, n_seq, scale, cap, window,
+                  More{sinks, nullptr, 0, false}, d_out, out_pitch, d_ws, ws_bytes);
+}
+
+int frq_kv_attn_tree_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, size_t n_row, size_t n_head,
+                         const int32_t* d_pages, size_t pages_pitch, const int32_t* d_len, const int32_t* d_first,
+                         size_t n_seq, double scale, double cap, size_t window, size_t sinks, const uint64_t* d_tree,
+                         size_t tree_pitch, float* d_out, size_t out_pitch, void* d_ws, size_t ws_bytes) {
+    return attend(ctx, kv, d_q, q_pitch, n_row, n_head, d_pages, pages_pitch, d_len, d_first, n_seq, scale, cap, window,
+                  More{sinks, d_tree, tree_pitch, true}, d_out, out_pitch, d_ws, ws_bytes);
 }
 
 }  // extern "C"

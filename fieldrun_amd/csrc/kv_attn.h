@@ -219,10 +219,10 @@ __device__ __forceinline__ float fsum16(float v) {
     return v + __uint_as_float(xshfl<32>(__float_as_uint(v)));
 }
 
-// What out is multiplied by: a row that sees no key (its position below 0) is
-// zeros, one whose scores are all -inf is NaN, as the formula has it.
-__device__ __forceinline__ float over(float l, int pos) {
-    return l > 0.0f || l != l ? 1.0f / l : pos < 0 ? 0.0f : __builtin_nanf("");
+// What out is multiplied by: a row that sees no key is zeros, one whose scores
+// are all -inf is NaN, as the formula has it.
+__device__ __forceinline__ float over(float l, bool sees) {
+    return l > 0.0f || l != l ? 1.0f / l : !sees ? 0.0f : __builtin_nanf("");
 }
 
 // The loops read page 0 for a page id out of range.  Such an id is an error
@@ -236,6 +236,103 @@ __device__ __forceinline__ bool page_bad(const Args& a, int seq, int lo, int hi)
     for (int pg = lo >> a.c.shift; lo <= hi && pg <= hi >> a.c.shift; ++pg)
         if (page_ok(table[pg], a.kv.n_pages) < 0) return true;
     return false;
+}
+// The same for a chunk that takes sinks: `real` is where its keys v0 .. v1 - 1
+// lie, 16 by 16 in one page; rows see the first keys and those from lo to hi.
+template <typename F>
+__device__ __forceinline__ bool page_bad(const Args& a, int seq, int v0, int v1, int lo, int hi, F&& real) {
+    const int32_t* table = a.pages + (int64_t)seq * a.pages_pitch;
+    for (int v = v0; v < v1; v += 16) {
+        const int k0 = real(v), k1 = min(k0 + 15, hi);
+        if (k0 <= k1 && (k0 < a.c.sinks || k1 >= lo) && page_ok(table[k0 >> a.c.shift], a.kv.n_pages) < 0) return true;
+    }
+    return false;
+}
+
+// What a row sees.  EX: the calls with sinks or with trees of drafted tokens;
+// there the keys lo .. hi, the first `sinks` of those up to hi, and of a tree
+// the keys base + t whose bit t of its mask is set.  (A row of a tree stands as
+// far behind the cached tokens as its mask has tokens.)
+struct Run {  // keys from `key` on against lo .. hi
+    int key, lo, hi;
+    __device__ __forceinline__ bool operator[](int j) const { return key + j >= lo && key + j <= hi; }
+};
+struct Bits {
+    uint32_t x;
+    __device__ __forceinline__ bool operator[](int j) const { return x >> j & 1; }
+};
+template <bool EX>
+struct Sight {
+    int lo, hi;
+    __device__ __forceinline__ bool any() const { return hi >= 0; }
+    __device__ __forceinline__ int first() const { return lo; }
+    template <int N>
+    __device__ __forceinline__ Run seen(int key) const {  // of the N keys from `key` on
+        return Run{key, lo, hi};
+    }
+};
+template <>
+struct Sight<true> {
+    int lo, hi, sinks, base, n;  // n: drafted tokens (0: no tree)
+    bool some;
+    const uint64_t* mask;
+    __device__ __forceinline__ bool any() const { return some; }
+    __device__ __forceinline__ int first() const { return sinks ? 0 : n && lo > base ? base : lo; }
+    template <int N>
+    __device__ __forceinline__ Bits seen(int key) const {
+        static_assert(N <= 16, "");
+        uint32_t x = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) x |= (key + j >= lo || key + j < sinks) && key + j <= hi ? 1u << j : 0u;
+        return Bits{x | tree_bits<N>(mask, n, key - base)};
+    }
+};
+template <bool EX>
+__device__ __forceinline__ Sight<EX> sight_of(const Args& a, int row0, int rows, int len, int row) {
+    Sight<EX> s;
+    if constexpr (!EX) {
+        s.hi = len - rows + row;
+        s.lo = key_lo(a.c, s.hi);
+    } else {
+        s.sinks = a.c.sinks;
+        s.base = len - rows;
+        s.n = 0;
+        s.mask = nullptr;
+        if (!a.c.tree) {
+            s.hi = s.base + row;
+            s.lo = key_lo(a.c, s.hi);
+            s.some = s.hi >= 0;
+        } else {
+            s.n = rows;
+            s.mask = a.c.tree + (int64_t)(row0 + row) * a.c.tree_pitch;
+            int depth = 0;
+            for (int w = 0; 64 * w < rows; ++w) {
+                const int left = rows - 64 * w;
+                depth += __builtin_popcountll(s.mask[w] & (left < 64 ? ((uint64_t)1 << left) - 1 : ~(uint64_t)0));
+            }
+            s.hi = s.base - 1;
+            s.lo = key_lo(a.c, s.base - 1 + depth);
+            s.some = depth > 0 || s.lo <= s.hi || (s.sinks > 0 && s.hi >= 0);
+        }
+    }
+    return s;
+}
+// The same of all rows of a tile: its first and last key, the keys from which
+// on and up to which every row sees all (of a tree a bound of each).
+struct Bounds {
+    int lo_a, lo_b;  // the first row's and the last row's first key
+    int hi_a, hi_b;  // their last
+};
+template <bool EX>
+__device__ __forceinline__ Bounds bounds_of(const Args& a, int rows, int len, int row_a, int row_b) {
+    const int base = len - rows;
+    const bool tree = EX && a.c.tree;
+    Bounds b;
+    b.hi_a = tree ? base - 1 : base + row_a;
+    b.hi_b = tree ? len - 1 : base + row_b;
+    b.lo_a = key_lo(a.c, b.hi_a);
+    b.lo_b = key_lo(a.c, b.hi_b);
+    return b;
 }
 
 // tanh to about 2e-7 of its value: a polynomial near zero, where
@@ -434,7 +531,7 @@ __device__ __forceinline__ void load_q(const float* q, float sign, int g, QOp<DT
 // (batch, long, window): loads past the caches 47, 110, 122 us; eight waves a
 // workgroup 55 and 168 (batch, window); a wave's tiles side by side 107 and 131
 // (long, window).
-template <int DT, int HD, int NW>
+template <int DT, int HD, int NW, bool EX>
 __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(const Args a) {
     using T = Type<DT>;
     constexpr int NS = (HD + T::KS - 1) / T::KS, NT = HD / 16;
@@ -458,13 +555,16 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
     const int p0 = it.tile * 16, np = min(16, pairs - p0);
     const int pr = p0 + min(col, np - 1);
     const int row = pr / a.c.rep, head = kvh * a.c.rep + pr % a.c.rep;
-    const int pos = it.q.len - it.q.rows + row;
+    const Sight<EX> sight = sight_of<EX>(a, it.q.row0, it.q.rows, it.q.len, row);
     // the tile's first and last row
-    const int pos_a = uni(it.q.len - it.q.rows + p0 / a.c.rep);
-    const int pos_b = uni(it.q.len - it.q.rows + (p0 + np - 1) / a.c.rep);
-    const int see_lo = key_lo(a.c, pos), lo_a = key_lo(a.c, pos_a), lo_b = key_lo(a.c, pos_b);
-    const int64_t beg64 = tile_lo(a.c, pos_a) + (int64_t)it.chunk * it.klen;
-    const int end = uni((int)min(beg64 + it.klen, (int64_t)pos_b + 1));
+    const Bounds bd = bounds_of<EX>(a, it.q.rows, it.q.len, uni(p0 / a.c.rep), uni((p0 + np - 1) / a.c.rep));
+    const int pos_a = uni(bd.hi_a), pos_b = uni(bd.hi_b), lo_a = uni(bd.lo_a), lo_b = uni(bd.lo_b);
+    // the chunk's keys; EX: counted as span_at takes them, real() is the key
+    const Span sp = EX ? span_at(a.c, pos_a) : Span{0, 0};
+    const int span = uni(sp.span), gap = uni(sp.gap), sinks = EX ? a.c.sinks : 0;
+    auto real = [&](int v) { return EX && v >= span ? v + gap : v; };
+    const int64_t beg64 = (EX ? 0 : tile_lo(a.c, pos_a)) + (int64_t)it.chunk * it.klen;
+    const int end = uni((int)min(beg64 + it.klen, (int64_t)pos_b + 1 - gap));
     const int beg = uni((int)min(beg64, (int64_t)max(end, 0)));
     const int tiles = end > beg ? (end - beg + KT - 1) / KT : 0;
     QOp<DT, NS> q;
@@ -489,7 +589,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
     float l = 0.0f;
     int ev = 0;  // int8: out is held times 2^(W_EXP - ev)
     uint32_t odd = 0;
-    const bool alike = lo_a == lo_b && pos_a == pos_b;  // every pair sees the same
+    const bool alike = lo_a == lo_b && pos_a == pos_b && !(EX && a.c.tree);  // every pair sees the same
 
     // the page ids of a tile's two halves, loaded a tile ahead of the loads
     // that use them; a bad one reads page 0 and is looked into at the end
@@ -540,16 +640,16 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
         }
     };
     if (wave < tiles) {
-        ids(beg + wave * KT);
+        ids(real(beg + wave * KT));
         pages();
-        ids(beg + (wave + NW) * KT);
-        load_k(beg + wave * KT);
-        load_v(beg + wave * KT);
+        ids(real(beg + (wave + NW) * KT));
+        load_k(real(beg + wave * KT));
+        load_v(real(beg + wave * KT));
     }
     for (int ti = wave; ti < tiles; ti += NW) {
-        const int base = beg + ti * KT;
+        const int base = real(beg + ti * KT);
         const bool more = ti + NW < tiles;
-        const int next = base + NW * KT;
+        const int next = real(beg + (ti + NW) * KT);
         // ---- scores: s[4 u + i] is key base + PL g + 4 u + i of this lane's pair
         f4 sc[NU];
 #pragma unroll
@@ -586,7 +686,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
         }
         if (more) {
             pages();
-            ids(next + NW * KT);
+            ids(real(beg + (ti + 2 * NW) * KT));
             load_k(next);
         }
         if (capped) {
@@ -594,12 +694,12 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
             for (int j = 0; j < 4 * NU; ++j) s[j] = (a.cap * LOG2E) * tanh_f(s[j] * rcap);
         }
         // keys that not every pair of the tile sees
-        const bool edge = base < lo_b || base + KT - 1 > pos_a;
+        const bool edge = (base < lo_b && !(EX && base + KT <= sinks)) || base + KT - 1 > pos_a;
         if (edge) {
+            const auto sees = sight.template seen<4 * NU>(base + T::PL * g);
 #pragma unroll
             for (int j = 0; j < 4 * NU; ++j) {
-                const int key = base + T::PL * g + j;
-                if (key < see_lo || key > pos) {
+                if (!sees[j]) {
                     s[j] = -__builtin_inff();
                     if constexpr (T::I8) vcur[j] = 0.0f;  // its step may be anything
                 }
@@ -652,7 +752,8 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
 #pragma unroll
                 for (int j = 0; j < T::PL; ++j) {
                     const int key = base + T::PL * g + j;
-                    const uint32_t w = key < lo_a || key > pos_b ? 0u : PW == 1 ? ~0u : j & 1 ? 0xFFFF0000u : 0x0000FFFFu;
+                    const bool none = (key < lo_a && !(EX && key < sinks)) || key > pos_b;
+                    const uint32_t w = none ? 0u : PW == 1 ? ~0u : j & 1 ? 0xFFFF0000u : 0x0000FFFFu;
                     keep[j / PW] = j % PW ? keep[j / PW] | w : w;
                 }
 #pragma unroll
@@ -694,12 +795,12 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
     if constexpr (!T::I8) {
         // rare: the keys of those tiles again, one by one
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0) != 0, 0)) {
-            for (int key = beg; key < end; ++key) {
-                const int t0 = (key - beg) / KT, base = beg + t0 * KT;
-                if (t0 % NW != wave || (base >= lo_b && base + KT - 1 <= pos_a)) continue;
+            for (int v = beg; v < end; ++v) {
+                const int t0 = (v - beg) / KT, base = real(beg + t0 * KT), key = real(v);
+                if (t0 % NW != wave || ((base >= lo_b || (EX && base + KT <= sinks)) && base + KT - 1 <= pos_a)) continue;
                 const int64_t pg = max(page_ok(table[key >> shift], a.kv.n_pages), 0);
                 const char* p = vb + pg * a.kv.stride + (int64_t)(key & (page - 1)) * T::SZ;
-                const bool sees = key >= see_lo && key <= pos;
+                const bool sees = sight.template seen<1>(key)[0];
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -747,13 +848,18 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
         __syncthreads();
     }
     if (wave != 0) return;
-    if (__builtin_expect(hole, 0) && page_bad(a, it.seq, max(lo_a, beg), min(pos_b, end - 1))) {
-        note_hole(a, blockIdx.x / n_kv, it.seq);
-        lsum = HOLE;
+    if (__builtin_expect(hole, 0)) {
+        bool gone;
+        if constexpr (EX) gone = page_bad(a, it.seq, beg, end, -wave_most(-sight.lo), pos_b, real);
+        else gone = page_bad(a, it.seq, max(lo_a, beg), min(pos_b, end - 1));
+        if (gone) {
+            note_hole(a, blockIdx.x / n_kv, it.seq);
+            lsum = HOLE;
+        }
     }
     if (col >= np) return;
     if (it.chunks == 1) {
-        const float r = over(lsum, pos);
+        const float r = over(lsum, sight.any());
         float* d = a.out + (int64_t)(it.q.row0 + row) * a.out_pitch + (int64_t)head * hd + 4 * g;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -855,7 +961,7 @@ struct Prompt {
     static constexpr int LDS = 2 * NBUF * NA * BUF * 2 + (DT == FRQ_DT_ROWI8 ? 2 * 2 * KT * 4 : 0);
 };
 
-template <int DT, int HD>
+template <int DT, int HD, bool EX>
 __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel(const Args a) {
     using P = Prompt<DT, HD>;
     using Op = typename P::Op;
@@ -864,6 +970,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     constexpr int NS = HD / 16, NH = P::N32, NK = P::KT / 32, KT = P::KT, IPW = P::IPW;
     extern __shared__ __align__(1024) char lds[];
     __shared__ int flag, hole;  // a value was taken out; a page id was bad
+    __shared__ int least;       // EX: the first key that a row sees behind the sinks
     uint16_t* lk = reinterpret_cast<uint16_t*>(lds);                   // [NBUF][NA][KT][HP]
     uint16_t* lv = lk + NBUF * NA * P::BUF;                            // [NBUF][NA][HP][KT]
     float* lks = reinterpret_cast<float*>(lv + NBUF * NA * P::BUF);    // [2][KT] int8 steps
@@ -877,21 +984,27 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     const int col = lane & 31, h = lane >> 5;
     constexpr int hd = HD;
     const int page = a.kv.page, shift = a.c.shift, rep = a.c.rep;
-    const int pairs = it.q.rows * rep, off = it.q.len - it.q.rows;
+    const int pairs = it.q.rows * rep;
     // the workgroup's pairs and keys
     const int t0 = it.tile * 128, tn = min(128, pairs - t0);
-    const int wpos_a = uni(off + t0 / rep), wpos_b = uni(off + (t0 + tn - 1) / rep);  // its first and last row
-    const int64_t beg64 = tile_lo(a.c, wpos_a) + (int64_t)it.chunk * it.klen;
-    const int end = uni((int)min(beg64 + it.klen, (int64_t)wpos_b + 1));
+    const Bounds wbd = bounds_of<EX>(a, it.q.rows, it.q.len, uni(t0 / rep), uni((t0 + tn - 1) / rep));
+    const int wpos_a = uni(wbd.hi_a), wpos_b = uni(wbd.hi_b);  // its first and last row
+    // the chunk's keys; EX: counted as span_at takes them, real() is the key
+    const Span sp = EX ? span_at(a.c, wpos_a) : Span{0, 0};
+    const int span = uni(sp.span), gap = uni(sp.gap), sinks = EX ? a.c.sinks : 0;
+    auto real = [&](int v) { return EX && v >= span ? v + gap : v; };
+    const int64_t beg64 = (EX ? 0 : tile_lo(a.c, wpos_a)) + (int64_t)it.chunk * it.klen;
+    const int end = uni((int)min(beg64 + it.klen, (int64_t)wpos_b + 1 - gap));
     const int beg = uni((int)min(beg64, (int64_t)max(end, 0)));
     const int tiles = end > beg ? (end - beg + KT - 1) / KT : 0;
     // the wave's, the lane's; columns past the last pair repeat it
     const int p0 = t0 + min(32 * wave, tn - 1), np = max(1, min(32, tn - 32 * wave));
     const bool idle = 32 * wave >= tn;
     const int pr = p0 + min(col, np - 1);
-    const int row = pr / rep, head = kvh * rep + pr % rep, pos = off + row;
-    const int pos_a = uni(off + p0 / rep), pos_b = uni(off + (p0 + np - 1) / rep);
-    const int see_lo = key_lo(a.c, pos), lo_a = key_lo(a.c, pos_a), lo_b = key_lo(a.c, pos_b);
+    const int row = pr / rep, head = kvh * rep + pr % rep;
+    const Sight<EX> sight = sight_of<EX>(a, it.q.row0, it.q.rows, it.q.len, row);
+    const Bounds bd = bounds_of<EX>(a, it.q.rows, it.q.len, uni(p0 / rep), uni((p0 + np - 1) / rep));
+    const int pos_a = uni(bd.hi_a), pos_b = uni(bd.hi_b), lo_a = uni(bd.lo_a), lo_b = uni(bd.lo_b);
 
     // ---- q, times a power of two (f16), as the B operands of the scores
     Op qv[NS][NB];
@@ -998,9 +1111,11 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     // zero probability would carry them to pairs that do not see them) are
     // zeroed; the second are noted and given to their pairs after the loop.
     // (int8 values are finite, and a key that is not seen has weight zero.)
-    const int wlo_a = key_lo(a.c, wpos_a), wlo_b = key_lo(a.c, wpos_b);
+    const int wlo_a = uni(wbd.lo_a), wlo_b = uni(wbd.lo_b);
+    auto none = [&](int key) { return (key < wlo_a && !(EX && key < sinks)) || key > wpos_b; };
+    auto whole = [&](int base) { return (base >= wlo_b || (EX && base + KT <= sinks)) && base + KT - 1 <= wpos_a; };
     auto land = [&](int base, int buf) {
-        const bool edge = base < wlo_b || base + KT - 1 > wpos_a;
+        const bool edge = !whole(base);
         if constexpr (I8) {
 #pragma unroll
             for (int i = 0; i < IPW; ++i) {
@@ -1022,7 +1137,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
                     y[j] = __uint_as_float(rv[i][j / 4][j % 4]);
                     if (edge) {
                         const int key = base + vd + j;
-                        const bool seen = key >= wlo_a && key <= wpos_b, fin = y[j] - y[j] == 0.0f;
+                        const bool seen = !none(key), fin = y[j] - y[j] == 0.0f;
                         odd |= seen && !fin;
                         y[j] = seen && fin ? y[j] : 0.0f;
                     }
@@ -1048,7 +1163,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int key = base + vd + j;
-                    if (key < wlo_a || key > wpos_b) v[j / 2] &= j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                    if (none(key)) v[j / 2] &= j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -1073,29 +1188,33 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     float l = 0.0f;
     int ev = 0;
     const int krow = (col & 19) | (col & 4) << 1 | (col & 8) >> 1;  // the key of this lane's score row
-    if (tid == 0) flag = hole = 0;
+    if (tid == 0) {
+        flag = hole = 0;
+        least = 0x7FFFFFFF;
+    }
     // two workgroups share a CU, the second 256 behind the first: one ahead of
     // the other keeps the one's products over the other's softmax
     if ((blockIdx.x >> 8) & 1) __builtin_amdgcn_s_setprio(2);
     __syncthreads();
     if (tiles) {
-        ids(beg);
-        fetch(beg, 0);
-        land(beg, 0);
-        if (tiles > 1) ids(beg + KT);
+        ids(real(beg));
+        fetch(real(beg), 0);
+        land(real(beg), 0);
+        if (tiles > 1) ids(real(beg + KT));
     }
     __syncthreads();
     for (int ti = 0; ti < tiles; ++ti) {
-        const int base = beg + ti * KT, buf = NBUF == 1 ? 0 : ti & 1, other = NBUF - 1 - buf;
+        const int base = real(beg + ti * KT), next = real(beg + (ti + 1) * KT);
+        const int buf = NBUF == 1 ? 0 : ti & 1, other = NBUF - 1 - buf;
         if (ti + 1 < tiles) {
-            fetch(base + KT, other);
-            if (ti + 2 < tiles) ids(base + 2 * KT);
+            fetch(next, other);
+            if (ti + 2 < tiles) ids(real(beg + (ti + 2) * KT));
         }
         if (!idle) {
 #pragma unroll 1
             for (int u = 0; u < NK; ++u) {
                 const int kb0 = base + 32 * u;
-                if (kb0 > pos_b || kb0 + 31 < lo_a) continue;
+                if (kb0 > pos_b || (kb0 + 31 < lo_a && !(EX && kb0 < sinks))) continue;
                 // operands are read a group ahead of their products, the
                 // first of the values ahead of the softmax
                 // piece (2 st + h) ^ (row mod) of the key row, 4 u + 2 k + h
@@ -1150,7 +1269,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
 #pragma unroll
                 for (int i = 0; i < G; ++i)
                     if (i < 2 * NH) val_op(i, xa[i]);
-                const bool edge = kb0 < lo_b || kb0 + 31 > pos_a;
+                const bool edge = (kb0 < lo_b && !(EX && kb0 + 32 <= sinks)) || kb0 + 31 > pos_a;
                 if constexpr (I8) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[i] *= lks[buf * KT + 32 * u + 16 * (i / 8) + 8 * h + i % 8];
@@ -1161,9 +1280,11 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
                 }
                 if (edge) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int key = kb0 + 16 * (i / 8) + 8 * h + i % 8;
-                        if (key < see_lo || key > pos) s[i] = -__builtin_inff();
+                    for (int t = 0; t < 2; ++t) {
+                        const auto sees = sight.template seen<8>(kb0 + 16 * t + 8 * h);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (!sees[j]) s[8 * t + j] = -__builtin_inff();
                     }
                 }
                 float mx = s[0];
@@ -1254,19 +1375,23 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
             }
         }
         if (NBUF == 1) __syncthreads();
-        if (ti + 1 < tiles) land(base + KT, other);
+        if (ti + 1 < tiles) land(next, other);
         __syncthreads();
     }
     if (bad) hole = 1;  // (each wave has looked at the ids of its own pieces)
+    if constexpr (EX) {
+        const int lo = -wave_most(-sight.lo);
+        if (lane == 0) atomicMin(&least, lo);
+    }
     __syncthreads();
     if constexpr (!I8) {
         if (flag) {  // rare: the keys of those tiles again, one by one (the last barrier was after the last note)
-            for (int key = beg; key < end; ++key) {
-                const int base = beg + (key - beg) / KT * KT;
-                if (base >= wlo_b && base + KT - 1 <= wpos_a) continue;
+            for (int v = beg; v < end; ++v) {
+                const int base = real(beg + (v - beg) / KT * KT), key = real(v);
+                if (whole(base)) continue;
                 const int64_t pg = max(page_ok(table[key >> shift], a.kv.n_pages), 0);
                 const char* p = vb + pg * a.kv.stride + (int64_t)(key & (page - 1)) * SZ;
-                const bool sees = key >= see_lo && key <= pos;
+                const bool sees = sight.template seen<1>(key)[0];
 #pragma unroll
                 for (int t = 0; t < NH; ++t)
 #pragma unroll
@@ -1282,14 +1407,19 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     }
     if constexpr (I8) l = __builtin_ldexpf(l, -down);
     l += __uint_as_float(xshfl<32>(__float_as_uint(l)));
-    if (__builtin_expect(hole, 0) && page_bad(a, it.seq, max(wlo_a, beg), min(wpos_b, end - 1))) {
-        note_hole(a, blockIdx.x / n_kv, it.seq);
-        l = HOLE;
+    if (__builtin_expect(hole, 0)) {
+        bool gone;
+        if constexpr (EX) gone = page_bad(a, it.seq, beg, end, least, wpos_b, real);
+        else gone = page_bad(a, it.seq, max(wlo_a, beg), min(wpos_b, end - 1));
+        if (gone) {
+            note_hole(a, blockIdx.x / n_kv, it.seq);
+            l = HOLE;
+        }
     }
     if (idle || col >= np) return;
     const float m = top.m * mul;
     if (it.chunks == 1) {
-        const float r = over(l, pos);
+        const float r = over(l, sight.any());
         float* d = a.out + (int64_t)(it.q.row0 + row) * a.out_pitch + (int64_t)head * hd + 4 * h;
 #pragma unroll
         for (int t = 0; t < NH; ++t)
@@ -1336,7 +1466,7 @@ __device__ __forceinline__ float entry(const char* p) {  // a stored key's or va
 // page ids out of range: a wave a pair, eight keys at a time, a lane every 64th
 // channel.  For calls in error, and no faster than that: one f16 sequence of
 // 131071 tokens 0.11 s, 2048 rows over 8192 tokens 47 ms.
-template <int DT, int TP>
+template <int DT, int TP, bool EX>
 __device__ __forceinline__ void redo_share(const Args& a, const Record& it, int kvh, int beg, int end) {
     constexpr bool I8 = DT == FRQ_DT_ROWI8;
     constexpr int SZ = DT == FRQ_DT_F32 ? 4 : I8 ? 1 : 2;
@@ -1344,7 +1474,8 @@ __device__ __forceinline__ void redo_share(const Args& a, const Record& it, int 
     const int32_t* table = a.pages + (int64_t)(it.seq < 0 ? ~it.seq : it.seq) * a.pages_pitch;
     const int p0 = it.tile * TP, h4 = hd / 4;
     for (int pair = beg / h4 + uni(threadIdx.x >> 6); pair * h4 < end; pair += 4) {
-        const int row = (p0 + pair) / rep, head = kvh * rep + (p0 + pair) % rep, pos = it.len - it.rows + row;
+        const int row = (p0 + pair) / rep, head = kvh * rep + (p0 + pair) % rep;
+        const Sight<EX> sight = sight_of<EX>(a, it.row0, it.rows, it.len, row);
         const float* q = a.q + (int64_t)(it.row0 + row) * a.q_pitch + (int64_t)head * hd;
         float x[4], o[4], m = -__builtin_inff(), l = 0.0f;
         int e = 0;  // q is held times 2^-e, as by the loops
@@ -1360,11 +1491,15 @@ __device__ __forceinline__ void redo_share(const Args& a, const Record& it, int 
         const int down = down_of(it.len);
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = __builtin_ldexpf(x[i], -e);
-        int seen = -1;  // (over's place of a row: below 0 if it sees nothing)
+        bool some = false;
         constexpr int U = 8;  // keys at once, one page's
-        const int lo = key_lo(a.c, pos);
+        const int last = EX && a.c.tree ? it.len - 1 : sight.hi;
 #pragma unroll 1
-        for (int k0 = lo & -U; k0 <= pos; k0 += U) {
+        for (int k0 = sight.first() & -U; k0 <= last; k0 += U) {
+            const auto sees = sight.template seen<U>(k0);
+            if constexpr (EX) {
+                if (!sees.x) continue;
+            }
             const int64_t pg = page_ok(table[k0 >> a.c.shift], a.kv.n_pages);
             if (pg < 0) continue;
             const int at = k0 & (page - 1);
@@ -1385,7 +1520,7 @@ __device__ __forceinline__ void redo_share(const Args& a, const Record& it, int 
                 z[u] = wave_sum(z[u]);
                 if constexpr (I8) z[u] *= a.kv.ks[step + u];
                 z[u] = a.cap > 0.0f ? (a.cap * LOG2E) * tanh_f(z[u] * (scl / a.cap)) : z[u] * (scl * LOG2E);
-                if (k0 + u < lo || k0 + u > pos) z[u] = -__builtin_inff();
+                if (!sees[u]) z[u] = -__builtin_inff();
                 mn = fmaxf(mn, z[u]);
             }
             const float mr = mn == -__builtin_inff() ? 0.0f : mn, alpha = __builtin_amdgcn_exp2f(m - mr);
@@ -1395,7 +1530,7 @@ __device__ __forceinline__ void redo_share(const Args& a, const Record& it, int 
             for (int i = 0; i < 4; ++i) o[i] *= alpha;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (k0 + u < lo || k0 + u > pos) continue;
+                if (!sees[u]) continue;
                 float w = __builtin_ldexpf(__builtin_amdgcn_exp2f(z[u] - mr), -down);
                 l += w;
                 if constexpr (I8) w *= a.kv.vs[step + u];
@@ -1403,9 +1538,9 @@ __device__ __forceinline__ void redo_share(const Args& a, const Record& it, int 
                 for (int i = 0; i < 4; ++i)
                     if (64 * i + lane < hd) o[i] += w * entry<DT>(v + ((int64_t)(64 * i + lane) * page + u) * SZ);
             }
-            seen = 0;
+            some = true;
         }
-        const float r = over(l, seen);
+        const float r = over(l, some);
         float* d = a.out + (int64_t)(it.row0 + row) * a.out_pitch + (int64_t)head * hd;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -1414,11 +1549,11 @@ __device__ __forceinline__ void redo_share(const Args& a, const Record& it, int 
         }
     }
 }
-template <int TP>
+template <int TP, bool EX>
 __device__ __forceinline__ void redo_share(const Args& a, const Record& it, int kvh, int beg, int end) {
-    if (a.dtype == FRQ_DT_F32) redo_share<FRQ_DT_F32, TP>(a, it, kvh, beg, end);
-    else if (a.dtype == FRQ_DT_F16) redo_share<FRQ_DT_F16, TP>(a, it, kvh, beg, end);
-    else redo_share<FRQ_DT_ROWI8, TP>(a, it, kvh, beg, end);
+    if (a.dtype == FRQ_DT_F32) redo_share<FRQ_DT_F32, TP, EX>(a, it, kvh, beg, end);
+    else if (a.dtype == FRQ_DT_F16) redo_share<FRQ_DT_F16, TP, EX>(a, it, kvh, beg, end);
+    else redo_share<FRQ_DT_ROWI8, TP, EX>(a, it, kvh, beg, end);
 }
 
 // ---- joining the chunks' parts ----------------------------------------------
@@ -1429,13 +1564,13 @@ __device__ __forceinline__ void redo_share(const Args& a, const Record& it, int 
 // latency: 4.5 to 5.5 us at 60 to 280 chunks of 16 pairs of 128 channels, 10 us for
 // 7 prompts' 128 pairs (a float4 a thread at a time: 585 rows of 8 heads of 256
 // 64 us in all against 57).
-template <int TP>
+template <int TP, bool EX>
 __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so, float* sm, float* sl) {
     const int n_kv = a.c.n_kv, kvh = block % n_kv;
     const Record it = a.rec[block / n_kv];
     if (it.chunks <= 1) {
         if (__builtin_expect(it.seq < 0, 0))
-            redo_share<TP>(a, it, kvh, 0, min(TP, it.rows * a.c.rep - it.tile * TP) * (a.kv.hd / 4));
+            redo_share<TP, EX>(a, it, kvh, 0, min(TP, it.rows * a.c.rep - it.tile * TP) * (a.kv.hd / 4));
         return;
     }
     if (it.slot < 0 || it.slot + it.chunks > a.slots) return;
@@ -1450,7 +1585,7 @@ __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so,
     const float* part = a.part + (it.slot * n_kv + kvh) * (int64_t)(TP * (hd + 2));
     auto store = [&](int pair, int c4, f4 o, float l) {
         const int pr = p0 + pair, row = pr / a.c.rep, head = kvh * a.c.rep + pr % a.c.rep;
-        const float r = over(l, it.len - it.rows + row);
+        const float r = over(l, sight_of<EX>(a, it.row0, it.rows, it.len, row).any());
         F4 y;
 #pragma unroll
         for (int i = 0; i < 4; ++i) y.v[i] = o[i] * r;
@@ -1533,7 +1668,7 @@ __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so,
         }
         if (run == 0 && in) store(pair, c4, o, l);
     }
-    if (__builtin_expect(__syncthreads_or(hole), 0)) redo_share<TP>(a, it, kvh, beg, end);
+    if (__builtin_expect(__syncthreads_or(hole), 0)) redo_share<TP, EX>(a, it, kvh, beg, end);
 }
 
 // The launchers of one stored type (each in a file of its own).
@@ -1547,6 +1682,13 @@ hipError_t launch_decode_i8(const Args& a, const Launch& l);
 hipError_t launch_prompt_f32(const Args& a, const Launch& l);
 hipError_t launch_prompt_f16(const Args& a, const Launch& l);
 hipError_t launch_prompt_i8(const Args& a, const Launch& l);
+// of calls with sinks or trees
+hipError_t launch_decode_ex_f32(const Args& a, const Launch& l);
+hipError_t launch_decode_ex_f16(const Args& a, const Launch& l);
+hipError_t launch_decode_ex_i8(const Args& a, const Launch& l);
+hipError_t launch_prompt_ex_f32(const Args& a, const Launch& l);
+hipError_t launch_prompt_ex_f16(const Args& a, const Launch& l);
+hipError_t launch_prompt_ex_i8(const Args& a, const Launch& l);
 
 // Every width has a kernel of its own: with the steps of a width known only at
 // run time (the next of 64, 128 and 256, masked) 192 channels took 21 us where
@@ -1580,30 +1722,30 @@ hipError_t by_width(int hd, F&& f) {
     return hipErrorNotSupported;  // not a width that the checks let through
 }
 
-template <int DT>
+template <int DT, bool EX>
 hipError_t launch_decode(const Args& a, const Launch& l) {
     return by_width<256>(a.kv.hd, [&](auto w) {
-        kv_decode_kernel<DT, decltype(w)::value, 4><<<dim3(l.grid), dim3(256), 0, l.s>>>(a);
+        kv_decode_kernel<DT, decltype(w)::value, 4, EX><<<dim3(l.grid), dim3(256), 0, l.s>>>(a);
         return hipGetLastError();
     });
 }
 
-template <int DT, int HD>
+template <int DT, int HD, bool EX>
 hipError_t run_prompt(const Args& a, const Launch& l) {
     constexpr int lds = Prompt<DT, HD>::LDS;
     static_assert(lds <= 160 * 1024, "LDS of a CU");
     if (lds > 48 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kv_prompt_kernel<DT, HD>),
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kv_prompt_kernel<DT, HD, EX>),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
     }
-    kv_prompt_kernel<DT, HD><<<dim3(l.grid), dim3(256), lds, l.s>>>(a);
+    kv_prompt_kernel<DT, HD, EX><<<dim3(l.grid), dim3(256), lds, l.s>>>(a);
     return hipGetLastError();
 }
-template <int DT>
+template <int DT, bool EX>
 hipError_t launch_prompt(const Args& a, const Launch& l) {
     return by_width<DT == FRQ_DT_F32 ? 128 : 256>(a.kv.hd,
-                                                  [&](auto w) { return run_prompt<DT, decltype(w)::value>(a, l); });
+                                                  [&](auto w) { return run_prompt<DT, decltype(w)::value, EX>(a, l); });
 }
 
 }  // namespace kv

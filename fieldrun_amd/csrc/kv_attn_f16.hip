@@ -3,7 +3,7 @@
 
 namespace frq {
 namespace kv {
-hipError_t launch_decode_f16(const Args& a, const Launch& l) { return launch_decode<FRQ_DT_F16>(a, l); }
-hipError_t launch_prompt_f16(const Args& a, const Launch& l) { return launch_prompt<FRQ_DT_F16>(a, l); }
+hipError_t launch_decode_f16(const Args& a, const Launch& l) { return launch_decode<FRQ_DT_F16, false>(a, l); }
+hipError_t launch_prompt_f16(const Args& a, const Launch& l) { return launch_prompt<FRQ_DT_F16, false>(a, l); }
 }  // namespace kv
 }  // namespace frq

@@ -3,7 +3,7 @@
 
 namespace frq {
 namespace kv {
-hipError_t launch_decode_i8(const Args& a, const Launch& l) { return launch_decode<FRQ_DT_ROWI8>(a, l); }
-hipError_t launch_prompt_i8(const Args& a, const Launch& l) { return launch_prompt<FRQ_DT_ROWI8>(a, l); }
+hipError_t launch_decode_i8(const Args& a, const Launch& l) { return launch_decode<FRQ_DT_ROWI8, false>(a, l); }
+hipError_t launch_prompt_i8(const Args& a, const Launch& l) { return launch_prompt<FRQ_DT_ROWI8, false>(a, l); }
 }  // namespace kv
 }  // namespace frq

@@ -36,6 +36,9 @@ struct Call {
     int64_t target;        // items wanted over all kv heads
     int min_chunk;         // keys a chunk at least, 64, 128 or 256
     const int32_t* plan;   // of many sequences: the chunk length and 0, then before each 64 sequences (items, slots)
+    int sinks, sink_span;  // with a window: first keys seen besides, and as a tile spans them (sink_keys; 0: none)
+    const uint64_t* tree;  // bit masks of drafted tokens, a row of q each (null: rows see what lies before them)
+    int64_t tree_pitch;    // words between the masks
 };
 
 struct Seq {
@@ -57,12 +60,18 @@ KV_HD Seq seq_of(const Call& c, int len, int r0, int r1) {
         q.len = 0;
         q.bad = true;
     }
+    if (c.tree && (q.rows > q.len || (q.rows + 63) / 64 > c.tree_pitch)) {  // no room for its tree
+        q.row0 = q.rows = q.len = 0;
+        q.bad = true;
+        return q;
+    }
     const int64_t pairs = (int64_t)q.rows * c.rep;
     if (pairs < c.min_pairs || pairs > c.max_pairs) return q;
     q.tiles = (int)((pairs + c.tp - 1) / c.tp);
-    // its window and its rows after the first, and the rounding of tile_lo
-    const int most = (c.tp - 1) / c.rep + 2, rows = q.rows < most ? q.rows : most;
-    const int64_t span = (int64_t)c.window + rows - 1 + ALIGN - 1;
+    // its window and its rows after the first (of a tree all, and the place
+    // before it), the rounding of tile_lo, the sinks
+    const int most = (c.tp - 1) / c.rep + 2, rows = c.tree ? q.rows + 1 : q.rows < most ? q.rows : most;
+    const int64_t span = (int64_t)c.window + rows - 1 + ALIGN - 1 + c.sink_span;
     q.ext = c.window && span < q.len ? (int)span : q.len;
     return q;
 }
@@ -118,6 +127,37 @@ KV_HD int64_t max_slots(int64_t target, int n_kv) { return 2 * (target / n_kv + 
 KV_HD int key_lo(const Call& c, int pos) { return c.window && pos - c.window + 1 > 0 ? pos - c.window + 1 : 0; }
 
 KV_HD int tile_lo(const Call& c, int pos) { return key_lo(c, pos) / ALIGN * ALIGN; }
+
+// With sinks a tile takes the keys 0 .. span - 1 first, and then goes on at
+// key span + gap; where its window begins no later, the keys from 0 on.
+// Without, it begins at key gap.
+struct Span {
+    int span, gap;
+};
+KV_HD Span span_at(const Call& c, int pos) {
+    const int lo = tile_lo(c, pos);
+    if (!c.sinks) return Span{0, lo};
+    return lo > c.sink_span ? Span{c.sink_span, lo - c.sink_span} : Span{0, 0};
+}
+KV_HD int sink_keys(int64_t sinks, int step) { return (int)((sinks + step - 1) / step * step); }  // whole tiles
+
+// Which of the N drafted tokens from t on (t may be below 0) a mask of n tokens
+// has, as bits; n 0: no mask is read.
+template <int N>
+KV_HD uint32_t tree_bits(const uint64_t* mask, int n, int t) {
+    static_assert(N <= 16, "");
+    if (n <= 0 || t <= -N || t >= n) return 0;
+    const int w = t > 0 ? t >> 6 : 0, sh = t & 63;
+    uint64_t m = mask[w];
+    if (t < 0) {
+        m <<= -t;
+    } else if (sh) {
+        m >>= sh;
+        if (sh > 64 - N && 64 * (w + 1) < n) m |= mask[w + 1] << (64 - sh);
+    }
+    const int left = n - t;  // bits past the tree count for nothing
+    return (uint32_t)m & ((1u << (left < N ? left : N)) - 1);
+}
 
 // A key's page id where the table holds one, else -1.
 KV_HD int page_ok(int id, int64_t n_pages) { return id >= 0 && (int64_t)id < n_pages ? id : -1; }

@@ -308,6 +308,38 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q,
                     double scale, double cap, size_t window, float* d_out,
                     size_t out_pitch, void* d_ws, size_t ws_bytes);
 
+/* frq_kv_attn_dev with more to see than a window: a row at position p sees the
+ * tokens j <= p of p - j < window and of j < sinks, a sequence's first ones,
+ * which stay (window 0: all).  Their pages stay in the table; those between them
+ * and the window may be gone.  Workspace and all else as there. */
+int frq_kv_attn_sink_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q,
+                         size_t q_pitch, size_t n_row, size_t n_head,
+                         const int32_t* d_pages, size_t pages_pitch,
+                         const int32_t* d_len, const int32_t* d_first,
+                         size_t n_seq, double scale, double cap, size_t window,
+                         size_t sinks, float* d_out, size_t out_pitch,
+                         void* d_ws, size_t ws_bytes);
+/* Attention for a tree of drafted tokens: the r rows of a sequence are its
+ * last r tokens, drafted ones in the order of its rows, and row i (row d_first[s]
+ * + i of q) sees those whose bit is set in its mask: bit t % 64 of word t / 64 of
+ * d_tree + (d_first[s] + i) * tree_pitch for the t-th, its ancestors' and its
+ * own (any set will do; bits from r on count for nothing).  Of the n = len - r
+ * tokens before it sees all, or with a window those of p - j < window and of j <
+ * sinks, where p = n - 1 + the number of drafted tokens it sees: its place in
+ * the sequence that its branch would make.  A row that sees nothing gets zeros.
+ * A sequence of fewer tokens than rows, or of more rows than 64 tree_pitch, is
+ * out of range: its rows stay as they were, and the next frq_sync reports it; the
+ * pages of its drafted tokens have to be there whether a row sees them or not.
+ * tree_pitch is 1 or more.  Workspace and all else as frq_kv_attn_dev. */
+int frq_kv_attn_tree_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q,
+                         size_t q_pitch, size_t n_row, size_t n_head,
+                         const int32_t* d_pages, size_t pages_pitch,
+                         const int32_t* d_len, const int32_t* d_first,
+                         size_t n_seq, double scale, double cap, size_t window,
+                         size_t sinks, const uint64_t* d_tree, size_t tree_pitch,
+                         float* d_out, size_t out_pitch, void* d_ws,
+                         size_t ws_bytes);
+
 /* ---- the unembed: Bundle::rowdot_f32 (src/bundle.rs:958-987) -----------
  * out[r] = dot(W[r], x) for every row of a frq_upload_rows table (out has
  * rows entries, x has d), bit-identical to the reference's order (f32/f16:

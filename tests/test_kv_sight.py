@@ -1,0 +1,178 @@
+"""Attention with sinks and trees without a GPU: the refusals, and the index
+arithmetic of kv_index.h on the host: the chunks of a tile cover every key that
+one of its rows sees once, within the bounds that the host launches by."""
+import ctypes as C
+import os
+import random
+import subprocess
+
+import pytest
+
+import fieldrun_amd as fa
+from test_kv import A, BAD_CACHES, ROOT, desc, message
+
+
+def call(d=None, tree=A, tree_pitch=1, sinks=4, q=A, qp=256, n_row=3, n_head=4, pages=A, width=5, lens=A, first=None, n_seq=3,
+         scale=0.1, cap=0.0, window=9, out=A, op=256, ws=A, ws_bytes=1 << 40, trees=True):
+    d = C.byref(desc()) if d is None else d
+    args = (None, d, q, qp, n_row, n_head, pages, width, lens, first, n_seq, scale, cap, window, sinks)
+    to = (out, op, ws, ws_bytes)
+    if trees:
+        return fa.lib.frq_kv_attn_tree_dev(*args, tree, tree_pitch, *to)
+    return fa.lib.frq_kv_attn_sink_dev(*args, *to)
+
+
+@pytest.mark.parametrize("trees", [False, True])
+@pytest.mark.parametrize("change,code,word", BAD_CACHES)
+def test_bad_descriptors_are_refused(change, code, word, trees):
+    assert call(C.byref(desc(**change)), trees=trees) == code and word in message(), message()
+
+
+@pytest.mark.parametrize("trees", [False, True])
+@pytest.mark.parametrize("change,word", [
+    (dict(n_head=3), "n_head"), (dict(n_row=4), "one row"), (dict(qp=255), "pitch"), (dict(op=100), "pitch"),
+    (dict(n_row=1 << 31, n_seq=1 << 31), "too many"), (dict(width=1 << 28), "2^31"), (dict(scale=float("nan")), "scale"),
+    (dict(cap=-1.0), "cap"), (dict(q=None), "null"), (dict(out=None), "null"), (dict(lens=None), "null"),
+    (dict(pages=None), "null"), (dict(ws=A + 4), "16-byte"), ({}, "null context"), (dict(sinks=1 << 63), "null context"),
+    (dict(window=0, sinks=0), "null context"), (dict(n_row=0, n_seq=0, q=None, out=None, lens=None), "null context"),
+])
+def test_bad_calls_are_refused(change, word, trees):
+    assert call(trees=trees, **change) == fa.FRQ_ERR_ARG and word in message(), message()
+
+
+@pytest.mark.parametrize("change,word", [(dict(tree=None), "null pointer"), (dict(tree_pitch=0), "tree"),
+                                         (dict(tree_pitch=1 << 41), "tree"),
+                                         (dict(tree=None, n_row=0, n_seq=0), "null context")])
+def test_bad_trees_are_refused(change, word):
+    assert call(**change) == fa.FRQ_ERR_ARG and word in message(), message()
+
+
+SRC = r"""
+#include "kv_index.h"
+using namespace frq::kv;
+struct Row { int32_t seq, tile, chunk, chunks, row0, rows, len, span, gap, ext, klen; };
+extern "C" int64_t plan(const int32_t* len, const int32_t* first, int n_seq, int n_row, int rep, int window, int sinks, int step,
+                        int trees, int tree_pitch, int n_kv, int tp, int64_t target, int min_chunk, Row* out, int64_t cap,
+                        int64_t* bounds, int* bad) {
+    Call c{len, first, n_seq, n_row, 8192, 4, rep, window, n_kv, tp, 1, 0x7FFFFFFF, target, min_chunk};
+    c.sinks = sinks;
+    c.sink_span = sink_keys(sinks, step);
+    c.tree = trees ? (const uint64_t*)8 : nullptr;
+    c.tree_pitch = tree_pitch;
+    int64_t total = 0, n = 0, slots = 0;
+    *bad = 0;
+    for (int s = 0; s < n_seq; ++s) { const Seq q = seq_at(c, s); total += keys_of(q); *bad += q.bad; }
+    const int klen = chunk_of(c, total);
+    for (int s = 0; s < n_seq; ++s) {
+        const Seq q = seq_at(c, s);
+        const int m = chunks_of(q, klen);
+        for (int t = 0; t < q.tiles; ++t)
+            for (int k = 0; k < m; ++k) {
+                const int base = q.len - q.rows;
+                const Span sp = span_at(c, trees ? base - 1 : base + (int)((int64_t)t * tp / rep));
+                if (n < cap) out[n] = Row{s, t, k, m, q.row0, q.rows, q.len, sp.span, sp.gap, q.ext, even_chunk(q, m)};
+                ++n;
+                if (m > 1) ++slots;
+            }
+    }
+    bounds[0] = max_items(c);
+    bounds[1] = max_slots(target, n_kv);
+    bounds[2] = slots;
+    return n;
+}
+extern "C" uint32_t bits(const uint64_t* mask, int n, int t, int of) {
+    return of == 1 ? tree_bits<1>(mask, n, t) : of == 4 ? tree_bits<4>(mask, n, t) : of == 8 ? tree_bits<8>(mask, n, t)
+                                                                                            : tree_bits<16>(mask, n, t);
+}
+"""
+
+
+class Row(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("seq", "tile", "chunk", "chunks", "row0", "rows", "len", "span", "gap", "ext", "klen")]
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    d = tmp_path_factory.mktemp("kv_sight")
+    (d / "plan.cpp").write_text(SRC)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", "-I",
+                    os.path.join(ROOT, "fieldrun_amd", "csrc"), str(d / "plan.cpp"), "-o", str(d / "plan.so")], check=True)
+    lib = C.CDLL(str(d / "plan.so"))
+    lib.plan.restype = C.c_int64
+    lib.plan.argtypes = [C.c_void_p, C.c_void_p] + [C.c_int] * 10 + [C.c_int64, C.c_int, C.c_void_p, C.c_int64, C.c_void_p,
+                                                                     C.c_void_p]
+    lib.bits.restype = C.c_uint32
+    lib.bits.argtypes = [C.c_void_p] + [C.c_int] * 3
+    return lib
+
+
+@pytest.mark.parametrize("of", [1, 4, 8, 16])
+def test_bits_of_a_mask(host, of):
+    """Around a tree's first and last token and its words' borders; bits past
+    its tokens count for nothing, and without a tree nothing is read."""
+    rng = random.Random(of)
+    for n in (1, 3, 63, 64, 65, 127, 128, 129, 200):
+        words = -(-n // 64)
+        mask = [rng.getrandbits(64) for _ in range(words)]
+        m = (C.c_uint64 * words)(*mask)  # not a word more
+        for t in range(-20, n + 20):
+            want = sum((0 <= t + j < n and mask[(t + j) // 64] >> (t + j) % 64 & 1) << j for j in range(of))
+            assert host.bits(m, n, t, of) == want
+    for t in range(-20, 20):
+        assert host.bits(None, 0, t, of) == 0
+
+
+def plan(host, lens, first, rep, window, sinks, step, trees, pitch=64, n_kv=4, tp=16, target=512, least=256):
+    n, cap = len(lens), 200000
+    out, bounds, bad = (Row * cap)(), (C.c_int64 * 3)(), C.c_int()
+    cf = (C.c_int32 * (n + 1))(*first) if first else None
+    m = host.plan((C.c_int32 * n)(*lens), cf, n, first[-1] if first else n, rep, window, sinks, step, int(trees), pitch, n_kv,
+                  tp, target, least, out, cap, bounds, C.byref(bad))
+    assert m <= cap
+    return [out[i] for i in range(m)], list(bounds), bad.value
+
+
+def test_chunks_cover_what_rows_see(host):
+    rng = random.Random(4)
+    for _ in range(400):
+        n = rng.choice([1, 2, 5, 70])
+        top = rng.choice([40, 700, 9000, 100000])
+        trees = rng.random() < 0.5
+        lens = [rng.choice([0, 1, rng.randint(0, top), top]) for _ in range(n)]
+        decode = rng.random() < 0.4 and all(lens)
+        rows = [1] * n if decode else [rng.choice([0, 1, rng.randint(0, 300)]) for _ in range(n)]
+        if trees:
+            rows = [min(a, b) for a, b in zip(rows, lens)]
+        first = None if decode else [sum(rows[:i]) for i in range(n + 1)]
+        window = rng.choice([0, 1, 33, 100, 4096])
+        sinks = rng.choice([0, 1, 4, 33, 64, 500, 100000]) if window else 0
+        rep, tp, step = rng.choice([1, 3, 7, 16]), rng.choice([16, 128]), rng.choice([32, 64])
+        items, bounds, bad = plan(host, lens, first, rep, window, sinks, step, trees, tp=tp)
+        assert bad == 0 and len(items) <= bounds[0] and bounds[2] <= bounds[1]
+        parts = {}
+        for i in items:
+            parts.setdefault((i.seq, i.tile), []).append(i)
+        assert len(parts) == sum(-(-r * rep // tp) for r in rows)
+        for (s, t), p in parts.items():
+            span, gap, base = p[0].span, p[0].gap, lens[s] - rows[s]
+            assert span % step == 0 and gap % 32 == 0 and gap >= 0
+            assert [x.chunk for x in p] == list(range(p[0].chunks))
+            a, b = t * tp // rep, (min((t + 1) * tp, rows[s] * rep) - 1) // rep
+            last = lens[s] - 1 if trees else base + b
+            # the tile's keys are 0 .. span - 1 and span + gap .. last, in runs of klen
+            assert p[0].chunks * p[0].klen >= last + 1 - gap
+            lows = [base - 1, base] if trees else [base + a]  # the places that the first row may stand at
+            for low in lows:
+                lo = max(0, low - window + 1) if window else 0
+                assert span + gap <= lo or (span == 0 and gap <= lo) or (span + gap == 0)
+                if sinks and low >= 0 and span + gap > 0:
+                    assert span >= min(sinks, lo)
+
+
+def test_trees_without_room_are_told(host):
+    for lens, first, pitch, want in (([70], [0, 70], 2, 0), ([70], [0, 70], 1, 1), ([69], [0, 70], 2, 1), ([64], [0, 64], 1, 0),
+                                     ([0, 5], [0, 1, 3], 1, 1), ([0, 5], [0, 0, 5], 1, 0), ([5, -1], [0, 5, 7], 1, 1)):
+        items, _, bad = plan(host, lens, first, 3, 0, 0, 32, True, pitch)
+        assert bad == want
+        assert all(i.rows <= i.len for i in items)
+    assert plan(host, [5], [0, 9], 3, 0, 0, 32, False)[2] == 0  # more rows than tokens: not of trees alone
