@@ -105,6 +105,8 @@ SIGNATURES = {
     "frq_norm_quant_i8_dev": (_I, [_P, _P, _P, _P, C.c_double, _S, _S, _P, _P, _P, _P, _P]),
     "frq_kv_write_dev": (_I, [_P, _P, _P, _P, _S, _P, _S]),
     "frq_kv_read_dev": (_I, [_P, _P, _P, _S, _P, _P, _S]),
+    "frq_sample_ws": (_S, [_S, _S]),
+    "frq_sample_dev": (_I, [_P, _P, _S, _S, _S, _P, _P, _P, _P, _P, _P, _P, _P, _S]),
     "frq_kv_append_dev": (_I, [_P, _P, _P, _P, _S, _S, _P, _P, _S, _P, _S]),
     "frq_kv_attn_ws": (_S, [_P, _S, _S, _S, _S]),
     "frq_kv_attn_dev": (_I, [_P, _P, _P, _S, _S, _S, _P, _S, _P, _P, _S, C.c_double, C.c_double, _S, _P, _S, _P, _S]),
@@ -200,6 +202,20 @@ class Context:
         rows quant_dev gives for it, on device pointers, for Weight.mm_q_dev."""
         _check(lib.frq_norm_quant_i8_dev(self.h, x_ptr, y_ptr, w_ptr, eps, m, k, sum_ptr, a8_ptr, sa_ptr, oidx_ptr,
                                          oval_ptr))
+
+    def sample_ws_bytes(self, m: int, n: int) -> int:
+        """Bytes of the workspace sample_dev takes for m rows of n logits."""
+        return lib.frq_sample_ws(m, n)
+
+    def sample_dev(self, logits_ptr: int, m: int, n: int, u_ptr: int, token_ptr: int, temp_ptr: int | None = None,
+                   topk_ptr: int | None = None, topp_ptr: int | None = None, minp_ptr: int | None = None,
+                   prob_ptr: int | None = None, pitch: int | None = None, ws_ptr: int | None = None, ws_bytes: int = 0):
+        """A token (int64) for each of m rows of n logits by its random number
+        u in [0, 1), temperature (0: the largest), top-k (int32), top-p and
+        min-p, arrays of m on the device (None: 1, all, all, all), and the
+        token's share of what was kept (frq_sample_dev)."""
+        _check(lib.frq_sample_dev(self.h, logits_ptr, n if pitch is None else pitch, m, n, temp_ptr, topk_ptr, topp_ptr,
+                                  minp_ptr, u_ptr, token_ptr, prob_ptr, ws_ptr, ws_bytes))
 
     # ---- uploads ----
     def upload_i8(self, wt_nk: np.ndarray, scale: np.ndarray) -> "Weight":

@@ -18,7 +18,7 @@ LIB = os.path.join(HERE, "libfrq.so")
 SOURCES = ["api.hip", "quant.hip", "gemv_i8.hip", "skinny_i8.hip", "gemm_i8.hip", "i4.hip", "moe.hip", "rowdot.hip",
            "bundle.hip", "gpt2.hip", "q4a.hip", "gemma.hip",
            "mm_f32.hip", "kv.hip", "kv_append.hip", "kv_attn_f32.hip", "kv_attn_f16.hip", "kv_attn_i8.hip",
-           "kv_attn_ex_f32.hip", "kv_attn_ex_f16.hip", "kv_attn_ex_i8.hip", "norm_quant.hip"]
+           "kv_attn_ex_f32.hip", "kv_attn_ex_f16.hip", "kv_attn_ex_i8.hip", "norm_quant.hip", "sample.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",

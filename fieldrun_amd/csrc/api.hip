@@ -34,7 +34,7 @@ struct frq_ctx {
     hipStream_t stream = nullptr;
     void* ws = nullptr;
     size_t ws_bytes = 0;
-    int* err = nullptr;  // device word: kernels atomically OR 1 on NaN input, 2 on a bad index (kv_attn.h)
+    int* err = nullptr;  // device word: kernels atomically OR 1 on NaN input, 2 on a bad index or parameter (kv_attn.h, sample.hip)
 };
 
 // Scratch of frq_mm_dev_noalloc: one static array per GPU (each device that
@@ -216,7 +216,7 @@ int check_err_word(frq_ctx* c) {
     if (h) {
         const int left = h & 1 ? h & ~1 : 0;  // one error a call; the index is told by the next
         HIPCHK(hipMemcpy(c->err, &left, sizeof(int), hipMemcpyHostToDevice), "hipMemcpy(err)");
-        if (!(h & 1)) return fail(FRQ_ERR_ARG, "a page, slot, length or row offset of the cache was out of range");
+        if (!(h & 1)) return fail(FRQ_ERR_ARG, "a page, slot, length or row offset of the cache, or a sampling parameter, was out of range");
         return fail(FRQ_ERR_NAN, "NaN in activations (the reference panics in partial_cmp().unwrap())");
     }
     return FRQ_OK;

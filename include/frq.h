@@ -115,8 +115,8 @@ int frq_set_stream(frq_ctx* ctx, void* hip_stream);
 void* frq_get_stream(frq_ctx* ctx);
 /* Wait for the ctx stream; returns FRQ_ERR_NAN if a _dev call since the last
  * sync saw a NaN activation, FRQ_ERR_ARG if one saw an index of the paged
- * cache out of range (of both the NaN first, the index by the next frq_sync),
- * else FRQ_OK / FRQ_ERR_HIP. */
+ * cache or a sampling parameter out of range (of both the NaN first, the other by
+ * the next frq_sync), else FRQ_OK / FRQ_ERR_HIP. */
 int frq_sync(frq_ctx* ctx);
 
 /* ---- weight upload (one-time, into persistent HBM) ---------------------- */
@@ -356,6 +356,32 @@ int frq_rowdot_f32_subset(frq_ctx* ctx, const frq_w* w, const float* x,
 int frq_rowdot_f32_subset_dev(frq_ctx* ctx, const frq_w* w, const float* d_x,
                               const int64_t* d_cand, size_t ncand,
                               float* d_out);
+
+/* ---- the token -----------------------------------------------------------
+ * A token for each of m rows of n logits (row i at d_logits + i * pitch), by its
+ * own parameters (device arrays of m; NULL: 1, no bound, 1 and 0 for all):
+ *   w_j = exp((x_j - max x) / d_temp[i]);  d_temp 0: the largest x (of equal ones
+ *   the lowest index), as the engines choose;
+ *   the d_topk[i] largest (0 and below, n and above: all; of equal ones those of
+ *   the lowest index); of these, from the largest on, those with less than
+ *   d_topp[i] of their sum before them (the first always; 1 and above: all); of
+ *   these those of w_j >= d_minp[i] (0: all);
+ *   d_token[i]: the first, in the tokens' order, up to which these sum to more
+ *   than d_u[i] (0 <= d_u < 1; a number outside counts as the nearest inside) of
+ *   their sum; d_prob[i] (nullable): its share of the sum.
+ * Weights are summed as whole numbers, in steps of 2^(log2(n) - 62), 2^-50 or
+ * more, of a largest one between 1/2 and 1 (none below half a step): the token
+ * does not depend on how the row was split.  A logit of -inf is never
+ * chosen.  A row with a NaN, or without a finite maximum, gets token -1 and share
+ * 0, and the next frq_sync returns FRQ_ERR_NAN; so does one whose temperature
+ * (negative, infinite) or another parameter (NaN) is none, as FRQ_ERR_ARG.
+ * n up to 2^24.  d_ws: frq_sample_ws bytes of device memory, 16-byte aligned, as
+ * in frq_kv_attn_dev; NULL: the context's, which a call under capture may not. */
+size_t frq_sample_ws(size_t m, size_t n);
+int frq_sample_dev(frq_ctx* ctx, const float* d_logits, size_t pitch, size_t m,
+                   size_t n, const float* d_temp, const int32_t* d_topk,
+                   const float* d_topp, const float* d_minp, const float* d_u,
+                   int64_t* d_token, float* d_prob, void* d_ws, size_t ws_bytes);
 
 /* ---- MoE experts: expert_f32 + expert_mm (src/bundle.rs:404-461) and the
  * routed branch of src/qwen3moe.rs:120-158 / src/gemma4.rs:131-187 -------- */
