@@ -9,29 +9,33 @@
 //
 // Weights are whole numbers, round(2^s w'), s up to 50 and s + log2(n) at most 62,
 // so that every sum is exact and the same in any order: a row is cut over
-// workgroups, and their sums meet in atomics, without the token depending on it.
+// workgroups, and sums meet in atomics, without the token depending on it.
 // (w' is w times a factor for all of a row that puts the largest between 1/2 and
 // 1; at 152064 tokens a step is 2^-44, and what is below half of it is none.)
 //
-// Nothing is sorted but a few candidates.  Three launches: each chunk's maximum
-// and its histogram over the logarithm of w, ten bins a factor of two; the bins
-// summed for the row, which gives those that are kept whole and those (one, mostly)
-// where a cut falls; then each chunk's sum of what is kept whole, and the elements
-// of the bins between as a list, which the row's last workgroup sorts, cuts, and
-// walks to the token.  A list that is too long (many equal logits) is cut by
-// radix selection over the row instead.
+// The row is never sorted.  Four launches: each chunk's maximum and its
+// histogram over the logarithm of w, ten bins a factor of two, from one reading
+// into registers; the bins summed for the row, which gives those that are kept
+// whole and those (one, mostly) where a cut falls; each chunk's sum of what is
+// kept whole, and the elements of the bins between as a list; the cuts in the list
+// (through finer bins where it is long), the chunk of the token, and the token.  A list that is too long (many equal logits)
+// is cut by radix selection over the row instead.
 #include "frq_internal.h"
 
 namespace frq {
 namespace smp {
 namespace {
 
-constexpr int NT = 256;           // threads
-constexpr int NB = 512, PER = 10; // bins, bins a factor of two: 51 of them
-constexpr int MAX_S = 50;         // E - v <= s + 1 where a weight is not zero
-constexpr int CAP = 2048;         // candidates of a row's list
+constexpr int NT = 512;            // threads
+constexpr int NB = 512, PER = 10;  // bins, bins a factor of two: 51 of them
+constexpr int MAX_S = 50;          // E - v <= s + 1 where a weight is not zero
+constexpr int CAP = 16384;         // elements of a row's list
+constexpr int FT = 512;            // threads of a row's last launch
+constexpr int FEW = FT;            // elements that are put in order
 constexpr int MAX_N = 1 << 24;
-constexpr int MAX_CHUNKS = 64;
+constexpr int MAX_V = 8;           // quads a thread at most
+constexpr int MAX_CHUNKS = MAX_N / (4 * NT * MAX_V);
+static_assert(NB == NT && NB == FT && MAX_CHUNKS <= 2 * FT, "");
 constexpr int ERR_NAN_BIT = 1, ERR_ARG_BIT = 2;
 
 struct __attribute__((packed, aligned(4))) F4 {
@@ -54,7 +58,7 @@ struct Row {
     int count_below;
     int k;              // 0: no bound
     float p;            // 1: no bound
-    int listed, ticket; // the list's length (may pass CAP), workgroups done
+    int listed;         // the list's length (may pass CAP)
 };
 
 struct Args {
@@ -140,39 +144,57 @@ __device__ __forceinline__ F4 load4(const float* x, int i, int end) {
     return f;
 }
 
-// Over the workgroup.
-__device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor((unsigned long long)v, d, 64);
-    return v;
+// Sums over the lanes up to and with each (DPP: within rows of 16, then the
+// rows' ends), and over the workgroup.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_add(uint64_t x) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xF, false);
+    return x + ((uint64_t)hi << 32 | lo);
 }
-__device__ uint64_t group_sum(uint64_t v, uint64_t* tmp) {  // tmp: [NT / 64]
-    v = wave_sum(v);
+__device__ __forceinline__ uint64_t lane_sums(uint64_t x) {
+    x = dpp_add<0x111, 0xF>(x);
+    x = dpp_add<0x112, 0xF>(x);
+    x = dpp_add<0x114, 0xF>(x);
+    x = dpp_add<0x118, 0xF>(x);
+    x = dpp_add<0x142, 0xA>(x);
+    return dpp_add<0x143, 0xC>(x);
+}
+__device__ __forceinline__ uint64_t last_lane(uint64_t x) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, 63);
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), 63) << 32 | lo;
+}
+template <int T>
+__device__ __forceinline__ uint64_t group_sum(uint64_t v, uint64_t* tmp) {  // tmp: [T / 64]
+    v = lane_sums(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63) tmp[threadIdx.x >> 6] = v;
     __syncthreads();
     v = 0;
 #pragma unroll
-    for (int i = 0; i < NT / 64; ++i) v += tmp[i];
+    for (int i = 0; i < T / 64; ++i) v += tmp[i];
     return v;
 }
-// The sum of the threads before.
-__device__ uint64_t group_before(uint64_t v, uint64_t* tmp) {
+// The sum of the threads before, and of all.
+template <int T>
+__device__ __forceinline__ uint64_t group_before(uint64_t v, uint64_t* tmp, uint64_t* all = nullptr) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    uint64_t x = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = __shfl_up((unsigned long long)x, d, 64);
-        if (lane >= d) x += o;
-    }
+    const uint64_t x = lane_sums(v);
     __syncthreads();
     if (lane == 63) tmp[w] = x;
     __syncthreads();
-    uint64_t before = x - v;
-    for (int i = 0; i < w; ++i) before += tmp[i];
+    uint64_t before = x - v, total = 0;
+#pragma unroll
+    for (int i = 0; i < T / 64; ++i) {
+        const uint64_t t = tmp[i];
+        total += t;
+        if (i < w) before += t;
+    }
+    if (all) *all = total;
     return before;
 }
 
+template <int NV>
 __global__ __launch_bounds__(NT) void sample_bins_kernel(const Args a) {
     __shared__ unsigned long long weight[NB];
     __shared__ uint32_t count[NB];
@@ -181,21 +203,25 @@ __global__ __launch_bounds__(NT) void sample_bins_kernel(const Args a) {
     const int r = blockIdx.x / a.chunks, ch = blockIdx.x % a.chunks, tid = threadIdx.x;
     const float* x = a.x + (int64_t)r * a.pitch;
     const int beg = ch * a.len, end = min(beg + a.len, a.n);
+    F4 f[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) f[i] = load4(x, beg + 4 * (i * NT + tid), end);
     const Ask q = ask_of(a, r);
+    weight[tid] = 0;
+    count[tid] = 0;
     float most = -__builtin_inff();
-    int at = beg < end ? beg : 0;
+    int at = beg;
     bool nan = false;
-    for (int i = beg + 4 * tid; i < end; i += 4 * NT) {
-        const F4 f = load4(x, i, end);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            nan |= f.v[j] != f.v[j];
-            if (f.v[j] > most) {
-                most = f.v[j];
-                at = i + j;
+            nan |= f[i].v[j] != f[i].v[j];
+            if (f[i].v[j] > most) {
+                most = f[i].v[j];
+                at = beg + 4 * (i * NT + tid) + j;
             }
         }
-    }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         const float o = __shfl_xor(most, d, 64);
@@ -219,17 +245,12 @@ __global__ __launch_bounds__(NT) void sample_bins_kernel(const Args a) {
     const double e = __builtin_ceil((double)most * q.c);
     if (tid == 0) a.chunk[(int64_t)r * a.chunks + ch] = Chunk{e, most, nan ? -1 : at};
     if ((!q.k && q.p == 1.0f) || q.greedy || q.bad) return;
-    for (int i = tid; i < NB; i += NT) {
-        weight[i] = 0;
-        count[i] = 0;
-    }
-    __syncthreads();
     if (!nan && most > -__builtin_inff() && most < __builtin_inff()) {
-        for (int i = beg + 4 * tid; i < end; i += 4 * NT) {
-            const F4 f = load4(x, i, end);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const double v = (double)f.v[j] * q.c;
+                const double v = (double)f[i].v[j] * q.c;
                 const uint64_t w = weight_of(v - e + (double)a.s);
                 if (w) {
                     const int b = min(bin_of(e, v), NB - 1);
@@ -237,14 +258,11 @@ __global__ __launch_bounds__(NT) void sample_bins_kernel(const Args a) {
                     atomicAdd(&count[b], 1u);
                 }
             }
-        }
     }
     __syncthreads();
     const int64_t to = ((int64_t)r * a.chunks + ch) * NB;
-    for (int i = tid; i < NB; i += NT) {
-        a.weight[to + i] = weight[i];
-        a.count[to + i] = count[i];
-    }
+    a.weight[to + tid] = weight[tid];
+    a.count[to + tid] = count[tid];
 }
 
 // f total for f of [0, 1), down to a whole number and whether it is more; exact
@@ -268,27 +286,63 @@ __device__ __forceinline__ uint64_t share_of(float p, uint64_t total) {
     return t > 0 ? t : 1;
 }
 
-__global__ __launch_bounds__(NT) void sample_row_kernel(const Args a) {
-    __shared__ uint64_t tmp[NT / 64];
-    __shared__ int kbin, lo, hi;
-    __shared__ uint64_t klo;
+constexpr int RT = 1024;  // threads of a row's launch: two a bin
+__global__ __launch_bounds__(RT) void sample_row_kernel(const Args a) {
+    __shared__ uint64_t half_w[NB], tmp[NT / 64];
+    __shared__ uint32_t half_n[NB];
+    __shared__ double we[RT / 64];
+    __shared__ float wmost[RT / 64];
+    __shared__ int wat[RT / 64];
+    __shared__ int kbin, lo, hi, count_below;
+    __shared__ uint64_t klo, below;
     __shared__ int shift[MAX_CHUNKS];  // whole factors of two between a chunk's scale and the row's; -1: too many
-    const int r = blockIdx.x, tid = threadIdx.x;
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const Ask q = ask_of(a, r);
     const Chunk* chunk = a.chunk + (int64_t)r * a.chunks;
     Row* row = a.row + r;
     float most = -__builtin_inff();
-    int at = 0;
+    int at = 0x7FFFFFFF;
     bool nan = false;
     double e = -__builtin_inf();
-    for (int i = 0; i < a.chunks; ++i) {
-        const Chunk c = chunk[i];
-        nan |= c.at < 0;
-        if (c.most > most) {
-            most = c.most;
-            at = c.at;
+    static_assert(MAX_CHUNKS <= RT, "");
+    if (tid < a.chunks) {
+        const Chunk c = chunk[tid];
+        nan = c.at < 0;
+        most = c.most;
+        at = c.at;
+        e = c.e;
+    }
+    const double mine = e;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const float o = __shfl_xor(most, d, 64);
+        const int oa = __shfl_xor(at, d, 64);
+        e = fmax(e, __shfl_xor(e, d, 64));
+        if (o > most || (o == most && oa < at)) {
+            most = o;
+            at = oa;
         }
-        e = fmax(e, c.e);
+    }
+    if (lane == 0) {
+        wmost[tid >> 6] = most;
+        wat[tid >> 6] = at;
+        we[tid >> 6] = e;
+    }
+    if (tid == 0) {
+        kbin = NB;
+        lo = NB;
+        hi = -1;
+        klo = 0;
+        below = 0;
+        count_below = 0;
+    }
+    nan = __syncthreads_or(nan);
+    for (int i = 0; i < min(RT / 64, (a.chunks + 63) / 64); ++i) {
+        e = fmax(e, we[i]);
+        if (wmost[i] > most || (wmost[i] == most && wat[i] < at)) {
+            most = wmost[i];
+            at = wat[i];
+        }
     }
     const bool finite = most > -__builtin_inff() && most < __builtin_inff();
     if (q.bad || nan || !finite || q.greedy) {
@@ -301,127 +355,172 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const Args a) {
         }
         return;
     }
-    uint64_t before[2] = {0, 0}, w[2] = {0, 0}, all = 0, below = 0;
-    uint32_t cbefore[2] = {0, 0}, n[2] = {0, 0};
-    int count_below = 0, k = 0;
-    if (tid == 0) {
-        kbin = NB;
-        lo = NB;
-        hi = -1;
-        klo = 0;
-    }
-    __syncthreads();
+    uint64_t all = 0;
+    int k = 0;
     if (q.k || q.p < 1.0f) {
         if (tid < a.chunks) {
-            const double de = e - chunk[tid].e;  // whole, or infinite
+            const double de = e - mine;  // whole, or infinite
             shift[tid] = de <= 51.0 ? (int)de : -1;
         }
         __syncthreads();
+        uint64_t w = 0;
+        uint32_t n = 0;
+        const int bin = tid % NB;
 #pragma unroll 8
-        for (int i = 0; i < a.chunks; ++i) {
-            const int sh = shift[i];
-            const int64_t from = ((int64_t)r * a.chunks + i) * NB;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int b = 2 * tid + j - PER * sh;
-                const bool in = sh >= 0 && b >= 0;
-                const int64_t at = from + (in ? b : 0);  // (loads without a branch, to be in flight together)
-                const uint64_t wb = a.weight[at];
-                const uint32_t nb = a.count[at];
-                w[j] += in ? wb >> sh : 0;
-                n[j] += in ? nb : 0;
+        for (int i = tid / NB; i < a.chunks; i += RT / NB) {
+            const int sh = shift[i], b = bin - PER * sh;
+            const bool in = sh >= 0 && b >= 0;
+            const int64_t from = ((int64_t)r * a.chunks + i) * NB + (in ? b : 0);  // (loads without a branch: all in flight)
+            const uint64_t wb = a.weight[from];
+            const uint32_t nb = a.count[from];
+            w += in ? wb >> sh : 0;
+            n += in ? nb : 0;
+        }
+        if (tid >= NB) {
+            half_w[bin] = w;
+            half_n[bin] = n;
+        }
+        __syncthreads();
+        // the first NB threads go on, a bin each; the others keep to the barriers
+        const bool on = tid < NB;
+        if (on) {
+            w += half_w[bin];
+            n += half_n[bin];
+        }
+        const uint64_t x = lane_sums(w);
+        const uint32_t c = (uint32_t)lane_sums(n);
+        if (on && lane == 63) {
+            tmp[tid >> 6] = x;
+            wat[tid >> 6] = (int)c;
+        }
+        __syncthreads();
+        uint64_t before = x - w;
+        uint32_t cbefore = c - n;
+        for (int i = 0; i < NB / 64; ++i) {
+            all += tmp[i];
+            if (i < tid >> 6) {
+                before += tmp[i];
+                cbefore += (uint32_t)wat[i];
             }
         }
-        before[0] = group_before(w[0] + w[1], tmp);
-        cbefore[0] = (uint32_t)group_before(n[0] + n[1], tmp);
-        before[1] = before[0] + w[0];
-        cbefore[1] = cbefore[0] + n[0];
-        all = group_sum(w[0] + w[1], tmp);
         // the bin where the k largest end
-        if (q.k) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (cbefore[j] < (uint32_t)q.k && cbefore[j] + n[j] >= (uint32_t)q.k) {
-                    kbin = 2 * tid + j;
-                    klo = before[j];
-                }
+        if (on && q.k && cbefore < (uint32_t)q.k && cbefore + n >= (uint32_t)q.k) {
+            kbin = bin;
+            klo = before;
         }
         __syncthreads();
         k = kbin < NB ? q.k : 0;
-        const int kb = kbin;
-        const uint64_t sure = k ? klo : all;
-        if (q.p < 1.0f) {
-            const uint64_t t = share_of(q.p, sure);
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (w[j] && before[j] <= t) {
-                    if (before[j] + w[j] > t) atomicMin(&lo, 2 * tid + j);
-                    if (before[j] < t) atomicMax(&hi, 2 * tid + j);
-                }
+        if (on && q.p < 1.0f && w) {
+            const uint64_t t = share_of(q.p, k ? klo : all);
+            if (before <= t && before + w > t) atomicMin(&lo, bin);
+            if (before < t) atomicMax(&hi, bin);
         }
         __syncthreads();
         if (tid == 0) {
             if (k) {
-                lo = min(lo, kb);
-                hi = kb;
+                lo = min(lo, kbin);
+                hi = kbin;
             } else if (q.p < 1.0f && lo > hi) {
                 lo = hi + 1;  // the cut falls between two bins
             }
         }
         __syncthreads();
-        // what lies before the list
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            if (2 * tid + j < lo) {
-                below += w[j];
-                count_below += (int)n[j];
-            }
+        if (on && bin == lo) {  // what lies before the list
+            below = before;
+            count_below = (int)cbefore;
         }
-        below = group_sum(below, tmp);
-        count_below = (int)group_sum((uint64_t)count_below, tmp);
+        __syncthreads();
     }
-    if (tid == 0) {
+    if (tid == 0)
         *row = Row{q.c, e, q.minp > 0.0f ? (double)most * q.c + log2((double)q.minp) : -__builtin_inf(),
-                   below, all, 0, lo, hi, count_below, k, q.p, 0, 0};
-    }
+                   below, all, 0, lo, hi, count_below, k, q.p, 0};
 }
 
-struct Last {  // the row's last workgroup
-    unsigned long long list[CAP];
+template <int NV>
+__global__ __launch_bounds__(NT) void sample_take_kernel(const Args a) {
+    __shared__ uint64_t tmp[NT / 64];
+    __shared__ int place;
+    const int r = blockIdx.x / a.chunks, ch = blockIdx.x % a.chunks, tid = threadIdx.x;
+    Row* rp = a.row + r;
+    const float* x = a.x + (int64_t)r * a.pitch;
+    const int beg = ch * a.len, end = min(beg + a.len, a.n);
+    F4 f[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) f[i] = load4(x, beg + 4 * (i * NT + tid), end);
+    if (rp->done) return;
+    const double c = rp->c, e = rp->e, least = rp->least;
+    const int lo = rp->lo, hi = rp->hi;
+    const double ce = a.chunk[(int64_t)r * a.chunks + ch].e, de = e - ce;
+    uint64_t sum = 0;
+    uint32_t in = 0;  // which of the thread's elements go to the list
+    if (de <= 51.0) {
+        const int sh = PER * (int)de;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const double v = (double)f[i].v[j] * c;  // (past the end: -inf)
+                const int b = bin_of(ce, v) + sh;
+                if (b < lo && v >= least) sum += weight_of(v - e + (double)a.s);
+                in |= b >= lo && b <= hi && beg + 4 * (i * NT + tid) + j < end ? 1u << (4 * i + j) : 0u;
+            }
+    }
+    sum = group_sum<NT>(sum, tmp);
+    if (tid == 0) a.kept[(int64_t)r * a.chunks + ch] = sum;
+    if (hi < lo) return;
+    uint64_t mine;  // one atomic a workgroup
+    int to = (int)group_before<NT>((uint64_t)__builtin_popcount(in), tmp, &mine);
+    if (tid == 0 && mine) place = atomicAdd(&rp->listed, (int)mine);
+    __syncthreads();
+    if (!in) return;
+    to += place;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (in >> (4 * i + j) & 1) {
+                if (to < CAP) a.list[(int64_t)r * CAP + to] = key_of(f[i].v[j], beg + 4 * (i * NT + tid) + j);
+                ++to;
+            }
+}
+
+struct Last {  // the row's last launch
     uint64_t kept[MAX_CHUNKS];
-    uint64_t tmp[NT / 64];
-    uint32_t count[256];
-    unsigned long long weight[256];
-    uint64_t cut, target;
-    int at, last;
+    double e[MAX_CHUNKS];
+    uint64_t few[FEW], order[FEW];
+    uint64_t tmp[FT / 64];
+    unsigned long long weight[NB];
+    uint32_t count[NB];
+    uint64_t rest, before;
+    int at, chunk, bin, n;
+    uint64_t list[1];  // CAP, where it is needed
 };
 
-// Descending, `size` (a power of two) keys.
-__device__ void sort_list(unsigned long long* v, int size) {
-    for (int k = 2; k <= size; k <<= 1)
-        for (int j = k >> 1; j; j >>= 1) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < size / 2; i += NT) {
-                const int lo = 2 * j * (i / j) + i % j, hi = lo + j;
-                const unsigned long long x = v[lo], y = v[hi];
-                if ((x < y) == !(lo & k)) {
-                    v[lo] = y;
-                    v[hi] = x;
-                }
-            }
-        }
+// few[0 .. n - 1], n up to FEW different keys, in descending order.
+__device__ __forceinline__ void put_in_order(Last& L, int n) {
+    __syncthreads();
+    const int tid = threadIdx.x;
+    if (tid < (n + 63) / 64 * 64) {  // whole waves
+        const uint64_t mine = tid < n ? L.few[tid] : 0;
+        int place = 0;
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) place += L.few[i] > mine;
+        if (tid < n) L.order[place] = mine;
+    }
     __syncthreads();
 }
 
-// Runs f(key, weight) over the row's elements of the list's bins.
+// Runs f(key, v, chunk) over the row's elements of the list's bins.
 template <typename F>
-__device__ __forceinline__ void over_list(const Args& a, const Row& row, const Chunk* chunk, const float* x, F&& f) {
+__device__ __forceinline__ void over_row(const Args& a, const Row& row, const Last& L, const float* x, F&& f) {
+#pragma unroll 1
     for (int ch = 0; ch < a.chunks; ++ch) {
         const int end = min((ch + 1) * a.len, a.n);
-        const double ce = chunk[ch].e, de = row.e - ce;
+        const double ce = L.e[ch], de = row.e - ce;
         if (!(de <= 51.0)) continue;
         const int sh = PER * (int)de;
-        for (int i = ch * a.len + 4 * (int)threadIdx.x; i < end; i += 4 * NT) {
+#pragma unroll 1
+        for (int i = ch * a.len + 4 * (int)threadIdx.x; i < end; i += 4 * FT) {
             const F4 v4 = load4(x, i, end);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -432,22 +531,27 @@ __device__ __forceinline__ void over_list(const Args& a, const Row& row, const C
         }
     }
 }
+__device__ __forceinline__ double v_of(const Row& row, uint64_t key) {
+    return (double)value_of((uint32_t)(key >> 32)) * row.c;
+}
 
-// The last key of the list's elements that is kept, where they do not fit: of
-// the first `want` (weight 0), or of those with less than `want` before them,
-// `before` with the bins before.  Eight bits of the order at a time, then the
-// index among equal ones.  Adds up what is kept into *sum.
-__device__ uint64_t select_cut(const Args& a, const Row& row, const Chunk* chunk, const float* x, Last& L, bool by_weight,
-                               uint64_t before, uint64_t want, uint64_t limit, uint64_t* sum) {
+// The last key that is kept of the elements of the list's bins with keys of
+// `limit` and more: of the first `want`, or (by_weight) of those with less than
+// `want` before them, `before` with the bins before.  *sum: the weight kept, with
+// `before`.  Over the row: eight bits of the order at a time, then the index among
+// equal ones.
+__device__ __forceinline__ uint64_t cut_row(const Args& a, const Row& row, const float* x, Last& L, bool by_weight,
+                                            uint64_t before, uint64_t want, uint64_t limit, uint64_t* sum) {
     const int tid = threadIdx.x;
     uint32_t prefix = 0;
     uint64_t total = before, n = 0;  // of larger keys
+#pragma unroll 1
     for (int shift = 24; shift >= 0; shift -= 8) {
         __syncthreads();
         L.count[tid] = 0;
         L.weight[tid] = 0;
         __syncthreads();
-        over_list(a, row, chunk, x, [&](uint64_t key, double v, int) {
+        over_row(a, row, L, x, [&](uint64_t key, double v, int) {
             const uint32_t o = (uint32_t)(key >> 32);
             if (key < limit || (shift < 24 && o >> (shift + 8) != prefix)) return;
             atomicAdd(&L.weight[o >> shift & 255], (unsigned long long)weight_of(v - row.e + (double)a.s));
@@ -466,181 +570,243 @@ __device__ uint64_t select_cut(const Args& a, const Row& row, const Chunk* chunk
     const uint64_t w = weight_of((double)value_of(prefix) * row.c - row.e + (double)a.s), ties = L.count[prefix & 255];
     uint64_t take = by_weight ? (total >= want ? 0 : w ? (want - total + w - 1) / w : ties) : want - n;
     if (take > ties) take = ties;
-    *sum = total + take * w - before;
+    *sum = total + take * w;
     if (!take) return prefix == 0xFFFFFFFFu ? ~0ull : (uint64_t)(prefix + 1) << 32;  // none of them
     uint64_t seen = 0;
     __syncthreads();
     if (tid == 0) L.at = -1;
-    for (int base = 0; base < a.n && seen < take; base += NT) {
+    for (int base = 0; base < a.n && seen < take; base += FT) {
         const int i = base + tid;
         const uint64_t mine = i < a.n && order_of(x[i]) == prefix && key_of(x[i], i) >= limit;
-        const uint64_t prior = seen + group_before(mine, L.tmp);
+        uint64_t all;
+        const uint64_t prior = seen + group_before<FT>(mine, L.tmp, &all);
         if (mine && prior + 1 == take) L.at = i;
-        seen += group_sum(mine, L.tmp);
+        seen += all;
     }
     __syncthreads();
     return (uint64_t)prefix << 32 | (uint32_t)~L.at;
 }
 
-__device__ void finish_row(const Args& a, int r, Last& L) {
+// The same over the list (FEW < n <= CAP, in LDS): bins of equal width over the
+// list's, then the elements of one in order.  False where that one has too many.
+__device__ __forceinline__ bool cut_list(const Args& a, const Row& row, int n, Last& L, bool by_weight, uint64_t before,
+                                         uint64_t want, uint64_t limit, uint64_t* sum, uint64_t* cut) {
     const int tid = threadIdx.x;
-    const Row row = a.row[r];
-    const float* x = a.x + (int64_t)r * a.pitch;
-    const Chunk* chunk = a.chunk + (int64_t)r * a.chunks;
-    const int n = row.listed;
-    const double s = (double)a.s;
-    for (int i = tid; i < a.chunks; i += NT) L.kept[i] = a.kept[(int64_t)r * a.chunks + i];
-    uint64_t cut = 0;  // the last key of the list that is kept
-    if (n > 0 && n <= CAP) {
-        int size = 2;
-        while (size < n) size <<= 1;
-        for (int i = tid; i < size; i += NT) L.list[i] = i < n ? a.list[(int64_t)r * CAP + i] : 0;
-        sort_list(L.list, size);
-        const int per = (size + NT - 1) / NT;  // a run of the order a thread
-        const int beg = tid * per, end = min(beg + per, n), held = row.k ? row.k - row.count_below : n;
-        auto weight = [&](int i) { return weight_of((double)value_of((uint32_t)(L.list[i] >> 32)) * row.c - row.e + s); };
-        uint64_t mine = 0, got = 0;
-        for (int i = beg; i < end; ++i) {
-            const uint64_t w = weight(i);
-            mine += w;
-            if (i < held) got += w;
-        }
-        uint64_t before = row.below + group_before(mine, L.tmp);
-        const uint64_t total = row.k ? row.below + group_sum(got, L.tmp) : row.all;
-        const uint64_t want = row.p < 1.0f ? share_of(row.p, total) : ~0ull;
-        uint64_t taken = 0;
-        for (int i = beg; i < end; ++i) {
-            taken += i < held && before < want;
-            before += weight(i);
-        }
-        taken = group_sum(taken, L.tmp);
-        cut = taken ? L.list[taken - 1] : ~0ull;
-        __syncthreads();
-        for (int i = tid; i < (int)taken; i += NT) {
-            const float v = value_of((uint32_t)(L.list[i] >> 32));
-            const int at = (int)~(uint32_t)L.list[i];
-            if ((double)v * row.c >= row.least)
-                atomicAdd((unsigned long long*)&L.kept[at / a.len], (unsigned long long)weight(i));
-        }
-    } else if (n > CAP) {
-        uint64_t total = row.all, sum = 0;
-        if (row.k) {
-            cut = select_cut(a, row, chunk, x, L, false, row.below, (uint64_t)(row.k - row.count_below), 0, &sum);
-            total = row.below + sum;
-        }
-        if (row.p < 1.0f) {
-            const uint64_t pcut = select_cut(a, row, chunk, x, L, true, row.below, share_of(row.p, total), cut, &sum);
-            cut = cut > pcut ? cut : pcut;
-        }
-        __syncthreads();
-        over_list(a, row, chunk, x, [&](uint64_t key, double v, int ch) {
-            if (key >= cut && v >= row.least)
-                atomicAdd((unsigned long long*)&L.kept[ch], (unsigned long long)weight_of(v - row.e + s));
-        });
+    if (by_weight && before >= want) {  // none
+        *sum = before;
+        *cut = ~0ull;
+        return true;
+    }
+    const double scale = (double)NB / (double)(row.hi - row.lo + 1);
+    auto bin = [&](uint64_t key) {  // (falls with the key)
+        const double d = ((row.e - v_of(row, key)) * (double)PER - (double)row.lo) * scale;
+        return d < (double)(NB - 1) ? d > 0.0 ? (int)d : 0 : NB - 1;
+    };
+    auto weight = [&](uint64_t key) { return weight_of(v_of(row, key) - row.e + (double)a.s); };
+    __syncthreads();
+    L.count[tid] = 0;
+    L.weight[tid] = 0;
+    if (tid == 0) {
+        L.bin = -1;
+        L.n = 0;
     }
     __syncthreads();
-    // the chunk, then the token
-    uint64_t total = 0;
-    for (int i = 0; i < a.chunks; ++i) total += L.kept[i];
-    const float u = fminf(fmaxf(a.u[r], 0.0f), 0.999999940395355225f);  // below 1: 1 - 2^-24
-    bool more;
-    uint64_t target = part_of(u, total, &more);  // below total, which holds the largest weight
-    int ch = 0;
-    while (ch + 1 < a.chunks && target >= L.kept[ch]) target -= L.kept[ch++];
-    const int first = ch * a.len, end = min(first + a.len, a.n);
-    const double ce = chunk[ch].e;
-    const int sh = PER * (int)(row.e - ce);
-    if (tid == 0) L.at = -1;
-    __syncthreads();
-    for (int base = first; base < end; base += 4 * NT) {
-        const int i = base + 4 * tid;
-        uint64_t w[4] = {0, 0, 0, 0}, mine = 0;
-        if (i < end) {
-            const F4 f = load4(x, i, end);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const double v = (double)f.v[j] * row.c;
-                const int b = bin_of(ce, v) + sh;
-                const bool in = i + j < end && v >= row.least &&
-                                (b < row.lo || (b <= row.hi && key_of(f.v[j], i + j) >= cut));
-                w[j] = in ? weight_of(v - row.e + s) : 0;
-                mine += w[j];
-            }
-        }
-        uint64_t before = group_before(mine, L.tmp);
-        const uint64_t sum = group_sum(mine, L.tmp);
-        if (target < sum) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (w[j] && target >= before && target < before + w[j]) {
-                    a.token[r] = i + j;
-                    if (a.prob) a.prob[r] = (float)((double)w[j] / (double)total);
-                }
-                before += w[j];
-            }
-            break;
-        }
-        target -= sum;
+#pragma unroll 1
+    for (int i = tid; i < n; i += FT) {
+        const uint64_t key = L.list[i];
+        if (key < limit) continue;
+        const int b = bin(key);
+        atomicAdd(&L.weight[b], (unsigned long long)weight(key));
+        atomicAdd(&L.count[b], 1u);
     }
+    __syncthreads();
+    const uint64_t w = L.weight[tid], c = L.count[tid];
+    uint64_t all;
+    const uint64_t wb = before + group_before<FT>(w, L.tmp, &all), cb = group_before<FT>(c, L.tmp);
+    if (c && (by_weight ? wb < want && wb + w >= want : cb < want && cb + c >= want)) {
+        L.bin = tid;
+        L.before = wb;
+        L.chunk = (int)cb;
+    }
+    __syncthreads();
+    const int at = L.bin;
+    if (at < 0) {  // all of them
+        *sum = before + all;
+        *cut = limit;
+        return true;
+    }
+    if (L.count[at] > FEW) return false;
+    const uint64_t start = L.before, first = (uint64_t)L.chunk;
+#pragma unroll 1
+    for (int i = tid; i < n; i += FT) {
+        const uint64_t key = L.list[i];
+        if (key >= limit && bin(key) == at) L.few[atomicAdd(&L.n, 1)] = key;
+    }
+    __syncthreads();
+    const int m = L.n;
+    put_in_order(L, m);
+    const uint64_t mine = tid < m ? weight(L.order[tid]) : 0;
+    const uint64_t prior = start + group_before<FT>(mine, L.tmp);
+    const bool in = tid < m && (by_weight ? prior < want : first + (uint64_t)tid < want);
+    const int taken = __syncthreads_count(in);
+    *sum = start + group_sum<FT>(in ? mine : 0, L.tmp);
+    *cut = L.order[taken - 1];  // (the bin holds the last one)
+    __syncthreads();
+    return true;
 }
 
-__global__ __launch_bounds__(NT) void sample_take_kernel(const Args a) {
-    __shared__ Last L;
-    const int r = blockIdx.x / a.chunks, ch = blockIdx.x % a.chunks, tid = threadIdx.x, lane = tid & 63;
-    Row* rp = a.row + r;
-    if (rp->done) return;
-    const double c = rp->c, e = rp->e, least = rp->least;
-    const int lo = rp->lo, hi = rp->hi;
-    const float* x = a.x + (int64_t)r * a.pitch;
-    const int beg = ch * a.len, end = min(beg + a.len, a.n);
-    const double ce = a.chunk[(int64_t)r * a.chunks + ch].e, de = e - ce;
-    uint64_t sum = 0;
-    if (de <= 51.0) {
-        const int sh = PER * (int)de;
-        for (int i = beg + 4 * tid; i - 4 * lane < end; i += 4 * NT) {  // whole waves
-            F4 f;
-            if (i < end) f = load4(x, i, end);
+// A workgroup a row.  Bound by latency: what it runs is one chain of a dozen loads
+// and barriers, so it keeps its code short and its sums in few steps.
+__global__ __launch_bounds__(FT) void sample_token_kernel(const Args a) {
+    extern __shared__ __align__(16) char lds[];
+    Last& L = *reinterpret_cast<Last*>(lds);
+    const int r = blockIdx.x, tid = threadIdx.x;
+    const Row row = a.row[r];
+    const uint64_t* list = a.list + (int64_t)r * CAP;
+    const uint64_t ahead = list[tid];  // (memory of the list, whatever its length)
+    uint64_t two[2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const double v = i + j < end ? (double)f.v[j] * c : -__builtin_inf();
-                const int b = bin_of(ce, v) + sh;
-                if (b < lo && v >= least) sum += weight_of(v - e + (double)a.s);
-                const bool in = b >= lo && b <= hi;
-                const uint64_t who = __builtin_amdgcn_ballot_w64(in);
-                if (who) {  // one place a wave
-                    int at = 0;
-                    if (lane == __builtin_ctzll(who)) at = atomicAdd(&rp->listed, __builtin_popcountll(who));
-                    at = __builtin_amdgcn_readlane(at, __builtin_ctzll(who)) +
-                         __builtin_popcountll(who & (((uint64_t)1 << lane) - 1));
-                    if (in && at < CAP) a.list[(int64_t)r * CAP + at] = key_of(f.v[j], i + j);
-                }
-            }
+    for (int j = 0; j < 2; ++j) two[j] = tid + j * FT < a.chunks ? a.kept[(int64_t)r * a.chunks + tid + j * FT] : 0;
+    if (row.done) return;
+    const float* x = a.x + (int64_t)r * a.pitch;
+    const int n = row.listed;
+    const double s = (double)a.s;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        if (tid + j * FT < a.chunks) {
+            L.kept[tid + j * FT] = two[j];
+            L.e[tid + j * FT] = a.chunk[(int64_t)r * a.chunks + tid + j * FT].e;
+        }
+    uint64_t cut = 0;  // the last key of the list that is kept
+    auto weight = [&](uint64_t key) { return weight_of(v_of(row, key) - row.e + s); };
+    auto keep = [&](uint64_t key) {
+        if (v_of(row, key) >= row.least)
+            atomicAdd((unsigned long long*)&L.kept[(int)~(uint32_t)key / a.len], (unsigned long long)weight(key));
+    };
+    if (n > 0 && n <= FEW) {
+        L.few[tid] = ahead;
+        put_in_order(L, n);
+        const uint64_t key = L.order[tid < n ? tid : 0], w = tid < n ? weight(key) : 0;
+        const bool first = tid < (row.k ? min(n, row.k - row.count_below) : n);
+        uint64_t total = row.all;
+        const uint64_t before = row.below + group_before<FT>(w, L.tmp);
+        if (row.k) total = row.below + group_sum<FT>(first ? w : 0, L.tmp);
+        const bool in = first && (row.p == 1.0f || before < share_of(row.p, total));
+        const int taken = __syncthreads_count(in);
+        cut = taken ? L.order[taken - 1] : ~0ull;
+        if (in) keep(key);
+    } else if (n > FEW) {
+        const bool here = n <= CAP;
+        if (here) {
+            L.list[tid] = ahead;
+#pragma unroll 4
+            for (int i = tid + FT; i < n; i += FT) L.list[i] = list[i];
+        }
+        __syncthreads();
+        // by the number, then by the share
+        uint64_t total = row.all;
+#pragma unroll 1
+        for (int by = row.k ? 0 : 1; by < (row.p < 1.0f ? 2 : 1); ++by) {
+            const uint64_t want = by ? share_of(row.p, total) : (uint64_t)(row.k - row.count_below), limit = cut;
+            uint64_t sum;
+            if (!here || !cut_list(a, row, n, L, by, row.below, want, limit, &sum, &cut))
+                cut = cut_row(a, row, x, L, by, row.below, want, limit, &sum);
+            cut = cut > limit ? cut : limit;
+            total = sum;
+        }
+        __syncthreads();
+        if (here) {
+#pragma unroll 1
+            for (int i = tid; i < n; i += FT)
+                if (L.list[i] >= cut) keep(L.list[i]);
+        } else {
+            over_row(a, row, L, x, [&](uint64_t key, double, int) {
+                if (key >= cut) keep(key);
+            });
         }
     }
-    sum = group_sum(sum, L.tmp);
-    if (tid == 0) a.kept[(int64_t)r * a.chunks + ch] = sum;
-    // the row's last workgroup goes on
-    __threadfence();
+    if (tid == 0) {
+        L.chunk = 0;
+        L.rest = ~0ull;
+    }
     __syncthreads();
-    if (tid == 0) L.last = __hip_atomic_fetch_add(&rp->ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == a.chunks - 1;
+    // the chunk of the token (two a thread)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) two[j] = 2 * tid + j < a.chunks ? L.kept[2 * tid + j] : 0;
+    uint64_t total;
+    uint64_t before = group_before<FT>(two[0] + two[1], L.tmp, &total);
+    const float u = fminf(fmaxf(a.u[r], 0.0f), 0.999999940395355225f);  // below 1: 1 - 2^-24
+    bool more;
+    const uint64_t target = part_of(u, total, &more);  // below total, which holds the largest weight
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        if (target >= before && target - before < two[j]) {
+            L.chunk = 2 * tid + j;
+            L.rest = target - before;
+        }
+        before += two[j];
+    }
     __syncthreads();
-    if (!L.last) return;
-    __threadfence();
-    finish_row(a, r, L);
+    // the token: the chunk in runs of four a thread
+    const int ch = L.chunk, end = min((ch + 1) * a.len, a.n);
+    const double ce = L.e[ch];
+    const int sh = PER * (int)(row.e - ce);
+    uint64_t rest = L.rest;
+    int i = ch * a.len + 4 * tid;
+    F4 f = load4(x, i, end);
+#pragma unroll 1
+    for (;;) {
+        const F4 next = load4(x, i + 4 * FT, end);
+        uint64_t w[4], mine = 0, sum;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const double v = (double)f.v[j] * row.c;
+            const int b = bin_of(ce, v) + sh;
+            const bool in = i + j < end && v >= row.least && (b < row.lo || (b <= row.hi && key_of(f.v[j], i + j) >= cut));
+            w[j] = in ? weight_of(v - row.e + s) : 0;
+            mine += w[j];
+        }
+        before = group_before<FT>(mine, L.tmp, &sum);
+        if (rest < sum || i - 4 * tid + 4 * FT >= end) {
+            if (rest >= before && rest - before < mine) {
+                rest -= before;
+                int j = 0;
+                uint64_t wj = w[0];
+#pragma unroll
+                for (int k = 1; k < 4; ++k)
+                    if (j == k - 1 && rest >= wj) {
+                        rest -= wj;
+                        wj = w[k];
+                        j = k;
+                    }
+                a.token[r] = i + j;
+                if (a.prob) a.prob[r] = (float)((double)wj / (double)total);
+            }
+            return;
+        }
+        rest -= sum;
+        i += 4 * FT;
+        f = next;
+    }
 }
 
 // How a call's rows are cut, and its workspace.
 struct Plan {
-    int chunks, len, s;
+    int quads, chunks, len, s;  // quads a thread; logits a chunk
     size_t row, chunk, weight, count, kept, list, bytes;
 };
 Plan plan_of(size_t m, size_t n) {
     Plan p{};
-    size_t want = (768 + m - 1) / m;
-    want = std::min(want, (n + 2047) / 2048);
-    want = std::max<size_t>(1, std::min<size_t>(want, 40));
-    p.len = (int)round_up((n + want - 1) / want, 4);
-    p.chunks = (int)((n + p.len - 1) / p.len);
+    p.quads = MAX_V;
+    auto cut = [&]() {
+        p.len = 4 * NT * p.quads;
+        p.chunks = (int)((n + p.len - 1) / p.len);
+    };
+    cut();
+    while (p.quads > 1 && m * p.chunks < 1024 && p.chunks < 20) {
+        p.quads /= 2;
+        cut();
+    }
     int bits = 0;
     while (((size_t)1 << bits) < n) ++bits;
     p.s = std::min(MAX_S, 62 - bits);
@@ -713,14 +879,28 @@ int frq_sample_dev(frq_ctx* ctx, const float* d_logits, size_t pitch, size_t m, 
         if (st != hipStreamCaptureStatusNone) return bad("under graph capture the caller gives the workspace");
         if (int rc = ctx_ws(ctx, p.bytes, &d_ws)) return rc;
     }
+    constexpr int LAST = sizeof(Last) + CAP * 8;
+    static_assert(LAST <= 160 * 1024, "LDS of a CU");
+    if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(sample_token_kernel),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, LAST);
+        e != hipSuccess)
+        return set_error(FRQ_ERR_HIP, std::string("hipFuncSetAttribute: ") + hipGetErrorString(e));
     char* ws = (char*)d_ws;
     const Args a{d_logits, (int64_t)pitch, (int)n, p.s, p.chunks, p.len, d_temp, d_topp, d_minp, d_u, d_topk, d_token, d_prob,
                  (Row*)(ws + p.row), (Chunk*)(ws + p.chunk), (uint64_t*)(ws + p.weight), (uint32_t*)(ws + p.count),
                  (uint64_t*)(ws + p.kept), (uint64_t*)(ws + p.list), ctx_err(ctx)};
-    const dim3 all((unsigned)(m * p.chunks)), rows((unsigned)m), b(NT);
-    sample_bins_kernel<<<all, b, 0, s>>>(a);
-    sample_row_kernel<<<rows, b, 0, s>>>(a);
-    sample_take_kernel<<<all, b, 0, s>>>(a);
+    const dim3 all((unsigned)(m * p.chunks)), rows((unsigned)m);
+    auto go = [&](auto quads) {
+        constexpr int NV = decltype(quads)::value;
+        sample_bins_kernel<NV><<<all, dim3(NT), 0, s>>>(a);
+        sample_row_kernel<<<rows, dim3(RT), 0, s>>>(a);
+        sample_take_kernel<NV><<<all, dim3(NT), 0, s>>>(a);
+        sample_token_kernel<<<rows, dim3(FT), LAST, s>>>(a);
+    };
+    if (p.quads == 1) go(std::integral_constant<int, 1>{});
+    else if (p.quads == 2) go(std::integral_constant<int, 2>{});
+    else if (p.quads == 4) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 8>{});
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? FRQ_OK : set_error(FRQ_ERR_HIP, std::string("launch sample: ") + hipGetErrorString(e));
 }

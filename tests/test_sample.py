@@ -25,4 +25,4 @@ def test_workspace():
     assert size(0, 5) == size(5, 0) == size(1, (1 << 24) + 1) == size((1 << 20) + 1, 5) == 0
     for m in (1, 7, 64, 1000, 1 << 20):
         for n in (1, 3, 5000, 152064, 1 << 24):
-            assert 0 < size(m, n) < m * 32768 + (40 << 20)
+            assert 0 < size(m, n) < m * (140000 + (n // 16384 + 41) * 7000)
