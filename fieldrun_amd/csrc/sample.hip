@@ -32,6 +32,7 @@ constexpr int MAX_S = 50;          // E - v <= s + 1 where a weight is not zero
 constexpr int CAP = 16384;         // elements of a row's list
 constexpr int FT = 512;            // threads of a row's last launch
 constexpr int FEW = FT;            // elements that are put in order
+constexpr int LISTED = 2048;        // top-k up to this: the list holds all of them
 constexpr int MAX_N = 1 << 24;
 constexpr int MAX_V = 8;           // quads a thread at most
 constexpr int MAX_CHUNKS = MAX_N / (4 * NT * MAX_V);
@@ -84,6 +85,10 @@ struct Ask {  // a row's parameters
     float p, minp;
     int k;
     bool greedy, bad;
+    // which histograms the row needs: up to LISTED of the largest are all listed,
+    // and their weights are taken from the list
+    __device__ __forceinline__ bool counts() const { return k > 0; }
+    __device__ __forceinline__ bool weights() const { return p < 1.0f && (k == 0 || k > LISTED); }
 };
 __device__ __forceinline__ Ask ask_of(const Args& a, int r) {
     Ask q;
@@ -124,6 +129,12 @@ __device__ __forceinline__ uint64_t weight_of(double y) {
 __device__ __forceinline__ int bin_of(double e, double v) {
     const double d = (e - v) * (double)PER;
     return d < (double)NB ? (int)d : NB;
+}
+// A number that every x with x c above v (in log2, give or take the roundings of
+// numbers as large as e) is not below.
+__device__ __forceinline__ float floor_of(double v, double e, double c) {
+    const float f = (float)((v - 0.01 - __builtin_fabs(e) * 0x1p-48) / c);
+    return f - __builtin_fabsf(f) * 0x1p-22f - 1e-37f;
 }
 // The order of finite floats as whole numbers (both zeros alike).
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -244,25 +255,42 @@ __global__ __launch_bounds__(NT) void sample_bins_kernel(const Args a) {
         }
     const double e = __builtin_ceil((double)most * q.c);
     if (tid == 0) a.chunk[(int64_t)r * a.chunks + ch] = Chunk{e, most, nan ? -1 : at};
-    if ((!q.k && q.p == 1.0f) || q.greedy || q.bad) return;
+    if ((!q.counts() && !q.weights()) || q.greedy || q.bad) return;
     if (!nan && most > -__builtin_inff() && most < __builtin_inff()) {
+        const float least = floor_of(e - (double)(a.s + 1), e, q.c);  // below: no weight
+        if (q.weights()) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+            for (int i = 0; i < NV; ++i) {
+                const float top = fmaxf(fmaxf(f[i].v[0], f[i].v[1]), fmaxf(f[i].v[2], f[i].v[3]));
+                if (!__builtin_amdgcn_ballot_w64(top >= least)) continue;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const double v = (double)f[i].v[j] * q.c;
-                const uint64_t w = weight_of(v - e + (double)a.s);
-                if (w) {
-                    const int b = min(bin_of(e, v), NB - 1);
-                    atomicAdd(&weight[b], (unsigned long long)w);
-                    atomicAdd(&count[b], 1u);
+                for (int j = 0; j < 4; ++j) {
+                    const double v = (double)f[i].v[j] * q.c;
+                    const uint64_t w = weight_of(v - e + (double)a.s);
+                    if (w) {
+                        const int b = min(bin_of(e, v), NB - 1);
+                        atomicAdd(&weight[b], (unsigned long long)w);
+                        if (q.counts()) atomicAdd(&count[b], 1u);
+                    }
                 }
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const float top = fmaxf(fmaxf(f[i].v[0], f[i].v[1]), fmaxf(f[i].v[2], f[i].v[3]));
+                if (!__builtin_amdgcn_ballot_w64(top >= least)) continue;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int b = bin_of(e, (double)f[i].v[j] * q.c);
+                    if (b < NB) atomicAdd(&count[b], 1u);
+                }
+            }
+        }
     }
     __syncthreads();
     const int64_t to = ((int64_t)r * a.chunks + ch) * NB;
-    a.weight[to + tid] = weight[tid];
-    a.count[to + tid] = count[tid];
+    if (q.weights()) a.weight[to + tid] = weight[tid];
+    if (q.counts()) a.count[to + tid] = count[tid];
 }
 
 // f total for f of [0, 1), down to a whole number and whether it is more; exact
@@ -270,13 +298,19 @@ __global__ __launch_bounds__(NT) void sample_bins_kernel(const Args a) {
 __device__ __forceinline__ uint64_t part_of(float f, uint64_t total, bool* more) {
     const uint32_t u = __float_as_uint(f), e = u >> 23, m = e ? (u & 0x7FFFFFu) | 0x800000u : u & 0x7FFFFFu;
     const int sh = 150 - (int)(e ? e : 1);  // f = m 2^-sh, sh of 24 and more
-    const unsigned __int128 x = (unsigned __int128)total * m;
-    if (sh >= 128) {
-        *more = x != 0;
+    // m total = hi 2^32 + lo, hi below 2^54
+    const uint64_t a = (uint64_t)(uint32_t)total * m, hi = (total >> 32) * m + (a >> 32);
+    const uint32_t lo = (uint32_t)a;
+    if (sh >= 96) {
+        *more = hi || lo;
         return 0;
     }
-    *more = (x & (((unsigned __int128)1 << sh) - 1)) != 0;
-    return (uint64_t)(x >> sh);
+    if (sh >= 32) {
+        *more = lo || (hi & (((uint64_t)1 << (sh - 32)) - 1));
+        return hi >> (sh - 32);
+    }
+    *more = lo & ((1u << sh) - 1);
+    return hi << (32 - sh) | lo >> sh;
 }
 // ceil(p total), at least one: what lies before an element is less than that
 // where the element is kept.
@@ -286,47 +320,38 @@ __device__ __forceinline__ uint64_t share_of(float p, uint64_t total) {
     return t > 0 ? t : 1;
 }
 
-constexpr int RT = 1024;  // threads of a row's launch: two a bin
+// A workgroup a row.  Bound by latency, the loads of the chunks' histograms and
+// the fetching of its own code, which is run once.
+constexpr int RT = 1024;  // threads: two a bin
 __global__ __launch_bounds__(RT) void sample_row_kernel(const Args a) {
-    __shared__ uint64_t half_w[NB], tmp[NT / 64];
-    __shared__ uint32_t half_n[NB];
-    __shared__ double we[RT / 64];
+    __shared__ uint64_t half_w[NB], tmp[NB / 64];
+    __shared__ uint32_t half_n[NB], tmp_n[NB / 64];
     __shared__ float wmost[RT / 64];
     __shared__ int wat[RT / 64];
     __shared__ int kbin, lo, hi, count_below;
     __shared__ uint64_t klo, below;
     __shared__ int shift[MAX_CHUNKS];  // whole factors of two between a chunk's scale and the row's; -1: too many
-    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Ask q = ask_of(a, r);
-    const Chunk* chunk = a.chunk + (int64_t)r * a.chunks;
     Row* row = a.row + r;
+    static_assert(MAX_CHUNKS <= RT && MAX_CHUNKS <= 64 * (RT / 64), "");
     float most = -__builtin_inff();
-    int at = 0x7FFFFFFF;
-    bool nan = false;
-    double e = -__builtin_inf();
-    static_assert(MAX_CHUNKS <= RT, "");
+    int at = 0;
+    double mine = 0.0;
     if (tid < a.chunks) {
-        const Chunk c = chunk[tid];
-        nan = c.at < 0;
+        const Chunk c = a.chunk[(int64_t)r * a.chunks + tid];
         most = c.most;
         at = c.at;
-        e = c.e;
+        mine = c.e;
     }
-    const double mine = e;
+    // the first chunk with the largest number holds its first index
+    float top = most;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const float o = __shfl_xor(most, d, 64);
-        const int oa = __shfl_xor(at, d, 64);
-        e = fmax(e, __shfl_xor(e, d, 64));
-        if (o > most || (o == most && oa < at)) {
-            most = o;
-            at = oa;
-        }
-    }
-    if (lane == 0) {
-        wmost[tid >> 6] = most;
-        wat[tid >> 6] = at;
-        we[tid >> 6] = e;
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(most == top) | (1ull << 63));
+    if (lane == who) {
+        wmost[wave] = top;
+        wat[wave] = at;
     }
     if (tid == 0) {
         kbin = NB;
@@ -336,14 +361,14 @@ __global__ __launch_bounds__(RT) void sample_row_kernel(const Args a) {
         below = 0;
         count_below = 0;
     }
-    nan = __syncthreads_or(nan);
-    for (int i = 0; i < min(RT / 64, (a.chunks + 63) / 64); ++i) {
-        e = fmax(e, we[i]);
-        if (wmost[i] > most || (wmost[i] == most && wat[i] < at)) {
+    const bool nan = __syncthreads_or(at < 0);
+    most = wmost[0];
+    at = wat[0];
+    for (int i = 1; i < (a.chunks + 63) / 64; ++i)
+        if (wmost[i] > most) {
             most = wmost[i];
             at = wat[i];
         }
-    }
     const bool finite = most > -__builtin_inff() && most < __builtin_inff();
     if (q.bad || nan || !finite || q.greedy) {
         if (tid == 0) {
@@ -355,9 +380,11 @@ __global__ __launch_bounds__(RT) void sample_row_kernel(const Args a) {
         }
         return;
     }
+    const double e = __builtin_ceil((double)most * q.c);
+    const bool ws = q.weights(), ns = q.counts();
     uint64_t all = 0;
     int k = 0;
-    if (q.k || q.p < 1.0f) {
+    if (ws || ns) {
         if (tid < a.chunks) {
             const double de = e - mine;  // whole, or infinite
             shift[tid] = de <= 51.0 ? (int)de : -1;
@@ -366,15 +393,25 @@ __global__ __launch_bounds__(RT) void sample_row_kernel(const Args a) {
         uint64_t w = 0;
         uint32_t n = 0;
         const int bin = tid % NB;
+        const int64_t base = (int64_t)r * a.chunks * NB;
+        // (loads without a branch: all in flight)
+        if (ws) {
+#pragma unroll 4
+            for (int i = tid / NB; i < a.chunks; i += RT / NB) {
+                const int sh = shift[i], b = bin - PER * sh;
+                const bool in = sh >= 0 && b >= 0;
+                const uint64_t wb = a.weight[base + i * NB + (in ? b : 0)];
+                w += in ? wb >> sh : 0;
+            }
+        }
+        if (ns) {
 #pragma unroll 8
-        for (int i = tid / NB; i < a.chunks; i += RT / NB) {
-            const int sh = shift[i], b = bin - PER * sh;
-            const bool in = sh >= 0 && b >= 0;
-            const int64_t from = ((int64_t)r * a.chunks + i) * NB + (in ? b : 0);  // (loads without a branch: all in flight)
-            const uint64_t wb = a.weight[from];
-            const uint32_t nb = a.count[from];
-            w += in ? wb >> sh : 0;
-            n += in ? nb : 0;
+            for (int i = tid / NB; i < a.chunks; i += RT / NB) {
+                const int sh = shift[i], b = bin - PER * sh;
+                const bool in = sh >= 0 && b >= 0;
+                const uint32_t nb = a.count[base + i * NB + (in ? b : 0)];
+                n += in ? nb : 0;
+            }
         }
         if (tid >= NB) {
             half_w[bin] = w;
@@ -390,27 +427,28 @@ __global__ __launch_bounds__(RT) void sample_row_kernel(const Args a) {
         const uint64_t x = lane_sums(w);
         const uint32_t c = (uint32_t)lane_sums(n);
         if (on && lane == 63) {
-            tmp[tid >> 6] = x;
-            wat[tid >> 6] = (int)c;
+            tmp[wave] = x;
+            tmp_n[wave] = c;
         }
         __syncthreads();
         uint64_t before = x - w;
         uint32_t cbefore = c - n;
+#pragma unroll
         for (int i = 0; i < NB / 64; ++i) {
             all += tmp[i];
-            if (i < tid >> 6) {
+            if (i < wave) {
                 before += tmp[i];
-                cbefore += (uint32_t)wat[i];
+                cbefore += tmp_n[i];
             }
         }
         // the bin where the k largest end
-        if (on && q.k && cbefore < (uint32_t)q.k && cbefore + n >= (uint32_t)q.k) {
+        if (on && ns && cbefore < (uint32_t)q.k && cbefore + n >= (uint32_t)q.k) {
             kbin = bin;
             klo = before;
         }
         __syncthreads();
         k = kbin < NB ? q.k : 0;
-        if (on && q.p < 1.0f && w) {
+        if (on && ws && w) {
             const uint64_t t = share_of(q.p, k ? klo : all);
             if (before <= t && before + w > t) atomicMin(&lo, bin);
             if (before < t) atomicMax(&hi, bin);
@@ -418,10 +456,14 @@ __global__ __launch_bounds__(RT) void sample_row_kernel(const Args a) {
         __syncthreads();
         if (tid == 0) {
             if (k) {
-                lo = min(lo, kbin);
+                lo = ws ? min(lo, kbin) : q.p < 1.0f ? 0 : kbin;
                 hi = kbin;
-            } else if (q.p < 1.0f && lo > hi) {
+            } else if (ws && lo > hi) {
                 lo = hi + 1;  // the cut falls between two bins
+            } else if (q.p < 1.0f && !ws) {
+                lo = 0;  // fewer than k are in the bins: all of them are listed
+                hi = NB - 1;
+                k = q.k;
             }
         }
         __syncthreads();
@@ -433,7 +475,7 @@ __global__ __launch_bounds__(RT) void sample_row_kernel(const Args a) {
     }
     if (tid == 0)
         *row = Row{q.c, e, q.minp > 0.0f ? (double)most * q.c + log2((double)q.minp) : -__builtin_inf(),
-                   below, all, 0, lo, hi, count_below, k, q.p, 0};
+                   below, ws ? all : 0, 0, lo, hi, count_below, k, q.p, 0};
 }
 
 template <int NV>
@@ -455,8 +497,15 @@ __global__ __launch_bounds__(NT) void sample_take_kernel(const Args a) {
     uint32_t in = 0;  // which of the thread's elements go to the list
     if (de <= 51.0) {
         const int sh = PER * (int)de;
+        // what lies past the bins, or has no weight, or (without a list) is below
+        // min_p, by whole waves
+        double past = fmax(e - (double)(hi >= lo ? hi + 1 : lo) / (double)PER, e - (double)(a.s + 1));
+        if (hi < lo) past = fmax(past, least);
+        const float skip = floor_of(past, e, c);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            const float top = fmaxf(fmaxf(f[i].v[0], f[i].v[1]), fmaxf(f[i].v[2], f[i].v[3]));
+            if (!__builtin_amdgcn_ballot_w64(top >= skip)) continue;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const double v = (double)f[i].v[j] * c;  // (past the end: -inf)
@@ -464,6 +513,7 @@ __global__ __launch_bounds__(NT) void sample_take_kernel(const Args a) {
                 if (b < lo && v >= least) sum += weight_of(v - e + (double)a.s);
                 in |= b >= lo && b <= hi && beg + 4 * (i * NT + tid) + j < end ? 1u << (4 * i + j) : 0u;
             }
+        }
     }
     sum = group_sum<NT>(sum, tmp);
     if (tid == 0) a.kept[(int64_t)r * a.chunks + ch] = sum;
