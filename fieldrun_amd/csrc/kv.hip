@@ -162,9 +162,9 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const Move m) {
 template <bool EX>
 __global__ __launch_bounds__(256) void kv_join_kernel(const Args a, const Args b, unsigned grid_a) {
     __shared__ f4 so[256];
-    __shared__ float sm[256], sl[256];
-    if (blockIdx.x < grid_a) join_item<16, EX>(a, blockIdx.x, so, sm, sl);
-    else join_item<128, EX>(b, blockIdx.x - grid_a, so, sm, sl);
+    __shared__ float sm[256], sl[256], fac[EX ? JOIN_FACTORS : 1];
+    if (blockIdx.x < grid_a) join_item<16, EX>(a, blockIdx.x, so, sm, sl, fac);
+    else join_item<128, EX>(b, blockIdx.x - grid_a, so, sm, sl, fac);
 }
 
 // The plans of many sequences (workgroup 0: the decode launch's, 1: the
@@ -274,6 +274,25 @@ constexpr int64_t PROMPT_TARGET = 400, PROMPT_TARGET_WIDE = 240;
 // 8 times over 2000 71, 49.5).
 constexpr int DEC_PAIRS = 128;
 
+// Trees: a sequence's rows all see (nearly) the same keys, so the prompt kernel's
+// tiles of 128 pairs save their reading anew, from little more than a tile of the
+// decode kernel on: 16 f16 sequences of up to 4000 tokens with 112 pairs 126 us
+// on the decode kernel, 60 on the prompt kernel, 4 of 128 pairs 68, 46, one of 256
+// pairs over 32768 tokens 238, 97.  Where the whole call is small its latency
+// counts: one sequence of 112 pairs over 8000 tokens 27, 32 us, of 56 over 211
+// 9.7, 19.6, of 336 over 2000 27, 27.  (The tokens are those that the table has room
+// for; lengths are device data.)
+constexpr int TREE_PAIRS = 32;
+constexpr double TREE_WORK = 6e6;  // rows x heads x tokens
+// With sinks or trees the items fill the chip's workgroups once, less the chunks
+// that every tile is rounded up by (half a target at least): one tree of 256 pairs
+// over 32768 f16 tokens 106 us at 400 items, 97 at 496; 16 int8 ones of up to 182
+// pairs 75 us at 400, 88 at 512; 4 f32 ones, one workgroup a CU, 121 at 400, 82 at 220.
+int64_t ex_target(const frq_kv* kv, const Call& prompt) {
+    const int64_t slots = kv->dtype == FRQ_DT_F32 || kv->hd > 128 ? 256 : 512;
+    return std::max(slots / 2, slots - max_tiles(prompt) * prompt.n_kv);
+}
+
 // The work of an attention call, and its workspace: the items' records, the
 // decode tiles' parts, where a sequence may ask with several rows the prompt
 // tiles', and for many sequences both launches' plans.
@@ -281,7 +300,9 @@ struct Plan {
     Call dec, prompt;
     size_t rec_dec, rec_prompt, part_dec, part_prompt, plan_dec, plan_prompt, bytes;  // offsets, the whole
 };
-Plan plan_of(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq) {
+// tokens: those that a table has room for, for calls with trees (0: none); ex: with
+// trees or sinks.
+Plan plan_of(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq, bool ex, size_t tokens) {
     Plan p{};
     Call& c = p.dec;
     c.n_seq = (int)n_seq;
@@ -299,10 +320,11 @@ Plan plan_of(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq) {
     c.tp = 16;
     c.target = DEC_TARGET;
     p.prompt = c;
-    p.prompt.min_pairs = DEC_PAIRS + 1;
+    p.prompt.min_pairs = 1 + (tokens ? (double)n_row * (double)n_head * (double)tokens > TREE_WORK ? TREE_PAIRS : 0x7FFFFFFE
+                                     : DEC_PAIRS);
     p.prompt.tp = 128;
     // (n_row <= n_seq: no room for parts, every tile's keys in one run)
-    p.prompt.target = n_row <= n_seq ? 1 : kv->hd > 128 ? PROMPT_TARGET_WIDE : PROMPT_TARGET;
+    p.prompt.target = n_row <= n_seq ? 1 : ex ? ex_target(kv, p.prompt) : kv->hd > 128 ? PROMPT_TARGET_WIDE : PROMPT_TARGET;
     p.prompt.min_chunk = 128;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -356,7 +378,8 @@ int attend(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, siz
     if (d_ws && ((uintptr_t)d_ws & 15)) return bad("the workspace must be 16-byte aligned");
     if (!ctx) return bad("null context");
     if (!n_row || !n_seq) return FRQ_OK;
-    const Plan plan = plan_of(kv, n_row, n_head, n_seq);
+    const bool ex = sinks || more.trees;
+    const Plan plan = plan_of(kv, n_row, n_head, n_seq, ex, more.trees ? std::max<size_t>(1, pages_pitch << shift) : 0);
     const size_t need = plan.bytes;
     if (d_ws && ws_bytes < need) return bad("the workspace is below frq_kv_attn_ws");
     Guard g(ctx_device(ctx));
@@ -400,9 +423,9 @@ int attend(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, siz
     // decode kernel against the prompt kernel: 256 channels 288, 340 us over
     // themselves, 72, 78 at 600 rows, 1612, 1508 over 8192 tokens; 192 channels 225,
     // 202 and 1280, 676.  Widths of an odd number of 32s do not fit the LDS.)
-    const bool prompts = d_first && n_row * (size_t)a.c.rep > (size_t)DEC_PAIRS &&
+    const bool prompts = d_first && n_row * (size_t)a.c.rep >= (size_t)plan.prompt.min_pairs &&
                          !(kv->dtype == FRQ_DT_F32 && kv->hd > 128);
-    a.c.max_pairs = prompts ? DEC_PAIRS : 0x7FFFFFFF;
+    a.c.max_pairs = prompts ? plan.prompt.min_pairs - 1 : 0x7FFFFFFF;
     char* ws = (char*)d_ws;
     a.rec = (Record*)(ws + plan.rec_dec);
     a.part = (float*)(ws + plan.part_dec);
@@ -429,7 +452,7 @@ int attend(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, siz
         a.c.plan = pa;
         b.c.plan = pb;
     }
-    const bool ex = sinks || more.trees, f32 = kv->dtype == FRQ_DT_F32, f16 = kv->dtype == FRQ_DT_F16;
+    const bool f32 = kv->dtype == FRQ_DT_F32, f16 = kv->dtype == FRQ_DT_F16;
     if (ex) e = f32 ? launch_decode_ex_f32(a, la) : f16 ? launch_decode_ex_f16(a, la) : launch_decode_ex_i8(a, la);
     else e = f32 ? launch_decode_f32(a, la) : f16 ? launch_decode_f16(a, la) : launch_decode_i8(a, la);
     if (e != hipSuccess) return hip_bad(e, "launch kv_decode");
@@ -486,7 +509,7 @@ size_t frq_kv_attn_ws(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_se
     if (!kv || !kv->n_kv || kv->n_kv > 65535 || kv->hd > MAX_HD || !n_head || n_head % kv->n_kv ||
         n_head / kv->n_kv > 65535 || n_row > 0x7FFFFFFF || n_seq > 0x7FFFFFFF)
         return 0;
-    return plan_of(kv, n_row, n_head, n_seq).bytes;
+    return std::max(plan_of(kv, n_row, n_head, n_seq, false, 0).bytes, plan_of(kv, n_row, n_head, n_seq, true, 0).bytes);
 }
 
 int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, size_t n_row, size_t n_head,

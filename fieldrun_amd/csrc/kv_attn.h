@@ -1564,8 +1564,62 @@ __device__ __forceinline__ void redo_share(const Args& a, const Record& it, int 
 // latency: 4.5 to 5.5 us at 60 to 280 chunks of 16 pairs of 128 channels, 10 us for
 // 7 prompts' 128 pairs (a float4 a thread at a time: 585 rows of 8 heads of 256
 // 64 us in all against 57).
+// EX: trees have tiles of 128 pairs in many chunks.  There the factors of a
+// share's pairs, exp2(m_c - m) / sum, are formed first, so that the chunks' outputs
+// are added without waiting for one another (256 pairs in 26 chunks 8.6 us against
+// 17.4; in 3 to 8 chunks 15.2 against 11.9).
+constexpr int JOIN_CHUNKS = 12;
+constexpr int JOIN_FACTORS = 128 + 3 * 512;  // pairs of a share times chunks, at most
+template <int TP>
+__device__ __forceinline__ bool join_share(const Args& a, const Record& it, int kvh, int beg, int end, float* fac) {
+    const int n_kv = a.c.n_kv, hd = a.kv.hd, h4 = hd / 4, tid = threadIdx.x, p0 = it.tile * TP, nc = it.chunks;
+    const int64_t pitch = (int64_t)TP * (hd + 2) * n_kv;
+    const float* part = a.part + (it.slot * n_kv + kvh) * (int64_t)(TP * (hd + 2));
+    const int first = beg / h4, pairs = (end - 1) / h4 - first + 1;
+    bool hole = false;
+    // 16 lanes a pair
+    for (int p = tid / 16; p < (pairs + 15) / 16 * 16; p += 16) {
+        const int pair = first + min(p, pairs - 1);
+        float m = -__builtin_inff(), l = 0.0f;
+        for (int c = tid % 16; c < nc; c += 16) {
+            const float mc = part[c * pitch + 2 * pair], lc = part[c * pitch + 2 * pair + 1];
+            hole |= lc == HOLE;
+            const float mn = fmaxf(m, mc), mr = mn == -__builtin_inff() ? 0.0f : mn;
+            l = l * __builtin_amdgcn_exp2f(m - mr) + lc * __builtin_amdgcn_exp2f(mc - mr);
+            m = mn;
+        }
+        auto merge = [&](uint32_t om, uint32_t ol) {
+            const float mo = __uint_as_float(om), lo = __uint_as_float(ol);
+            const float mn = fmaxf(m, mo), mr = mn == -__builtin_inff() ? 0.0f : mn;
+            l = l * __builtin_amdgcn_exp2f(m - mr) + lo * __builtin_amdgcn_exp2f(mo - mr);
+            m = mn;
+        };
+        merge(xshfl<1>(__float_as_uint(m)), xshfl<1>(__float_as_uint(l)));
+        merge(xshfl<2>(__float_as_uint(m)), xshfl<2>(__float_as_uint(l)));
+        merge(xshfl<4>(__float_as_uint(m)), xshfl<4>(__float_as_uint(l)));
+        merge(xshfl<8>(__float_as_uint(m)), xshfl<8>(__float_as_uint(l)));
+        const float mr = m == -__builtin_inff() ? 0.0f : m;
+        const float r = over(l, sight_of<true>(a, it.row0, it.rows, it.len, (p0 + pair) / a.c.rep).any());
+        if (p < pairs)
+            for (int c = tid % 16; c < nc; c += 16)
+                fac[p * nc + c] = __builtin_amdgcn_exp2f(part[c * pitch + 2 * pair] - mr) * r;
+    }
+    if (__syncthreads_or(hole)) return false;
+    for (int e = beg + tid; e < end; e += 256) {
+        const int pair = e / h4, c4 = e - pair * h4;
+        const float* f = fac + (pair - first) * nc;
+        const float* d = part + 2 * TP + (int64_t)pair * hd + 4 * c4;
+        f4 o{0, 0, 0, 0};
+#pragma unroll 8
+        for (int c = 0; c < nc; ++c) o += *reinterpret_cast<const f4*>(d + c * pitch) * f[c];
+        const int pr = p0 + pair, row = pr / a.c.rep, head = kvh * a.c.rep + pr % a.c.rep;
+        *reinterpret_cast<F4*>(a.out + (int64_t)(it.row0 + row) * a.out_pitch + (int64_t)head * hd + 4 * c4) =
+            F4{{o[0], o[1], o[2], o[3]}};
+    }
+    return true;
+}
 template <int TP, bool EX>
-__device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so, float* sm, float* sl) {
+__device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so, float* sm, float* sl, float* fac) {
     const int n_kv = a.c.n_kv, kvh = block % n_kv;
     const Record it = a.rec[block / n_kv];
     if (it.chunks <= 1) {
@@ -1578,6 +1632,13 @@ __device__ __forceinline__ void join_item(const Args& a, unsigned block, f4* so,
     const int p0 = it.tile * TP, np = min(TP, it.rows * a.c.rep - p0);
     const int n4 = np * (hd / 4), per = (n4 + it.chunks - 1) / it.chunks;
     const int beg = it.chunk * per, end = min(n4, beg + per);
+    if constexpr (EX) {
+        // (a share is ceil(pairs / chunks) pairs and part of two more)
+        if (it.chunks > JOIN_CHUNKS && ((end - 1) / (hd / 4) - beg / (hd / 4) + 1) * it.chunks <= JOIN_FACTORS) {
+            if (beg < end && !join_share<TP>(a, it, kvh, beg, end, fac)) redo_share<TP, true>(a, it, kvh, beg, end);
+            return;
+        }
+    }
     int pe = 1;
     while (pe < per && pe < 256) pe *= 2;
     const int runs = 256 / pe, run = tid / pe;
