@@ -129,7 +129,12 @@ __device__ __forceinline__ void append_values(const Append& a, unsigned block, E
     store_values<E, WR>(m, kvh, at, lv);
 }
 
-constexpr int MAX_ROWS = 8;  // a workgroup's, of queries and keys
+// Workgroups of values, then of queries and keys: some rows and heads, four heads
+// a lane in flight, the rows' turns in LDS.  Bound by memory for long prompts: 8192
+// rows of 36 heads of 128 channels, int8 pages, 277 MB in 66 us (4.2 TB/s); 8 rows
+// a workgroup 76, 4 70, 1 68; two heads in flight 77 at 8 rows.  A step's few rows
+// are bound by latency: one f16 row of 18 heads of 64 2.8 us, 61 f32 rows of 25 of 80 3.7.
+constexpr int MAX_ROWS = 2;  // a workgroup's, of queries and keys
 template <int DT, int G, int WR>
 __global__ __launch_bounds__(256) void kv_append_kernel(const Append a) {
     using E = Elem<DT>;
@@ -170,6 +175,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const Append a) {
     for (int p = 0; p < items; p += NB * NG) {
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
+            if (p + i * NG >= items) break;  // (of all lanes)
             const int it = p + i * NG + first, r = it & rmask, u = min(u0 + (it >> a.rshift), u1 - 1);
             const int64_t row = r0 + r;
             const bool in = act && it < items && row < m.n, key = u >= a.n_head;
@@ -256,12 +262,12 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const Append a) {
 
 template <int DT, int G, int WR>
 void launch_append(Append& a, hipStream_t s) {
-    // Rows and heads a workgroup: 8 rows with all heads, less where that leaves
+    // Rows and heads a workgroup: 2 rows with all heads, less where that leaves
     // the chip unfilled, down to one pass over a workgroup's lanes.
     constexpr int NG = 256 / G;
     const int all = a.n_head + a.m.n_kv;
     auto groups = [&]() { return ((a.m.n + (1 << a.rshift) - 1) >> a.rshift) * ((all + a.units - 1) / a.units); };
-    a.rshift = 3;
+    a.rshift = 1;
     a.units = all;
     while (a.rshift && (groups() < 1024 || (int64_t)1 << a.rshift >= 2 * a.m.n)) --a.rshift;
     while (groups() < 1024 && a.units << a.rshift > NG && a.units > 1) a.units = (a.units + 1) / 2;
