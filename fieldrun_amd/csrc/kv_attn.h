@@ -266,7 +266,7 @@ struct Sight {
     int lo, hi;
     __device__ __forceinline__ bool any() const { return hi >= 0; }
     __device__ __forceinline__ int first() const { return lo; }
-    template <int N>
+    template <int N, bool HELD = false>
     __device__ __forceinline__ Run seen(int key) const {  // of the N keys from `key` on
         return Run{key, lo, hi};
     }
@@ -276,14 +276,18 @@ struct Sight<true> {
     int lo, hi, sinks, base, n;  // n: drafted tokens (0: no tree)
     bool some;
     const uint64_t* mask;
+    uint64_t word;  // its first word, for HELD: most trees have no second
     __device__ __forceinline__ bool any() const { return some; }
     __device__ __forceinline__ int first() const { return sinks ? 0 : n && lo > base ? base : lo; }
-    template <int N>
+    template <int N, bool HELD = false>
     __device__ __forceinline__ Bits seen(int key) const {
         static_assert(N <= 16, "");
         uint32_t x = 0;
 #pragma unroll
         for (int j = 0; j < N; ++j) x |= (key + j >= lo || key + j < sinks) && key + j <= hi ? 1u << j : 0u;
+        if constexpr (HELD) {
+            if (n <= 64) return Bits{x | tree_bits<N>(&word, n, key - base)};
+        }
         return Bits{x | tree_bits<N>(mask, n, key - base)};
     }
 };
@@ -298,6 +302,7 @@ __device__ __forceinline__ Sight<EX> sight_of(const Args& a, int row0, int rows,
         s.base = len - rows;
         s.n = 0;
         s.mask = nullptr;
+        s.word = 0;
         if (!a.c.tree) {
             s.hi = s.base + row;
             s.lo = key_lo(a.c, s.hi);
@@ -305,10 +310,14 @@ __device__ __forceinline__ Sight<EX> sight_of(const Args& a, int row0, int rows,
         } else {
             s.n = rows;
             s.mask = a.c.tree + (int64_t)(row0 + row) * a.c.tree_pitch;
+            s.word = s.mask[0];
             int depth = 0;
-            for (int w = 0; 64 * w < rows; ++w) {
-                const int left = rows - 64 * w;
-                depth += __builtin_popcountll(s.mask[w] & (left < 64 ? ((uint64_t)1 << left) - 1 : ~(uint64_t)0));
+            if (a.c.window || s.base <= 0) {  // (else every row sees all that was cached)
+                for (int w = 0; 64 * w < rows; ++w) {
+                    const int left = rows - 64 * w;
+                    const uint64_t m = w ? s.mask[w] : s.word;
+                    depth += __builtin_popcountll(m & (left < 64 ? ((uint64_t)1 << left) - 1 : ~(uint64_t)0));
+                }
             }
             s.hi = s.base - 1;
             s.lo = key_lo(a.c, s.base - 1 + depth);
@@ -696,7 +705,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
         // keys that not every pair of the tile sees
         const bool edge = (base < lo_b && !(EX && base + KT <= sinks)) || base + KT - 1 > pos_a;
         if (edge) {
-            const auto sees = sight.template seen<4 * NU>(base + T::PL * g);
+            const auto sees = sight.template seen<4 * NU, true>(base + T::PL * g);
 #pragma unroll
             for (int j = 0; j < 4 * NU; ++j) {
                 if (!sees[j]) {
