@@ -17,9 +17,14 @@
 // histogram over the logarithm of w, ten bins a factor of two, from one reading
 // into registers; the bins summed for the row, which gives those that are kept
 // whole and those (one, mostly) where a cut falls; each chunk's sum of what is
-// kept whole, and the elements of the bins between as a list; the cuts in the list
-// (through finer bins where it is long), the chunk of the token, and the token.  A list that is too long (many equal logits)
-// is cut by radix selection over the row instead.
+// kept whole, and the elements of the bins between as a list; the cuts in the
+// list (through finer bins where it is long), the chunk of the token, and the
+// token.  A list that is too long (many equal logits) is cut by radix selection
+// over the row instead.  Short rows take one launch (sample_one_kernel).
+//
+// Few rows are bound by the launches' latency (one row of 152064 logits 23 us, 9
+// of 50257 28 us), many by the two readings of the logits: 64 rows of 152064 (39
+// MB) 48 us, of which the histograms 15 and the second reading 16.
 #include "frq_internal.h"
 
 namespace frq {
@@ -205,88 +210,127 @@ __device__ __forceinline__ uint64_t group_before(uint64_t v, uint64_t* tmp, uint
     return before;
 }
 
+// A thread's quads of a chunk: quad i of thread t lies at beg + 4 (i NT + t).  Held
+// in registers, or (one launch for all: its code is run once, and loops are shorter)
+// in LDS.
 template <int NV>
-__global__ __launch_bounds__(NT) void sample_bins_kernel(const Args a) {
-    __shared__ unsigned long long weight[NB];
-    __shared__ uint32_t count[NB];
-    __shared__ float wmost[NT / 64];
-    __shared__ int wat[NT / 64];
-    const int r = blockIdx.x / a.chunks, ch = blockIdx.x % a.chunks, tid = threadIdx.x;
-    const float* x = a.x + (int64_t)r * a.pitch;
-    const int beg = ch * a.len, end = min(beg + a.len, a.n);
+struct Held {
     F4 f[NV];
+    template <typename F>
+    __device__ __forceinline__ void each(F&& use) const {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) f[i] = load4(x, beg + 4 * (i * NT + tid), end);
-    const Ask q = ask_of(a, r);
-    weight[tid] = 0;
-    count[tid] = 0;
-    float most = -__builtin_inff();
-    int at = beg;
+        for (int i = 0; i < NV; ++i) use(i, f[i]);
+    }
+};
+struct Staged {
+    const F4* x;
+    int quads;
+    template <typename F>
+    __device__ __forceinline__ void each(F&& use) const {
+#pragma unroll 1
+        for (int i = 0; i < quads; ++i) use(i, x[i * NT + threadIdx.x]);
+    }
+};
+__device__ __forceinline__ float top_of(const F4& f) { return fmaxf(fmaxf(f.v[0], f.v[1]), fmaxf(f.v[2], f.v[3])); }
+
+// The largest of a chunk's numbers and its first index; whether one is a NaN.
+struct Most {
+    float wave[NT / 64];
+    int at[NT / 64];
+};
+template <typename H>
+__device__ __forceinline__ bool most_of(const H& held, int beg, Most& L, float& most, int& at) {
+    const int tid = threadIdx.x;
+    float top = -__builtin_inff();
+    int where = beg;
     bool nan = false;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
+    held.each([&](int i, const F4& f) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            nan |= f[i].v[j] != f[i].v[j];
-            if (f[i].v[j] > most) {
-                most = f[i].v[j];
-                at = beg + 4 * (i * NT + tid) + j;
+            nan |= f.v[j] != f.v[j];
+            if (f.v[j] > top) {
+                top = f.v[j];
+                where = beg + 4 * (i * NT + tid) + j;
             }
         }
+    });
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const float o = __shfl_xor(most, d, 64);
-        const int oa = __shfl_xor(at, d, 64);
-        if (o > most || (o == most && oa < at)) {
-            most = o;
-            at = oa;
+        const float o = __shfl_xor(top, d, 64);
+        const int oa = __shfl_xor(where, d, 64);
+        if (o > top || (o == top && oa < where)) {
+            top = o;
+            where = oa;
         }
     }
     if ((tid & 63) == 0) {
-        wmost[tid >> 6] = most;
-        wat[tid >> 6] = at;
+        L.wave[tid >> 6] = top;
+        L.at[tid >> 6] = where;
     }
     nan = __syncthreads_or(nan);
 #pragma unroll
     for (int i = 0; i < NT / 64; ++i)
-        if (wmost[i] > most || (wmost[i] == most && wat[i] < at)) {
-            most = wmost[i];
-            at = wat[i];
+        if (L.wave[i] > top || (L.wave[i] == top && L.at[i] < where)) {
+            top = L.wave[i];
+            where = L.at[i];
         }
+    most = top;
+    at = where;
+    return nan;
+}
+// The chunk's histograms, added to weight and count (as the row needs them).
+template <typename H>
+__device__ __forceinline__ void add_bins(const H& held, const Ask& q, double e, int s, unsigned long long* weight,
+                                         uint32_t* count) {
+    const float least = floor_of(e - (double)(s + 1), e, q.c);  // below: no weight
+    const bool counts = q.counts();
+    if (q.weights()) {
+        held.each([&](int, const F4& f) {
+            if (!__builtin_amdgcn_ballot_w64(top_of(f) >= least)) return;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const double v = (double)f.v[j] * q.c;
+                const uint64_t w = weight_of(v - e + (double)s);
+                if (w) {
+                    const int b = min(bin_of(e, v), NB - 1);
+                    atomicAdd(&weight[b], (unsigned long long)w);
+                    if (counts) atomicAdd(&count[b], 1u);
+                }
+            }
+        });
+    } else {
+        held.each([&](int, const F4& f) {
+            if (!__builtin_amdgcn_ballot_w64(top_of(f) >= least)) return;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int b = bin_of(e, (double)f.v[j] * q.c);
+                if (b < NB) atomicAdd(&count[b], 1u);
+            }
+        });
+    }
+}
+
+template <int NV>
+__global__ __launch_bounds__(NT) void sample_bins_kernel(const Args a) {
+    __shared__ unsigned long long weight[NB];
+    __shared__ uint32_t count[NB];
+    __shared__ Most tops;
+    const int r = blockIdx.x / a.chunks, ch = blockIdx.x % a.chunks, tid = threadIdx.x;
+    const float* x = a.x + (int64_t)r * a.pitch;
+    const int beg = ch * a.len, end = min(beg + a.len, a.n);
+    Held<NV> held;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) held.f[i] = load4(x, beg + 4 * (i * NT + tid), end);
+    const Ask q = ask_of(a, r);
+    weight[tid] = 0;
+    count[tid] = 0;
+    float most;
+    int at;
+    const bool nan = most_of(held, beg, tops, most, at);
     const double e = __builtin_ceil((double)most * q.c);
     if (tid == 0) a.chunk[(int64_t)r * a.chunks + ch] = Chunk{e, most, nan ? -1 : at};
     if ((!q.counts() && !q.weights()) || q.greedy || q.bad) return;
-    if (!nan && most > -__builtin_inff() && most < __builtin_inff()) {
-        const float least = floor_of(e - (double)(a.s + 1), e, q.c);  // below: no weight
-        if (q.weights()) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const float top = fmaxf(fmaxf(f[i].v[0], f[i].v[1]), fmaxf(f[i].v[2], f[i].v[3]));
-                if (!__builtin_amdgcn_ballot_w64(top >= least)) continue;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const double v = (double)f[i].v[j] * q.c;
-                    const uint64_t w = weight_of(v - e + (double)a.s);
-                    if (w) {
-                        const int b = min(bin_of(e, v), NB - 1);
-                        atomicAdd(&weight[b], (unsigned long long)w);
-                        if (q.counts()) atomicAdd(&count[b], 1u);
-                    }
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const float top = fmaxf(fmaxf(f[i].v[0], f[i].v[1]), fmaxf(f[i].v[2], f[i].v[3]));
-                if (!__builtin_amdgcn_ballot_w64(top >= least)) continue;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int b = bin_of(e, (double)f[i].v[j] * q.c);
-                    if (b < NB) atomicAdd(&count[b], 1u);
-                }
-            }
-        }
-    }
+    if (!nan && most > -__builtin_inff() && most < __builtin_inff()) add_bins(held, q, e, a.s, weight, count);
     __syncthreads();
     const int64_t to = ((int64_t)r * a.chunks + ch) * NB;
     if (q.weights()) a.weight[to + tid] = weight[tid];
@@ -320,16 +364,100 @@ __device__ __forceinline__ uint64_t share_of(float p, uint64_t total) {
     return t > 0 ? t : 1;
 }
 
+// Where the cuts fall: weight w and number n of this thread's bin (the first NB
+// threads have one each; the others keep to the barriers).
+struct Cuts {
+    uint64_t tmp[NB / 64], klo, below;
+    uint32_t tmp_n[NB / 64];
+    int kbin, lo, hi, count_below;
+};
+struct Cut {
+    uint64_t below, all;
+    int lo, hi, count_below, k;
+};
+__device__ __forceinline__ void cut_start(Cuts& L) {  // by one thread, a barrier before cut_bins
+    L.kbin = NB;
+    L.lo = NB;
+    L.hi = -1;
+    L.klo = 0;
+    L.below = 0;
+    L.count_below = 0;
+}
+__device__ __forceinline__ Cut cut_bins(const Ask& q, Cuts& L, uint64_t w, uint32_t n) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bin = tid % NB;
+    const bool on = tid < NB, ws = q.weights(), ns = q.counts();
+    const uint64_t x = lane_sums(w);
+    const uint32_t c = (uint32_t)lane_sums(n);
+    if (on && lane == 63) {
+        L.tmp[wave] = x;
+        L.tmp_n[wave] = c;
+    }
+    __syncthreads();
+    uint64_t before = x - w, all = 0;
+    uint32_t cbefore = c - n;
+#pragma unroll
+    for (int i = 0; i < NB / 64; ++i) {
+        all += L.tmp[i];
+        if (i < wave) {
+            before += L.tmp[i];
+            cbefore += L.tmp_n[i];
+        }
+    }
+    // the bin where the k largest end
+    if (on && ns && cbefore < (uint32_t)q.k && cbefore + n >= (uint32_t)q.k) {
+        L.kbin = bin;
+        L.klo = before;
+    }
+    __syncthreads();
+    int k = L.kbin < NB ? q.k : 0;
+    if (on && ws && w) {
+        const uint64_t t = share_of(q.p, k ? L.klo : all);
+        if (before <= t && before + w > t) atomicMin(&L.lo, bin);
+        if (before < t) atomicMax(&L.hi, bin);
+    }
+    __syncthreads();
+    int lo = L.lo, hi = L.hi;
+    if (k) {
+        lo = ws ? min(lo, L.kbin) : q.p < 1.0f ? 0 : L.kbin;
+        hi = L.kbin;
+    } else if (ws && lo > hi) {
+        lo = hi + 1;  // the cut falls between two bins
+    } else if (q.p < 1.0f && !ws) {
+        lo = 0;  // fewer than k are in the bins: all of them are listed
+        hi = NB - 1;
+        k = q.k;
+    }
+    if (on && bin == lo) {  // what lies before the list
+        L.below = before;
+        L.count_below = (int)cbefore;
+    }
+    __syncthreads();
+    return Cut{L.below, ws ? all : 0, lo, hi, L.count_below, k};
+}
+// v = x c of min_p.
+__device__ __forceinline__ double least_of(const Ask& q, float most) {
+    return q.minp > 0.0f ? (double)most * q.c + log2((double)q.minp) : -__builtin_inf();
+}
+// A row that needs no weights, or has none: its token, by one thread.
+__device__ __forceinline__ void told(const Args& a, int r, const Ask& q, bool ok, int at) {
+    a.token[r] = ok ? at : -1;
+    if (a.prob) a.prob[r] = ok ? 1.0f : 0.0f;
+    if (!ok) atomicOr(a.err, q.bad ? ERR_ARG_BIT : ERR_NAN_BIT);
+}
+
+__device__ __forceinline__ Row row_of(const Ask& q, double e, double least, const Cut& c) {
+    return Row{q.c, e, least, c.below, c.all, 0, c.lo, c.hi, c.count_below, c.k, q.p, 0};
+}
+
 // A workgroup a row.  Bound by latency, the loads of the chunks' histograms and
 // the fetching of its own code, which is run once.
 constexpr int RT = 1024;  // threads: two a bin
 __global__ __launch_bounds__(RT) void sample_row_kernel(const Args a) {
-    __shared__ uint64_t half_w[NB], tmp[NB / 64];
-    __shared__ uint32_t half_n[NB], tmp_n[NB / 64];
+    __shared__ uint64_t half_w[NB];
+    __shared__ uint32_t half_n[NB];
+    __shared__ Cuts cuts;
     __shared__ float wmost[RT / 64];
     __shared__ int wat[RT / 64];
-    __shared__ int kbin, lo, hi, count_below;
-    __shared__ uint64_t klo, below;
     __shared__ int shift[MAX_CHUNKS];  // whole factors of two between a chunk's scale and the row's; -1: too many
     const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Ask q = ask_of(a, r);
@@ -353,14 +481,7 @@ __global__ __launch_bounds__(RT) void sample_row_kernel(const Args a) {
         wmost[wave] = top;
         wat[wave] = at;
     }
-    if (tid == 0) {
-        kbin = NB;
-        lo = NB;
-        hi = -1;
-        klo = 0;
-        below = 0;
-        count_below = 0;
-    }
+    if (tid == 0) cut_start(cuts);
     const bool nan = __syncthreads_or(at < 0);
     most = wmost[0];
     at = wat[0];
@@ -372,18 +493,14 @@ __global__ __launch_bounds__(RT) void sample_row_kernel(const Args a) {
     const bool finite = most > -__builtin_inff() && most < __builtin_inff();
     if (q.bad || nan || !finite || q.greedy) {
         if (tid == 0) {
-            const bool ok = !q.bad && !nan && finite;
-            a.token[r] = ok ? at : -1;
-            if (a.prob) a.prob[r] = ok ? 1.0f : 0.0f;
-            if (!ok) atomicOr(a.err, q.bad ? ERR_ARG_BIT : ERR_NAN_BIT);
+            told(a, r, q, !q.bad && !nan && finite, at);
             row->done = 1;
         }
         return;
     }
     const double e = __builtin_ceil((double)most * q.c);
     const bool ws = q.weights(), ns = q.counts();
-    uint64_t all = 0;
-    int k = 0;
+    Cut cut{0, 0, NB, -1, 0, 0};
     if (ws || ns) {
         if (tid < a.chunks) {
             const double de = e - mine;  // whole, or infinite
@@ -418,64 +535,50 @@ __global__ __launch_bounds__(RT) void sample_row_kernel(const Args a) {
             half_n[bin] = n;
         }
         __syncthreads();
-        // the first NB threads go on, a bin each; the others keep to the barriers
-        const bool on = tid < NB;
-        if (on) {
+        if (tid < NB) {
             w += half_w[bin];
             n += half_n[bin];
         }
-        const uint64_t x = lane_sums(w);
-        const uint32_t c = (uint32_t)lane_sums(n);
-        if (on && lane == 63) {
-            tmp[wave] = x;
-            tmp_n[wave] = c;
-        }
-        __syncthreads();
-        uint64_t before = x - w;
-        uint32_t cbefore = c - n;
-#pragma unroll
-        for (int i = 0; i < NB / 64; ++i) {
-            all += tmp[i];
-            if (i < wave) {
-                before += tmp[i];
-                cbefore += tmp_n[i];
-            }
-        }
-        // the bin where the k largest end
-        if (on && ns && cbefore < (uint32_t)q.k && cbefore + n >= (uint32_t)q.k) {
-            kbin = bin;
-            klo = before;
-        }
-        __syncthreads();
-        k = kbin < NB ? q.k : 0;
-        if (on && ws && w) {
-            const uint64_t t = share_of(q.p, k ? klo : all);
-            if (before <= t && before + w > t) atomicMin(&lo, bin);
-            if (before < t) atomicMax(&hi, bin);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            if (k) {
-                lo = ws ? min(lo, kbin) : q.p < 1.0f ? 0 : kbin;
-                hi = kbin;
-            } else if (ws && lo > hi) {
-                lo = hi + 1;  // the cut falls between two bins
-            } else if (q.p < 1.0f && !ws) {
-                lo = 0;  // fewer than k are in the bins: all of them are listed
-                hi = NB - 1;
-                k = q.k;
-            }
-        }
-        __syncthreads();
-        if (on && bin == lo) {  // what lies before the list
-            below = before;
-            count_below = (int)cbefore;
-        }
-        __syncthreads();
+        cut = cut_bins(q, cuts, w, n);
     }
-    if (tid == 0)
-        *row = Row{q.c, e, q.minp > 0.0f ? (double)most * q.c + log2((double)q.minp) : -__builtin_inf(),
-                   below, ws ? all : 0, 0, lo, hi, count_below, k, q.p, 0};
+    if (tid == 0) *row = row_of(q, e, least_of(q, most), cut);
+}
+
+// Adds up what of a chunk is kept whole; returns which of the thread's elements go
+// to the list (bit 4 i + j: element j of quad i).
+template <typename H>
+__device__ __forceinline__ uint32_t split_chunk(const H& held, int beg, int end, double c, double e, double ce,
+                                                double least, int lo, int hi, int s, uint64_t& sum) {
+    const int sh = PER * (int)(e - ce);
+    // what lies past the bins, or has no weight, or (without a list) is below
+    // min_p, by whole waves
+    double past = fmax(e - (double)(hi >= lo ? hi + 1 : lo) / (double)PER, e - (double)(s + 1));
+    if (hi < lo) past = fmax(past, least);
+    const float skip = floor_of(past, e, c);
+    uint32_t in = 0;
+    held.each([&](int i, const F4& f) {
+        if (!__builtin_amdgcn_ballot_w64(top_of(f) >= skip)) return;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const double v = (double)f.v[j] * c;  // (past the end: -inf)
+            const int b = bin_of(ce, v) + sh;
+            if (b < lo && v >= least) sum += weight_of(v - e + (double)s);
+            in |= b >= lo && b <= hi && beg + 4 * (i * NT + (int)threadIdx.x) + j < end ? 1u << (4 * i + j) : 0u;
+        }
+    });
+    return in;
+}
+// The thread's elements of the list, from place `to` on, up to CAP.
+template <typename H>
+__device__ __forceinline__ void put_list(const H& held, int beg, uint32_t in, int to, uint64_t* list) {
+    held.each([&](int i, const F4& f) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (in >> (4 * i + j) & 1) {
+                if (to < CAP) list[to] = key_of(f.v[j], beg + 4 * (i * NT + (int)threadIdx.x) + j);
+                ++to;
+            }
+    });
 }
 
 template <int NV>
@@ -486,35 +589,16 @@ __global__ __launch_bounds__(NT) void sample_take_kernel(const Args a) {
     Row* rp = a.row + r;
     const float* x = a.x + (int64_t)r * a.pitch;
     const int beg = ch * a.len, end = min(beg + a.len, a.n);
-    F4 f[NV];
+    Held<NV> held;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) f[i] = load4(x, beg + 4 * (i * NT + tid), end);
+    for (int i = 0; i < NV; ++i) held.f[i] = load4(x, beg + 4 * (i * NT + tid), end);
     if (rp->done) return;
     const double c = rp->c, e = rp->e, least = rp->least;
     const int lo = rp->lo, hi = rp->hi;
     const double ce = a.chunk[(int64_t)r * a.chunks + ch].e, de = e - ce;
     uint64_t sum = 0;
-    uint32_t in = 0;  // which of the thread's elements go to the list
-    if (de <= 51.0) {
-        const int sh = PER * (int)de;
-        // what lies past the bins, or has no weight, or (without a list) is below
-        // min_p, by whole waves
-        double past = fmax(e - (double)(hi >= lo ? hi + 1 : lo) / (double)PER, e - (double)(a.s + 1));
-        if (hi < lo) past = fmax(past, least);
-        const float skip = floor_of(past, e, c);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const float top = fmaxf(fmaxf(f[i].v[0], f[i].v[1]), fmaxf(f[i].v[2], f[i].v[3]));
-            if (!__builtin_amdgcn_ballot_w64(top >= skip)) continue;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const double v = (double)f[i].v[j] * c;  // (past the end: -inf)
-                const int b = bin_of(ce, v) + sh;
-                if (b < lo && v >= least) sum += weight_of(v - e + (double)a.s);
-                in |= b >= lo && b <= hi && beg + 4 * (i * NT + tid) + j < end ? 1u << (4 * i + j) : 0u;
-            }
-        }
-    }
+    uint32_t in = 0;
+    if (de <= 51.0) in = split_chunk(held, beg, end, c, e, ce, least, lo, hi, a.s, sum);
     sum = group_sum<NT>(sum, tmp);
     if (tid == 0) a.kept[(int64_t)r * a.chunks + ch] = sum;
     if (hi < lo) return;
@@ -523,15 +607,7 @@ __global__ __launch_bounds__(NT) void sample_take_kernel(const Args a) {
     if (tid == 0 && mine) place = atomicAdd(&rp->listed, (int)mine);
     __syncthreads();
     if (!in) return;
-    to += place;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (in >> (4 * i + j) & 1) {
-                if (to < CAP) a.list[(int64_t)r * CAP + to] = key_of(f[i].v[j], beg + 4 * (i * NT + tid) + j);
-                ++to;
-            }
+    put_list(held, beg, in, to + place, a.list + (int64_t)r * CAP);
 }
 
 struct Last {  // the row's last launch
@@ -705,28 +781,14 @@ __device__ __forceinline__ bool cut_list(const Args& a, const Row& row, int n, L
     return true;
 }
 
-// A workgroup a row.  Bound by latency: what it runs is one chain of a dozen loads
-// and barriers, so it keeps its code short and its sums in few steps.
-__global__ __launch_bounds__(FT) void sample_token_kernel(const Args a) {
-    extern __shared__ __align__(16) char lds[];
-    Last& L = *reinterpret_cast<Last*>(lds);
-    const int r = blockIdx.x, tid = threadIdx.x;
-    const Row row = a.row[r];
-    const uint64_t* list = a.list + (int64_t)r * CAP;
-    const uint64_t ahead = list[tid];  // (memory of the list, whatever its length)
-    uint64_t two[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) two[j] = tid + j * FT < a.chunks ? a.kept[(int64_t)r * a.chunks + tid + j * FT] : 0;
-    if (row.done) return;
-    const float* x = a.x + (int64_t)r * a.pitch;
-    const int n = row.listed;
+// The cuts in the row's list of n (in few where it is short, else in list where
+// that holds it), its token and share; kept, e: of the chunks, what of them is kept
+// whole and their scales.  Bound by latency: one chain of a dozen barriers, whose
+// code is run once, and so is kept short.
+__device__ __forceinline__ void finish_row(const Args& a, const float* x, const Row& row, int r, int n, Last& L) {
+    const int tid = threadIdx.x;
     const double s = (double)a.s;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-        if (tid + j * FT < a.chunks) {
-            L.kept[tid + j * FT] = two[j];
-            L.e[tid + j * FT] = a.chunk[(int64_t)r * a.chunks + tid + j * FT].e;
-        }
+    uint64_t two[2];
     uint64_t cut = 0;  // the last key of the list that is kept
     auto weight = [&](uint64_t key) { return weight_of(v_of(row, key) - row.e + s); };
     auto keep = [&](uint64_t key) {
@@ -734,7 +796,6 @@ __global__ __launch_bounds__(FT) void sample_token_kernel(const Args a) {
             atomicAdd((unsigned long long*)&L.kept[(int)~(uint32_t)key / a.len], (unsigned long long)weight(key));
     };
     if (n > 0 && n <= FEW) {
-        L.few[tid] = ahead;
         put_in_order(L, n);
         const uint64_t key = L.order[tid < n ? tid : 0], w = tid < n ? weight(key) : 0;
         const bool first = tid < (row.k ? min(n, row.k - row.count_below) : n);
@@ -747,11 +808,6 @@ __global__ __launch_bounds__(FT) void sample_token_kernel(const Args a) {
         if (in) keep(key);
     } else if (n > FEW) {
         const bool here = n <= CAP;
-        if (here) {
-            L.list[tid] = ahead;
-#pragma unroll 4
-            for (int i = tid + FT; i < n; i += FT) L.list[i] = list[i];
-        }
         __syncthreads();
         // by the number, then by the share
         uint64_t total = row.all;
@@ -840,11 +896,93 @@ __global__ __launch_bounds__(FT) void sample_token_kernel(const Args a) {
     }
 }
 
+__global__ __launch_bounds__(FT) void sample_token_kernel(const Args a) {
+    extern __shared__ __align__(16) char lds[];
+    Last& L = *reinterpret_cast<Last*>(lds);
+    const int r = blockIdx.x, tid = threadIdx.x;
+    const Row row = a.row[r];
+    const uint64_t* list = a.list + (int64_t)r * CAP;
+    const uint64_t ahead = list[tid];  // (memory of the list, whatever its length)
+    uint64_t two[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) two[j] = tid + j * FT < a.chunks ? a.kept[(int64_t)r * a.chunks + tid + j * FT] : 0;
+    if (row.done) return;
+    const int n = row.listed;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        if (tid + j * FT < a.chunks) {
+            L.kept[tid + j * FT] = two[j];
+            L.e[tid + j * FT] = a.chunk[(int64_t)r * a.chunks + tid + j * FT].e;
+        }
+    if (n <= FEW) {
+        L.few[tid] = ahead;
+    } else if (n <= CAP) {
+        L.list[tid] = ahead;
+#pragma unroll 4
+        for (int i = tid + FT; i < n; i += FT) L.list[i] = list[i];
+    }
+    finish_row(a, a.x + (int64_t)r * a.pitch, row, r, n, L);
+}
+
+// Rows of up to ONE logits: all of it in one launch, a workgroup a row, the logits
+// in LDS and nothing else read.  Latency bounds it.  Against the four launches, in us:
+// a row of 1000 14 -> 6, 7 rows of 5000 22 -> 19, 256 rows of 2000 24 -> 15; 64 rows
+// of 16384 in one chunk 26 -> 29, so ONE lies below that.
+constexpr int ONE = 8192;
+__global__ __launch_bounds__(NT) void sample_one_kernel(const Args a) {
+    extern __shared__ __align__(16) char lds[];
+    __shared__ Most tops;
+    __shared__ Cuts cuts;
+    Last& L = *reinterpret_cast<Last*>(lds);
+    static_assert(NT == FT && ONE / (4 * NT) * 4 <= 32 && offsetof(Last, list) % 16 == 0, "");
+    const int r = blockIdx.x, tid = threadIdx.x;
+    const float* x = a.x + (int64_t)r * a.pitch;
+    F4* quad = reinterpret_cast<F4*>(L.list + (a.n > FEW ? (a.n + 1) / 2 * 2 : 0));
+    const Staged held{quad, a.len / (4 * NT)};
+#pragma unroll 4
+    for (int i = 0; i < held.quads; ++i) quad[i * NT + tid] = load4(x, 4 * (i * NT + tid), a.n);  // (each thread its own)
+    const Ask q = ask_of(a, r);
+    L.weight[tid] = 0;
+    L.count[tid] = 0;
+    if (tid == 0) cut_start(cuts);
+    float most;
+    int at;
+    const bool nan = most_of(held, 0, tops, most, at), finite = most > -__builtin_inff() && most < __builtin_inff();
+    if (q.bad || nan || !finite || q.greedy) {
+        if (tid == 0) told(a, r, q, !q.bad && !nan && finite, at);
+        return;
+    }
+    const double e = __builtin_ceil((double)most * q.c), least = least_of(q, most);
+    Cut cut{0, 0, NB, -1, 0, 0};
+    if (q.weights() || q.counts()) {
+        add_bins(held, q, e, a.s, L.weight, L.count);
+        __syncthreads();
+        cut = cut_bins(q, cuts, L.weight[tid], L.count[tid]);
+    }
+    uint64_t sum = 0, n = 0;
+    const uint32_t in = split_chunk(held, 0, a.n, q.c, e, e, least, cut.lo, cut.hi, a.s, sum);
+    sum = group_sum<NT>(sum, L.tmp);
+    if (cut.hi >= cut.lo) {
+        const int to = (int)group_before<NT>((uint64_t)__builtin_popcount(in), L.tmp, &n);
+        if (in) put_list(held, 0, in, to, n <= FEW ? L.few : L.list);
+    }
+    if (tid == 0) {
+        L.kept[0] = sum;
+        L.e[0] = e;
+    }
+    finish_row(a, reinterpret_cast<const float*>(quad), row_of(q, e, least, cut), r, (int)n, L);
+}
+
 // How a call's rows are cut, and its workspace.
 struct Plan {
     int quads, chunks, len, s;  // quads a thread; logits a chunk
     size_t row, chunk, weight, count, kept, list, bytes;
 };
+int s_of(size_t n) {
+    int bits = 0;
+    while (((size_t)1 << bits) < n) ++bits;
+    return std::min(MAX_S, 62 - bits);
+}
 Plan plan_of(size_t m, size_t n) {
     Plan p{};
     p.quads = MAX_V;
@@ -853,13 +991,17 @@ Plan plan_of(size_t m, size_t n) {
         p.chunks = (int)((n + p.len - 1) / p.len);
     };
     cut();
+    p.s = s_of(n);
+    if (n <= (size_t)ONE) {
+        p.quads = (int)((n + 4 * NT - 1) / (4 * NT));
+        cut();
+        p.bytes = 256;  // nothing is kept between launches
+        return p;
+    }
     while (p.quads > 1 && m * p.chunks < 1024 && p.chunks < 20) {
         p.quads /= 2;
         cut();
     }
-    int bits = 0;
-    while (((size_t)1 << bits) < n) ++bits;
-    p.s = std::min(MAX_S, 62 - bits);
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t q = at;
@@ -891,6 +1033,31 @@ struct Guard {
 };
 
 constexpr size_t MAX_M = 1 << 20;
+
+template <typename K>
+hipError_t with_lds(K kernel, int lds) {
+    if (lds <= 48 * 1024) return hipSuccess;
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+}
+hipError_t launch_one(const Args& a, size_t m, hipStream_t s) {
+    static_assert(sizeof(Last) + ONE * 8 + ONE * 4 + 1024 <= 160 * 1024, "LDS of a CU");
+    const int lds = (int)sizeof(Last) + (a.n > FEW ? (a.n + 1) / 2 * 16 : 0) + a.len * 4;
+    if (const hipError_t e = with_lds(sample_one_kernel, lds); e != hipSuccess) return e;
+    sample_one_kernel<<<dim3((unsigned)m), dim3(NT), lds, s>>>(a);
+    return hipGetLastError();
+}
+template <int NV>
+hipError_t launch(const Args& a, size_t m, hipStream_t s) {
+    static_assert(sizeof(Last) + CAP * 8 + 1024 <= 160 * 1024, "LDS of a CU");
+    const dim3 rows((unsigned)m), all((unsigned)(m * a.chunks));
+    const int lds = (int)sizeof(Last) + CAP * 8;
+    if (const hipError_t e = with_lds(sample_token_kernel, lds); e != hipSuccess) return e;
+    sample_bins_kernel<NV><<<all, dim3(NT), 0, s>>>(a);
+    sample_row_kernel<<<rows, dim3(RT), 0, s>>>(a);
+    sample_take_kernel<NV><<<all, dim3(NT), 0, s>>>(a);
+    sample_token_kernel<<<rows, dim3(FT), lds, s>>>(a);
+    return hipGetLastError();
+}
 
 }  // namespace
 }  // namespace smp
@@ -929,29 +1096,16 @@ int frq_sample_dev(frq_ctx* ctx, const float* d_logits, size_t pitch, size_t m, 
         if (st != hipStreamCaptureStatusNone) return bad("under graph capture the caller gives the workspace");
         if (int rc = ctx_ws(ctx, p.bytes, &d_ws)) return rc;
     }
-    constexpr int LAST = sizeof(Last) + CAP * 8;
-    static_assert(LAST <= 160 * 1024, "LDS of a CU");
-    if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(sample_token_kernel),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, LAST);
-        e != hipSuccess)
-        return set_error(FRQ_ERR_HIP, std::string("hipFuncSetAttribute: ") + hipGetErrorString(e));
     char* ws = (char*)d_ws;
     const Args a{d_logits, (int64_t)pitch, (int)n, p.s, p.chunks, p.len, d_temp, d_topp, d_minp, d_u, d_topk, d_token, d_prob,
                  (Row*)(ws + p.row), (Chunk*)(ws + p.chunk), (uint64_t*)(ws + p.weight), (uint32_t*)(ws + p.count),
                  (uint64_t*)(ws + p.kept), (uint64_t*)(ws + p.list), ctx_err(ctx)};
-    const dim3 all((unsigned)(m * p.chunks)), rows((unsigned)m);
-    auto go = [&](auto quads) {
-        constexpr int NV = decltype(quads)::value;
-        sample_bins_kernel<NV><<<all, dim3(NT), 0, s>>>(a);
-        sample_row_kernel<<<rows, dim3(RT), 0, s>>>(a);
-        sample_take_kernel<NV><<<all, dim3(NT), 0, s>>>(a);
-        sample_token_kernel<<<rows, dim3(FT), LAST, s>>>(a);
-    };
-    if (p.quads == 1) go(std::integral_constant<int, 1>{});
-    else if (p.quads == 2) go(std::integral_constant<int, 2>{});
-    else if (p.quads == 4) go(std::integral_constant<int, 4>{});
-    else go(std::integral_constant<int, 8>{});
-    const hipError_t e = hipGetLastError();
+    hipError_t e = hipSuccess;
+    if (n <= (size_t)ONE) e = launch_one(a, m, s);
+    else if (p.quads == 1) e = launch<1>(a, m, s);
+    else if (p.quads == 2) e = launch<2>(a, m, s);
+    else if (p.quads == 4) e = launch<4>(a, m, s);
+    else e = launch<8>(a, m, s);
     return e == hipSuccess ? FRQ_OK : set_error(FRQ_ERR_HIP, std::string("launch sample: ") + hipGetErrorString(e));
 }
 
