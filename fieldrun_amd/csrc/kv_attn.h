@@ -912,7 +912,7 @@ __device__ __forceinline__ int pick4(int j, int a, int b, int c, int d) {
 // Bound by the matrix cores, and by the clock under them (1.7 GHz, the cores
 // busy half the time): f16, 28 heads of 128 channels over 4, 2048 rows after
 // 6144 cached tokens, is 210 GFLOP of the formula, which the two halves of q
-// and p make 420, in 464 us; int8, 7 sequences of up to 1501 tokens, 24 GFLOP,
+// and p make 420, in 430 us; int8, 7 sequences of up to 1501 tokens, 24 GFLOP,
 // in 101.  One f16 for p would cost its bits below 2^-11.  128 pairs a workgroup
 // let two fit a CU (64 KB of LDS, 256 registers); equal priorities of both 503 us
 // against 481.
@@ -1202,8 +1202,19 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
         least = 0x7FFFFFFF;
     }
     // two workgroups share a CU, the second 256 behind the first: one ahead of
-    // the other keeps the one's products over the other's softmax
-    if ((blockIdx.x >> 8) & 1) __builtin_amdgcn_s_setprio(2);
+    // the other keeps the one's products over the other's softmax, and products
+    // ahead of every softmax (PHASES) keep the matrix cores fed, an instruction of
+    // them taking the place of eight others.  (The f16 case 457 us without phases,
+    // 430 with; 16 int8 trees of up to 182 pairs over 6001 tokens 77, 74; but 7 int8
+    // prompts, more workgroups than two a CU, 116, 125.)
+    constexpr bool PHASES = F16 || (I8 && EX);
+    const bool second = (blockIdx.x >> 8) & 1;
+    auto prio = [&](bool products) {
+        if (products) __builtin_amdgcn_s_setprio(3);
+        else if (second) __builtin_amdgcn_s_setprio(2);
+        else __builtin_amdgcn_s_setprio(0);
+    };
+    if (!PHASES && second) __builtin_amdgcn_s_setprio(2);
     __syncthreads();
     if (tiles) {
         ids(real(beg));
@@ -1247,6 +1258,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
                 constexpr int G = F32 ? 2 : 4;  // operands a group
                 Op xa[G][NA], xb[G][NA];
                 f16v s;  // s[8 t + j] is key kb0 + 16 t + 8 h + j
+                if constexpr (PHASES) prio(true);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
@@ -1278,6 +1290,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
 #pragma unroll
                 for (int i = 0; i < G; ++i)
                     if (i < 2 * NH) val_op(i, xa[i]);
+                if constexpr (PHASES) prio(false);
                 const bool edge = (kb0 < lo_b && !(EX && kb0 + 32 <= sinks)) || kb0 + 31 > pos_a;
                 if constexpr (I8) {
 #pragma unroll
@@ -1356,6 +1369,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
                     for (int j = 0; j < 8; ++j) x[j] = s[8 * t + j];
                     split8(x, pv[t]);
                 }
+                if constexpr (PHASES) prio(true);
 #pragma unroll
                 for (int g = 0; g < 2 * NH; g += 2 * G) {
 #pragma unroll
