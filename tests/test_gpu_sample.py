@@ -130,6 +130,17 @@ def test_tokens(ctx, kind, m, n):
         Call(ctx, x, u=rng.random(m), pad=i % 3, **how).check()
 
 
+@pytest.mark.parametrize("n", [511, 512, 513, 2047, 2048, 4096, 8191, 8192, 8193, 16385])
+def test_widths_about_the_kernels_own(ctx, n):
+    """Rows that fit a launch and rows one longer, with and without room for all
+    of them in order, as few and many, also those that miss every alignment."""
+    for i, kind in enumerate(KINDS):
+        rng = np.random.default_rng(n + i)
+        m = [2, 5, 33][i % 3]
+        for mode in MODES[i % 2::2]:
+            Call(ctx, rows(rng, m, n, kind), u=rng.random(m), pad=1 + 2 * (i % 2), **mode).check()
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_rows_of_their_own_parameters(ctx, kind):
     """Rows of every mode in one call, and each alone: the same bits, however
