@@ -283,13 +283,24 @@ constexpr int DEC_PAIRS = 128;
 // 9.7, 19.6, of 336 over 2000 27, 27.  (The tokens are those that the table has room
 // for; lengths are device data.)
 constexpr int TREE_PAIRS = 32;
-constexpr double TREE_WORK = 6e6;  // rows x heads x tokens
+constexpr double EX_WORK = 6e6;  // rows x heads x keys
+// With sinks or trees the prompt kernel serves every sequence where they have more
+// than EX_PAIRS pairs in the mean (without trees, in a small call or over f32 keys, more
+// than the decode kernel's; calls with neither keep each row's kernel, and so its
+// bits), and their tiles fit the chip at once or are mostly large sequences': the
+// launch of the other takes longer than what it saves.  Both launches against one:
+// 2048 f16 rows of 28 heads in windows of 1024 89, 86 us, 500 rows beside 31 of one
+// row 71, 56, 20 sequences of 84 pairs 54, 37, int8 in windows of 4000 117, 77; trees:
+// 4 of 128 pairs 45, 41, 16 int8 of up to 182 72, 67.  But f32, 72 pairs 76, 99; 2000 rows
+// beside 31 of one 109, 127; trees of 24 pairs, f16 of 64 channels 39, 55.
+constexpr size_t EX_PAIRS = 64;
 // With sinks or trees the items fill the chip's workgroups once, less the chunks
 // that every tile is rounded up by (half a target at least): one tree of 256 pairs
 // over 32768 f16 tokens 106 us at 400 items, 97 at 496; 16 int8 ones of up to 182
 // pairs 75 us at 400, 88 at 512; 4 f32 ones, one workgroup a CU, 121 at 400, 82 at 220.
+int64_t ex_slots(const frq_kv* kv) { return kv->dtype == FRQ_DT_F32 || kv->hd > 128 ? 256 : 512; }
 int64_t ex_target(const frq_kv* kv, const Call& prompt) {
-    const int64_t slots = kv->dtype == FRQ_DT_F32 || kv->hd > 128 ? 256 : 512;
+    const int64_t slots = ex_slots(kv);
     return std::max(slots / 2, slots - max_tiles(prompt) * prompt.n_kv);
 }
 
@@ -300,9 +311,8 @@ struct Plan {
     Call dec, prompt;
     size_t rec_dec, rec_prompt, part_dec, part_prompt, plan_dec, plan_prompt, bytes;  // offsets, the whole
 };
-// tokens: those that a table has room for, for calls with trees (0: none); ex: with
-// trees or sinks.
-Plan plan_of(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq, bool ex, size_t tokens) {
+// ex: with trees or sinks; keys: those that a row sees at most, by the table's room.
+Plan plan_of(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq, bool ex, bool trees, size_t keys) {
     Plan p{};
     Call& c = p.dec;
     c.n_seq = (int)n_seq;
@@ -320,11 +330,17 @@ Plan plan_of(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq, bool e
     c.tp = 16;
     c.target = DEC_TARGET;
     p.prompt = c;
-    p.prompt.min_pairs = 1 + (tokens ? (double)n_row * (double)n_head * (double)tokens > TREE_WORK ? TREE_PAIRS : 0x7FFFFFFE
-                                     : DEC_PAIRS);
+    const bool big = (double)n_row * (double)n_head * (double)keys > EX_WORK;
+    p.prompt.min_pairs = 1 + (!trees ? DEC_PAIRS : big ? TREE_PAIRS : 0x7FFFFFFE);
     p.prompt.tp = 128;
     // (n_row <= n_seq: no room for parts, every tile's keys in one run)
     p.prompt.target = n_row <= n_seq ? 1 : ex ? ex_target(kv, p.prompt) : kv->hd > 128 ? PROMPT_TARGET_WIDE : PROMPT_TARGET;
+    // (f32 keys of over 128 channels have no prompt kernel)
+    const bool f32 = kv->dtype == FRQ_DT_F32;
+    const size_t pairs = n_row * c.rep, mean = big && (trees || !f32) ? EX_PAIRS : DEC_PAIRS;
+    if (ex && n_row > n_seq && !(f32 && kv->hd > 128) && (big || !trees) && pairs > mean * n_seq &&
+        (pairs >= 4 * DEC_PAIRS * n_seq || max_tiles(p.prompt) * c.n_kv <= ex_slots(kv)))
+        p.prompt.min_pairs = 1;
     p.prompt.min_chunk = 128;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -379,7 +395,8 @@ int attend(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, siz
     if (!ctx) return bad("null context");
     if (!n_row || !n_seq) return FRQ_OK;
     const bool ex = sinks || more.trees;
-    const Plan plan = plan_of(kv, n_row, n_head, n_seq, ex, more.trees ? std::max<size_t>(1, pages_pitch << shift) : 0);
+    const size_t keys = std::min(pages_pitch << shift, window ? window + sinks : SIZE_MAX);
+    const Plan plan = plan_of(kv, n_row, n_head, n_seq, ex, more.trees, keys);
     const size_t need = plan.bytes;
     if (d_ws && ws_bytes < need) return bad("the workspace is below frq_kv_attn_ws");
     Guard g(ctx_device(ctx));
@@ -440,7 +457,7 @@ int attend(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, siz
     b.rec = (Record*)(ws + plan.rec_prompt);
     b.part = (float*)(ws + plan.part_prompt);
     b.slots = n_row > n_seq ? max_slots(b.c.target, a.c.n_kv) : 0;
-    const int64_t ga = max_items(a.c) * a.c.n_kv, gb = prompts ? max_items(b.c) * b.c.n_kv : 0;
+    const int64_t ga = a.c.max_pairs ? max_items(a.c) * a.c.n_kv : 0, gb = prompts ? max_items(b.c) * b.c.n_kv : 0;
     if (ga + gb > 0x7FFFFFFF) return bad("too many rows or sequences");
     const Launch la{(unsigned)ga, s}, lb{(unsigned)gb, s};
     hipError_t e = hipSuccess;
@@ -453,7 +470,8 @@ int attend(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, siz
         b.c.plan = pb;
     }
     const bool f32 = kv->dtype == FRQ_DT_F32, f16 = kv->dtype == FRQ_DT_F16;
-    if (ex) e = f32 ? launch_decode_ex_f32(a, la) : f16 ? launch_decode_ex_f16(a, la) : launch_decode_ex_i8(a, la);
+    if (!ga) e = hipSuccess;
+    else if (ex) e = f32 ? launch_decode_ex_f32(a, la) : f16 ? launch_decode_ex_f16(a, la) : launch_decode_ex_i8(a, la);
     else e = f32 ? launch_decode_f32(a, la) : f16 ? launch_decode_f16(a, la) : launch_decode_i8(a, la);
     if (e != hipSuccess) return hip_bad(e, "launch kv_decode");
     if (prompts) {
@@ -509,7 +527,8 @@ size_t frq_kv_attn_ws(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_se
     if (!kv || !kv->n_kv || kv->n_kv > 65535 || kv->hd > MAX_HD || !n_head || n_head % kv->n_kv ||
         n_head / kv->n_kv > 65535 || n_row > 0x7FFFFFFF || n_seq > 0x7FFFFFFF)
         return 0;
-    return std::max(plan_of(kv, n_row, n_head, n_seq, false, 0).bytes, plan_of(kv, n_row, n_head, n_seq, true, 0).bytes);
+    return std::max(plan_of(kv, n_row, n_head, n_seq, false, false, 0).bytes,
+                    plan_of(kv, n_row, n_head, n_seq, true, false, 0).bytes);
 }
 
 int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, size_t n_row, size_t n_head,

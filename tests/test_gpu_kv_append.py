@@ -7,6 +7,8 @@ what 64 bits leave: 2^-48 of the head's terms, some 30 operations of 2^-53 each
 (the angle's own rounding is the same on both sides).  Keys and values then
 take frq_kv_write_dev's rounding: the bytes have to be those that call writes for
 the f32 rows that an f32 cache holds."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -238,3 +240,30 @@ def test_slots_beyond_32_bits(ctx):
     want, size = r.want()
     check_rows(ok.numpy(), want[:, 2:3], size[:, 2:3])
     check_rows(ov.numpy(), want[:, 3:], 0 * size[:, 3:])
+
+
+def test_another_stream_and_two_contexts_at_once(ctx):
+    r = Rows(ctx, 2, 3, 64, 70, 64, qn=True, seed=11)
+    p, slots = Pool(ctx, "rowi8", 6, 16, 2, 64), np.arange(70)
+    q, pages = r.call(p, slots), raw(p)
+    other = fa.Context(0)
+    s = Rows(other, 2, 3, 64, 70, 64, qn=True, seed=11)
+    o = Pool(other, "rowi8", 6, 16, 2, 64)
+    stream = C.c_void_p()
+    hip._chk(hip._hip.hipStreamCreate(C.byref(stream)), "hipStreamCreate")
+    try:
+        other.set_stream(stream.value)
+        assert same(s.call(o, slots), q)
+        for _ in range(10):
+            for x, c in ((r, p), (s, o)):
+                c.c.append_dev(x.dx.ptr, x.heads, x.dpos.ptr, x.ds.ptr, 70, x.dq.ptr, x.how)
+        ctx.sync()
+        other.sync()
+        for x, c in ((r, p), (s, o)):
+            assert same(x.dq.numpy()[:70].reshape(q.shape), q)
+            assert all(np.array_equal(a, b) for a, b in zip(raw(c), pages))
+    finally:
+        other.sync()
+        other.set_stream(None)
+        hip._chk(hip._hip.hipStreamDestroy(stream), "hipStreamDestroy")
+        other.close()

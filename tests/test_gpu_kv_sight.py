@@ -406,6 +406,43 @@ def test_pages_of_trees_out_of_range_take_no_part(ctx, kind, rows):
     hold(runs[0], *b.want(20.0, gone))
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("many", [False, True])
+def test_small_sequences_beside_large_ones(ctx, kind, many):
+    """Calls of many pairs a sequence, where one kernel serves them all: rows of
+    sequences of a token or none, of one row or none, beside large ones; then a
+    length that no table holds."""
+    lens, rows = [900, 1, 40, 0, 333, 17], [200, 1, 1, 2, 90, 17]
+    if many:
+        lens, rows = lens + [25, 0, 3, 60] * 20, rows + [25, 1, 0, 57] * 20
+    b = More(ctx, kind, 16, 2, 7, 64, lens, rows, seed=5, window=64, sinks=5)
+    b.check(cap=20.0)
+    want, tol = b.want()
+    put(b.dev[1], np.array([900, 1, 2 ** 30, 0, 333, 17] + lens[6:], np.int32))
+    with pytest.raises(fa.FrqError) as e:
+        b.run()
+    assert e.value.code == fa.FRQ_ERR_ARG
+    ctx.sync()
+    got, other = b.do.numpy()[:b.n_row], np.arange(b.n_row) != b.first[2]
+    assert (got[~other] == 0.0).all()
+    hold(got[other], want[other], tol[other])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (300, 4)])
+def test_small_trees_beside_large_ones(ctx, kind, window, sinks):
+    rng = np.random.default_rng(9)
+    lens, rows = [9000, 1, 40, 0, 700, 17], [130, 1, 1, 0, 30, 17]
+    trees = [grow(rng, r) for r in rows]
+    More(ctx, kind, 64, 4, 7, 32, lens, rows, seed=6, trees=trees, window=window, sinks=sinks).check()
+
+
+@pytest.mark.parametrize("rep", [70, 130])
+def test_many_heads_and_a_row_a_sequence(ctx, rep):
+    More(ctx, "f16", 16, 1, rep, 32, [700, 33], [1, 1], seed=rep, window=90, sinks=4).check()
+    More(ctx, "f16", 16, 1, rep, 32, [700, 33], [1, 1], seed=rep, trees=[[{0}], [{0}]]).check()
+
+
 def test_captured_and_replayed(ctx):
     """A speculative step's attention in a graph, over changing trees, lengths
     and queries, with eager calls and synchronizations between."""
