@@ -8,10 +8,13 @@
 //   sum_{j <= i} w_j > u sum(w)
 //
 // Weights are whole numbers, round(2^s w'), s up to 50 and s + log2(n) at most 62,
-// so that every sum is exact and the same in any order: a row is cut over
-// workgroups, and sums meet in atomics, without the token depending on it.
-// (w' is w times a factor for all of a row that puts the largest between 1/2 and
-// 1; at 152064 tokens a step is 2^-44, and what is below half of it is none.)
+// so that every sum is exact and the same in any order: sums meet in atomics
+// without the token depending on timing.  (w' is w times a factor for all of a row
+// that puts the largest between 1/2 and 1; at 152064 tokens a step is 2^-44, and
+// what is below half of it is none.)  A row is cut into chunks over workgroups, by
+// n and the number of rows.  Top-p's bound alone knows how: a chunk's bins are
+// whole numbers of its own largest weight, so that their sums are off the row's by
+// up to a step a logit.
 //
 // The row is never sorted.  Four launches: each chunk's maximum and its
 // histogram over the logarithm of w, ten bins a factor of two, from one reading

@@ -369,12 +369,14 @@ int frq_rowdot_f32_subset_dev(frq_ctx* ctx, const frq_w* w, const float* d_x,
  *   d_token[i]: the first, in the tokens' order, up to which these sum to more
  *   than d_u[i] (0 <= d_u < 1; a number outside counts as the nearest inside) of
  *   their sum; d_prob[i] (nullable): its share of the sum.
- * Weights are summed as whole numbers, in steps of 2^(log2(n) - 62), 2^-50 or
- * more, of a largest one between 1/2 and 1 (none below half a step): the token
- * does not depend on how the row was split.  A logit of -inf is never
- * chosen.  A row with a NaN, or without a finite maximum, gets token -1 and share
- * 0, and the next frq_sync returns FRQ_ERR_NAN; so does one whose temperature
- * (negative, infinite) or another parameter (NaN) is none, as FRQ_ERR_ARG.
+ * Weights are summed as whole numbers, in steps of 2^(log2(n) - 62) (log2 rounded
+ * up), 2^-50 or more, of a largest one between 1/2 and 1, none below half a step:
+ * the token does not depend on timing.  How a row is split between workgroups goes
+ * by m and n; top-p's sums alone may differ by up to a step a logit between splits.
+ * A logit of -inf is never chosen.  A row with a NaN, or without a finite maximum,
+ * gets token -1 and share 0, and the next frq_sync returns FRQ_ERR_NAN; so does one
+ * whose temperature (negative, infinite) or another parameter (NaN) is none, as
+ * FRQ_ERR_ARG.
  * n up to 2^24.  d_ws: frq_sample_ws bytes of device memory, 16-byte aligned, as
  * in frq_kv_attn_dev; NULL: the context's, which a call under capture may not. */
 size_t frq_sample_ws(size_t m, size_t n);
