@@ -20,8 +20,12 @@ The classes mirror the reference's interface for this path
                           and rowdot_f32_subset (995-1015)
 
   KvCache                 a paged key / value cache in the caller's device
-                          memory: rows written (quantised) and read back,
-                          attention over it (decode and prompt rows)
+                          memory: rows written (quantised) and read back, or
+                          appended from fused q | k | v rows as Rotary says;
+                          attention over it (decode and prompt rows, windows
+                          with sinks, trees of drafted tokens)
+  Context.sample_dev      a token a row of logits: temperature, top-k, top-p,
+                          min-p
 
 Errors the reference raises by panicking come back as FrqError carrying the
 library's status code and message.

@@ -278,7 +278,7 @@ constexpr int DEC_PAIRS = 128;
 // tiles of 128 pairs save their reading anew, from little more than a tile of the
 // decode kernel on: 16 f16 sequences of up to 4000 tokens with 112 pairs 126 us
 // on the decode kernel, 60 on the prompt kernel, 4 of 128 pairs 68, 46, one of 256
-// pairs over 32768 tokens 238, 97.  Where the whole call is small its latency
+// pairs over 32768 tokens 238, 95.  Where the whole call is small its latency
 // counts: one sequence of 112 pairs over 8000 tokens 27, 32 us, of 56 over 211
 // 9.7, 19.6, of 336 over 2000 27, 27.  (The tokens are those that the table has room
 // for; lengths are device data.)
@@ -296,8 +296,9 @@ constexpr double EX_WORK = 6e6;  // rows x heads x keys
 constexpr size_t EX_PAIRS = 64;
 // With sinks or trees the items fill the chip's workgroups once, less the chunks
 // that every tile is rounded up by (half a target at least): one tree of 256 pairs
-// over 32768 f16 tokens 106 us at 400 items, 97 at 496; 16 int8 ones of up to 182
-// pairs 75 us at 400, 88 at 512; 4 f32 ones, one workgroup a CU, 121 at 400, 82 at 220.
+// over 32768 f16 tokens 104 us at 400 items, 95 at the rule's 496; 16 int8 ones of up to
+// 182 pairs 84 at 512, 70 at the rule's 388; 2048 rows in windows of 1024 111, 88 at the
+// rule's 256; 4 f32 trees of 182 pairs, one workgroup a CU, 119 at 400, 90 at the rule's.
 int64_t ex_slots(const frq_kv* kv) { return kv->dtype == FRQ_DT_F32 || kv->hd > 128 ? 256 : 512; }
 int64_t ex_target(const frq_kv* kv, const Call& prompt) {
     const int64_t slots = ex_slots(kv);
