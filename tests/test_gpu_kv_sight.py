@@ -437,6 +437,28 @@ def test_small_trees_beside_large_ones(ctx, kind, window, sinks):
     More(ctx, kind, 64, 4, 7, 32, lens, rows, seed=6, trees=trees, window=window, sinks=sinks).check()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("page", [16, 128, 1024])
+def test_pages_and_pitches(ctx, kind, page):
+    """Strided pages of every size, rows of q and out that lie apart."""
+    rng = np.random.default_rng(10)
+    for lens, rows in (([1500, 90, 3], [1, 1, 1]), ([1500, 90, 40], [70, 5, 40])):
+        for trees in (None, [grow(rng, r) for r in rows]):
+            b = More(ctx, kind, page, 2, 3, 64, lens, rows, seed=page, pad=1, window=200, sinks=17, trees=trees)
+            want = b.check()
+            n, heads, wide = b.n_row, 6, 6 * 64
+            q = np.full((n, wide + 5), np.nan, np.float32)
+            q[:, :wide] = b.q.reshape(n, wide)
+            dq, do = hip.DeviceArray.from_numpy(q), hip.DeviceArray.from_numpy(np.full((n, wide + 3), 7.0, np.float32))
+            t, ln, f = b.dev
+            b.p.c.attn_dev(dq.ptr, n, heads, t.ptr, b.width, ln.ptr, len(lens), do.ptr, f.ptr, window=200, sinks=17,
+                           q_pitch=wide + 5, out_pitch=wide + 3, ws_ptr=b.ws.ptr, ws_bytes=b.ws.nbytes,
+                           tree_ptr=b.dtree and b.dtree.ptr, tree_pitch=b.pitch if b.dtree else 1)
+            ctx.sync()
+            out = do.numpy()
+            assert same(out[:, :wide].copy().reshape(want.shape), want) and (out[:, wide:] == 7.0).all()
+
+
 @pytest.mark.parametrize("rep", [70, 130])
 def test_many_heads_and_a_row_a_sequence(ctx, rep):
     More(ctx, "f16", 16, 1, rep, 32, [700, 33], [1, 1], seed=rep, window=90, sinks=4).check()

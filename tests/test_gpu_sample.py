@@ -342,3 +342,88 @@ def test_the_widest_rows(ctx):
     x = (2 * rng.standard_normal((1, n))).astype(np.float32)
     for mode in (dict(p=0.9), dict(k=100), dict(mp=0.01), dict(temp=0.0)):
         Call(ctx, x, u=0.6, **mode).check()
+
+
+@pytest.mark.parametrize("n", [3001, 20011, 40009])
+@pytest.mark.parametrize("temp", [1e-45, 1e-30, 1e-3, 0.1, 40.0, 1e6, 3e38])
+def test_temperatures_over_several_chunks(ctx, n, temp):
+    rng = np.random.default_rng(n)
+    for kind in KINDS:
+        x = rows(rng, 4, n, kind)
+        for mode in (dict(), dict(k=30), dict(p=0.9), dict(k=5000, p=0.99), dict(k=100, p=0.5, mp=0.01)):
+            Call(ctx, x, temp=temp, u=rng.random(4), **mode).check()
+
+
+@pytest.mark.parametrize("n", [2000, 20011])
+def test_logits_of_any_size_over_several_chunks(ctx, n):
+    rng = np.random.default_rng(15)
+    for scale in (1e-44, 1e-38, 1e-20, 1e10, 1e30, 3e38):
+        x = (rng.uniform(-1, 1, (5, n)) * scale).astype(np.float32)
+        x[1, n - 7] = -x[1].min()
+        x[2] = np.float32(scale)
+        x[3, ::2], x[3, 1::2] = 0.0, -0.0  # equal
+        x[4] = np.float32(-scale)
+        x[4, n - 1] = np.float32(-scale / 2)
+        for mode in (dict(), dict(k=30), dict(p=0.5), dict(k=3000, p=0.9), dict(mp=0.5)):
+            Call(ctx, x, u=rng.random(5), **mode).check()
+
+
+@pytest.mark.parametrize("n", [8192, 70001])
+def test_chunks_far_below_the_row(ctx, n):
+    """Chunks of -inf alone, of the type's lowest value, of weights that are none,
+    and one element that stands above all others, in the first chunk or the last."""
+    rng = np.random.default_rng(16)
+    x = rows(rng, 8, n, "flat")
+    x[0, :n // 2] = -np.inf
+    x[1, n // 3:] = -np.inf
+    x[2, 5000:] = np.finfo(np.float32).min
+    x[3, :n - 9] -= 1000
+    x[4, 11:] -= 30
+    x[5, n - 1] = 200
+    x[6, 0] = 40
+    x[7] = -np.inf
+    x[7, [0, n // 2, n - 1]] = [-3, -2, -3]
+    for mode in MODES:
+        Call(ctx, x, u=rng.random(8), pad=1, **mode).check()
+
+
+@pytest.mark.parametrize("n", [900, 50021])
+def test_rows_and_parameters_that_are_none(ctx, n):
+    """As above in a row of one launch and of several chunks, beside good ones."""
+    rng = np.random.default_rng(17)
+    x = rows(rng, 9, n, "peaked")
+    how = dict(k=40, p=0.9, mp=0.001, u=rng.random(9))
+    good = Call(ctx, x, **how).check()
+    y, nan = x.copy(), np.nan
+    y[1, n - 1], y[2, 0], y[3, n // 2], y[4] = nan, np.inf, nan, -np.inf
+    bad = np.arange(9) >= 1
+    bad[[5, 8]] = False
+    c = Call(ctx, y, temp=[1, 1, 1, 0, 1, 1, -0.5, nan, 1], **how)
+    c()
+    with pytest.raises(fa.FrqError) as e:
+        ctx.sync()
+    assert e.value.code == fa.FRQ_ERR_NAN  # of both the NaN first
+    with pytest.raises(fa.FrqError) as e:
+        ctx.sync()
+    assert e.value.code == fa.FRQ_ERR_ARG
+    ctx.sync()
+    t, p = c.token.numpy()[:9], c.prob.numpy()[:9]
+    assert (t[bad] == -1).all() and (p[bad] == 0).all()
+    assert np.array_equal(t[~bad], good[0][~bad]) and same(p[~bad], good[1][~bad])
+
+
+def test_short_rows_captured_and_replayed(ctx):
+    rng = np.random.default_rng(18)
+    c = Call(ctx, rows(rng, 7, 2000, "peaked"), temp=1.0, k=50, p=0.9, u=0.5)
+    c.check()
+    graph = Graph(ctx, c)
+    for i in range(5):
+        c.x, c.u = rows(rng, 7, 2000, KINDS[i]), rng.random(7).astype(np.float32)
+        put(c.dx, c.x)
+        put(c.du, c.u)
+        for how in (graph.replay, c, graph.replay):
+            put(c.token, np.full(9, 77, np.int64))
+            how()
+            ctx.sync()
+            assert c.token.numpy()[:7].tolist() == [w[0] for w in c.want()]
+    graph.close()
