@@ -83,6 +83,12 @@ struct Item {
 };
 
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// A word of memory that no one writes during the launch, the address the same in
+// all lanes: through the scalar cache.
+__device__ __forceinline__ int scalar_at(const int32_t* p, int64_t i) {
+    typedef const int32_t __attribute__((address_space(4))) word;
+    return reinterpret_cast<word*>(reinterpret_cast<uint64_t>(p))[i];
+}
 template <typename T>
 __device__ __forceinline__ T lane_bcast(T v, int src) {
     if constexpr (sizeof(T) == 8) {
@@ -1064,38 +1070,46 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     const int vr0 = (wave * IPW * 64 + lane) / P::VC;     // channel of piece 0
     const int vd = 8 * ((lane % P::VC) ^ (vr0 & P::VX));  // its first token
     bool bad = false;
-    int g0 = 0, g1 = 0, g2 = 0, g3 = 0;  // the ids of the tile's 16-token groups
+    struct Ids {  // of the tile's 16-token groups
+        int g0, g1, g2, g3;
+    } group{0, 0, 0, 0};
     auto ids = [&](int base) {
-        g0 = table[min(base >> shift, last_page)];
-        g1 = table[min((base + 16) >> shift, last_page)];
+        Ids g{0, 0, 0, 0};
+        g.g0 = scalar_at(table, min(base >> shift, last_page));
+        g.g1 = scalar_at(table, min((base + 16) >> shift, last_page));
         if (KT == 64) {
-            g2 = table[min((base + 32) >> shift, last_page)];
-            g3 = table[min((base + 48) >> shift, last_page)];
+            g.g2 = scalar_at(table, min((base + 32) >> shift, last_page));
+            g.g3 = scalar_at(table, min((base + 48) >> shift, last_page));
         }
+        return g;
     };
-    auto page_of = [&](int id) -> int64_t {
-        const int ok = page_ok(id, a.kv.n_pages);
-        bad |= ok < 0;
-        return max(ok, 0);
+    auto page_of = [&](int id) {
+        const bool ok = (uint32_t)id < (uint32_t)a.kv.n_pages;  // (n_pages below 2^31)
+        bad |= !ok;
+        return ok ? id : 0;
     };
     using Raw = std::conditional_t<I8, u2, u4>;
     constexpr int NR = F32 ? 2 : 1;  // loads a piece
     Raw rk[F16 ? 1 : IPW][NR], rv[F16 ? 1 : IPW][NR];
     float rs = 0.0f;
     auto fetch = [&](int base, int buf) {
-        int ln = lane;
+        const int g0 = page_of(group.g0), g1 = page_of(group.g1), g2 = KT == 64 ? page_of(group.g2) : 0,
+                  g3 = KT == 64 ? page_of(group.g3) : 0;
+        uint32_t ln = lane;
         asm volatile("" : "+v"(ln));  // addresses are formed anew for every tile, not held over the products
-        const int r0 = wave * (IPW * VR) + ln / P::VC, tok = 8 * ((ln % P::VC) ^ (r0 & P::VX));
-        const char* rows = kb + page_of(pick4(wave * (KT / 4) / 16, g0, g1, g2, g3)) * a.kv.stride +
+        const uint32_t r0 = wave * (IPW * VR) + ln / P::VC, tok = 8 * ((ln % P::VC) ^ (r0 & P::VX));
+        const char* rows = kb + pick4(wave * (KT / 4) / 16, g0, g1, g2, g3) * a.kv.stride +
                            (int64_t)((base + wave * (KT / 4)) & (page - 1)) * (hd * SZ);
-        const char* toks = vb + page_of(pick4(tok / 16, g0, g1, g2, g3)) * a.kv.stride + ((base + tok) & (page - 1)) * SZ;
+        const int64_t v0 = g0 * a.kv.stride, v1 = g1 * a.kv.stride, v2 = g2 * a.kv.stride, v3 = g3 * a.kv.stride;
+        const int64_t vlo = tok & 16 ? v1 : v0, vhi = tok & 16 ? v3 : v2;
+        const char* toks = vb + (KT == 64 && (tok & 32) ? vhi : vlo) + (uint32_t)(((base + (int)tok) & (page - 1)) * SZ);
 #pragma unroll
         for (int i = 0; i < IPW; ++i) {
-            const int d = (i * 64 + ln) / P::KC, r = r0 + i * VR;
-            const int c = 8 * (((i * 64 + ln) % P::KC) ^ ((wave * (KT / 4) + d) & P::KX));
+            const uint32_t d = (i * 64 + ln) / P::KC, r = r0 + i * VR;
+            const uint32_t c = 8 * (((i * 64 + ln) % P::KC) ^ ((wave * (KT / 4) + d) & P::KX));
             // past hd q is zero, any piece will do; channels past hd are not kept
             const char* pk = rows + (d * hd + (P::HP == hd || c < hd ? c : 0)) * SZ;
-            const char* pv = toks + (P::HP == hd || r < hd ? r : 0) * page * SZ;
+            const char* pv = toks + (((P::HP == hd || r < hd ? r : 0) << shift) * SZ);
             if constexpr (!F16) {
 #pragma unroll
                 for (int x = 0; x < NR; ++x) {
@@ -1110,7 +1124,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
         if constexpr (I8) {
             if (tid < 2 * KT) {  // the steps, a thread a key of each
                 const int d = tid % KT;
-                const int64_t at = page_of(pick4(d / 16, g0, g1, g2, g3)) * a.kv.sstride + kvh * page + ((base + d) & (page - 1));
+                const int64_t at = pick4(d / 16, g0, g1, g2, g3) * a.kv.sstride + kvh * page + ((base + d) & (page - 1));
                 rs = tid < KT ? a.kv.ks[at] : a.kv.vs[at];
             }
         }
@@ -1217,18 +1231,19 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     if (!PHASES && second) __builtin_amdgcn_s_setprio(2);
     __syncthreads();
     if (tiles) {
-        ids(real(beg));
+        group = ids(real(beg));
         fetch(real(beg), 0);
         land(real(beg), 0);
-        if (tiles > 1) ids(real(beg + KT));
+        if (tiles > 1) group = ids(real(beg + KT));
     }
     __syncthreads();
     for (int ti = 0; ti < tiles; ++ti) {
         const int base = real(beg + ti * KT), next = real(beg + (ti + 1) * KT);
         const int buf = NBUF == 1 ? 0 : ti & 1, other = NBUF - 1 - buf;
         if (ti + 1 < tiles) {
+            const Ids ahead = ids(real(beg + min(ti + 2, tiles - 1) * KT));
             fetch(next, other);
-            if (ti + 2 < tiles) ids(real(beg + (ti + 2) * KT));
+            group = ahead;
         }
         if (!idle) {
 #pragma unroll 1
@@ -1267,23 +1282,24 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
 #pragma unroll
                 for (int g = 0; g < NS; g += 2 * G) {
 #pragma unroll
-                    for (int i = 0; i < G; ++i)
-                        if (g + G + i < NS) key_op(g + G + i, xb[i]);
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
                     for (int i = 0; i < G; ++i) {
-                        if (g + i >= NS) continue;
-                        s = product(xa[i], qv[(g + i) % NS], s);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (g + i < NS) s = product(xa[i], qv[(g + i) % NS], s);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (i > 0) continue;
+#pragma unroll
+                        for (int j = 0; j < G; ++j)
+                            if (g + G + j < NS) key_op(g + G + j, xb[j]);
                     }
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int i = 0; i < G; ++i)
-                        if (g + 2 * G + i < NS) key_op(g + 2 * G + i, xa[i]);
-                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int i = 0; i < G; ++i) {
-                        if (g + G + i >= NS) continue;
-                        s = product(xb[i], qv[(g + G + i) % NS], s);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (g + G + i < NS) s = product(xb[i], qv[(g + G + i) % NS], s);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (i > 0) continue;
+#pragma unroll
+                        for (int j = 0; j < G; ++j)
+                            if (g + 2 * G + j < NS) key_op(g + 2 * G + j, xa[j]);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -1373,25 +1389,26 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
 #pragma unroll
                 for (int g = 0; g < 2 * NH; g += 2 * G) {
 #pragma unroll
-                    for (int i = 0; i < G; ++i)
-                        if (g + G + i < 2 * NH) val_op(g + G + i, xb[i]);
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
                     for (int i = 0; i < G; ++i) {
                         const int t = (g + i) / 2;
-                        if (g + i >= 2 * NH) continue;
-                        o[t % NH] = product(xa[i], pv[i % 2], o[t % NH]);
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (g + i < 2 * NH) o[t % NH] = product(xa[i], pv[i % 2], o[t % NH]);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (i > 0) continue;
 #pragma unroll
-                    for (int i = 0; i < G; ++i)
-                        if (g + 2 * G + i < 2 * NH) val_op(g + 2 * G + i, xa[i]);
-                    __builtin_amdgcn_sched_barrier(0);
+                        for (int j = 0; j < G; ++j)
+                            if (g + G + j < 2 * NH) val_op(g + G + j, xb[j]);
+                    }
 #pragma unroll
                     for (int i = 0; i < G; ++i) {
                         const int t = (g + G + i) / 2;
-                        if (g + G + i >= 2 * NH) continue;
-                        o[t % NH] = product(xb[i], pv[i % 2], o[t % NH]);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (g + G + i < 2 * NH) o[t % NH] = product(xb[i], pv[i % 2], o[t % NH]);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (i > 0) continue;
+#pragma unroll
+                        for (int j = 0; j < G; ++j)
+                            if (g + 2 * G + j < 2 * NH) val_op(g + 2 * G + j, xa[j]);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
