@@ -918,8 +918,12 @@ __device__ __forceinline__ int pick4(int j, int a, int b, int c, int d) {
 // Bound by the matrix cores, and by the clock under them (1.7 GHz, the cores
 // busy half the time): f16, 28 heads of 128 channels over 4, 2048 rows after
 // 6144 cached tokens, is 210 GFLOP of the formula, which the two halves of q
-// and p make 420, in 430 us; int8, 7 sequences of up to 1501 tokens, 24 GFLOP,
-// in 101.  One f16 for p would cost its bits below 2^-11.  128 pairs a workgroup
+// and p make 420, in 420 us; int8, 7 sequences of up to 1501 tokens, 24 GFLOP,
+// in 101.  A tile of 64 keys takes a wave 7000 to 8500 cycles beside another's: its
+// loads' issue 1400 to 2000 (before their addresses moved to the scalar unit, 439 us
+// the whole), scores 1700 to 2200, softmax 2000, values 1100 to 1500 (1024 of each
+// product's are its instructions', which take two fifths of the vector unit's turns
+// as well).  One f16 for p would cost its bits below 2^-11.  128 pairs a workgroup
 // let two fit a CU (64 KB of LDS, 256 registers); equal priorities of both 503 us
 // against 481.
 //
