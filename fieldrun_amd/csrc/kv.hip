@@ -261,6 +261,15 @@ hipError_t launch_move(const Move& m, int dtype, hipStream_t s) {
 // 48 int8 sequences of up to 6001 tokens 65, 47, 55, 56 us; one of 131071 f16
 // 103, 109, 115, 109; 16 f32 windows of 4096 164, 124, 123, 133).
 constexpr int64_t DEC_TARGET = 512;
+// With sinks or trees one round of half of that (chunk_of_even) where the tiles have
+// nearly the same keys (windows mostly, and one sequence always) and memory or one
+// workgroup a CU bounds them: windows over f32 keys, over 192 channels, one sequence.
+// 512 against it: 16 f32 windows of 4096 by 256 channels 121, 107 us, 35 of 325 52, 35, 20
+// f16 ones of 1000 34, 29, f32 of 128 channels 28, 25, one int8 window of 50000 34, 31, 16
+// rows of one f16 tree over 8000 27.7, 25.8.  But 20 f32 sequences of 100 to 6001 by 256
+// channels 101, 129 (of 256 items: these keep the target), 8 f16 trees of 35 pairs over
+// 2000 27, 33, f32 49, 54.
+constexpr int64_t EVEN_TARGET = 256;
 // Prompt items wanted: a round and not quite two a CU; more cost the joining
 // more than the balance gives (400, 640, 1024, 1536: kernel and join of 7 ragged
 // int8 prompts 123 + 8, 127 + 18, 110 + 24, 108 + 24 us; of 2048 rows over 8192
@@ -331,6 +340,7 @@ Plan plan_of(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq, bool e
     c.tp = 16;
     c.target = DEC_TARGET;
     p.prompt = c;
+    if (ex && ((kv->dtype == FRQ_DT_F32 && !trees) || kv->hd > 192 || n_seq == 1)) c.even = EVEN_TARGET;
     const bool big = (double)n_row * (double)n_head * (double)keys > EX_WORK;
     p.prompt.min_pairs = 1 + (!trees ? DEC_PAIRS : big ? TREE_PAIRS : 0x7FFFFFFE);
     p.prompt.tp = 128;

@@ -39,6 +39,7 @@ struct Call {
     int sinks, sink_span;  // with a window: first keys seen besides, and as a tile spans them (sink_keys; 0: none)
     const uint64_t* tree;  // bit masks of drafted tokens, a row of q each (null: rows see what lies before them)
     int64_t tree_pitch;    // words between the masks
+    int64_t even;          // items wanted where the tiles have nearly the same keys, up to target (0: target)
 };
 
 struct Seq {
@@ -88,10 +89,19 @@ KV_HD int round_keys(uint32_t keys, int step) {  // up to a multiple of step, a 
     const uint32_t up = (keys + (uint32_t)step - 1) & ~((uint32_t)step - 1);
     return up > (uint32_t)MOST ? MOST : (int)up;
 }
-KV_HD int chunk_of(const Call& c, int64_t total) {
-    const uint64_t x = (uint64_t)total * (uint64_t)c.n_kv + (uint64_t)c.target - 1;
-    const uint64_t per = x >> 32 ? x / (uint64_t)c.target : (uint64_t)((uint32_t)x / (uint32_t)c.target);
+KV_HD int chunk_of(const Call& c, int64_t total, int64_t target) {
+    const uint64_t x = (uint64_t)total * (uint64_t)c.n_kv + (uint64_t)target - 1;
+    const uint64_t per = x >> 32 ? x / (uint64_t)target : (uint64_t)((uint32_t)x / (uint32_t)target);
     const int up = round_keys(per > (uint64_t)MOST ? (uint32_t)MOST : (uint32_t)per, c.min_chunk);
+    return up < c.min_chunk ? c.min_chunk : up;
+}
+KV_HD int chunk_of(const Call& c, int64_t total) { return chunk_of(c, total, c.target); }
+// The same where c.even is set, of `tiles` tiles of up to `most` keys.
+KV_HD int chunk_of_even(const Call& c, int64_t total, int64_t tiles, int most) {
+    if ((int64_t)most * tiles > total + total / 4) return chunk_of(c, total);
+    if (!tiles || tiles * c.n_kv > c.even) return chunk_of(c, total, c.even);
+    const uint32_t n = (uint32_t)c.even / ((uint32_t)tiles * (uint32_t)c.n_kv);  // chunks a tile: one round
+    const int up = round_keys(((uint32_t)most + n - 1) / n, c.min_chunk);
     return up < c.min_chunk ? c.min_chunk : up;
 }
 KV_HD int chunks_of(const Seq& q, int chunk) {

@@ -6,6 +6,7 @@ import os
 import random
 import subprocess
 
+import numpy as np
 import pytest
 
 import fieldrun_amd as fa
@@ -176,3 +177,66 @@ def test_trees_without_room_are_told(host):
         assert bad == want
         assert all(i.rows <= i.len for i in items)
     assert plan(host, [5], [0, 9], 3, 0, 0, 32, False)[2] == 0  # more rows than tokens: not of trees alone
+
+
+EVEN = r"""
+#include "kv_index.h"
+using namespace frq::kv;
+extern "C" int64_t even(int n_seq, const int32_t* tiles, const int32_t* ext, int n_row, int rep, int n_kv, int tp, int64_t target,
+                        int64_t even, int min_chunk, int64_t* out) {
+    Call c{nullptr, nullptr, n_seq, n_row, 8192, 4, rep, 0, n_kv, tp, 1, 0x7FFFFFFF, target, min_chunk};
+    c.even = even;
+    int64_t total = 0, all = 0, items = 0, slots = 0;
+    int most = 0;
+    for (int s = 0; s < n_seq; ++s) {
+        total += (int64_t)tiles[s] * ext[s];
+        all += tiles[s];
+        if (tiles[s] && ext[s] > most) most = ext[s];
+    }
+    const int klen = chunk_of_even(c, total, all, most);
+    for (int s = 0; s < n_seq; ++s) {
+        Seq q{0, 0, 0, ext[s], tiles[s], false};
+        const int n = chunks_of(q, klen);
+        items += (int64_t)tiles[s] * n;
+        if (n > 1) slots += (int64_t)tiles[s] * n;
+    }
+    out[0] = klen;
+    out[1] = items;
+    out[2] = slots;
+    out[3] = all + target / n_kv + 1;
+    out[4] = max_slots(target, n_kv);
+    return chunk_of(c, total);
+}
+"""
+
+
+def test_chunks_of_even_tiles_keep_the_bounds(tmp_path):
+    """Tiles of nearly the same keys fill one round of `even` items and no more,
+    others are cut as ever; neither passes the host's bounds."""
+    (tmp_path / "even.cpp").write_text(EVEN)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", "-I",
+                    os.path.join(ROOT, "fieldrun_amd", "csrc"), str(tmp_path / "even.cpp"), "-o", str(tmp_path / "even.so")],
+                   check=True)
+    lib = C.CDLL(str(tmp_path / "even.so"))
+    lib.even.restype = C.c_int64
+    lib.even.argtypes = [C.c_int, C.c_void_p, C.c_void_p] + [C.c_int] * 4 + [C.c_int64] * 2 + [C.c_int, C.c_void_p]
+    rng = np.random.default_rng(3)
+    rounds = 0
+    for i in range(3000):
+        n = int(rng.integers(1, 65))
+        most = int(10 ** rng.uniform(0, 9 if i % 3 == 0 else 5))
+        low = most if i % 2 else max(0, int(most * rng.uniform(0.5, 1)))
+        ext = rng.integers(low, most + 1, n).astype(np.int32) if i % 5 else rng.integers(0, most + 1, n).astype(np.int32)
+        tiles = rng.integers(0, 4, n).astype(np.int32) if i % 4 else np.ones(n, np.int32)
+        kv, step = int(rng.choice([1, 2, 4, 5, 8, 64, 600])), int(rng.choice([128, 256]))
+        out = np.zeros(5, np.int64)
+        plain = lib.even(n, tiles.ctypes.data, ext.ctypes.data, n, 1, kv, 16, 512, 256, step, out.ctypes.data)
+        klen, items, slots, most_items, most_slots = out.tolist()
+        assert klen % 64 == 0 and klen >= step and items <= most_items and slots <= most_slots, (i, out)
+        total, top = int((tiles.astype(np.int64) * ext).sum()), int(ext[tiles > 0].max(initial=0))
+        if top * int(tiles.sum()) > total + total // 4:
+            assert klen == plain
+        elif 0 < int(tiles.sum()) * kv <= 256:
+            rounds += 1
+            assert items * kv <= 256
+    assert rounds > 300
