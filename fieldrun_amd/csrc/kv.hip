@@ -463,6 +463,7 @@ int attend(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, siz
     b.c.max_pairs = plan.prompt.max_pairs;
     b.c.tp = plan.prompt.tp;
     b.c.target = plan.prompt.target;
+    b.c.even = 0;
     b.c.min_chunk = plan.prompt.min_chunk;
     b.c.sink_span = sink_keys((int64_t)sinks, 64);
     b.rec = (Record*)(ws + plan.rec_prompt);
