@@ -173,24 +173,32 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const Args a, const Args b
 // two passes over the lengths.
 __global__ __launch_bounds__(1024) void kv_plan_kernel(const Call ca, const Call cb, int32_t* plan_a, int32_t* plan_b,
                                                        int* err) {
-    __shared__ int64_t keys[16];
+    __shared__ int64_t keys[16], tiles[16];
     const bool dec = blockIdx.x == 0;
     const Call c = dec ? ca : cb;
     int32_t* plan = dec ? plan_a : plan_b;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, blocks = (c.n_seq + 63) / 64;
-    int64_t total = 0;
+    int64_t total = 0, all = 0;
     for (int64_t s = threadIdx.x; s < c.n_seq; s += 1024) {
         const Seq q = seq_at(c, (int)s);
         total += keys_of(q);
+        all += q.tiles;
         if (q.bad && dec) atomicOr(err, ERR_INDEX);
     }
     total = wave_total(total);
-    if (lane == 0) keys[w] = total;
+    all = wave_total(all);
+    if (lane == 0) {
+        keys[w] = total;
+        tiles[w] = all;
+    }
     __syncthreads();
-    total = 0;
+    total = all = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) total += keys[i];
-    const int klen = chunk_of(c, total);
+    for (int i = 0; i < 16; ++i) {
+        total += keys[i];
+        all += tiles[i];
+    }
+    const int klen = chunk_of(c, total, wanted(c, all));
     for (int b = w; b < blocks; b += 16) {
         Seq q{};
         if (b * 64 + lane < c.n_seq) q = seq_at(c, b * 64 + lane);
@@ -304,16 +312,12 @@ constexpr double EX_WORK = 6e6;  // rows x heads x keys
 // beside 31 of one 109, 127; trees of 24 pairs, f16 of 64 channels 39, 55.
 constexpr size_t EX_PAIRS = 64;
 // With sinks or trees the items fill the chip's workgroups once, less the chunks
-// that every tile is rounded up by (half a target at least): one tree of 256 pairs
-// over 32768 f16 tokens 104 us at 400 items, 95 at the rule's 496; 16 int8 ones of up to
-// 182 pairs 84 at 512, 70 at the rule's 388; 2048 rows in windows of 1024 111, 88 at the
-// rule's 256; 4 f32 trees of 182 pairs, one workgroup a CU, 119 at 400, 90 at the rule's.
+// that every tile is rounded up by (wanted(), from the lengths): one tree of 256 pairs
+// over 32768 f16 tokens 104 us at 400 items, 91 at the rule's 496; 16 int8 ones of up to
+// 182 pairs 84 at 512, 63 at the rule's 424 (65 at 388, the host's bound of the tiles;
+// 20 f16 ones 77 by that, 72); 2048 rows in windows of 1024 111, 85 at the rule's 256; 4
+// f32 trees of 182 pairs, one workgroup a CU, 119 at 400, 79 at the rule's.
 int64_t ex_slots(const frq_kv* kv) { return kv->dtype == FRQ_DT_F32 || kv->hd > 128 ? 256 : 512; }
-int64_t ex_target(const frq_kv* kv, const Call& prompt) {
-    const int64_t slots = ex_slots(kv);
-    return std::max(slots / 2, slots - max_tiles(prompt) * prompt.n_kv);
-}
-
 // The work of an attention call, and its workspace: the items' records, the
 // decode tiles' parts, where a sequence may ask with several rows the prompt
 // tiles', and for many sequences both launches' plans.
@@ -345,7 +349,8 @@ Plan plan_of(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq, bool e
     p.prompt.min_pairs = 1 + (!trees ? DEC_PAIRS : big ? TREE_PAIRS : 0x7FFFFFFE);
     p.prompt.tp = 128;
     // (n_row <= n_seq: no room for parts, every tile's keys in one run)
-    p.prompt.target = n_row <= n_seq ? 1 : ex ? ex_target(kv, p.prompt) : kv->hd > 128 ? PROMPT_TARGET_WIDE : PROMPT_TARGET;
+    p.prompt.target = n_row <= n_seq ? 1 : ex ? ex_slots(kv) : kv->hd > 128 ? PROMPT_TARGET_WIDE : PROMPT_TARGET;
+    if (ex && n_row > n_seq) p.prompt.slots = p.prompt.target;
     // (f32 keys of over 128 channels have no prompt kernel)
     const bool f32 = kv->dtype == FRQ_DT_F32;
     const size_t pairs = n_row * c.rep, mean = big && (trees || !f32) ? EX_PAIRS : DEC_PAIRS;
@@ -464,6 +469,7 @@ int attend(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, siz
     b.c.tp = plan.prompt.tp;
     b.c.target = plan.prompt.target;
     b.c.even = 0;
+    b.c.slots = plan.prompt.slots;
     b.c.min_chunk = plan.prompt.min_chunk;
     b.c.sink_span = sink_keys((int64_t)sinks, 64);
     b.rec = (Record*)(ws + plan.rec_prompt);

@@ -176,7 +176,7 @@ __device__ __forceinline__ Item find_item(const Call& c, int id, int* err) {
     if (!c.plan) {
         if (q.bad && id == 0 && threadIdx.x < 64) atomicOr(err, ERR_INDEX);
         const int64_t total = c.n_seq > 1 ? wave_total(keys_of(q)) : lane_bcast(keys_of(q), 0);
-        if (!c.even) klen = chunk_of(c, total);
+        if (!c.even) klen = chunk_of(c, total, c.slots ? wanted(c, wave_total(q.tiles)) : c.target);
         else klen = chunk_of_even(c, total, wave_total(q.tiles), wave_most(q.tiles ? q.ext : 0));
     }
     const int n = q.tiles ? chunks_of(q, klen) : 1, own = even_chunk(q, n), mine = q.tiles * n;

@@ -40,6 +40,7 @@ struct Call {
     const uint64_t* tree;  // bit masks of drafted tokens, a row of q each (null: rows see what lies before them)
     int64_t tree_pitch;    // words between the masks
     int64_t even;          // items wanted where the tiles have nearly the same keys, up to target (0: target)
+    int64_t slots;         // or the items that fill the chip, up to target, for wanted() (0: target)
 };
 
 struct Seq {
@@ -96,6 +97,13 @@ KV_HD int chunk_of(const Call& c, int64_t total, int64_t target) {
     return up < c.min_chunk ? c.min_chunk : up;
 }
 KV_HD int chunk_of(const Call& c, int64_t total) { return chunk_of(c, total, c.target); }
+// The items that fill the chip less the chunks that every tile is rounded up by,
+// half of them at least.
+KV_HD int64_t wanted(const Call& c, int64_t tiles) {
+    if (!c.slots) return c.target;
+    const int64_t left = c.slots - tiles * c.n_kv;
+    return left > c.slots / 2 ? left : c.slots / 2;
+}
 // The same where c.even is set, of `tiles` tiles of up to `most` keys.
 KV_HD int chunk_of_even(const Call& c, int64_t total, int64_t tiles, int most) {
     if ((int64_t)most * tiles > total + total / 4) return chunk_of(c, total);

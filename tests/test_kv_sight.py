@@ -240,3 +240,29 @@ def test_chunks_of_even_tiles_keep_the_bounds(tmp_path):
             rounds += 1
             assert items * kv <= 256
     assert rounds > 300
+
+
+WANTED = r"""
+#include "kv_index.h"
+using namespace frq::kv;
+extern "C" int64_t items(int64_t slots, int64_t target, int64_t tiles, int n_kv) {
+    Call c{};
+    c.target = target;
+    c.slots = slots;
+    c.n_kv = n_kv;
+    return wanted(c, tiles);
+}
+"""
+
+
+def test_items_wanted_stay_within_the_target(tmp_path):
+    (tmp_path / "w.cpp").write_text(WANTED)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", "-I",
+                    os.path.join(ROOT, "fieldrun_amd", "csrc"), str(tmp_path / "w.cpp"), "-o", str(tmp_path / "w.so")], check=True)
+    lib = C.CDLL(str(tmp_path / "w.so"))
+    lib.items.restype = C.c_int64
+    lib.items.argtypes = [C.c_int64] * 3 + [C.c_int]
+    for tiles in (0, 1, 20, 64, 128, 1000, 1 << 31):
+        for kv in (1, 4, 65535):
+            assert lib.items(0, 400, tiles, kv) == 400
+            assert lib.items(512, 512, tiles, kv) == max(256, 512 - tiles * kv)
