@@ -109,8 +109,12 @@ KV_HD int chunk_of_even(const Call& c, int64_t total, int64_t tiles, int most) {
     if ((int64_t)most * tiles > total + total / 4) return chunk_of(c, total);
     if (!tiles || tiles * c.n_kv > c.even) return chunk_of(c, total, c.even);
     const uint32_t n = (uint32_t)c.even / ((uint32_t)tiles * (uint32_t)c.n_kv);  // chunks a tile: one round
-    const int up = round_keys(((uint32_t)most + n - 1) / n, c.min_chunk);
-    return up < c.min_chunk ? c.min_chunk : up;
+    // (chunks of half the least for a few hundred keys, where a tile's latency counts: one
+    // sequence of 1000 keys, 4 int8 heads of 128, 14.4 us in five chunks, 12.8 in nine; two
+    // for 200 keys or sixteen for 2000 cost the joining more, 10.0 / 11.3, 12.1 / 13.1)
+    const int least = most > 256 && most <= 12 * 128 && c.min_chunk > 128 ? 128 : c.min_chunk;
+    const int up = round_keys(((uint32_t)most + n - 1) / n, least);
+    return up < least ? least : up;
 }
 KV_HD int chunks_of(const Seq& q, int chunk) {
     const int n = (int)(((uint32_t)q.ext + (uint32_t)chunk - 1) / (uint32_t)chunk);
