@@ -245,7 +245,7 @@ __device__ __forceinline__ bool page_bad(const Args& a, int seq, int lo, int hi)
     return false;
 }
 // The same for a chunk that takes sinks: `real` is where its keys v0 .. v1 - 1
-// lie, 16 by 16 in one page; rows see the first keys and those from lo to hi.
+// lie, 16 by 16 in one page; rows see the sinks and keys from lo (Sight::low) to hi.
 template <typename F>
 __device__ __forceinline__ bool page_bad(const Args& a, int seq, int v0, int v1, int lo, int hi, F&& real) {
     const int32_t* table = a.pages + (int64_t)seq * a.pages_pitch;
@@ -285,7 +285,9 @@ struct Sight<true> {
     const uint64_t* mask;
     uint64_t word;  // its first word, for HELD: most trees have no second
     __device__ __forceinline__ bool any() const { return some; }
-    __device__ __forceinline__ int first() const { return sinks ? 0 : n && lo > base ? base : lo; }
+    // the first key behind the sinks that may be seen (a drafted one however deep its row)
+    __device__ __forceinline__ int low() const { return n && lo > base ? base : lo; }
+    __device__ __forceinline__ int first() const { return sinks ? 0 : low(); }
     template <int N, bool HELD = false>
     __device__ __forceinline__ Bits seen(int key) const {
         static_assert(N <= 16, "");
@@ -871,7 +873,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
     if (wave != 0) return;
     if (__builtin_expect(hole, 0)) {
         bool gone;
-        if constexpr (EX) gone = page_bad(a, it.seq, beg, end, -wave_most(-sight.lo), pos_b, real);
+        if constexpr (EX) gone = page_bad(a, it.seq, beg, end, -wave_most(-sight.low()), pos_b, real);
         else gone = page_bad(a, it.seq, max(lo_a, beg), min(pos_b, end - 1));
         if (gone) {
             note_hole(a, blockIdx.x / n_kv, it.seq);
@@ -995,7 +997,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     constexpr int NS = HD / 16, NH = P::N32, NK = P::KT / 32, KT = P::KT, IPW = P::IPW;
     extern __shared__ __align__(1024) char lds[];
     __shared__ int flag, hole;  // a value was taken out; a page id was bad
-    __shared__ int least;       // EX: the first key that a row sees behind the sinks
+    __shared__ int least;       // EX: the first key behind the sinks that a row may see
     uint16_t* lk = reinterpret_cast<uint16_t*>(lds);                   // [NBUF][NA][KT][HP]
     uint16_t* lv = lk + NBUF * NA * P::BUF;                            // [NBUF][NA][HP][KT]
     float* lks = reinterpret_cast<float*>(lv + NBUF * NA * P::BUF);    // [2][KT] int8 steps
@@ -1430,7 +1432,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     }
     if (bad) hole = 1;  // (each wave has looked at the ids of its own pieces)
     if constexpr (EX) {
-        const int lo = -wave_most(-sight.lo);
+        const int lo = -wave_most(-sight.low());
         if (lane == 0) atomicMin(&least, lo);
     }
     __syncthreads();

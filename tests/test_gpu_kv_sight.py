@@ -407,6 +407,34 @@ def test_pages_of_trees_out_of_range_take_no_part(ctx, kind, rows):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("every", [False, True])
+@pytest.mark.parametrize("window,sinks,length,rows,page", [
+    (1, 0, 300, 70, 15), (10, 0, 300, 70, 15), (10, 5, 300, 70, 14), (16, 40, 131, 64, 5),  # the decode kernel
+    (10, 1000, 1500, 200, 85), (190, 0, 900, 400, 32), (190, 0, 900, 400, 31),  # the prompt kernel
+])
+def test_pages_of_drafted_tokens_count_past_the_window(ctx, kind, every, window, sinks, length, rows, page):
+    """A drafted token stays seen however deep its row, so a page id out of range
+    under one is reported and its tokens left out of every row: chains longer
+    than the window, and rows that see all drafted tokens."""
+    trees = [[set(range(r if every else i + 1)) for i in range(r)] for r in (rows, 7)]
+    rep = 3 if rows < 100 else 21 if sinks else 42
+    b = More(ctx, kind, 16, 2, rep, 16, [length, 40], [rows, 7], seed=window, trees=trees, window=window, sinks=sinks)
+    table = b.table.copy()
+    assert (page + 1) * 16 > length - rows and page * 16 + 15 < length
+    table[0, page] = b.p.n_pages
+    put(b.dev[0], table)
+    runs = []
+    for _ in range(2):
+        with pytest.raises(fa.FrqError) as e:
+            b.run()
+        assert e.value.code == fa.FRQ_ERR_ARG
+        ctx.sync()
+        runs.append(b.do.numpy()[:b.n_row])
+    assert same(*runs)
+    hold(runs[0], *b.want(gone={0: range(16 * page, 16 * page + 16)}))
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("many", [False, True])
 def test_small_sequences_beside_large_ones(ctx, kind, many):
     """Calls of many pairs a sequence, where one kernel serves them all: rows of
