@@ -168,21 +168,24 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const Args a, const Args b
 }
 
 // The plans of many sequences (workgroup 0: the decode launch's, 1: the
-// prompt's): the call's keys, then the items and slots before each 64
-// sequences.  16 waves, 64 sequences each at a time, bound by the latency of
-// two passes over the lengths.
+// prompt's): which launch serves those of c.uncut pairs, the call's keys, then the
+// items and slots before each 64 sequences.  16 waves, 64 sequences each at a
+// time, bound by the latency of two passes over the lengths.
+template <bool EX>
 __global__ __launch_bounds__(1024) void kv_plan_kernel(const Call ca, const Call cb, int32_t* plan_a, int32_t* plan_b,
                                                        int* err) {
-    __shared__ int64_t keys[16], tiles[16];
+    __shared__ int64_t keys[16], tiles[16], uncut_keys[16], walked[16];
+    __shared__ int longest[16];
     const bool dec = blockIdx.x == 0;
     const Call c = dec ? ca : cb;
+    const int pairs = EX ? c.uncut : 0;
     int32_t* plan = dec ? plan_a : plan_b;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, blocks = (c.n_seq + 63) / 64;
-    int64_t total = 0, all = 0;
+    int64_t total = 0, all = 0;  // keys, tiles; (pairs: wanted() asks for none) sequences of `pairs` and more
     for (int64_t s = threadIdx.x; s < c.n_seq; s += 1024) {
         const Seq q = seq_at(c, (int)s);
         total += keys_of(q);
-        all += q.tiles;
+        all += pairs ? (int64_t)q.rows * c.rep >= pairs : q.tiles;
         if (q.bad && dec) atomicOr(err, ERR_INDEX);
     }
     total = wave_total(total);
@@ -198,10 +201,41 @@ __global__ __launch_bounds__(1024) void kv_plan_kernel(const Call ca, const Call
         total += keys[i];
         all += tiles[i];
     }
+    bool filled = false;
+    if (__builtin_expect(pairs && all, 0)) {
+        int64_t uncut = 0, walk = 0;
+        int most = 0;
+        for (int64_t s = threadIdx.x; s < c.n_seq; s += 1024) {
+            const Seq q = seq_at(c, (int)s);
+            if ((int64_t)q.rows * c.rep < pairs) continue;
+            const int own = lone_keys(c, q);
+            uncut += keys_of(q);
+            walk += lone_tiles(c, q) * own;
+            most = max(most, own);
+        }
+        uncut = wave_total(uncut);
+        walk = wave_total(walk);
+        most = wave_most(most);
+        if (lane == 0) {
+            uncut_keys[w] = uncut;
+            walked[w] = walk;
+            longest[w] = most;
+        }
+        __syncthreads();
+        uncut = walk = 0;
+        for (int i = 0; i < 16; ++i) {
+            uncut += uncut_keys[i];
+            walk += walked[i];
+            most = max(most, longest[i]);
+        }
+        filled = fills(walk, most, c.n_kv);
+        if (filled != c.prompt) total -= uncut;
+    }
     const int klen = chunk_of(c, total, wanted(c, all));
     for (int b = w; b < blocks; b += 16) {
         Seq q{};
         if (b * 64 + lane < c.n_seq) q = seq_at(c, b * 64 + lane);
+        if (pairs && all) drop_uncut(c, filled, q);
         const int n = q.tiles ? chunks_of(q, klen) : 1, mine = q.tiles * n;
         const int items = lane_sums(mine), slots = lane_sums(n > 1 ? mine : 0);
         if (lane == 63) {
@@ -213,7 +247,7 @@ __global__ __launch_bounds__(1024) void kv_plan_kernel(const Call ca, const Call
     if (w) return;
     if (lane == 0) {
         plan[0] = klen;
-        plan[1] = 0;
+        plan[1] = filled;
     }
     int items = 0, slots = 0;
     for (int b0 = 0; b0 < blocks; b0 += 64) {
@@ -318,6 +352,16 @@ constexpr size_t EX_PAIRS = 64;
 // 20 f16 ones 77 by that, 72); 2048 rows in windows of 1024 111, 85 at the rule's 256; 4
 // f32 trees of 182 pairs, one workgroup a CU, 119 at 400, 79 at the rule's.
 int64_t ex_slots(const frq_kv* kv) { return kv->dtype == FRQ_DT_F32 || kv->hd > 128 ? 256 : 512; }
+// A batch with idle sequences, no more rows than sequences, has no room for prompt
+// tiles' parts (n_row <= n_seq below): with sinks or trees the prompt kernel takes
+// sequences there only where they fill it (fills(), kv_index.h, from the lengths), and
+// none of a batch that needs no plan, which has 64 rows at most.  Prompt kernel, decode
+// kernel: 64 slots and one tree of 112 pairs over 32768 tokens, 2 kv heads of 64, f16
+// 902, 29 us, int8 1253, 27, f32 2124, 55; over 211 f16 21, 11; 2048 slots, 4 kv heads of
+// 128, one prompt of 2800 pairs with a window of 1000 f16 76, 65, int8 90, 62, f32 151,
+// 109; of 5600 83, 113, 96, 103, 158, 202; 40 trees of 70 pairs over 2000 tokens 104, 130,
+// 135, 114, 234, 252.  The choice costs the plan 3 to 5 us.  (Without sinks or trees these
+// batches keep their kernels, and so their bits.)
 // The work of an attention call, and its workspace: the items' records, the
 // decode tiles' parts, where a sequence may ask with several rows the prompt
 // tiles', and for many sequences both launches' plans.
@@ -347,6 +391,10 @@ Plan plan_of(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq, bool e
     if (ex && ((kv->dtype == FRQ_DT_F32 && !trees) || kv->hd > 192 || n_seq == 1)) c.even = EVEN_TARGET;
     const bool big = (double)n_row * (double)n_head * (double)keys > EX_WORK;
     p.prompt.min_pairs = 1 + (!trees ? DEC_PAIRS : big ? TREE_PAIRS : 0x7FFFFFFE);
+    if (ex && n_row <= n_seq) {
+        if (n_seq > (size_t)PLAN_SEQS) p.prompt.uncut = p.prompt.min_pairs;
+        else p.prompt.min_pairs = 0x7FFFFFFF;
+    }
     p.prompt.tp = 128;
     // (n_row <= n_seq: no room for parts, every tile's keys in one run)
     p.prompt.target = n_row <= n_seq ? 1 : ex ? ex_slots(kv) : kv->hd > 128 ? PROMPT_TARGET_WIDE : PROMPT_TARGET;
@@ -458,7 +506,9 @@ int attend(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, siz
     // 202 and 1280, 676.  Widths of an odd number of 32s do not fit the LDS.)
     const bool prompts = d_first && n_row * (size_t)a.c.rep >= (size_t)plan.prompt.min_pairs &&
                          !(kv->dtype == FRQ_DT_F32 && kv->hd > 128);
-    a.c.max_pairs = prompts ? plan.prompt.min_pairs - 1 : 0x7FFFFFFF;
+    const int uncut = prompts ? plan.prompt.uncut : 0;
+    a.c.max_pairs = prompts && !uncut ? plan.prompt.min_pairs - 1 : 0x7FFFFFFF;
+    a.c.uncut = uncut;
     char* ws = (char*)d_ws;
     a.rec = (Record*)(ws + plan.rec_dec);
     a.part = (float*)(ws + plan.part_dec);
@@ -470,6 +520,7 @@ int attend(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, siz
     b.c.target = plan.prompt.target;
     b.c.even = 0;
     b.c.slots = plan.prompt.slots;
+    b.c.prompt = true;
     b.c.min_chunk = plan.prompt.min_chunk;
     b.c.sink_span = sink_keys((int64_t)sinks, 64);
     b.rec = (Record*)(ws + plan.rec_prompt);
@@ -481,7 +532,8 @@ int attend(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, siz
     hipError_t e = hipSuccess;
     if (n_seq > (size_t)PLAN_SEQS) {
         int32_t *pa = (int32_t*)(ws + plan.plan_dec), *pb = (int32_t*)(ws + plan.plan_prompt);
-        kv_plan_kernel<<<dim3(prompts ? 2 : 1), dim3(1024), 0, s>>>(a.c, b.c, pa, pb, a.err);
+        if (ex) kv_plan_kernel<true><<<dim3(prompts ? 2 : 1), dim3(1024), 0, s>>>(a.c, b.c, pa, pb, a.err);
+        else kv_plan_kernel<false><<<dim3(prompts ? 2 : 1), dim3(1024), 0, s>>>(a.c, b.c, pa, pb, a.err);
         e = hipGetLastError();
         if (e != hipSuccess) return hip_bad(e, "launch kv_plan");
         a.c.plan = pa;

@@ -151,6 +151,7 @@ __device__ __forceinline__ int wave_most(int v) {
 // 128 of 800, 47.6 / 41.5 at 256 of 400, 1669 / 305 at 4096 of 100.)  Of each 64 those with chunks longer
 // than half the longest come first, so that the last workgroups to start have
 // the least to do; a sequence's last tiles come first, which see the most.
+template <bool EX>
 __device__ __forceinline__ Item find_item(const Call& c, int id, int* err) {
     const int lane = threadIdx.x & 63;
     Item it{};
@@ -173,6 +174,7 @@ __device__ __forceinline__ Item find_item(const Call& c, int id, int* err) {
     }
     Seq q{};
     if (s0 + lane < c.n_seq) q = seq_at(c, s0 + lane);
+    if (EX && c.uncut) drop_uncut(c, c.plan[1], q);
     if (!c.plan) {
         if (q.bad && id == 0 && threadIdx.x < 64) atomicOr(err, ERR_INDEX);
         const int64_t total = c.n_seq > 1 ? wave_total(keys_of(q)) : lane_bcast(keys_of(q), 0);
@@ -566,7 +568,7 @@ __global__ __launch_bounds__(64 * NW, HD <= 192 ? 2 : 1) void kv_decode_kernel(c
     __shared__ int holes[NW];
     const int n_kv = a.c.n_kv;
     const int kvh = blockIdx.x % n_kv;
-    const Item it = find_item(a.c, blockIdx.x / n_kv, a.err);
+    const Item it = find_item<EX>(a.c, blockIdx.x / n_kv, a.err);
     if (kvh == 0) note_item(a.rec, blockIdx.x / n_kv, it);
     if (!it.found) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -1004,7 +1006,7 @@ __global__ __launch_bounds__(256, (Prompt<DT, HD>::WAVES)) void kv_prompt_kernel
     float* lvs = lks + 2 * KT;
     const int n_kv = a.c.n_kv;
     const int kvh = blockIdx.x % n_kv;
-    const Item it = find_item(a.c, blockIdx.x / n_kv, a.err);
+    const Item it = find_item<EX>(a.c, blockIdx.x / n_kv, a.err);
     if (kvh == 0) note_item(a.rec, blockIdx.x / n_kv, it);
     if (!it.found) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;

@@ -35,12 +35,14 @@ struct Call {
     int min_pairs, max_pairs;  // the sequences served: pairs in [min, max]
     int64_t target;        // items wanted over all kv heads
     int min_chunk;         // keys a chunk at least, 64, 128 or 256
-    const int32_t* plan;   // of many sequences: the chunk length and 0, then before each 64 sequences (items, slots)
+    const int32_t* plan;   // of many sequences: the chunk length and fills(), then before each 64 sequences (items, slots)
     int sinks, sink_span;  // with a window: first keys seen besides, and as a tile spans them (sink_keys; 0: none)
     const uint64_t* tree;  // bit masks of drafted tokens, a row of q each (null: rows see what lies before them)
     int64_t tree_pitch;    // words between the masks
     int64_t even;          // items wanted where the tiles have nearly the same keys, up to target (0: target)
     int64_t slots;         // or the items that fill the chip, up to target, for wanted() (0: target)
+    int uncut;             // with a plan: drop_uncut()'s pairs (0: all that is served)
+    bool prompt;           // and the launch
 };
 
 struct Seq {
@@ -139,6 +141,22 @@ KV_HD int64_t max_tiles(const Call& c) {
     return least < by_seq ? least : by_seq;
 }
 KV_HD int64_t max_items(const Call& c) { return max_tiles(c) + c.target / c.n_kv + 1; }
+// A prompt launch that has no room for parts takes its sequences, of uncut pairs and
+// more, where they fill it: their tiles' keys, of which a workgroup walks one tile's,
+// come to those of LONE workgroups with the longest.  Else the decode launch does.
+// (The keys without a window's rows and roundings: the same for both launches.)
+constexpr int LONE = 128;
+KV_HD int lone_keys(const Call& c, const Seq& q) {
+    const int64_t span = (int64_t)c.window + c.sinks;
+    return c.window && span < q.len ? (int)span : q.len;
+}
+KV_HD int64_t lone_tiles(const Call& c, const Seq& q) { return ((int64_t)q.rows * c.rep + 127) >> 7; }
+KV_HD bool fills(int64_t total, int most, int n_kv) { return total > 0 && total * n_kv >= (int64_t)most * LONE; }
+// What of a sequence one of both launches serves then (the decode launch's max_pairs
+// and the prompt launch's min_pairs let it through).
+KV_HD void drop_uncut(const Call& c, bool filled, Seq& q) {
+    if (c.prompt ? !filled : filled && (int64_t)q.rows * c.rep >= c.uncut) q.tiles = 0;
+}
 // More sequences than this are summed once for the call, into a plan.
 constexpr int PLAN_SEQS = 64;
 KV_HD int64_t plan_words(int64_t n_seq) { return n_seq > PLAN_SEQS ? 2 + (n_seq + 63) / 64 * 2 : 0; }

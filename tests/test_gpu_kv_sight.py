@@ -466,6 +466,52 @@ def test_small_trees_beside_large_ones(ctx, kind, window, sinks):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("trees", [False, True])
+def test_batches_with_idle_sequences(ctx, kind, trees):
+    """No more rows than sequences, most of them idle, sequences of a row beside
+    large ones: which do or do not fill a launch that cuts no keys, also behind
+    one another in a graph; and a length that no table holds."""
+    rng = np.random.default_rng(12)
+    for kv, rep, n, lens, rows in ((2, 7, 64, [4000, 300, 40], [16, 1, 5]), (8, 16, 200, [900, 300, 150, 7], [140, 1, 20, 2]),
+                                   (8, 16, 130, [1700, 0, 95], [95, 1, 30]), (1, 140, 70, [2000, 33], [9, 1]),
+                                   (8, 16, 90, [400, 50] * 5, [16, 2] * 5)):
+        rows, lens = rows + [0] * (n - len(rows)), lens + [0] * (n - len(lens))
+        if trees:
+            rows = [min(a, b) for a, b in zip(rows, lens)]
+        assert sum(rows) <= n
+        More(ctx, kind, 16, kv, rep, 32, lens, rows, seed=n, window=600, sinks=9,
+             trees=[grow(rng, r) for r in rows] if trees else None).check()
+    n, lens, rows = 200, [700, 300, 150, 400, 40] + [0] * 195, [120, 1, 20, 30, 2] + [0] * 195
+    b = More(ctx, kind, 16, 8, 16, 32, lens, rows, seed=n, window=600, sinks=9, trees=[grow(rng, r) for r in rows] if trees else None)
+    b.check()
+    graph, held = Graph(ctx, b.call), (list(b.k), list(b.v))
+    for first in (130, 700, 2 ** 30):  # the longest and its share of the keys
+        put(b.dev[1], np.array([first] + lens[1:], np.int32))
+        b.lens = [first if first < 2 ** 30 else 0] + lens[1:]
+        b.k, b.v = ([x[:n] for x, n in zip(y, b.lens)] for y in held)
+        outs = []
+        for how in (graph.replay, b.call):
+            put(b.do, np.full(b.do.shape, 7.0, np.float32))
+            how()
+            if first < 2 ** 30:
+                ctx.sync()
+            else:
+                with pytest.raises(fa.FrqError):
+                    ctx.sync()
+            outs.append(b.do.numpy()[:b.n_row])
+        assert same(*outs)
+        if first < 2 ** 30:
+            hold(outs[0], *b.want())
+        else:
+            assert (outs[0][:120] == (7.0 if trees else 0.0)).all()
+            b.lens[0], b.rows = 120, [120] + rows[1:]
+            b.k, b.v = ([x[:n] for x, n in zip(y, b.lens)] for y in held)
+            want, tol = b.want()
+            hold(outs[0][120:], want[120:], tol[120:])
+    graph.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("page", [16, 128, 1024])
 def test_pages_and_pitches(ctx, kind, page):
     """Strided pages of every size, rows of q and out that lie apart."""

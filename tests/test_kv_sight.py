@@ -266,3 +266,70 @@ def test_items_wanted_stay_within_the_target(tmp_path):
         for kv in (1, 4, 65535):
             assert lib.items(0, 400, tiles, kv) == 400
             assert lib.items(512, 512, tiles, kv) == max(256, 512 - tiles * kv)
+
+
+UNCUT = r"""
+#include "kv_index.h"
+using namespace frq::kv;
+// sequences that each launch serves, and whether the prompt launch is filled
+extern "C" int uncut(const int32_t* len, const int32_t* first, int n_seq, int rep, int n_kv, int window, int pairs, int* dec,
+                     int* prompt) {
+    Call a{len, first, n_seq, first[n_seq], 8192, 4, rep, window, n_kv, 16, 1, 0x7FFFFFFF, 512, 128};
+    Call b = a;
+    a.uncut = b.uncut = b.min_pairs = pairs;
+    b.tp = 128;
+    b.prompt = true;
+    int64_t total = 0;
+    int most = 0;
+    for (int s = 0; s < n_seq; ++s) {
+        const Seq x = seq_at(a, s), y = seq_at(b, s);  // (the launches sum their own)
+        if (!y.tiles) continue;
+        if (lone_tiles(a, x) != y.tiles || lone_tiles(b, y) != y.tiles || lone_keys(a, x) != lone_keys(b, y)) return -1;
+        total += lone_tiles(b, y) * lone_keys(b, y);
+        if (lone_keys(b, y) > most) most = lone_keys(b, y);
+    }
+    const bool filled = fills(total, most, n_kv);
+    for (int s = 0; s < n_seq; ++s) {
+        Seq x = seq_at(a, s), y = seq_at(b, s);
+        drop_uncut(a, filled, x);
+        drop_uncut(b, filled, y);
+        dec[s] = x.tiles;
+        prompt[s] = y.tiles;
+    }
+    return filled;
+}
+"""
+
+
+def test_a_launch_that_cuts_no_keys_is_filled(tmp_path):
+    """A batch with idle sequences: each sequence is served once, and by workgroups
+    that walk all of its keys only where all of these have 128 times the longest."""
+    (tmp_path / "u.cpp").write_text(UNCUT)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", "-I",
+                    os.path.join(ROOT, "fieldrun_amd", "csrc"), str(tmp_path / "u.cpp"), "-o", str(tmp_path / "u.so")], check=True)
+    lib = C.CDLL(str(tmp_path / "u.so"))
+    lib.uncut.argtypes = [C.c_void_p] * 2 + [C.c_int] * 5 + [C.c_void_p] * 2
+    rng = np.random.default_rng(7)
+    seen = [0, 0]
+    for _ in range(1500):
+        n = int(rng.integers(65, 400))
+        rows = np.where(rng.random(n) < 10.0 ** rng.uniform(-2.5, 0), 10.0 ** rng.uniform(0, rng.choice([1.0, 2.5])), 0).astype(np.int32)
+        lens = np.maximum(rows, 10.0 ** rng.uniform(0, rng.choice([2.0, 4.9]), n)).astype(np.int32)
+        first = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+        rep, kv, pairs = int(rng.choice([1, 4, 7, 64])), int(rng.choice([1, 2, 8, 129])), int(rng.choice([33, 129]))
+        window = int(rng.choice([0, 100]))
+        dec, prompt = np.zeros(n, np.int32), np.zeros(n, np.int32)
+        filled = lib.uncut(lens.ctypes.data, first.ctypes.data, n, rep, kv, window, pairs, dec.ctypes.data, prompt.ctypes.data)
+        large = rows.astype(np.int64) * rep >= pairs
+        assert ((dec > 0) != (prompt > 0))[rows > 0].all() and not (dec + prompt)[rows == 0].any()
+        assert ((prompt > 0) == (large & bool(filled))).all()
+        if large.any():
+            own = np.minimum(lens[large], window or 1 << 30)
+            assert bool(filled) == ((-(-rows[large].astype(np.int64) * rep // 128) * own).sum() * kv >= 128 * int(own.max()))
+        seen[filled] += 1
+    assert min(seen) > 200, seen
+    # one tree of 112 pairs beside idle sequences, many alike
+    for rows, want in (([16] + [0] * 79, 0), ([16] * 64 + [0] * 16, 1), ([16] * 63 + [0] * 17, 0)):
+        first = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+        lens, out = np.full(80, 32768, np.int32), np.zeros((2, 80), np.int32)
+        assert lib.uncut(lens.ctypes.data, first.ctypes.data, 80, 7, 2, 0, 33, out[0].ctypes.data, out[1].ctypes.data) == want
