@@ -333,3 +333,60 @@ def test_a_launch_that_cuts_no_keys_is_filled(tmp_path):
         first = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
         lens, out = np.full(80, 32768, np.int32), np.zeros((2, 80), np.int32)
         assert lib.uncut(lens.ctypes.data, first.ctypes.data, 80, 7, 2, 0, 33, out[0].ctypes.data, out[1].ctypes.data) == want
+
+
+FILLED = r"""
+#include "kv_index.h"
+using namespace frq::kv;
+extern "C" void filled(const int32_t* len, const int32_t* first, int n_seq, int rep, int n_kv, int window, int sinks, int trees,
+                       int64_t want, int least, int64_t* out) {
+    Call c{len, first, n_seq, first[n_seq], 1 << 17, 10, rep, window, n_kv, 128, least, 0x7FFFFFFF, want, 128};
+    c.sinks = sinks;
+    c.sink_span = sink_keys(sinks, 64);
+    c.tree = trees ? (const uint64_t*)8 : nullptr;
+    c.tree_pitch = 64;
+    c.slots = want;
+    int64_t total = 0, tiles = 0, items = 0, slots = 0;
+    for (int s = 0; s < n_seq; ++s) { const Seq q = seq_at(c, s); total += keys_of(q); tiles += q.tiles; }
+    const int klen = chunk_of(c, total, wanted(c, tiles));
+    for (int s = 0; s < n_seq; ++s) {
+        const Seq q = seq_at(c, s);
+        const int n = q.tiles ? chunks_of(q, klen) : 1;
+        items += (int64_t)q.tiles * n;
+        if (n > 1) slots += (int64_t)q.tiles * n;
+    }
+    out[0] = items;
+    out[1] = max_items(c);
+    out[2] = slots;
+    out[3] = max_slots(want, n_kv);
+}
+"""
+
+
+def test_chunks_of_the_items_wanted_keep_the_bounds(tmp_path):
+    """The prompt launch of calls with sinks or trees, as kernels cut it: no more
+    items than its grid and records, no more parts than its workspace."""
+    (tmp_path / "f.cpp").write_text(FILLED)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", "-I",
+                    os.path.join(ROOT, "fieldrun_amd", "csrc"), str(tmp_path / "f.cpp"), "-o", str(tmp_path / "f.so")], check=True)
+    lib = C.CDLL(str(tmp_path / "f.so"))
+    lib.filled.argtypes = [C.c_void_p] * 2 + [C.c_int] * 6 + [C.c_int64, C.c_int, C.c_void_p]
+    lib.filled.restype = None
+    rng, cut = np.random.default_rng(11), 0
+    for i in range(4000):
+        n = int(rng.choice([1, 2, 5, 20, 64, 300]))
+        lens = (10.0 ** rng.uniform(0, rng.choice([2.0, 4.5, 8.0]), n)).astype(np.int32)
+        rows = np.minimum(lens, 10.0 ** rng.uniform(0, rng.choice([1.0, 2.0, 3.6]), n)).astype(np.int32)
+        rows[rng.random(n) < rng.choice([0.0, 0.5])] = 0
+        if i % 3 == 0:
+            lens[:], rows[:] = lens[0], rows[0]
+        first = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+        window = int(rng.choice([0, 1, 100, 4096]))
+        out = np.zeros(4, np.int64)
+        lib.filled(lens.ctypes.data, first.ctypes.data, n, int(rng.choice([1, 3, 7, 16])), int(rng.choice([1, 2, 4, 5, 8, 64, 600])),
+                   window, int(rng.choice([0, 4, 500])) if window else 0, i % 2, int(rng.choice([256, 512])),
+                   int(rng.choice([1, 33, 129])), out.ctypes.data)
+        items, most_items, slots, most_slots = out.tolist()
+        assert items <= most_items and slots <= most_slots, (i, out)
+        cut += slots > 0
+    assert cut > 500
