@@ -311,8 +311,11 @@ extern "C" int frq_kv_append_dev(frq_ctx* ctx, const frq_kv* kv, const frq_rotar
     const size_t wide = (n_head + 2 * kv->n_kv) * kv->hd;
     if (pitch < wide || q_pitch < n_head * kv->hd || pitch > ((size_t)1 << 40) || q_pitch > ((size_t)1 << 40))
         return bad("pitch is below the heads' width");
-    // (a workgroup for every row and eight heads, and for eight rows of every kv head)
-    if (n > ((size_t)1 << 31) || n * (n_head + 2 * kv->n_kv) > 0x7FFFFFFF) return bad("too many rows");
+    // (many rows: a workgroup for every two, and for 32 of every kv head; a launch has
+    // fewer than 2^32 threads)
+    if (n > ((size_t)1 << 31) || n * (n_head + 2 * kv->n_kv) > 0x7FFFFFFF ||
+        ((n + 1) / 2 + (n + 31) / 32 * kv->n_kv) * 256 > 0xFFFFFFFFull)
+        return bad("too many rows");
     if (n && (!d_qkv || !d_q || !d_slot || (how->rot && (!d_pos || !how->freq)))) return bad("null pointer");
     if (!ctx) return bad("null context");
     if (!n) return FRQ_OK;

@@ -40,3 +40,13 @@ def test_null_rotary():
     d = C.byref(desc())
     assert fa.lib.frq_kv_append_dev(None, d, None, A, 512, 4, A, A, 1, A, 256) == fa.FRQ_ERR_ARG
     assert "null rotary" in message()
+
+
+def test_rows_that_no_launch_holds_are_refused():
+    """A grid has fewer than 2^32 threads: a workgroup for every two rows, one for
+    every 32 of each of 2 kv heads."""
+    most = (2 ** 24 - 1) * 16 // 9
+    for n in (most + 32, 1 << 25, 1 << 26):
+        assert append(n=n) == fa.FRQ_ERR_ARG and "too many" in message(), message()
+    for n in (most - 32, 1 << 24):
+        assert append(n=n) == fa.FRQ_ERR_ARG and "null context" in message(), message()
