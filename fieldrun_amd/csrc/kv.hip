@@ -311,7 +311,7 @@ constexpr int64_t DEC_TARGET = 512;
 // rows of one f16 tree over 8000 27.7, 25.8.  But 20 f32 sequences of 100 to 6001 by 256
 // channels 101, 129 (of 256 items: these keep the target), 8 f16 trees of 35 pairs over
 // 2000 27, 33, f32 49, 54.
-constexpr int64_t EVEN_TARGET = 256;
+constexpr int EVEN_TARGET = 256;
 // Prompt items wanted: a round and not quite two a CU; more cost the joining
 // more than the balance gives (400, 640, 1024, 1536: kernel and join of 7 ragged
 // int8 prompts 123 + 8, 127 + 18, 110 + 24, 108 + 24 us; of 2048 rows over 8192
@@ -398,7 +398,7 @@ Plan plan_of(const frq_kv* kv, size_t n_row, size_t n_head, size_t n_seq, bool e
     p.prompt.tp = 128;
     // (n_row <= n_seq: no room for parts, every tile's keys in one run)
     p.prompt.target = n_row <= n_seq ? 1 : ex ? ex_slots(kv) : kv->hd > 128 ? PROMPT_TARGET_WIDE : PROMPT_TARGET;
-    if (ex && n_row > n_seq) p.prompt.slots = p.prompt.target;
+    if (ex && n_row > n_seq) p.prompt.slots = (int)p.prompt.target;
     // (f32 keys of over 128 channels have no prompt kernel)
     const bool f32 = kv->dtype == FRQ_DT_F32;
     const size_t pairs = n_row * c.rep, mean = big && (trees || !f32) ? EX_PAIRS : DEC_PAIRS;

@@ -174,12 +174,13 @@ __device__ __forceinline__ Item find_item(const Call& c, int id, int* err) {
     }
     Seq q{};
     if (s0 + lane < c.n_seq) q = seq_at(c, s0 + lane);
-    if (EX && c.uncut) drop_uncut(c, c.plan[1], q);
     if (!c.plan) {
         if (q.bad && id == 0 && threadIdx.x < 64) atomicOr(err, ERR_INDEX);
         const int64_t total = c.n_seq > 1 ? wave_total(keys_of(q)) : lane_bcast(keys_of(q), 0);
         if (!c.even) klen = chunk_of(c, total, c.slots ? wanted(c, wave_total(q.tiles)) : c.target);
         else klen = chunk_of_even(c, total, wave_total(q.tiles), wave_most(q.tiles ? q.ext : 0));
+    } else if (EX && c.uncut) {
+        drop_uncut(c, c.plan[1], q);
     }
     const int n = q.tiles ? chunks_of(q, klen) : 1, own = even_chunk(q, n), mine = q.tiles * n;
     const int most = wave_most(own);

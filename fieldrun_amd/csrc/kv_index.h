@@ -39,8 +39,8 @@ struct Call {
     int sinks, sink_span;  // with a window: first keys seen besides, and as a tile spans them (sink_keys; 0: none)
     const uint64_t* tree;  // bit masks of drafted tokens, a row of q each (null: rows see what lies before them)
     int64_t tree_pitch;    // words between the masks
-    int64_t even;          // items wanted where the tiles have nearly the same keys, up to target (0: target)
-    int64_t slots;         // or the items that fill the chip, up to target, for wanted() (0: target)
+    int even;              // items wanted where the tiles have nearly the same keys, up to target (0: target)
+    int slots;             // or the items that fill the chip, up to target, for wanted() (0: target)
     int uncut;             // with a plan: drop_uncut()'s pairs (0: all that is served)
     bool prompt;           // and the launch
 };
