@@ -332,7 +332,8 @@ constexpr int DEC_PAIRS = 128;
 // pairs over 32768 tokens 238, 95.  Where the whole call is small its latency
 // counts: one sequence of 112 pairs over 8000 tokens 27, 32 us, of 56 over 211
 // 9.7, 19.6, of 336 over 2000 27, 27.  (The tokens are those that the table has room
-// for; lengths are device data.)
+// for, as lengths are device data: 56 pairs over 211 tokens with 4 heads of 128 take 13 us
+// with a table of 256 tokens, 23 with one of 32768.)
 constexpr int TREE_PAIRS = 32;
 constexpr double EX_WORK = 6e6;  // rows x heads x keys
 // With sinks or trees the prompt kernel serves every sequence where they have more
@@ -500,10 +501,11 @@ int attend(frq_ctx* ctx, const frq_kv* kv, const float* d_q, size_t q_pitch, siz
     // Each sequence is served by the kernel of its number of pairs; one that
     // no sequence can be for is not launched.
     // (f32 keys of over 128 channels stay with the decode kernel: three parts of
-    // q leave the prompt kernel one wave a SIMD.  2048 rows of 8 heads over 4, the
-    // decode kernel against the prompt kernel: 256 channels 288, 340 us over
-    // themselves, 72, 78 at 600 rows, 1612, 1508 over 8192 tokens; 192 channels 225,
-    // 202 and 1280, 676.  Widths of an odd number of 32s do not fit the LDS.)
+    // q leave the prompt kernel one wave a SIMD, and widths of an odd number of 32s
+    // do not fit the LDS.  2048 rows of 8 heads over 4, the decode kernel against the
+    // prompt kernel: 256 channels 288, 340 us over themselves, 72, 78 at 600 rows,
+    // 1612, 1508 over 8192 tokens.  At 192 channels, 225, 202 and 1280, 676, one rule
+    // for these widths costs time.)
     const bool prompts = d_first && n_row * (size_t)a.c.rep >= (size_t)plan.prompt.min_pairs &&
                          !(kv->dtype == FRQ_DT_F32 && kv->hd > 128);
     const int uncut = prompts ? plan.prompt.uncut : 0;

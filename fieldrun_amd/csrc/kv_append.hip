@@ -133,7 +133,7 @@ __device__ __forceinline__ void append_values(const Append& a, unsigned block, E
 // a lane in flight, the rows' turns in LDS.  Bound by memory for long prompts: 8192
 // rows of 36 heads of 128 channels, int8 pages, 277 MB in 66 us (4.2 TB/s); 8 rows
 // a workgroup 76, 4 70, 1 68; two heads in flight 77 at 8 rows.  A step's few rows
-// are bound by latency: one f16 row of 18 heads of 64 2.8 us, 61 f32 rows of 25 of 80 3.7.
+// are bound by latency: one f16 row of 18 heads of 64 3.0 us, 61 f32 rows of 25 of 80 3.7.
 constexpr int MAX_ROWS = 2;  // a workgroup's, of queries and keys
 template <int DT, int G, int WR>
 __global__ __launch_bounds__(256) void kv_append_kernel(const Append a) {

@@ -113,7 +113,9 @@ KV_HD int chunk_of_even(const Call& c, int64_t total, int64_t tiles, int most) {
     const uint32_t n = (uint32_t)c.even / ((uint32_t)tiles * (uint32_t)c.n_kv);  // chunks a tile: one round
     // (chunks of half the least for a few hundred keys, where a tile's latency counts: one
     // sequence of 1000 keys, 4 int8 heads of 128, 14.4 us in five chunks, 12.8 in nine; two
-    // for 200 keys or sixteen for 2000 cost the joining more, 10.0 / 11.3, 12.1 / 13.1)
+    // for 200 keys or sixteen for 2000 cost the joining more, 10.0 / 11.3, 12.1 / 13.1.
+    // Several, 4 heads of 256: 2 f16 ones of 600 19.2 / 16.4, 4 of 1000 20.0 / 17.2, 8 int8
+    // ones of 600 20.4 / 16.9; 16 and more the same but f16 of 1500, 27.3 / 29.7)
     const int least = most > 256 && most <= 12 * 128 && c.min_chunk > 128 ? 128 : c.min_chunk;
     const int up = round_keys(((uint32_t)most + n - 1) / n, least);
     return up < least ? least : up;

@@ -26,8 +26,8 @@
 // over the row instead.  Short rows take one launch (sample_one_kernel).
 //
 // Few rows are bound by the launches' latency (one row of 152064 logits 23 us, 9
-// of 50257 28 us), many by the two readings of the logits: 64 rows of 152064 (39
-// MB) 48 us, of which the histograms 15 and the second reading 16.
+// of 50257 25 us), many by the two readings of the logits: 64 rows of 152064 (39
+// MB) 53 us, of which the histograms 15 and the second reading 15.
 #include "frq_internal.h"
 
 namespace frq {
@@ -314,7 +314,7 @@ __device__ __forceinline__ void add_bins(const H& held, const Ask& q, double e, 
 }
 
 // A workgroup a chunk, its logits in registers between the maximum and the bins.  64
-// rows of 152064 (39 MB) in 14 us: the weights, some 35 operations of 64 bits a
+// rows of 152064 (39 MB) in 15 us: the weights, some 35 operations of 64 bits a
 // logit, take as long as the reading beside them.  Two or four copies of the
 // histograms against colliding atomics: the same; half the chunks, twice as long: 56
 // us the call against 49.
@@ -458,7 +458,7 @@ __device__ __forceinline__ Row row_of(const Ask& q, double e, double least, cons
 }
 
 // A workgroup a row.  Bound by latency, the loads of the chunks' histograms and
-// the fetching of its own code, which is run once: one row of 38 chunks 6 us; 10 and
+// the fetching of its own code, which is run once: one row of 38 chunks 7 us; 10 and
 // 20 loads a thread in flight instead of 4 and 8, 2 KB of code more, 4 us longer.
 constexpr int RT = 1024;  // threads: two a bin
 __global__ __launch_bounds__(RT) void sample_row_kernel(const Args a) {
@@ -590,7 +590,7 @@ __device__ __forceinline__ void put_list(const H& held, int beg, uint32_t in, in
     });
 }
 
-// A workgroup a chunk again (14 us there): the weights of what is kept whole, by the
+// A workgroup a chunk again (15 us there): the weights of what is kept whole, by the
 // row's scale, and the list's elements, one atomic a workgroup.
 template <int NV>
 __global__ __launch_bounds__(NT) void sample_take_kernel(const Args a) {
@@ -907,7 +907,7 @@ __device__ __forceinline__ void finish_row(const Args& a, const float* x, const 
     }
 }
 
-// A workgroup a row (finish_row): one row 6 us, 64 rows 10, those with the longest lists.
+// A workgroup a row (finish_row): one row 7 us, 64 rows 11, those with the longest lists.
 __global__ __launch_bounds__(FT) void sample_token_kernel(const Args a) {
     extern __shared__ __align__(16) char lds[];
     Last& L = *reinterpret_cast<Last*>(lds);

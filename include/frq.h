@@ -270,8 +270,8 @@ int frq_kv_read_dev(frq_ctx* ctx, const frq_kv* kv, const int64_t* d_slot,
  * bits and rounded to f32 once (angles up to 2^30 radians).  q goes to d_q (row
  * i at d_q + i * q_pitch; d_q may be d_qkv with its pitch, else it lies apart),
  * keys and values into their slots as frq_kv_write_dev puts them there; a row
- * without a place leaves its q alone.  d_pos (may be below 0) and freq may be
- * NULL where rot is 0. */
+ * without a place is left out there, its q is made all the same.  d_pos (may be
+ * below 0) and freq may be NULL where rot is 0. */
 int frq_kv_append_dev(frq_ctx* ctx, const frq_kv* kv, const frq_rotary* how,
                       const float* d_qkv, size_t pitch, size_t n_head,
                       const int32_t* d_pos, const int64_t* d_slot, size_t n,
@@ -311,7 +311,11 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q,
 /* frq_kv_attn_dev with more to see than a window: a row at position p sees the
  * tokens j <= p of p - j < window and of j < sinks, a sequence's first ones,
  * which stay (window 0: all).  Their pages stay in the table; those between them
- * and the window may be gone.  Workspace and all else as there. */
+ * and the window may be gone.  Positions are those in the whole sequence: keys are
+ * read as they were cached, and are not rotated anew to places within what is
+ * kept.  Workspace and all else as there; which kernel serves a sequence, and so
+ * its roundings, goes by the whole call, here and below: n_row, n_head, n_seq,
+ * and of the tokens by those that the table has room for, pages_pitch pages. */
 int frq_kv_attn_sink_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q,
                          size_t q_pitch, size_t n_row, size_t n_head,
                          const int32_t* d_pages, size_t pages_pitch,
