@@ -315,7 +315,8 @@ int frq_kv_attn_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q,
  * read as they were cached, and are not rotated anew to places within what is
  * kept.  Workspace and all else as there; which kernel serves a sequence, and so
  * its roundings, goes by the whole call, here and below: n_row, n_head, n_seq,
- * and of the tokens by those that the table has room for, pages_pitch pages. */
+ * the tokens that the table has room for (pages_pitch pages), and, where there are
+ * no more rows than sequences, the lengths. */
 int frq_kv_attn_sink_dev(frq_ctx* ctx, const frq_kv* kv, const float* d_q,
                          size_t q_pitch, size_t n_row, size_t n_head,
                          const int32_t* d_pages, size_t pages_pitch,
